@@ -35,6 +35,12 @@ EXPORTS = [
     "catccos_b200_packed_row_bytes",
     "catccos_b200_mx_quant_scatter_packed",
     "catccos_b200_mxfp8_matmul_reduce_scatter",
+    "catccos_b200_add_rms_norm_mx_quant",
+    "catccos_b200_moe_route",
+    "catccos_b200_moe_row_plan",
+    "catccos_b200_mx_grouped_gemm",
+    "catccos_b200_moe_combine",
+    "catccos_b200_mx_fp4_matvec",
     "catccos_b200_mx_quant_matmul_static",
     "catccos_b200_mx_quant_matmul_static_status",
     "catccos_b200_last_status",
@@ -96,6 +102,13 @@ def load() -> ctypes.CDLL:
     L.catccos_b200_packed_row_bytes.restype = sz
     L.catccos_b200_mx_quant_scatter_packed.argtypes = [vp, vp, vp, vp, u32, u32, u32]
     L.catccos_b200_mxfp8_matmul_reduce_scatter.argtypes = [vp, vp, vp, vp, vp, vp, vp, tp, u32]
+    f32 = ctypes.c_float
+    L.catccos_b200_add_rms_norm_mx_quant.argtypes = [vp, vp, vp, vp, f32, u32, u32, vp, vp, vp, vp]
+    L.catccos_b200_moe_route.argtypes = [vp, vp, i32, vp, u32, u32, u32, u32, u32, u32, i32, i32, f32, vp, vp]
+    L.catccos_b200_moe_row_plan.argtypes = [vp, vp, u32, u32, i32, vp, vp]
+    L.catccos_b200_mx_grouped_gemm.argtypes = [vp, vp, sz, vp, sz, vp, vp, vp, vp, u32, u32, u32, u32]
+    L.catccos_b200_moe_combine.argtypes = [vp, vp, u32, vp, vp, vp, vp, u32, u32, u32, i32]
+    L.catccos_b200_mx_fp4_matvec.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32]
     L.catccos_b200_mx_quant_matmul_static.argtypes = [vp, vp, vp, vp, vp, u32, u32, u32]
     L.catccos_b200_last_status.argtypes = [ctypes.POINTER(u32)]
     L.catccos_b200_mx_quant_matmul_static_status.argtypes = [ctypes.POINTER(u32)]
@@ -283,6 +296,88 @@ def mx_quant_scatter_packed(x_bf16, expanded_row_idx, packed_out, top_k: int) ->
     code = (_calls or _load_calls()).mx_quant_scatter_packed(x_bf16, expanded_row_idx, packed_out, top_k)
     if code:
         raise CatccosError("catccos_b200_mx_quant_scatter_packed", code)
+
+
+def add_rms_norm_mx_quant(x_bf16, residual, weight, eps: float, residual_out=None, norm_out=None):
+    """h = bf16(x + residual), y = h / sqrt(mean(h^2) + eps) * weight, MX-quantised: (codes uint8 [rows, n], scales uint8 [rows, n/32]).
+
+    h goes to residual_out, by default back into residual; residual None: h = x.  norm_out (bf16 [rows, n]) takes y as well."""
+    code, codes, scales = (_calls or _load_calls()).add_rms_norm_mx_quant(x_bf16, residual, weight, eps, residual_out, norm_out)
+    if code:
+        raise CatccosError("catccos_b200_add_rms_norm_mx_quant", code)
+    return codes, scales
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route(logits, top_k: int, bias=None, score: str = "softmax", groups: int = 1, top_groups: int = 1, group_best: int = 1,
+              renormalize: bool = True, scale: float = 1.0):
+    """Router logits [tokens, experts] (fp32 or bf16) -> (ids int32, weights fp32), both [tokens, top_k], best expert first.
+
+    Chosen by score + bias (fp32 [experts]) among the experts of the top_groups groups whose group_best best add up highest;
+    weighted by the score alone, renormalised over the chosen, times scale.  Places that cannot be filled: id -1, weight 0."""
+    if score not in _SCORES:
+        raise ValueError(f"score is one of {sorted(_SCORES)}, got {score!r}")
+    code, ids, weights = (_calls or _load_calls()).moe_route(logits, bias, top_k, groups, top_groups, group_best, _SCORES[score],
+                                                             1 if renormalize else 0, scale)
+    if code:
+        raise CatccosError("catccos_b200_moe_route", code)
+    return ids, weights
+
+
+def moe_row_plan(ids, experts: int, first_expert: int = 0):
+    """ids int32 [tokens, top_k] -> (row_index int32 [tokens, top_k], offsets int32 [experts + 1]): routes sorted by expert.
+
+    row_index is the expanded_row_idx of mx_quant_scatter_packed (-1: not one of this rank's experts first_expert ..
+    first_expert + experts - 1), rows offsets[e] .. offsets[e + 1] belong to expert first_expert + e."""
+    code, row_index, offsets = (_calls or _load_calls()).moe_row_plan(ids, experts, first_expert)
+    if code:
+        raise CatccosError("catccos_b200_moe_row_plan", code)
+    return row_index, offsets
+
+
+def mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out=None, out_dtype=None):
+    """c [rows, N]: rows offsets[e] .. offsets[e + 1] are dequant(a) x dequant(b[e]); b [experts, K, N], b_scales [experts, K/64, N, 2].
+
+    a_codes [rows, K] and a_scales [rows, K/32] may be columns of a wider tensor (packed[:, :K] and packed[:, K:K + K // 32] of
+    mx_quant_scatter_packed).  Rows outside the offsets stay as they are (of a tensor allocated here: unset)."""
+    if out is None:
+        import torch
+
+        out = torch.empty((a_codes.shape[0], b_scales.shape[-2]), dtype=out_dtype or torch.bfloat16, device=a_codes.device)
+    code = (_calls or _load_calls()).mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out)
+    if code:
+        raise CatccosError("catccos_b200_mx_grouped_gemm", code)
+    return out
+
+
+def moe_combine(expert_out, row_index, weights, shared=None, out=None):
+    """out [tokens, n] = sum over r of weights[t, r] * expert_out[row_index[t, r]] (+ shared[t]); bf16 or fp16, sums in fp32."""
+    if out is None:
+        import torch
+
+        out = torch.empty((row_index.shape[0], expert_out.shape[1]), dtype=expert_out.dtype, device=expert_out.device)
+    code = (_calls or _load_calls()).moe_combine(expert_out, row_index, weights, shared, out)
+    if code:
+        raise CatccosError("catccos_b200_moe_combine", code)
+    return out
+
+
+def mx_fp4_matvec(x_bf16, w, w_scales, ids=None, out=None, out_dtype=None):
+    """x [rows, K] x dequant(w): w packed E2M1 [K, N/2], w_scales [K/64, N, 2] -> [rows, N].
+
+    With ids int32 (any shape, i values): w [experts, K, N/2], w_scales [experts, K/64, N, 2] -> [i, N], row r with weight ids[r]
+    and x's row r // (i // rows); a negative id gives a row of zeros."""
+    if out is None:
+        import torch
+
+        out = torch.empty((x_bf16.shape[0] if ids is None else ids.numel(), w_scales.shape[-2]), dtype=out_dtype or torch.bfloat16,
+                          device=x_bf16.device)
+    code = (_calls or _load_calls()).mx_fp4_matvec(x_bf16, w, w_scales, ids, out)
+    if code:
+        raise CatccosError("catccos_b200_mx_fp4_matvec", code)
+    return out
 
 
 def mxfp8_matmul_reduce_scatter(a_codes, a_scales, b, b_scales, d, symm: int, world: int) -> None:

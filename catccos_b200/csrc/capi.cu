@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -17,10 +18,14 @@
 #include "bootstrap.hpp"
 #include "internal_options.h"
 #include "common.cuh"
+#include "fp4_matvec.cuh"
+#include "moe.cuh"
 #include "mx_gemm.cuh"
 #include "mx_gemm_pair.cuh"
 #include "mx_gemm_small.cuh"
+#include "mx_grouped_gemm.cuh"
 #include "mx_quant.cuh"
+#include "norm_quant.cuh"
 
 using namespace catccos;
 
@@ -442,10 +447,11 @@ struct MapKey {
     uint32_t box_inner, box_outer;
     bool fp4;
     uint32_t elem;
+    uint64_t pitch;
     bool operator==(const MapKey& o) const
     {
         return base == o.base && inner == o.inner && outer == o.outer && box_inner == o.box_inner &&
-               box_outer == o.box_outer && fp4 == o.fp4 && elem == o.elem;
+               box_outer == o.box_outer && fp4 == o.fp4 && elem == o.elem && pitch == o.pitch;
     }
 };
 constexpr int kMapCacheSize = 16;
@@ -457,13 +463,14 @@ struct MapCache {
 } g_maps;
 
 int encode_map_2d_uncached(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
-                           uint32_t box_outer, bool fp4, uint32_t elem);
+                           uint32_t box_outer, bool fp4, uint32_t elem, uint64_t pitch);
 
-// inner / outer / box in elements of `elem` bytes; fp4: two E2M1 values per byte in global memory
+// inner / outer / box in elements of `elem` bytes; fp4: two E2M1 values per byte in global memory; pitch: bytes from one row
+// to the next, 0 where they follow one another
 int encode_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
-                  uint32_t box_outer, bool fp4 = false, uint32_t elem = 1)
+                  uint32_t box_outer, bool fp4 = false, uint32_t elem = 1, uint64_t pitch = 0)
 {
-    const MapKey k{base, inner, outer, box_inner, box_outer, fp4, elem};
+    const MapKey k{base, inner, outer, box_inner, box_outer, fp4, elem, pitch};
     int victim = 0;
     for (int i = 0; i < kMapCacheSize; ++i) {
         if (g_maps.used[i] != 0 && g_maps.key[i] == k) {
@@ -475,7 +482,7 @@ int encode_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t o
             victim = i;
         }
     }
-    int rc = encode_map_2d_uncached(map, base, inner, outer, box_inner, box_outer, fp4, elem);
+    int rc = encode_map_2d_uncached(map, base, inner, outer, box_inner, box_outer, fp4, elem, pitch);
     if (rc == 0) {
         g_maps.key[victim] = k;
         g_maps.map[victim] = *map;
@@ -485,10 +492,10 @@ int encode_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t o
 }
 
 int encode_map_2d_uncached(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
-                           uint32_t box_outer, bool fp4, uint32_t elem)
+                           uint32_t box_outer, bool fp4, uint32_t elem, uint64_t pitch)
 {
     cuuint64_t dims[2] = {inner, outer};
-    cuuint64_t strides[1] = {fp4 ? inner / 2 : inner * elem};  // bytes; 4-bit elements are packed in pairs
+    cuuint64_t strides[1] = {pitch != 0 ? pitch : (fp4 ? inner / 2 : inner * elem)};  // bytes; 4-bit elements are packed in pairs
     cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
     // packed 4-bit values land in shared memory sixteen to a 16-byte chunk (8 bytes of values, 8 bytes of gap):
@@ -1386,6 +1393,139 @@ int allgather_matmul(void* stream, const void* a, const void* a_scale, bool preq
     return 0;
 }
 
+// ---------------------------------------------------------------------------------------------
+// the steps around the matmuls of a mixture-of-experts layer
+// ---------------------------------------------------------------------------------------------
+bool misaligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1u)) != 0; }
+
+// A launch of clusters (with the attribute of launch_after).
+template <typename... KArgs, typename... Args>
+cudaError_t launch_clusters_after(void (*kern)(KArgs...), dim3 grid, uint32_t cluster, uint32_t threads, size_t smem, cudaStream_t st,
+                                  Args&&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    g_launches++;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+// Kernels with more than 48 KB of shared memory say so once per device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, size_t bytes, bool (&done)[kMaxRanks * 2])
+{
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess || (dev < kMaxRanks * 2 && done[dev])) {
+        return err;
+    }
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (err == cudaSuccess && dev < kMaxRanks * 2) {
+        done[dev] = true;
+    }
+    return err;
+}
+
+template <uint32_t kPasses>
+int launch_norm(cudaStream_t st, const NormQuantParams& p)
+{
+    const uint32_t warps = (p.n + kNormColsPerWarp * kPasses - 1) / (kNormColsPerWarp * kPasses);
+    // rows of one warp share a CTA
+    const uint32_t rows_per_cta = warps == 1u ? std::min(8u, p.rows) : 1u;
+    const uint32_t grid = (p.rows + rows_per_cta - 1) / rows_per_cta;
+    CUDA_TRY(launch_after(g.a_dtype == 1 ? add_rms_norm_mx_quant_kernel<kPasses, true> : add_rms_norm_mx_quant_kernel<kPasses, false>,
+                          dim3(grid), 32u * warps * rows_per_cta, 0, st, p, warps));
+    return 0;
+}
+
+template <typename LogitT>
+int launch_route(cudaStream_t st, const RouteParams& p)
+{
+    const uint32_t per_lane = (p.experts + 31u) / 32u;
+    const dim3 grid((p.tokens + kRouteWarps - 1) / kRouteWarps);
+    const size_t smem = p.top_groups < p.groups ? (size_t)kRouteWarps * p.experts * sizeof(double) : 0;
+#define CATCCOS_ROUTE_CASE(VPL)                                                                          \
+    if (per_lane <= VPL) {                                                                               \
+        CUDA_TRY(launch_after(moe_route_kernel<VPL, LogitT>, grid, 32 * kRouteWarps, smem, st, p));      \
+        return 0;                                                                                        \
+    }
+    CATCCOS_ROUTE_CASE(1)
+    CATCCOS_ROUTE_CASE(2)
+    CATCCOS_ROUTE_CASE(4)
+    CATCCOS_ROUTE_CASE(8)
+    CATCCOS_ROUTE_CASE(16)
+    CATCCOS_ROUTE_CASE(32)
+#undef CATCCOS_ROUTE_CASE
+    return CATCCOS_B200_EINVAL;
+}
+
+template <uint32_t kSets>
+int launch_matvec(cudaStream_t st, const MatvecParams& p, int num_sms)
+{
+    const uint32_t slabs = (p.n + kMatvecCols - 1) / kMatvecCols;
+    const uint32_t blocks = p.ids != nullptr ? p.rows : (p.rows + 4 * kSets - 1) / (4 * kSets);
+    const uint32_t steps = p.k / kMatvecUnit;
+    // K is shared by more CTAs until two fit every SM, as long as each of their warps has a step
+    uint32_t ctas = 1;
+    while (ctas < kMatvecMaxCluster && (uint64_t)slabs * blocks * ctas < 2u * (uint32_t)num_sms && ctas * kMatvecWarps < steps) {
+        ctas *= 2;
+    }
+    CUDA_TRY(launch_clusters_after(g.c_dtype == 1 ? fp4_matvec_kernel<kSets, __half> : fp4_matvec_kernel<kSets, __nv_bfloat16>,
+                                   dim3(slabs * ctas, blocks), ctas, kMatvecThreads, 0, st, p));
+    return 0;
+}
+
+// Width of a grouped launch's column tiles.
+uint32_t grouped_block_n(const RankCtx& rc, uint32_t rows, uint32_t experts, uint32_t n)
+{
+    // narrower tiles until the experts that can have rows fill the SMs
+    const uint64_t tiles = rows / kGemmBlockM + std::min(rows, experts);
+    for (uint32_t bn : {256u, 128u}) {
+        if (tiles * ((n + bn - 1) / bn) >= 2ull * (uint32_t)rc.num_sms) {
+            return bn;
+        }
+    }
+    return 64;
+}
+
+template <uint32_t BLOCK_N, typename OutT>
+int launch_grouped_inst(uint32_t grid, cudaStream_t st, const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb,
+                        const GroupedParams& p)
+{
+    static bool done[kMaxRanks * 2] = {};
+    CUDA_TRY(allow_smem(mx_grouped_gemm_kernel<BLOCK_N, OutT>, GroupedSmem<BLOCK_N>::dynamic_bytes(kGroupedMaxExperts), done));
+    CUDA_TRY(launch_after(mx_grouped_gemm_kernel<BLOCK_N, OutT>, dim3(grid), kGemmThreads, GroupedSmem<BLOCK_N>::dynamic_bytes(p.experts),
+                          st, ta, ta32, tb, p));
+    return 0;
+}
+
+template <uint32_t BLOCK_N>
+int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
+{
+    CUtensorMap ta, ta32, tb;
+    int rcode = encode_map_2d(&ta, a, p.K, p.rows, kGemmBlockK, kGemmBlockM, false, 1, a_row_bytes);
+    if (rcode == 0) rcode = encode_map_2d(&ta32, a, p.K, p.rows, kGemmBlockK, 32, false, 1, a_row_bytes);
+    if (rcode == 0) rcode = encode_map_2d(&tb, b, p.N, (uint64_t)p.experts * p.K, GemmSmem<BLOCK_N>::kBRow, kGemmBlockK);
+    if (rcode != 0) return rcode;
+    // at most one row tile that is not full for every expert that has rows
+    const uint64_t tiles = p.rows / kGemmBlockM + std::min(p.rows, p.experts);
+    const uint64_t units = tiles * ((p.N + BLOCK_N - 1) / BLOCK_N);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(units, (uint64_t)rc.num_sms);
+    return g.c_dtype == 1 ? launch_grouped_inst<BLOCK_N, __half>(grid, st, ta, ta32, tb, p)
+                          : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, ta, ta32, tb, p);
+}
+
 }  // namespace
 
 // =============================================================================================
@@ -2079,6 +2219,252 @@ int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, cons
                           static_cast<const uint16_t*>(in_bf16), expanded_row_idx, static_cast<uint8_t*>(packed_out), tokens, n,
                           top_k, g.tiny_block_rule != 0 ? 1u : 0u));
     return 0;
+}
+
+int catccos_b200_add_rms_norm_mx_quant(void* stream, const void* x_bf16, const void* residual_bf16, const void* weight_bf16,
+                                       float eps, uint32_t rows, uint32_t n, void* residual_out, void* norm_out, void* codes,
+                                       void* scales)
+{
+    if (n == 0 || n % 32 != 0 || n > kNormMaxCols || !(eps > 0.0f) || std::isinf(eps)) {
+        ERROR_LOG("add_rms_norm_mx_quant: n must be a multiple of 32 up to %u, eps positive (got n=%u eps=%g)", kNormMaxCols, n, eps);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (g.a_dtype == 2) {
+        ERROR_LOG("add_rms_norm_mx_quant writes 8-bit codes: a_dtype 0 or 1");
+        return CATCCOS_B200_EINVAL;
+    }
+    if (rows == 0) {
+        return 0;
+    }
+    if (!x_bf16 || !weight_bf16 || !codes || !scales || (residual_bf16 == nullptr) != (residual_out == nullptr)) {
+        return CATCCOS_B200_EINVAL;
+    }
+    if (misaligned(x_bf16, 16) || misaligned(residual_bf16, 16) || misaligned(weight_bf16, 16) || misaligned(residual_out, 16) ||
+        misaligned(norm_out, 16) || misaligned(codes, 16) || (n % 128 == 0 && misaligned(scales, 4))) {
+        return CATCCOS_B200_EINVAL;  // 16 bytes at a time; the GEMMs read the scales of such rows as 32-bit words
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    NormQuantParams p = {};
+    p.x = static_cast<const uint8_t*>(x_bf16);
+    p.residual = static_cast<const uint8_t*>(residual_bf16);
+    p.weight = static_cast<const uint8_t*>(weight_bf16);
+    p.residual_out = static_cast<uint8_t*>(residual_out);
+    p.norm_out = static_cast<uint8_t*>(norm_out);
+    p.codes = static_cast<uint8_t*>(codes);
+    p.scales = static_cast<uint8_t*>(scales);
+    p.rows = rows;
+    p.n = n;
+    p.eps = eps;
+    p.inv_n = 1.0f / (float)n;
+    p.device_tiny = g.tiny_block_rule != 0 ? 1u : 0u;
+    const uint32_t one_pass = kNormColsPerWarp * kNormMaxWarps;
+    return n <= one_pass ? launch_norm<1>((cudaStream_t)stream, p)
+                         : (n <= 2 * one_pass ? launch_norm<2>((cudaStream_t)stream, p) : launch_norm<kNormMaxPasses>((cudaStream_t)stream, p));
+}
+
+int catccos_b200_moe_route(void* stream, const void* logits, int logits_bf16, const float* bias, uint32_t tokens, uint32_t experts,
+                           uint32_t top_k, uint32_t groups, uint32_t top_groups, uint32_t group_best, int score, int renormalize,
+                           float scale, int32_t* ids, float* weights)
+{
+    if (experts == 0 || experts > kRouteMaxExperts || groups == 0 || groups > kRouteMaxGroups || experts % groups != 0 ||
+        top_groups == 0 || top_groups > groups || group_best == 0 || group_best > 2 || top_k == 0 || top_k > kRouteMaxTopK ||
+        top_k > experts / groups * top_groups || score < 0 || score > 1 || logits_bf16 < 0 || logits_bf16 > 1 ||
+        !std::isfinite(scale)) {
+        ERROR_LOG("moe_route: up to %u experts in up to %u equal groups, top_groups of them, group_best 1 or 2, top_k up to %u and "
+                  "not above the experts of top_groups groups (got %u experts, %u groups, %u, %u, top_k %u)",
+                  kRouteMaxExperts, kRouteMaxGroups, kRouteMaxTopK, experts, groups, top_groups, group_best, top_k);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if (!logits || !ids || !weights || misaligned(logits, logits_bf16 ? 2 : 4) || misaligned(bias, 4) || misaligned(ids, 4) ||
+        misaligned(weights, 4) || (uint64_t)tokens * top_k > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    RouteParams p = {};
+    p.logits = logits;
+    p.bias = bias;
+    p.ids = ids;
+    p.weights = weights;
+    p.tokens = tokens;
+    p.experts = experts;
+    p.top_k = top_k;
+    p.groups = groups;
+    p.top_groups = top_groups;
+    p.group_best = group_best;
+    p.sigmoid = score == 1 ? 1u : 0u;
+    p.renormalize = renormalize != 0 ? 1u : 0u;
+    p.scale = scale;
+    p.group_size = experts / groups;
+    p.group_inv = (1u << 22) / p.group_size + 1u;
+    p.group_lanes = 1;
+    while (p.group_lanes * 2 * groups <= 32) {
+        p.group_lanes *= 2;
+    }
+    return logits_bf16 ? launch_route<__nv_bfloat16>((cudaStream_t)stream, p) : launch_route<float>((cudaStream_t)stream, p);
+}
+
+int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes, uint32_t experts, int32_t first_expert,
+                              int32_t* row_index, int32_t* offsets)
+{
+    if (experts == 0 || experts > kPlanMaxExperts || first_expert < 0 || routes > 0x7FFFFFFFu) {
+        ERROR_LOG("moe_row_plan: 1 to %u experts, first_expert not negative (got %u, %d)", kPlanMaxExperts, experts, first_expert);
+        return CATCCOS_B200_EINVAL;
+    }
+    if ((routes != 0 && (!ids || !row_index)) || !offsets || misaligned(ids, 4) || misaligned(row_index, 4) || misaligned(offsets, 4)) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    RowPlanParams p = {};
+    p.ids = ids;
+    p.row_index = row_index;
+    p.offsets = offsets;
+    p.routes = routes;
+    p.experts = experts;
+    p.first = first_expert;
+    const uint32_t ctas = routes > 4096 ? kPlanCluster : 1;
+    const uint32_t per_pass = ctas * kPlanThreads;
+    p.per_warp = std::max(1u, (routes + per_pass - 1) / per_pass) * 32;
+    static bool done[kMaxRanks * 2] = {};
+    CUDA_TRY(allow_smem(moe_row_plan_kernel, row_plan_smem(kPlanMaxExperts), done));
+    CUDA_TRY(launch_clusters_after(moe_row_plan_kernel, dim3(ctas), ctas, kPlanThreads, row_plan_smem(experts), (cudaStream_t)stream, p, ctas));
+    return 0;
+}
+
+int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows, const int32_t* row_index, const float* weights,
+                             const void* shared_out, void* out, uint32_t tokens, uint32_t n, uint32_t top_k, int f16)
+{
+    if (n == 0 || n % 8 != 0 || top_k == 0 || f16 < 0 || f16 > 1) {
+        ERROR_LOG("moe_combine: n must be a multiple of 8 (got %u), top_k at least 1 (got %u)", n, top_k);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if ((rows != 0 && !expert_out) || !row_index || !weights || !out || misaligned(expert_out, 16) || misaligned(shared_out, 16) ||
+        misaligned(out, 16) || misaligned(row_index, 4) || misaligned(weights, 4) || rows > 0x7FFFFFFFu) {
+        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    CombineParams p = {};
+    p.y = static_cast<const uint8_t*>(expert_out);
+    p.row_index = row_index;
+    p.weights = weights;
+    p.shared_out = static_cast<const uint8_t*>(shared_out);
+    p.out = static_cast<uint8_t*>(out);
+    p.tokens = tokens;
+    p.rows = rows;
+    p.n = n;
+    p.top_k = top_k;
+    p.vectors = n / 8;
+    p.slabs = p.vectors >= kCombineThreads ? (p.vectors + kCombineThreads - 1) / kCombineThreads : 0;
+    const uint64_t per_cta = p.slabs ? 1 : kCombineThreads / p.vectors;
+    const uint64_t grid = p.slabs ? (uint64_t)tokens * p.slabs : (tokens + per_cta - 1) / per_cta;
+    if (grid > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    CUDA_TRY(launch_after(f16 ? moe_combine_kernel<__half> : moe_combine_kernel<__nv_bfloat16>, dim3((unsigned)grid), kCombineThreads, 0,
+                          (cudaStream_t)stream, p));
+    return 0;
+}
+
+int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes, const void* a_scale, size_t a_scale_row_bytes,
+                                 const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows, uint32_t experts,
+                                 uint32_t n, uint32_t k)
+{
+    if (n == 0 || n % 16 != 0 || k == 0 || k % kGemmBlockK != 0 || experts == 0 || experts > kGroupedMaxExperts ||
+        (uint64_t)experts * k > 0x7FFFFFFFull || rows > 0x7FFFFFFFu) {
+        ERROR_LOG("mx grouped gemm needs K %% 128 == 0, N %% 16 == 0 and 1 to %u experts (got N=%u K=%u experts=%u)", kGroupedMaxExperts, n,
+                  k, experts);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (g.a_dtype == 2 || g.b_dtype == 2) {
+        ERROR_LOG("mx grouped gemm takes 8-bit operands: a_dtype and b_dtype 0 or 1");
+        return CATCCOS_B200_EINVAL;
+    }
+    if (rows == 0) {
+        return 0;
+    }
+    if (!a || !a_scale || !b || !b_scale || !offsets || !c) {
+        return CATCCOS_B200_EINVAL;
+    }
+    if (a_row_bytes < k || a_row_bytes % 16 != 0 || a_row_bytes >= (1ull << 40) || a_scale_row_bytes < k / 32 ||
+        a_scale_row_bytes % 4 != 0 || misaligned(a, 16) || misaligned(b, 16) || misaligned(c, 32) || misaligned(a_scale, 4) ||
+        misaligned(b_scale, 2) || misaligned(offsets, 4)) {
+        ERROR_LOG("mx grouped gemm: a, b and the rows of a 16-byte aligned, c 32-byte, the rows of a_scale 4-byte, b_scale 2-byte");
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    if (!g.drv.Load()) {
+        return CATCCOS_B200_ECUDA;
+    }
+    RankCtx& rc = cur();
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (dev != rc.device) {
+        return CATCCOS_B200_ESTATE;  // the record of its waits is on the rank's device
+    }
+    GroupedParams p = {};
+    p.a_scales = static_cast<const uint8_t*>(a_scale);
+    p.a_scale_stride = a_scale_row_bytes;
+    p.b_scales = static_cast<const uint8_t*>(b_scale);
+    p.offsets = offsets;
+    p.c = c;
+    p.rows = rows;
+    p.experts = experts;
+    p.N = n;
+    p.K = k;
+    p.a_fmt = g.a_dtype == 1 ? 1u : 0u;
+    p.b_fmt = g.b_dtype == 1 ? 1u : 0u;
+    p.bar_timeout_ns = 2 * g.timeout_ns + 1000000000ull;
+    p.status = rc.status;
+    const uint32_t bn = g.block_n != 0 ? (uint32_t)g.block_n : grouped_block_n(rc, rows, experts, n);
+    cudaStream_t st = (cudaStream_t)stream;
+    return bn == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p)
+                    : (bn == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p) : launch_grouped<256>(rc, st, a, a_row_bytes, b, p));
+}
+
+int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
+                               uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k)
+{
+    if (n == 0 || n % 16 != 0 || k == 0 || k % kMatvecUnit != 0 || experts == 0) {
+        ERROR_LOG("mx_fp4_matvec needs K %% 64 == 0, N %% 16 == 0 and a weight (got N=%u K=%u experts=%u)", n, k, experts);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (rows == 0) {
+        return 0;
+    }
+    if (x_rows == 0 || rows % x_rows != 0 || (ids == nullptr && (rows != x_rows || experts != 1)) || rows > 65535u) {
+        ERROR_LOG("mx_fp4_matvec: up to 65535 rows; with ids a multiple of the rows of x, without as many and one weight (got %u, %u, "
+                  "experts=%u)", rows, x_rows, experts);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (!x_bf16 || !w || !w_scale || !out || misaligned(x_bf16, 16) || misaligned(w, 16) || misaligned(w_scale, 16) ||
+        misaligned(ids, 4) || misaligned(out, 4)) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    MatvecParams p = {};
+    p.x = static_cast<const uint8_t*>(x_bf16);
+    p.w = static_cast<const uint8_t*>(w);
+    p.scales = static_cast<const uint8_t*>(w_scale);
+    p.ids = ids;
+    p.out = static_cast<uint8_t*>(out);
+    p.rows = rows;
+    p.n = n;
+    p.k = k;
+    p.experts = experts;
+    p.rows_per_x = rows / x_rows;
+    return ids != nullptr || rows <= 4 ? launch_matvec<1>((cudaStream_t)stream, p, cur().num_sms)
+                                       : launch_matvec<2>((cudaStream_t)stream, p, cur().num_sms);
 }
 
 int catccos_b200_last_status(uint32_t out[4])

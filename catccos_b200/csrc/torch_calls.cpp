@@ -12,9 +12,11 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/catccos_b200.h"
 
@@ -27,6 +29,12 @@ BOUND(mx_gemm);
 BOUND(mx_gemm_quant_out);
 BOUND(mx_quant_scatter_packed);
 BOUND(mxfp8_matmul_reduce_scatter);
+BOUND(add_rms_norm_mx_quant);
+BOUND(moe_route);
+BOUND(moe_row_plan);
+BOUND(mx_grouped_gemm);
+BOUND(moe_combine);
+BOUND(mx_fp4_matvec);
 BOUND(mx_quant_matmul_static);
 BOUND(mx_quant_allgather);
 BOUND(mx_quant_allgather_matmul);
@@ -193,6 +201,67 @@ void assert_activations(const at::Tensor& x)
     }
 }
 
+// ---- calls that check what they are given: element types, shapes, one device (which becomes the current one) -----------------
+[[noreturn]] void refuse(const char* what, const char* wanted)
+{
+    PyErr_Format(PyExc_ValueError, "%s: expected %s", what, wanted);
+    throw Error{};
+}
+
+float real(PyObject* number)
+{
+    const double v = PyFloat_AsDouble(number);
+    if (v == -1.0 && PyErr_Occurred()) {
+        throw Error{};
+    }
+    return (float)v;
+}
+
+int64_t whole(PyObject* number, const char* what)
+{
+    const long long v = PyLong_AsLongLong(number);
+    if (v == -1 && PyErr_Occurred()) {
+        throw Error{};
+    }
+    if (v < 0 || v > 0x7FFFFFFFll) {
+        refuse(what, "a number from 0 to 2^31 - 1");
+    }
+    return v;
+}
+
+// A CUDA tensor on `like`'s device (any, without one), of one of the types, contiguous.
+const at::Tensor& plain(PyObject* o, const char* what, const char* wanted, std::initializer_list<at::ScalarType> types, int dims,
+                        const at::Tensor* like = nullptr, bool contiguous = true)
+{
+    const at::Tensor& t = tensor(o);
+    bool ok = t.is_cuda() && (dims < 0 || t.dim() == dims) && (!contiguous || t.is_contiguous()) &&
+              (like == nullptr || t.device() == like->device());
+    bool type = false;
+    for (at::ScalarType s : types) {
+        type = type || t.scalar_type() == s;
+    }
+    if (!ok || !type) {
+        refuse(what, wanted);
+    }
+    for (int64_t s : t.sizes()) {
+        if (s > 0x7FFFFFFFll) {
+            refuse(what, "sizes below 2^31");
+        }
+    }
+    return t;
+}
+
+void* data_or_null(PyObject* o) { return o == Py_None ? nullptr : tensor(o).data_ptr(); }
+
+// The tensors' device for the rest of a call, and its current stream.
+struct OnDevice {
+    c10::cuda::CUDAGuard guard;
+    void* stream;
+    explicit OnDevice(const at::Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+constexpr auto kBf16 = at::kBFloat16, kF16 = at::kHalf, kF32 = at::kFloat, kI32 = at::kInt, kU8 = at::kByte;
+
 #define CALL(name, nargs) \
     PyObject* name(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(#name, nargs, n, name##_fn != nullptr, [&]() -> PyObject* {
 #define END_CALL }); }
@@ -290,6 +359,150 @@ CALL(fp4_mx_allgather_matmul, 7)
     return released([&] { return fp4_mx_allgather_matmul_fn(st, ac, b, as, bs, c, symm, &t, 0); });
 END_CALL
 
+// x, residual, weight, eps, residual_out, norm_out
+CALL(add_rms_norm_mx_quant, 6)
+    const char* same = "a contiguous bf16 CUDA matrix of x's shape on x's device";
+    const at::Tensor& x = plain(a[0], "x", "a contiguous bf16 CUDA matrix", {kBf16}, 2);
+    const int64_t rows = x.size(0), n = x.size(1);
+    PyObject* residual_out = a[4] == Py_None ? a[1] : a[4];
+    if (a[1] == Py_None && a[4] != Py_None) {
+        refuse("residual_out", "None where residual is None");
+    }
+    PyObject* others[3] = {a[1], residual_out, a[5]};
+    const char* names[3] = {"residual", "residual_out", "norm_out"};
+    for (int i = 0; i < 3; ++i) {
+        if (others[i] != Py_None && plain(others[i], names[i], same, {kBf16}, 2, &x).sizes() != x.sizes()) {
+            refuse(names[i], same);
+        }
+    }
+    if (plain(a[2], "weight", "a contiguous bf16 CUDA vector on x's device", {kBf16}, 1, &x).size(0) != n) {
+        refuse("weight", "one value for each column of x");
+    }
+    const float eps = real(a[3]);
+    const OnDevice on(x);
+    const at::Tensor codes = bytes_like(x, rows, n), scales = bytes_like(x, rows, n / 32);
+    void *in = x.data_ptr(), *r = data_or_null(a[1]), *w = pointer(a[2]), *ro = data_or_null(residual_out), *no = data_or_null(a[5]);
+    void *c = codes.data_ptr(), *s = scales.data_ptr();
+    return with_outputs(released([&] { return add_rms_norm_mx_quant_fn(on.stream, in, r, w, eps, (uint32_t)rows, (uint32_t)n, ro, no, c, s); }),
+                        codes, scales);
+END_CALL
+
+// logits, bias, top_k, groups, top_groups, group_best, score, renormalize, scale
+CALL(moe_route, 9)
+    const at::Tensor& l = plain(a[0], "logits", "a contiguous fp32 or bf16 CUDA matrix", {kF32, kBf16}, 2);
+    const int64_t tokens = l.size(0), experts = l.size(1);
+    if (a[1] != Py_None &&
+        plain(a[1], "bias", "a contiguous fp32 CUDA vector on the logits' device", {kF32}, 1, &l).size(0) != experts) {
+        refuse("bias", "one value for each expert");
+    }
+    const int64_t top_k = whole(a[2], "top_k"), groups = whole(a[3], "groups"), top_groups = whole(a[4], "top_groups"),
+                  group_best = whole(a[5], "group_best"), score = whole(a[6], "score"), renormalize = whole(a[7], "renormalize");
+    const float scale = real(a[8]);
+    const OnDevice on(l);
+    // a top_k that the library refuses is not allocated for
+    const int64_t k = top_k <= experts ? top_k : 0;
+    const at::Tensor ids = at::detail::empty_cuda({tokens, k}, kI32, l.device(), std::nullopt);
+    const at::Tensor weights = at::detail::empty_cuda({tokens, k}, kF32, l.device(), std::nullopt);
+    void *in = l.data_ptr(), *b = data_or_null(a[1]), *i = ids.data_ptr(), *w = weights.data_ptr();
+    return with_outputs(released([&] {
+                            return moe_route_fn(on.stream, in, l.scalar_type() == kBf16 ? 1 : 0, (const float*)b, (uint32_t)tokens,
+                                                (uint32_t)experts, (uint32_t)top_k, (uint32_t)groups, (uint32_t)top_groups,
+                                                (uint32_t)group_best, (int)score, (int)renormalize, scale, (int32_t*)i, (float*)w);
+                        }),
+                        ids, weights);
+END_CALL
+
+// ids, experts, first_expert
+CALL(moe_row_plan, 3)
+    const at::Tensor& ids = plain(a[0], "ids", "a contiguous int32 CUDA tensor", {kI32}, -1);
+    const int64_t experts = whole(a[1], "experts"), first = whole(a[2], "first_expert");
+    if (ids.numel() > 0x7FFFFFFFll) {
+        refuse("ids", "fewer than 2^31 routes");
+    }
+    const OnDevice on(ids);
+    const at::Tensor index = at::detail::empty_cuda(ids.sizes(), kI32, ids.device(), std::nullopt);
+    // as many experts as the library takes are allocated for
+    const at::Tensor offsets = at::detail::empty_cuda({experts <= 1024 ? experts + 1 : 1}, kI32, ids.device(), std::nullopt);
+    void *in = ids.data_ptr(), *i = index.data_ptr(), *o = offsets.data_ptr();
+    const uint32_t routes = (uint32_t)ids.numel();
+    return with_outputs(released([&] { return moe_row_plan_fn(on.stream, (const int32_t*)in, routes, (uint32_t)experts, (int32_t)first, (int32_t*)i, (int32_t*)o); }),
+                        index, offsets);
+END_CALL
+
+// a, a_scales, b, b_scales, offsets, out
+CALL(mx_grouped_gemm, 6)
+    const auto codes = {kU8, at::kFloat8_e4m3fn, at::kFloat8_e5m2};
+    const at::Tensor& x = plain(a[0], "a_codes", "a CUDA matrix of 8-bit codes, its columns next to one another", codes, 2, nullptr, false);
+    const at::Tensor& xs = plain(a[1], "a_scales", "a CUDA matrix of bytes on a_codes' device, its columns next to one another",
+                                 {kU8, at::kFloat8_e8m0fnu}, 2, &x, false);
+    const at::Tensor& b = plain(a[2], "b", "contiguous 8-bit codes [experts, K, N] on a_codes' device", codes, 3, &x);
+    const at::Tensor& bs = plain(a[3], "b_scales", "contiguous bytes [experts, K / 64, N, 2] on a_codes' device", {kU8, at::kFloat8_e8m0fnu}, 4, &x);
+    const at::Tensor& offsets = plain(a[4], "offsets", "a contiguous int32 vector on a_codes' device", {kI32}, 1, &x);
+    const at::Tensor& out = plain(a[5], "out", "a contiguous bf16 or fp16 matrix on a_codes' device", {kBf16, kF16}, 2, &x);
+    const int64_t rows = x.size(0), k = x.size(1), experts = b.size(0), n = b.size(2);
+    if ((k > 1 && x.stride(1) != 1) || (k >= 64 && xs.stride(1) != 1) || x.stride(0) < 0 || xs.stride(0) < 0) {
+        refuse("a_codes, a_scales", "columns next to one another");
+    }
+    if (xs.size(0) != rows || xs.size(1) != k / 32 || b.size(1) != k || bs.size(0) != experts || bs.size(1) != k / 64 || bs.size(2) != n ||
+        bs.size(3) != 2 || offsets.size(0) != experts + 1 || out.size(0) != rows || out.size(1) != n) {
+        refuse("mx_grouped_gemm", "a [rows, K], a_scales [rows, K / 32], b [experts, K, N], b_scales [experts, K / 64, N, 2], "
+                                  "offsets [experts + 1], out [rows, N]");
+    }
+    const OnDevice on(x);
+    // one row has no distance to the next
+    const size_t step = rows > 1 ? (size_t)x.stride(0) : (size_t)(k + 15) / 16 * 16, scale_step = rows > 1 ? (size_t)xs.stride(0) : (size_t)(k / 32 + 3) / 4 * 4;
+    void *ac = x.data_ptr(), *as = xs.data_ptr(), *bc = b.data_ptr(), *bf = bs.data_ptr(), *o = offsets.data_ptr(), *c = out.data_ptr();
+    return released([&] {
+        return mx_grouped_gemm_fn(on.stream, ac, step, as, scale_step, bc, bf, (const int32_t*)o, c, (uint32_t)rows, (uint32_t)experts,
+                                  (uint32_t)n, (uint32_t)k);
+    });
+END_CALL
+
+// expert_out, row_index, weights, shared, out
+CALL(moe_combine, 5)
+    const at::Tensor& y = plain(a[0], "expert_out", "a contiguous bf16 or fp16 CUDA matrix", {kBf16, kF16}, 2);
+    const at::ScalarType type = y.scalar_type();
+    const at::Tensor& index = plain(a[1], "row_index", "a contiguous int32 matrix on expert_out's device", {kI32}, 2, &y);
+    const at::Tensor& w = plain(a[2], "weights", "a contiguous fp32 matrix on expert_out's device", {kF32}, 2, &y);
+    const at::Tensor& out = plain(a[4], "out", "a contiguous matrix of expert_out's type and device", {type}, 2, &y);
+    const int64_t tokens = index.size(0), n = y.size(1);
+    if (w.sizes() != index.sizes() || out.size(0) != tokens || out.size(1) != n) {
+        refuse("moe_combine", "row_index and weights [tokens, top_k], out [tokens, n]");
+    }
+    if (a[3] != Py_None && plain(a[3], "shared", "a contiguous matrix of expert_out's type and device", {type}, 2, &y).sizes() != out.sizes()) {
+        refuse("shared", "out's shape");
+    }
+    const OnDevice on(y);
+    void *in = y.data_ptr(), *i = index.data_ptr(), *g = w.data_ptr(), *s = data_or_null(a[3]), *o = out.data_ptr();
+    const uint32_t top_k = (uint32_t)index.size(1), rows = (uint32_t)y.size(0);
+    return released([&] {
+        return moe_combine_fn(on.stream, in, rows, (const int32_t*)i, (const float*)g, s, o, (uint32_t)tokens, (uint32_t)n, top_k,
+                              type == kF16 ? 1 : 0);
+    });
+END_CALL
+
+// x, w, w_scales, ids, out
+CALL(mx_fp4_matvec, 5)
+    const bool many = a[3] != Py_None;
+    const at::Tensor& x = plain(a[0], "x", "a contiguous bf16 CUDA matrix", {kBf16}, 2);
+    const at::Tensor& w = plain(a[1], "w", "contiguous packed codes [K, N / 2], with ids [experts, K, N / 2], on x's device", {kU8}, many ? 3 : 2, &x);
+    const at::Tensor& ws = plain(a[2], "w_scales", "contiguous bytes [K / 64, N, 2], with ids [experts, K / 64, N, 2], on x's device",
+                                 {kU8, at::kFloat8_e8m0fnu}, many ? 4 : 3, &x);
+    const at::Tensor& out = plain(a[4], "out", "a contiguous bf16 or fp16 matrix on x's device", {kBf16, kF16}, 2, &x);
+    const int64_t x_rows = x.size(0), k = x.size(1), experts = many ? w.size(0) : 1, n = 2 * w.size(-1);
+    const int64_t rows = many ? plain(a[3], "ids", "a contiguous int32 tensor on x's device", {kI32}, -1, &x).numel() : x_rows;
+    if (w.size(-2) != k || ws.size(-3) != k / 64 || ws.size(-2) != n || ws.size(-1) != 2 || (many && ws.size(0) != experts) ||
+        out.size(0) != rows || out.size(1) != n || rows > 0x7FFFFFFFll) {
+        refuse("mx_fp4_matvec", "x [rows, K], w [.., K, N / 2], w_scales [.., K / 64, N, 2], out [rows or ids, N]");
+    }
+    const OnDevice on(x);
+    void *in = x.data_ptr(), *wp = w.data_ptr(), *sp = ws.data_ptr(), *i = data_or_null(a[3]), *o = out.data_ptr();
+    return released([&] {
+        return mx_fp4_matvec_fn(on.stream, in, wp, sp, (const int32_t*)i, o, (uint32_t)rows, (uint32_t)x_rows, (uint32_t)experts,
+                                (uint32_t)n, (uint32_t)k);
+    });
+END_CALL
+
 // bind(name, address): which function of the loaded library a call goes to
 PyObject* bind(PyObject*, PyObject* args)
 {
@@ -309,6 +522,12 @@ PyObject* bind(PyObject*, PyObject* args)
     BIND(mx_gemm_quant_out)
     BIND(mx_quant_scatter_packed)
     BIND(mxfp8_matmul_reduce_scatter)
+    BIND(add_rms_norm_mx_quant)
+    BIND(moe_route)
+    BIND(moe_row_plan)
+    BIND(mx_grouped_gemm)
+    BIND(moe_combine)
+    BIND(mx_fp4_matvec)
     BIND(mx_quant_matmul_static)
     BIND(mx_quant_allgather)
     BIND(mx_quant_allgather_matmul)
@@ -326,6 +545,12 @@ PyMethodDef methods[] = {
     METHOD(mx_gemm_quant_out),
     METHOD(mx_quant_scatter_packed),
     METHOD(mxfp8_matmul_reduce_scatter),
+    METHOD(add_rms_norm_mx_quant),
+    METHOD(moe_route),
+    METHOD(moe_row_plan),
+    METHOD(mx_grouped_gemm),
+    METHOD(moe_combine),
+    METHOD(mx_fp4_matvec),
     METHOD(mx_quant_matmul_static),
     METHOD(mx_quant_allgather),
     METHOD(mx_quant_allgather_matmul),

@@ -151,6 +151,78 @@ size_t catccos_b200_packed_row_bytes(uint32_t n);
 int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, const int32_t* expanded_row_idx, void* packed_out,
                                          uint32_t tokens, uint32_t n, uint32_t top_k);
 
+/* ---- the steps around the matmuls of a mixture-of-experts layer (one GPU; no counterpart in the reference, which takes
+ * expanded_row_idx and the activations from its caller) ------------------------------------------------------------------
+ * None of these calls allocates, keeps anything from one call to the next or shares a scratch with another: calls on
+ * different streams may overlap, and calls may be captured in CUDA graphs and replayed.  They run on the current device;
+ * `stream` is one of its streams.  Inputs and outputs must not overlap except where a comment says so.  An empty batch
+ * (no rows, tokens or routes) is CATCCOS_B200_OK. */
+
+/* Residual addition, root-mean-square norm and MX quantiser: the activations that catccos_b200_mx_gemm and the
+ * AllGather-Matmuls read, in one pass.  With h = bf16(x + residual) (or x, without a residual):
+ *   residual_out = h;  y = h / sqrt(mean(h^2) + eps) * weight;  norm_out = bf16(y);  codes, scales = MX(y)
+ * x, residual, residual_out, norm_out bf16 [rows, n]; weight bf16 [n]; codes uint8 [rows, n]; scales uint8 [rows, n/32].
+ * y stays in fp32 up to the codes (catccos_b200_mx_quant of norm_out would round twice); element type and small blocks
+ * follow the options "a_dtype" (0 or 1) and "tiny_block_rule", blocks with an infinity or NaN get 0xFF / 0x7F.
+ * residual and residual_out are both NULL or both given, norm_out may be NULL.  residual_out may be residual or x, norm_out
+ * may be x or (with another residual_out) residual.  n % 32 == 0, n <= 32768; eps > 0; everything 16-byte aligned, scales
+ * 4-byte where n % 128 == 0. */
+int catccos_b200_add_rms_norm_mx_quant(void* stream, const void* x_bf16, const void* residual_bf16, const void* weight_bf16,
+                                       float eps, uint32_t rows, uint32_t n, void* residual_out, void* norm_out, void* codes,
+                                       void* scales);
+
+/* Router scores to experts.  logits fp32 (logits_bf16 0) or bf16 (1) [tokens, experts], bias fp32 [experts] or NULL:
+ *   s = softmax(logits) (score 0) or sigmoid(logits) (score 1);   choice c = s + bias
+ *   a group's score = the sum of the group_best (1 or 2) highest c of its experts / groups consecutive experts
+ *   ids int32 [tokens, top_k] = the top_k experts by c within the top_groups best groups, best first
+ *   weights fp32 [tokens, top_k] = scale * s[id], with renormalize divided by the sum over the token's ids
+ * Choices are compared as 64-bit floats (scores without a bias as the logits order them); ties go to the lower index.  An
+ * expert whose logit or bias is minus infinity or NaN is not chosen (its logit adds nothing to the softmax), a group without
+ * any other counts for nothing, and places that cannot be filled get id -1 and weight 0.  experts <= 1024, groups <= 32 and a
+ * divisor of experts, top_k <= 32 and <= the experts of top_groups groups; scale finite. */
+int catccos_b200_moe_route(void* stream, const void* logits, int logits_bf16, const float* bias, uint32_t tokens, uint32_t experts,
+                           uint32_t top_k, uint32_t groups, uint32_t top_groups, uint32_t group_best, int score, int renormalize,
+                           float scale, int32_t* ids, float* weights);
+
+/* The rows of the dispatch: routes (ids int32 [routes], token-major) sorted by expert, routes of one expert in their order.
+ *   row_index int32 [routes] = a route's row, -1 where its id is outside [first_expert, first_expert + experts): the
+ *                              expanded_row_idx of catccos_b200_mx_quant_scatter_packed
+ *   offsets int32 [experts + 1]: rows [offsets[e], offsets[e + 1]) belong to expert first_expert + e
+ * 1 <= experts <= 1024, first_expert >= 0. */
+int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes, uint32_t experts, int32_t first_expert,
+                              int32_t* row_index, int32_t* offsets);
+
+/* The experts' products, catccos_b200_mx_gemm for every expert on its own rows:
+ *   c[offsets[e] .. offsets[e + 1])[n] = dequant(a) x dequant(b[e]),   e < experts
+ * a 8-bit codes [rows, k], rows a_row_bytes apart; a_scale E8M0 [rows, k/32], rows a_scale_row_bytes apart: packed rows of
+ * catccos_b200_mx_quant_scatter_packed are given in place, as a = packed, a_scale = packed + k, both strides
+ * catccos_b200_packed_row_bytes(k).  b [experts, k, n]; b_scale [experts, k/64, n, 2]; offsets int32 [experts + 1] in device
+ * memory, ascending, at most rows (offsets that are not give unspecified rows of c, never an access outside); c [rows, n], of
+ * which rows outside the offsets stay as they are.  Options "a_dtype" (0, 1), "b_dtype" (0, 1), "c_dtype".  k % 128 == 0,
+ * n % 16 == 0, experts <= 1024, experts * k < 2^31; a, b and a's rows 16-byte aligned, c 32-byte, a_scale's rows 4-byte,
+ * b_scale 2-byte.  On the acting rank's device. */
+int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes, const void* a_scale, size_t a_scale_row_bytes,
+                                 const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows, uint32_t experts,
+                                 uint32_t n, uint32_t k);
+
+/* The end of the layer: out[t] = sum over r of weights[t, r] * expert_out[row_index[t, r]] (+ shared_out[t]), r ascending, in
+ * fp32, rounded once.  expert_out [rows, n], shared_out (or NULL) and out [tokens, n]: bf16 (f16 0) or fp16 (f16 1); row_index
+ * int32 and weights fp32 [tokens, top_k].  A route whose row is negative or not below rows adds nothing.  out may be
+ * shared_out.  n % 8 == 0; rows 16-byte aligned. */
+int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows, const int32_t* row_index, const float* weights,
+                             const void* shared_out, void* out, uint32_t tokens, uint32_t n, uint32_t top_k, int f16);
+
+/* Products of one or a few tokens with FP4 weights, in the layout that catccos_b200_fp4_mx_allgather_matmul takes and without
+ * its re-laid copy: x bf16 (not quantised), w packed E2M1 [k, n/2], w_scale E8M0 [k/64, n, 2], out [rows, n] (option "c_dtype").
+ *   ids NULL: out = x x dequant(w); x_rows == rows, experts == 1
+ *   ids int32 [rows]: out[r] = x[r / (rows / x_rows)] x dequant(w[ids[r]]) with w [experts, k, n/2] and w_scale
+ *     [experts, k/64, n, 2]: rows == tokens * top_k with one row of x a token, or one a route.  A row whose id is negative or
+ *     not below experts is zero.
+ * The weight is read once for every eight rows (with ids, for every row): meant for decoding, where that is all the work.
+ * k % 64 == 0, n % 16 == 0, rows <= 65535; x, w and w_scale 16-byte aligned, out 4-byte. */
+int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
+                               uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k);
+
 /* Quantise + matmul on one GPU that allocates nothing.  It has no counterpart in the reference.
  * c [m, n] = dequant(quantise(a_bf16 [m, k])) x dequant(b [k, n], b_scale [k/64, n, 2]): the same two
  * stages as catccos_b200_mx_quant_allgather_matmul at rankSize 1, but the quantised copy of A
