@@ -1450,9 +1450,23 @@ int launch_norm(cudaStream_t st, const NormQuantParams& p)
 }
 
 template <typename LogitT>
-int launch_route(cudaStream_t st, const RouteParams& p)
+int launch_route(cudaStream_t st, RouteParams p)
 {
-    const uint32_t per_lane = (p.experts + 31u) / 32u;
+    uint32_t per_lane = 1;  // consecutive experts of a lane
+    while (per_lane * 32u < p.experts) {
+        per_lane *= 2;
+    }
+    const uint32_t load = std::min(16u, per_lane * (uint32_t)sizeof(LogitT));
+    p.vector = p.experts % per_lane == 0 && p.experts * sizeof(LogitT) % load == 0 && !misaligned(p.logits, load) ? 1u : 0u;
+    p.group_in_lanes = p.group_size % per_lane == 0 && ((p.group_size / per_lane) & (p.group_size / per_lane - 1u)) == 0 ? 1u : 0u;
+    p.group_lanes = p.group_in_lanes ? p.group_size / per_lane : 1;
+    while (!p.group_in_lanes && p.group_lanes * 2 * p.groups <= 32) {
+        p.group_lanes *= 2;
+    }
+    while ((1u << p.group_shift) < p.group_lanes) {
+        ++p.group_shift;
+    }
+    p.bias_vector = p.bias != nullptr && p.experts % per_lane == 0 && !misaligned(p.bias, std::min(16u, per_lane * 4u)) ? 1u : 0u;
     const dim3 grid((p.tokens + kRouteWarps - 1) / kRouteWarps);
     const size_t smem = p.top_groups < p.groups ? (size_t)kRouteWarps * p.experts * sizeof(double) : 0;
 #define CATCCOS_ROUTE_CASE(VPL)                                                                          \
@@ -1469,6 +1483,59 @@ int launch_route(cudaStream_t st, const RouteParams& p)
 #undef CATCCOS_ROUTE_CASE
     return CATCCOS_B200_EINVAL;
 }
+
+// CTAs of a plan, microseconds with 1 / 4 / 8 / 16 of them: 2048 routes over 64 experts 3.4 / 4.0 / 4.1 / 4.5 (a cluster costs
+// its launch and two meetings), 4096 4.4 / 4.0 / 4.1 / 4.5, 8192 6.1 / 4.5 / 4.2 / 4.6, 32768 20 / 7.2 / 5.7 / 5.1, 131072 over
+// 256 experts 83 / 24 / 14 / 8.9.
+uint32_t plan_ctas(uint32_t routes, uint32_t limit)
+{
+    return routes <= 2048 ? 1 : (routes <= 4096 ? 4 : (routes <= 16384 ? 8 : limit));
+}
+
+template <uint32_t kBits>
+int launch_row_plan(cudaStream_t st, RowPlanParams p)
+{
+    auto kern = moe_row_plan_kernel<kBits>;
+    // clusters of sixteen are more than every device promises: asked once for each
+    static uint32_t most[kMaxRanks * 2] = {};
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    uint32_t limit = dev < kMaxRanks * 2 ? most[dev] : 0;
+    if (limit == 0) {
+        const size_t smem = row_plan_smem(kPlanMaxExperts);
+        CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        limit = 8;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(kPlanMaxCluster);
+            cfg.blockDim = dim3(kPlanThreads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = kPlanMaxCluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            limit = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters >= 1 ? kPlanMaxCluster : 8;
+        }
+        cudaGetLastError();
+        if (dev < kMaxRanks * 2) {
+            most[dev] = limit;
+        }
+    }
+    const uint32_t ctas = plan_ctas(p.routes, limit);
+    const uint64_t threads = (uint64_t)ctas * kPlanThreads;
+    p.per_warp = (uint32_t)std::max<uint64_t>(1, (p.routes + threads - 1) / threads) * 32;
+    CUDA_TRY(launch_clusters_after(kern, dim3(ctas), ctas, kPlanThreads, row_plan_smem(p.experts), st, p, ctas));
+    return 0;
+}
+
+// The wide form of the combination (whole sectors a load, four rows on their way) against the narrow one (eight rows), in
+// microseconds: 512 x 7168 columns of 8 rows 7.9 against 12.4, 64 x 7168 3.0 against 3.8, 16 x 7168 2.6 either way; 16 x 2048 of
+// 4 rows 1.8 against 2.2; but where 5 to 8 rows are two round trips of the wide form and nothing else counts, 16 x 512 2.3
+// against 2.0.
+bool combine_wide(uint32_t tokens, uint32_t n, uint32_t top_k) { return top_k <= 4 || (uint64_t)tokens * n >= 1u << 18; }
 
 template <uint32_t kSets>
 int launch_matvec(cudaStream_t st, const MatvecParams& p, int num_sms)
@@ -2301,10 +2368,6 @@ int catccos_b200_moe_route(void* stream, const void* logits, int logits_bf16, co
     p.scale = scale;
     p.group_size = experts / groups;
     p.group_inv = (1u << 22) / p.group_size + 1u;
-    p.group_lanes = 1;
-    while (p.group_lanes * 2 * groups <= 32) {
-        p.group_lanes *= 2;
-    }
     return logits_bf16 ? launch_route<__nv_bfloat16>((cudaStream_t)stream, p) : launch_route<float>((cudaStream_t)stream, p);
 }
 
@@ -2327,13 +2390,8 @@ int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes,
     p.routes = routes;
     p.experts = experts;
     p.first = first_expert;
-    const uint32_t ctas = routes > 4096 ? kPlanCluster : 1;
-    const uint32_t per_pass = ctas * kPlanThreads;
-    p.per_warp = std::max(1u, (routes + per_pass - 1) / per_pass) * 32;
-    static bool done[kMaxRanks * 2] = {};
-    CUDA_TRY(allow_smem(moe_row_plan_kernel, row_plan_smem(kPlanMaxExperts), done));
-    CUDA_TRY(launch_clusters_after(moe_row_plan_kernel, dim3(ctas), ctas, kPlanThreads, row_plan_smem(experts), (cudaStream_t)stream, p, ctas));
-    return 0;
+    return experts <= 64 ? launch_row_plan<6>((cudaStream_t)stream, p)
+                         : (experts <= 256 ? launch_row_plan<8>((cudaStream_t)stream, p) : launch_row_plan<10>((cudaStream_t)stream, p));
 }
 
 int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows, const int32_t* row_index, const float* weights,
@@ -2360,7 +2418,9 @@ int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows
     p.rows = rows;
     p.n = n;
     p.top_k = top_k;
-    p.vectors = n / 8;
+    const bool wide = n % 16 == 0 && !misaligned(expert_out, 32) && !misaligned(shared_out, 32) && !misaligned(out, 32) &&
+                      combine_wide(tokens, n, top_k);
+    p.vectors = wide ? n / 16 : n / 8;
     p.slabs = p.vectors >= kCombineThreads ? (p.vectors + kCombineThreads - 1) / kCombineThreads : 0;
     const uint64_t per_cta = p.slabs ? 1 : kCombineThreads / p.vectors;
     const uint64_t grid = p.slabs ? (uint64_t)tokens * p.slabs : (tokens + per_cta - 1) / per_cta;
@@ -2369,8 +2429,9 @@ int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows
     }
     int rcode = ensure_init();
     if (rcode != 0) return rcode;
-    CUDA_TRY(launch_after(f16 ? moe_combine_kernel<__half> : moe_combine_kernel<__nv_bfloat16>, dim3((unsigned)grid), kCombineThreads, 0,
-                          (cudaStream_t)stream, p));
+    CUDA_TRY(launch_after(f16 ? (wide ? moe_combine_kernel<__half, true> : moe_combine_kernel<__half, false>)
+                              : (wide ? moe_combine_kernel<__nv_bfloat16, true> : moe_combine_kernel<__nv_bfloat16, false>),
+                          dim3((unsigned)grid), kCombineThreads, 0, (cudaStream_t)stream, p));
     return 0;
 }
 

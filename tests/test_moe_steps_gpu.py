@@ -80,6 +80,8 @@ ROUTERS = [
     (4, 512, 32, "softmax", False, 1, 1, 1, True),
     (3, 1024, 32, "sigmoid", True, 2, 1, 2, False),
     (11, 40, 5, "sigmoid", False, 1, 1, 1, True),
+    (21, 97, 5, "softmax", True, 1, 1, 1, True),  # no whole lanes
+    (6, 32, 32, "sigmoid", True, 1, 1, 1, True),
 ]
 
 
@@ -91,6 +93,14 @@ def test_routes(capi, cuda, tokens, experts, top_k, score, with_bias, groups, to
     logits = (torch.randn((tokens, experts), generator=gen, device="cuda") * 2).to(getattr(torch, dtype))
     bias = torch.randn(experts, generator=gen, device="cuda") * 0.1 if with_bias else None
     _check_route(capi, torch, logits, bias, top_k, score, groups, top_groups, group_best, renormalize, 2.5)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_logits_at_odd_addresses(capi, cuda, dtype):
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    base = torch.randn(9 * 128 + 1, generator=gen, device="cuda").to(getattr(torch, dtype))
+    _check_route(capi, torch, base[1:].view(9, 128), torch.randn(129, generator=gen, device="cuda")[1:], 8, "sigmoid", 4, 2, 2)
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
