@@ -1537,20 +1537,47 @@ int launch_row_plan(cudaStream_t st, RowPlanParams p)
 // against 2.0.
 bool combine_wide(uint32_t tokens, uint32_t n, uint32_t top_k) { return top_k <= 4 || (uint64_t)tokens * n >= 1u << 18; }
 
+// CTAs that share K: the fewest of those that take least, in microseconds.  A warp's step takes 0.82 with one CTA to an SM, 1.3
+// with two; the weights' bytes come at 5.5 TB/s at most; a cluster costs 1.  (Measured with one token: 32 blocks x 112 steps 8
+// CTAs 7.5, 4 8.1, 2 10.3, 1 16; 56 x 36 2 5.9, 4 6.4, 1 6.6; 8 x 16 1 4.0, 2 4.4; 56 x 128 4 10.8, 2 11.5, 8 13.4.)
+uint32_t matvec_ctas(uint64_t blocks, uint32_t steps, double megabytes, int num_sms)
+{
+    uint32_t best = 1;
+    double least = 0;
+    for (uint32_t ctas = 1; ctas <= kMatvecMaxCluster; ctas *= 2) {
+        const uint64_t grid = blocks * ctas, per_warp = (steps + ctas * kMatvecWarps - 1) / (ctas * kMatvecWarps);
+        const uint64_t waves = (grid + 2 * (uint64_t)num_sms - 1) / (2 * (uint64_t)num_sms);
+        const double work = (double)(waves * per_warp) * (grid <= (uint64_t)num_sms ? 0.82 : 1.3);
+        const double time = std::max(work, megabytes / 5.5) + (ctas > 1 ? 1.0 : 0.0);
+        if (ctas == 1 || time < least) {
+            best = ctas;
+            least = time;
+        }
+    }
+    return best;
+}
+
+template <uint32_t kSets, bool kWhole, typename OutT>
+int launch_matvec_inst(cudaStream_t st, const MatvecParams& p, uint32_t slabs, uint32_t blocks, uint32_t ctas)
+{
+    static bool done[kMaxRanks * 2] = {};
+    CUDA_TRY(allow_smem(fp4_matvec_kernel<kSets, kWhole, OutT>, kMatvecSmem<kSets>, done));
+    CUDA_TRY(launch_clusters_after(fp4_matvec_kernel<kSets, kWhole, OutT>, dim3(slabs * ctas, blocks), ctas, kMatvecThreads,
+                                   kMatvecSmem<kSets>, st, p));
+    return 0;
+}
+
 template <uint32_t kSets>
 int launch_matvec(cudaStream_t st, const MatvecParams& p, int num_sms)
 {
     const uint32_t slabs = (p.n + kMatvecCols - 1) / kMatvecCols;
     const uint32_t blocks = p.ids != nullptr ? p.rows : (p.rows + 4 * kSets - 1) / (4 * kSets);
-    const uint32_t steps = p.k / kMatvecUnit;
-    // K is shared by more CTAs until two fit every SM, as long as each of their warps has a step
-    uint32_t ctas = 1;
-    while (ctas < kMatvecMaxCluster && (uint64_t)slabs * blocks * ctas < 2u * (uint32_t)num_sms && ctas * kMatvecWarps < steps) {
-        ctas *= 2;
-    }
-    CUDA_TRY(launch_clusters_after(g.c_dtype == 1 ? fp4_matvec_kernel<kSets, __half> : fp4_matvec_kernel<kSets, __nv_bfloat16>,
-                                   dim3(slabs * ctas, blocks), ctas, kMatvecThreads, 0, st, p));
-    return 0;
+    const uint32_t ctas = matvec_ctas((uint64_t)slabs * blocks, p.k / kMatvecUnit, 0.53125e-6 * p.n * p.k * (p.ids ? p.rows : 1), num_sms);
+    // rows of whole 16-byte chunks, where they also begin on such
+    return p.n % 32 == 0 ? (g.c_dtype == 1 ? launch_matvec_inst<kSets, true, __half>(st, p, slabs, blocks, ctas)
+                                           : launch_matvec_inst<kSets, true, __nv_bfloat16>(st, p, slabs, blocks, ctas))
+                         : (g.c_dtype == 1 ? launch_matvec_inst<kSets, false, __half>(st, p, slabs, blocks, ctas)
+                                           : launch_matvec_inst<kSets, false, __nv_bfloat16>(st, p, slabs, blocks, ctas));
 }
 
 // Width of a grouped launch's column tiles.

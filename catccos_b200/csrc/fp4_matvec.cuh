@@ -2,6 +2,8 @@
 //   x   bf16 [m, k];   w packed E2M1 [k, n/2], low nibble = even column;   scales E8M0 [k/64, n, 2]
 // With ids the weight is one of several: row r of the result is x[r / (routes / x_rows)] x dequant(w[ids[r]]).
 //
+// Rows of the result that share a weight are multiplied together, four to a pass over it.
+//
 // Bound by the weights' bytes (half a byte and 1/32 per element), then by the instructions that unpack them: an SM takes in 46
 // weights a cycle at full memory rate.  So two weights are unpacked by one conversion (cvt.f16x2.e2m1x2, 64 lanes a cycle as
 // any integer instruction) and the products run on mma.sync m16n8k16 (f16 in, fp32 sums), where they cost nothing here.
@@ -12,6 +14,11 @@
 // x goes in as f16 after a power of two per token and 64 k that brings its largest magnitude to 2^14 .. 2^15: every bf16
 // within 2^-29 of the largest stays exact, smaller ones are off by at most 2^-40 of it, far below the fp32 sums' rounding.
 // Sums of 32 products share a weight scale, which is applied to them in fp32.
+//
+// Every warp has a ring of its own in shared memory, filled by asynchronous copies, two steps (10 KB) ahead; 150 KB an SM.  One
+// token and a weight of 330 MB run at 5.5 TB/s; small ones are some 5 us of launch, first and last step around that (one token,
+// 4096 x 7168: 7.1 us).  Half steps in rings of three, three CTAs an SM, took 10.0 us there, and the largest magnitude of x found
+// ahead of the loop 9.5.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -25,7 +32,18 @@ namespace catccos {
 constexpr uint32_t kMatvecWarps = 8, kMatvecThreads = kMatvecWarps * 32;
 constexpr uint32_t kMatvecCols = 128;  // of a CTA: 8 lane groups x 16
 constexpr uint32_t kMatvecUnit = 64;   // k of a warp's step: the two scale groups that lie together
+constexpr uint32_t kMatvecDepth = 2;   // steps of a warp's ring
 constexpr uint32_t kMatvecMaxCluster = 8;
+constexpr uint32_t kMatvecPartRow = kMatvecCols + 8;
+constexpr uint32_t kMatvecWindow = 1024;  // routes among which a weight's rows find one another
+
+// One step in a warp's ring: 64 rows of 64 bytes of the weight, 128 columns' scales, four tokens' (times kSets) values
+constexpr uint32_t kMatvecScalesOff = kMatvecUnit * kMatvecCols / 2;
+constexpr uint32_t kMatvecXOff = kMatvecScalesOff + kMatvecCols * 2;
+template <uint32_t kSets>
+constexpr uint32_t kMatvecStage = kMatvecXOff + kSets * 4 * kMatvecUnit * 2;
+template <uint32_t kSets>
+constexpr uint32_t kMatvecSmem = kMatvecWarps * kMatvecDepth * kMatvecStage<kSets>;
 
 struct MatvecParams {
     const uint8_t* x;       // bf16
@@ -38,31 +56,30 @@ struct MatvecParams {
     uint32_t rows_per_x;    // rows of the result that share a row of x (with ids)
 };
 
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t word, uint32_t byte)
+// The two E2M1 values of byte `byte` of a word as f16, the low nibble's in the low half.  The byte is named by the instruction
+// itself: shifting it down first made three of four conversions two instructions.
+template <uint32_t kByte>
+__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t word)
 {
     uint32_t r;
-    asm("{\n\t"
-        ".reg .b8 b;\n\t"
-        "cvt.u8.u32 b, %1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, b;\n\t"
-        "}"
-        : "=r"(r)
-        : "r"(word >> (8u * byte)));
+    if constexpr (kByte == 0) {
+        asm("{.reg .b8 b0, b1, b2, b3; mov.b32 {b0, b1, b2, b3}, %1; cvt.rn.f16x2.e2m1x2 %0, b0;}" : "=r"(r) : "r"(word));
+    } else if constexpr (kByte == 1) {
+        asm("{.reg .b8 b0, b1, b2, b3; mov.b32 {b0, b1, b2, b3}, %1; cvt.rn.f16x2.e2m1x2 %0, b1;}" : "=r"(r) : "r"(word));
+    } else if constexpr (kByte == 2) {
+        asm("{.reg .b8 b0, b1, b2, b3; mov.b32 {b0, b1, b2, b3}, %1; cvt.rn.f16x2.e2m1x2 %0, b2;}" : "=r"(r) : "r"(word));
+    } else {
+        asm("{.reg .b8 b0, b1, b2, b3; mov.b32 {b0, b1, b2, b3}, %1; cvt.rn.f16x2.e2m1x2 %0, b3;}" : "=r"(r) : "r"(word));
+    }
     return r;
 }
 
-// two E8M0 bytes -> two bf16 (0xFF becomes NaN)
-__device__ __forceinline__ uint32_t e8m0x2_to_bf16x2(uint32_t pair)
+// A word of E8M0 bytes as four bf16, two to a register (0xFF becomes NaN)
+__device__ __forceinline__ void e8m0x4_to_bf16(uint32_t word, uint32_t& lo, uint32_t& hi)
 {
-    uint32_t r;
-    asm("{\n\t"
-        ".reg .b16 h;\n\t"
-        "cvt.u16.u32 h, %1;\n\t"
-        "cvt.rn.bf16x2.ue8m0x2 %0, h;\n\t"
-        "}"
-        : "=r"(r)
-        : "r"(pair));
-    return r;
+    asm("{.reg .b16 h0, h1; mov.b32 {h0, h1}, %2; cvt.rn.bf16x2.ue8m0x2 %0, h0; cvt.rn.bf16x2.ue8m0x2 %1, h1;}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(word));
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -79,80 +96,181 @@ __device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t cta)
     return v;
 }
 
+// 8-byte copy global -> shared; zeros when !inside (then nothing is read).
+__device__ __forceinline__ void cp_async_8(uint32_t smem_dst, const void* gsrc, bool inside)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_dst), "l"(gsrc), "r"(inside ? 8u : 0u) : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
+__device__ __forceinline__ uint2 ld_shared_u2(uint32_t addr)
+{
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+
+// Half a step lies in slots of 64 bytes: slot s has row 8 (s & 3) + s / 4 (a load of the products takes rows r, 8 + r, 16 + r and
+// 24 + r of the eight lane groups), the last two of four slots their 16-byte chunks the other way round.  So no two lanes of a
+// half warp meet in a bank, and a copy, which fills slots that follow one another, none either.
+__device__ __forceinline__ uint32_t matvec_row(uint32_t slot) { return ((slot & 3u) << 3) | (slot >> 2); }
+__device__ __forceinline__ uint32_t matvec_chunk(uint32_t slot, uint32_t chunk) { return chunk ^ (slot & 2u); }
+
 // kSets sets of four tokens.  A cluster is one block of 128 columns of one set of rows; its CTAs and their warps share the
 // steps of 64 k.  The partial sums meet in shared memory, warp by warp and CTA by CTA in ascending order.
-template <uint32_t kSets, typename OutT>
+// kWhole: rows of the weight are multiples of 16 bytes.
+template <uint32_t kSets, bool kWhole, typename OutT>
 __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const MatvecParams p)
 {
     constexpr uint32_t kTokens = 4 * kSets;
-    __shared__ float part[kMatvecWarps][kTokens][kMatvecCols];
+    constexpr uint32_t kAll = 0xFFFFFFFFu;
+    extern __shared__ __align__(16) uint8_t matvec_smem[];
     __shared__ float total[kTokens][kMatvecCols];
+    __shared__ uint32_t same[kMatvecWindow / 32];
+    static_assert(kMatvecSmem<kSets> >= kMatvecWarps * kTokens * kMatvecPartRow * 4, "the partial sums take the rings' place");
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t g = lane >> 2, tig = lane & 3u;
-    uint32_t ctas, cta;
+    uint32_t ctas;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ctas));
-    cta = cluster_ctarank();
+    const uint32_t cta = cluster_ctarank();
     const uint32_t n0 = blockIdx.x / ctas * kMatvecCols;
-    const uint32_t row0 = p.ids != nullptr ? blockIdx.y : blockIdx.y * kTokens;
     grid_dep_wait();
     grid_dep_launch();
 
     const uint8_t* w = p.w;
     const uint8_t* scales = p.scales;
-    uint32_t tokens = min(kTokens, p.rows - row0), x_row = row0;
+    uint32_t rows[kTokens];  // of the result
+    uint32_t tokens;
     bool live = true;
-    if (p.ids != nullptr) {
-        const uint32_t id = (uint32_t)p.ids[row0];
-        tokens = 1u;
-        x_row = row0 / p.rows_per_x;
+    if (p.ids == nullptr) {
+        tokens = min(kTokens, p.rows - blockIdx.y * kTokens);
+#pragma unroll
+        for (uint32_t t = 0; t < kTokens; ++t) {
+            rows[t] = blockIdx.y * kTokens + t;
+        }
+    } else {
+        // this row and the next three of the same weight; a row that one in front of it takes along has nothing to do
+        const uint32_t row = blockIdx.y, base = row / kMatvecWindow * kMatvecWindow;
+        const uint32_t id = (uint32_t)p.ids[row];
         live = id < p.experts;  // a negative id is a dropped route: its row is zero
+#pragma unroll
+        for (uint32_t i = 0; i < kMatvecWindow / kMatvecThreads; ++i) {
+            const uint32_t at = base + i * kMatvecThreads + threadIdx.x;
+            const uint32_t mask = __ballot_sync(kAll, at < p.rows && (uint32_t)p.ids[min(at, p.rows - 1u)] == id);
+            if (lane == 0) {
+                same[i * kMatvecWarps + warp] = mask;
+            }
+        }
+        __syncthreads();
+        uint32_t before = 0;
+        const uint32_t word = (row - base) >> 5, bit = (row - base) & 31u;
+        for (uint32_t i = 0; i < word; ++i) {
+            before += (uint32_t)__popc(same[i]);
+        }
+        before += (uint32_t)__popc(same[word] & ((1u << bit) - 1u));
+        if (live && before % kTokens != 0u) {
+            return;  // the same answer for the whole cluster
+        }
+        tokens = 1;
+        rows[0] = row;
+        uint32_t i = word, left = same[word] & ~((2u << bit) - 1u);
+#pragma unroll
+        for (uint32_t t = 1; t < kTokens; ++t) {
+            rows[t] = row;
+            while (live && left == 0u && i + 1u < kMatvecWindow / 32u) {
+                left = same[++i];
+            }
+            if (live && left != 0u) {
+                rows[t] = base + i * 32u + (uint32_t)__ffs((int)left) - 1u;
+                left &= left - 1u;
+                tokens = t + 1u;
+            }
+        }
         if (live) {
             w += (size_t)id * p.k * (p.n / 2u);
             scales += (size_t)id * (p.k / 32u) * p.n;
         }
     }
-    const uint32_t col = n0 + g * 16u;
-    const bool col_ok = col < p.n;
     const uint32_t steps = live ? p.k / kMatvecUnit : 0u;
     // bytes of the other operand's registers: this lane's slot takes the token's value, the other one a zero
     const uint32_t sel_lo = (g & 1u) == 0u ? 0x4410u : 0x1044u, sel_hi = (g & 1u) == 0u ? 0x4432u : 0x3244u;
+    const uint32_t ring = smem_u32(matvec_smem) + warp * (kMatvecDepth * kMatvecStage<kSets>);
 
-    float sum[kSets][4][4] = {};
-    for (uint32_t step = cta * kMatvecWarps + warp; step < steps; step += ctas * kMatvecWarps) {
-        uint2 q[2][8];
-        uint4 f[2];
-        f[0] = f[1] = make_uint4(0, 0, 0, 0);
+    // where this lane copies from: token lane / 8 of each set
+    const uint8_t* x_src[kSets];
+    bool x_in[kSets];
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
+    for (uint32_t t = 0; t < kSets; ++t) {
+        uint32_t row = rows[t * 4u];
 #pragma unroll
-            for (uint32_t r = 0; r < 8; ++r) {
-                q[h][r] = make_uint2(0, 0);
-                if (col_ok) {
-                    q[h][r] = __ldcs(reinterpret_cast<const uint2*>(
-                        w + (size_t)(step * kMatvecUnit + h * 32u + tig * 8u + r) * (p.n / 2u) + col / 2u));
-                }
+        for (uint32_t j = 1; j < 4; ++j) {
+            row = (lane >> 3) == j ? rows[t * 4u + j] : row;
+        }
+        x_in[t] = t * 4u + (lane >> 3) < tokens;
+        x_src[t] = p.x + ((size_t)(x_in[t] ? row / p.rows_per_x : 0u) * p.k + (lane & 7u) * 8u) * 2u;
+    }
+    auto copy = [&](uint32_t step, uint32_t stage) {
+        const size_t pitch = p.n / 2u;
+        const uint8_t* src = w + (size_t)step * kMatvecUnit * pitch;
+        if constexpr (kWhole) {
+            const uint32_t chunk = lane & 3u;
+            const bool inside = n0 + chunk * 32u < p.n;
+            const uint8_t* from = src + (inside ? n0 / 2u + chunk * 16u : 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const uint32_t half = i >> 2, slot = (i & 3u) * 8u + (lane >> 2);
+                cp_async_16(stage + half * 2048u + slot * 64u + matvec_chunk(slot, chunk) * 16u,
+                            from + (half * 32u + matvec_row(slot)) * pitch, inside);
+            }
+        } else {
+            const uint32_t part = lane & 7u;
+            const bool inside = n0 + part * 16u < p.n;
+            const uint8_t* from = src + (inside ? n0 / 2u + part * 8u : 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t half = i >> 3, slot = (i & 7u) * 4u + (lane >> 3);
+                cp_async_8(stage + half * 2048u + slot * 64u + matvec_chunk(slot, part >> 1) * 16u + (part & 1u) * 8u,
+                           from + (half * 32u + matvec_row(slot)) * pitch, inside);
             }
         }
-        if (col_ok) {
-            const uint4* s = reinterpret_cast<const uint4*>(scales + ((size_t)step * p.n + col) * 2u);
-            f[0] = s[0];
-            f[1] = s[1];
+        if (lane < 16u) {
+            const bool inside = n0 + lane * 8u < p.n;
+            cp_async_16(stage + kMatvecScalesOff + lane * 16u, scales + ((size_t)step * p.n + (inside ? n0 + lane * 8u : 0u)) * 2u, inside);
         }
+#pragma unroll
+        for (uint32_t t = 0; t < kSets; ++t) {
+            cp_async_16(stage + kMatvecXOff + t * 512u + lane * 16u, x_src[t] + (size_t)step * (kMatvecUnit * 2u), x_in[t]);
+        }
+    };
+
+    float sum[kSets][4][4] = {};
+    const uint32_t first = cta * kMatvecWarps + warp, stride = ctas * kMatvecWarps;
+#pragma unroll
+    for (uint32_t d = 0; d < kMatvecDepth; ++d) {
+        if (first + d * stride < steps) {
+            copy(first + d * stride, ring + d * kMatvecStage<kSets>);
+        }
+        cp_async_commit();
+    }
+    uint32_t stage = ring;
+    for (uint32_t step = first; step < steps; step += stride) {
+        cp_async_wait<kMatvecDepth - 1>();
+        __syncwarp();
         // the tokens' values: lane (g, tig) holds token g / 2, k tig * 8 .. + 7 of both halves
         uint32_t xh[kSets][2][4];
         float back[kSets];
 #pragma unroll
         for (uint32_t t = 0; t < kSets; ++t) {
-            const uint32_t token = t * 4u + (g >> 1);
-            uint4 v[2];
-            v[0] = v[1] = make_uint4(0, 0, 0, 0);
-            if (token < tokens) {
-                const uint4* src = reinterpret_cast<const uint4*>(p.x + ((size_t)(x_row + token) * p.k + step * kMatvecUnit + tig * 8u) * 2u);
-                v[0] = src[0];
-                v[1] = src[4];
-            }
+            const uint32_t at = stage + kMatvecXOff + t * 512u + (g >> 1) * 128u + tig * 16u;
+            const uint4 v[2] = {ld_shared_u4(at), ld_shared_u4(at + 64u)};
             uint32_t top = max(absmax_bits8(v[0]), absmax_bits8(v[1]));
-            if (__any_sync(0xFFFFFFFFu, top >= 0x7F80u)) {
+            if (__any_sync(kAll, top >= 0x7F80u)) {
                 // an infinity or NaN does not set the scale: the finite values beside it must not become infinite
                 top = 0;
                 const uint32_t all[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
@@ -162,12 +280,12 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
                     top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
                 }
             }
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            top = max(top, __shfl_xor_sync(kAll, top, 1));
+            top = max(top, __shfl_xor_sync(kAll, top, 2));
             const int up = min(141 - (int)(top >> 7), 126);
             const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
             // this lane's sums belong to token tig of the set
-            back[t] = __uint_as_float((uint32_t)(127 - __shfl_sync(0xFFFFFFFFu, up, tig * 8u)) << 23);
+            back[t] = __uint_as_float((uint32_t)(127 - __shfl_sync(kAll, up, tig * 8u)) << 23);
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
                 const uint32_t a[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
@@ -177,12 +295,21 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
                 }
             }
         }
-        const uint32_t fw[8] = {f[0].x, f[0].y, f[0].z, f[0].w, f[1].x, f[1].y, f[1].z, f[1].w};
+        const uint4 f0 = ld_shared_u4(stage + kMatvecScalesOff + g * 32u), f1 = ld_shared_u4(stage + kMatvecScalesOff + g * 32u + 16u);
+        const uint32_t fw[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+        uint32_t scale[4][4];  // of columns 2j, 2j + 1, 8 + 2j, 9 + 2j, the first half's below, the second half's above
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            e8m0x4_to_bf16(fw[j], scale[j][0], scale[j][1]);
+            e8m0x4_to_bf16(fw[4 + j], scale[j][2], scale[j][3]);
+        }
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
             float d[kSets][4][4] = {};
 #pragma unroll
             for (uint32_t s = 0; s < 4; ++s) {
+                const uint32_t at = stage + h * 2048u + tig * 64u + matvec_chunk(tig, g >> 1) * 16u + (g & 1u) * 8u;
+                const uint2 q0 = ld_shared_u2(at + 2u * s * 256u), q1 = ld_shared_u2(at + (2u * s + 1u) * 256u);
                 uint32_t b0[kSets], b1[kSets];
 #pragma unroll
                 for (uint32_t t = 0; t < kSets; ++t) {
@@ -190,13 +317,15 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
                     b1[t] = __byte_perm(xh[t][h][s], 0u, sel_hi);
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t a0 = e2m1x2_to_f16x2(q[h][2 * s].x, j), a1 = e2m1x2_to_f16x2(q[h][2 * s].y, j);
-                    const uint32_t a2 = e2m1x2_to_f16x2(q[h][2 * s + 1].x, j), a3 = e2m1x2_to_f16x2(q[h][2 * s + 1].y, j);
-#pragma unroll
-                    for (uint32_t t = 0; t < kSets; ++t) {
-                        mma_f16(d[t][j], a0, a1, a2, a3, b0[t], b1[t]);
-                    }
+                for (uint32_t t = 0; t < kSets; ++t) {
+                    mma_f16(d[t][0], e2m1x2_to_f16x2<0>(q0.x), e2m1x2_to_f16x2<0>(q0.y), e2m1x2_to_f16x2<0>(q1.x),
+                            e2m1x2_to_f16x2<0>(q1.y), b0[t], b1[t]);
+                    mma_f16(d[t][1], e2m1x2_to_f16x2<1>(q0.x), e2m1x2_to_f16x2<1>(q0.y), e2m1x2_to_f16x2<1>(q1.x),
+                            e2m1x2_to_f16x2<1>(q1.y), b0[t], b1[t]);
+                    mma_f16(d[t][2], e2m1x2_to_f16x2<2>(q0.x), e2m1x2_to_f16x2<2>(q0.y), e2m1x2_to_f16x2<2>(q1.x),
+                            e2m1x2_to_f16x2<2>(q1.y), b0[t], b1[t]);
+                    mma_f16(d[t][3], e2m1x2_to_f16x2<3>(q0.x), e2m1x2_to_f16x2<3>(q0.y), e2m1x2_to_f16x2<3>(q1.x),
+                            e2m1x2_to_f16x2<3>(q1.y), b0[t], b1[t]);
                 }
             }
             // d[.][j][0..3]: columns 2j, 2j + 1, 8 + 2j, 9 + 2j of this lane's sixteen, token tig of the set
@@ -204,35 +333,45 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
             for (uint32_t j = 0; j < 4; ++j) {
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t pair = fw[(i >> 1) * 4u + j] >> (16u * (i & 1u));
-                    const uint32_t both = e8m0x2_to_bf16x2(pair);
-                    const float scale = __uint_as_float(h == 0u ? both << 16 : both & 0xFFFF0000u);
+                    const float f = __uint_as_float(h == 0u ? scale[j][i] << 16 : scale[j][i] & 0xFFFF0000u);
 #pragma unroll
                     for (uint32_t t = 0; t < kSets; ++t) {
-                        sum[t][j][i] = fmaf(d[t][j][i] * back[t], scale, sum[t][j][i]);
+                        sum[t][j][i] = fmaf(d[t][j][i] * back[t], f, sum[t][j][i]);
                     }
                 }
             }
         }
+        __syncwarp();  // everybody has read the stage
+        if (step + kMatvecDepth * stride < steps) {
+            copy(step + kMatvecDepth * stride, stage);
+        }
+        cp_async_commit();
+        stage = stage + kMatvecStage<kSets> == ring + kMatvecDepth * kMatvecStage<kSets> ? ring : stage + kMatvecStage<kSets>;
     }
+    cp_async_wait<0>();
+    __syncthreads();  // the rings are empty: their place takes the partial sums
+    // [warp][token][pair of columns of a lane][lane group]: a row of eight floats more keeps the four tokens a half warp stores
+    // out of one another's banks
+    float* part = reinterpret_cast<float*>(matvec_smem);
 #pragma unroll
     for (uint32_t t = 0; t < kSets; ++t) {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            float* dst = &part[warp][t * 4u + tig][g * 16u];
-            *reinterpret_cast<float2*>(dst + 2u * j) = make_float2(sum[t][j][0], sum[t][j][1]);
-            *reinterpret_cast<float2*>(dst + 8u + 2u * j) = make_float2(sum[t][j][2], sum[t][j][3]);
+            float* dst = part + (warp * kTokens + t * 4u + tig) * kMatvecPartRow + j * 16u + g * 2u;
+            *reinterpret_cast<float2*>(dst) = make_float2(sum[t][j][0], sum[t][j][1]);
+            *reinterpret_cast<float2*>(dst + 64u) = make_float2(sum[t][j][2], sum[t][j][3]);
         }
     }
     __syncthreads();
     const uint32_t values = tokens * kMatvecCols;
     for (uint32_t i = threadIdx.x; i < values; i += kMatvecThreads) {
+        const uint32_t token = i / kMatvecCols, at = i & (kMatvecCols - 1u);
         float v = 0.0f;
 #pragma unroll
         for (uint32_t o = 0; o < kMatvecWarps; ++o) {
-            v += (&part[o][0][0])[i];
+            v += part[(o * kTokens + token) * kMatvecPartRow + at];
         }
-        (&total[0][0])[i] = v;
+        total[token][at] = v;
     }
     __syncthreads();
     if (ctas > 1u) {
@@ -240,15 +379,21 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
     }
     // every CTA of the cluster writes its share of the pairs of columns
     for (uint32_t i = cta * kMatvecThreads + threadIdx.x; i < values / 2u; i += ctas * kMatvecThreads) {
-        const float* src = &total[0][0] + 2u * i;
+        const uint32_t token = i / (kMatvecCols / 2u), pair = i & (kMatvecCols / 2u - 1u);
+        const float* src = &total[token][(pair & 7u) * 16u + (pair >> 3) * 2u];  // pair & 7 names half and j: columns 8 half + 2 j
         float a = 0.0f, b = 0.0f;
         for (uint32_t o = 0; o < ctas; ++o) {
             a += ctas > 1u ? ld_cluster_f32(src, o) : src[0];
             b += ctas > 1u ? ld_cluster_f32(src + 1, o) : src[1];
         }
-        const uint32_t token = 2u * i / kMatvecCols, c = n0 + (2u * i & (kMatvecCols - 1u));
+        const uint32_t c = n0 + 2u * pair;
+        uint32_t row = rows[0];
+#pragma unroll
+        for (uint32_t t = 1; t < kTokens; ++t) {
+            row = token == t ? rows[t] : row;
+        }
         if (c < p.n) {
-            *reinterpret_cast<uint32_t*>(p.out + ((size_t)(row0 + token) * p.n + c) * 2u) = pack2<OutT>(a, b);
+            *reinterpret_cast<uint32_t*>(p.out + ((size_t)row * p.n + c) * 2u) = pack2<OutT>(a, b);
         }
     }
     if (ctas > 1u) {
