@@ -342,11 +342,7 @@ def mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out=None, out_dtype
 
     a_codes [rows, K] and a_scales [rows, K/32] may be columns of a wider tensor (packed[:, :K] and packed[:, K:K + K // 32] of
     mx_quant_scatter_packed).  Rows outside the offsets stay as they are (of a tensor allocated here: unset)."""
-    if out is None:
-        import torch
-
-        out = torch.empty((a_codes.shape[0], b_scales.shape[-2]), dtype=out_dtype or torch.bfloat16, device=a_codes.device)
-    code = (_calls or _load_calls()).mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out)
+    code, out = (_calls or _load_calls()).mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out, out_dtype)
     if code:
         raise CatccosError("catccos_b200_mx_grouped_gemm", code)
     return out
@@ -354,11 +350,7 @@ def mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out=None, out_dtype
 
 def moe_combine(expert_out, row_index, weights, shared=None, out=None):
     """out [tokens, n] = sum over r of weights[t, r] * expert_out[row_index[t, r]] (+ shared[t]); bf16 or fp16, sums in fp32."""
-    if out is None:
-        import torch
-
-        out = torch.empty((row_index.shape[0], expert_out.shape[1]), dtype=expert_out.dtype, device=expert_out.device)
-    code = (_calls or _load_calls()).moe_combine(expert_out, row_index, weights, shared, out)
+    code, out = (_calls or _load_calls()).moe_combine(expert_out, row_index, weights, shared, out)
     if code:
         raise CatccosError("catccos_b200_moe_combine", code)
     return out
@@ -369,12 +361,7 @@ def mx_fp4_matvec(x_bf16, w, w_scales, ids=None, out=None, out_dtype=None):
 
     With ids int32 (any shape, i values): w [experts, K, N/2], w_scales [experts, K/64, N, 2] -> [i, N], row r with weight ids[r]
     and x's row r // (i // rows); a negative id gives a row of zeros."""
-    if out is None:
-        import torch
-
-        out = torch.empty((x_bf16.shape[0] if ids is None else ids.numel(), w_scales.shape[-2]), dtype=out_dtype or torch.bfloat16,
-                          device=x_bf16.device)
-    code = (_calls or _load_calls()).mx_fp4_matvec(x_bf16, w, w_scales, ids, out)
+    code, out = (_calls or _load_calls()).mx_fp4_matvec(x_bf16, w, w_scales, ids, out, out_dtype)
     if code:
         raise CatccosError("catccos_b200_mx_fp4_matvec", code)
     return out

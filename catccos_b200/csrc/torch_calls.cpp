@@ -7,6 +7,7 @@
 //
 // The C ABI's functions are not linked but bound by address (bind()), so that they are those of the library that capi.py
 // has loaded.  Every function returns the C ABI's code (alone, or first in a tuple with the outputs).
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -251,6 +252,44 @@ const at::Tensor& plain(PyObject* o, const char* what, const char* wanted, std::
     return t;
 }
 
+// The result's tensor: the one that is given, checked, or a new one.
+at::Tensor result(PyObject* given, const char* wanted, std::initializer_list<at::ScalarType> types, const at::Tensor& like, int64_t rows,
+                  int64_t cols, at::ScalarType type)
+{
+    if (given == Py_None) {
+        return at::detail::empty_cuda({rows, cols}, type, like.device(), std::nullopt);
+    }
+    const at::Tensor& out = plain(given, "out", wanted, types, 2, &like);
+    if (out.size(0) != rows || out.size(1) != cols) {
+        refuse("out", wanted);
+    }
+    return out;
+}
+
+// torch.bfloat16, torch.float16, or None for the first
+at::ScalarType half_type(PyObject* dtype)
+{
+    if (dtype == Py_None) {
+        return at::kBFloat16;
+    }
+    const at::ScalarType type = THPDtype_Check(dtype) ? reinterpret_cast<THPDtype*>(dtype)->scalar_type : at::kFloat;
+    if (type != at::kBFloat16 && type != at::kHalf) {
+        refuse("out_dtype", "torch.bfloat16 or torch.float16");
+    }
+    return type;
+}
+
+PyObject* with_output(PyObject* code, PyObject* given, const at::Tensor& made)
+{
+    PyObject* out = PyTuple_New(2);
+    PyTuple_SET_ITEM(out, 0, code);
+    if (given != Py_None) {
+        Py_INCREF(given);
+    }
+    PyTuple_SET_ITEM(out, 1, given != Py_None ? given : THPVariable_Wrap(made));
+    return out;
+}
+
 void* data_or_null(PyObject* o) { return o == Py_None ? nullptr : tensor(o).data_ptr(); }
 
 // The tensors' device for the rest of a call, and its current stream.
@@ -429,8 +468,8 @@ CALL(moe_row_plan, 3)
                         index, offsets);
 END_CALL
 
-// a, a_scales, b, b_scales, offsets, out
-CALL(mx_grouped_gemm, 6)
+// a, a_scales, b, b_scales, offsets, out, out_dtype
+CALL(mx_grouped_gemm, 7)
     const auto codes = {kU8, at::kFloat8_e4m3fn, at::kFloat8_e5m2};
     const at::Tensor& x = plain(a[0], "a_codes", "a CUDA matrix of 8-bit codes, its columns next to one another", codes, 2, nullptr, false);
     const at::Tensor& xs = plain(a[1], "a_scales", "a CUDA matrix of bytes on a_codes' device, its columns next to one another",
@@ -438,24 +477,25 @@ CALL(mx_grouped_gemm, 6)
     const at::Tensor& b = plain(a[2], "b", "contiguous 8-bit codes [experts, K, N] on a_codes' device", codes, 3, &x);
     const at::Tensor& bs = plain(a[3], "b_scales", "contiguous bytes [experts, K / 64, N, 2] on a_codes' device", {kU8, at::kFloat8_e8m0fnu}, 4, &x);
     const at::Tensor& offsets = plain(a[4], "offsets", "a contiguous int32 vector on a_codes' device", {kI32}, 1, &x);
-    const at::Tensor& out = plain(a[5], "out", "a contiguous bf16 or fp16 matrix on a_codes' device", {kBf16, kF16}, 2, &x);
     const int64_t rows = x.size(0), k = x.size(1), experts = b.size(0), n = b.size(2);
     if ((k > 1 && x.stride(1) != 1) || (k >= 64 && xs.stride(1) != 1) || x.stride(0) < 0 || xs.stride(0) < 0) {
         refuse("a_codes, a_scales", "columns next to one another");
     }
     if (xs.size(0) != rows || xs.size(1) != k / 32 || b.size(1) != k || bs.size(0) != experts || bs.size(1) != k / 64 || bs.size(2) != n ||
-        bs.size(3) != 2 || offsets.size(0) != experts + 1 || out.size(0) != rows || out.size(1) != n) {
+        bs.size(3) != 2 || offsets.size(0) != experts + 1) {
         refuse("mx_grouped_gemm", "a [rows, K], a_scales [rows, K / 32], b [experts, K, N], b_scales [experts, K / 64, N, 2], "
-                                  "offsets [experts + 1], out [rows, N]");
+                                  "offsets [experts + 1]");
     }
     const OnDevice on(x);
+    const at::Tensor out = result(a[5], "a contiguous bf16 or fp16 matrix [rows, N] on a_codes' device", {kBf16, kF16}, x, rows, n, half_type(a[6]));
     // one row has no distance to the next
     const size_t step = rows > 1 ? (size_t)x.stride(0) : (size_t)(k + 15) / 16 * 16, scale_step = rows > 1 ? (size_t)xs.stride(0) : (size_t)(k / 32 + 3) / 4 * 4;
     void *ac = x.data_ptr(), *as = xs.data_ptr(), *bc = b.data_ptr(), *bf = bs.data_ptr(), *o = offsets.data_ptr(), *c = out.data_ptr();
-    return released([&] {
-        return mx_grouped_gemm_fn(on.stream, ac, step, as, scale_step, bc, bf, (const int32_t*)o, c, (uint32_t)rows, (uint32_t)experts,
-                                  (uint32_t)n, (uint32_t)k);
-    });
+    return with_output(released([&] {
+                           return mx_grouped_gemm_fn(on.stream, ac, step, as, scale_step, bc, bf, (const int32_t*)o, c, (uint32_t)rows,
+                                                     (uint32_t)experts, (uint32_t)n, (uint32_t)k);
+                       }),
+                       a[5], out);
 END_CALL
 
 // expert_out, row_index, weights, shared, out
@@ -464,43 +504,46 @@ CALL(moe_combine, 5)
     const at::ScalarType type = y.scalar_type();
     const at::Tensor& index = plain(a[1], "row_index", "a contiguous int32 matrix on expert_out's device", {kI32}, 2, &y);
     const at::Tensor& w = plain(a[2], "weights", "a contiguous fp32 matrix on expert_out's device", {kF32}, 2, &y);
-    const at::Tensor& out = plain(a[4], "out", "a contiguous matrix of expert_out's type and device", {type}, 2, &y);
     const int64_t tokens = index.size(0), n = y.size(1);
-    if (w.sizes() != index.sizes() || out.size(0) != tokens || out.size(1) != n) {
-        refuse("moe_combine", "row_index and weights [tokens, top_k], out [tokens, n]");
+    if (w.sizes() != index.sizes()) {
+        refuse("moe_combine", "row_index and weights [tokens, top_k]");
     }
-    if (a[3] != Py_None && plain(a[3], "shared", "a contiguous matrix of expert_out's type and device", {type}, 2, &y).sizes() != out.sizes()) {
-        refuse("shared", "out's shape");
-    }
+    const char* wanted = "a contiguous matrix [tokens, n] of expert_out's type and device";
     const OnDevice on(y);
+    const at::Tensor out = result(a[4], wanted, {type}, y, tokens, n, type);
+    if (a[3] != Py_None && plain(a[3], "shared", wanted, {type}, 2, &y).sizes() != out.sizes()) {
+        refuse("shared", wanted);
+    }
     void *in = y.data_ptr(), *i = index.data_ptr(), *g = w.data_ptr(), *s = data_or_null(a[3]), *o = out.data_ptr();
     const uint32_t top_k = (uint32_t)index.size(1), rows = (uint32_t)y.size(0);
-    return released([&] {
-        return moe_combine_fn(on.stream, in, rows, (const int32_t*)i, (const float*)g, s, o, (uint32_t)tokens, (uint32_t)n, top_k,
-                              type == kF16 ? 1 : 0);
-    });
+    return with_output(released([&] {
+                           return moe_combine_fn(on.stream, in, rows, (const int32_t*)i, (const float*)g, s, o, (uint32_t)tokens,
+                                                 (uint32_t)n, top_k, type == kF16 ? 1 : 0);
+                       }),
+                       a[4], out);
 END_CALL
 
-// x, w, w_scales, ids, out
-CALL(mx_fp4_matvec, 5)
+// x, w, w_scales, ids, out, out_dtype
+CALL(mx_fp4_matvec, 6)
     const bool many = a[3] != Py_None;
     const at::Tensor& x = plain(a[0], "x", "a contiguous bf16 CUDA matrix", {kBf16}, 2);
     const at::Tensor& w = plain(a[1], "w", "contiguous packed codes [K, N / 2], with ids [experts, K, N / 2], on x's device", {kU8}, many ? 3 : 2, &x);
     const at::Tensor& ws = plain(a[2], "w_scales", "contiguous bytes [K / 64, N, 2], with ids [experts, K / 64, N, 2], on x's device",
                                  {kU8, at::kFloat8_e8m0fnu}, many ? 4 : 3, &x);
-    const at::Tensor& out = plain(a[4], "out", "a contiguous bf16 or fp16 matrix on x's device", {kBf16, kF16}, 2, &x);
     const int64_t x_rows = x.size(0), k = x.size(1), experts = many ? w.size(0) : 1, n = 2 * w.size(-1);
     const int64_t rows = many ? plain(a[3], "ids", "a contiguous int32 tensor on x's device", {kI32}, -1, &x).numel() : x_rows;
     if (w.size(-2) != k || ws.size(-3) != k / 64 || ws.size(-2) != n || ws.size(-1) != 2 || (many && ws.size(0) != experts) ||
-        out.size(0) != rows || out.size(1) != n || rows > 0x7FFFFFFFll) {
-        refuse("mx_fp4_matvec", "x [rows, K], w [.., K, N / 2], w_scales [.., K / 64, N, 2], out [rows or ids, N]");
+        rows > 0x7FFFFFFFll) {
+        refuse("mx_fp4_matvec", "x [rows, K], w [.., K, N / 2], w_scales [.., K / 64, N, 2]");
     }
     const OnDevice on(x);
+    const at::Tensor out = result(a[4], "a contiguous bf16 or fp16 matrix [rows or ids, N] on x's device", {kBf16, kF16}, x, rows, n, half_type(a[5]));
     void *in = x.data_ptr(), *wp = w.data_ptr(), *sp = ws.data_ptr(), *i = data_or_null(a[3]), *o = out.data_ptr();
-    return released([&] {
-        return mx_fp4_matvec_fn(on.stream, in, wp, sp, (const int32_t*)i, o, (uint32_t)rows, (uint32_t)x_rows, (uint32_t)experts,
-                                (uint32_t)n, (uint32_t)k);
-    });
+    return with_output(released([&] {
+                           return mx_fp4_matvec_fn(on.stream, in, wp, sp, (const int32_t*)i, o, (uint32_t)rows, (uint32_t)x_rows,
+                                                   (uint32_t)experts, (uint32_t)n, (uint32_t)k);
+                       }),
+                       a[4], out);
 END_CALL
 
 // bind(name, address): which function of the loaded library a call goes to
