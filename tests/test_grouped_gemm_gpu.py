@@ -99,8 +99,23 @@ def test_many_experts(capi, cuda):
     _run(cuda, capi, offsets[-1] + 5, 336, 128, offsets)
 
 
-def test_several_rounds_of_tiles(capi, cuda):
-    _run(cuda, capi, 2500, 2304, 256, [0, 100, 612, 613, 1500, 2500])
+def test_as_many_experts_as_there_may_be(capi, cuda):
+    counts = [(i * 7919) % 41 if i % 97 == 5 else 0 for i in range(1024)]
+    offsets = [0]
+    for v in counts:
+        offsets.append(offsets[-1] + v)
+    _run(cuda, capi, offsets[-1], 32, 128, offsets)
+
+
+@pytest.mark.parametrize("block_n", [0, 64, 128])
+def test_several_rounds_of_tiles(capi, cuda, block_n):
+    _run(cuda, capi, 2500, 2304, 256, [0, 100, 612, 613, 1500, 2500], block_n=block_n)
+
+
+@pytest.mark.parametrize("block_n", [64, 128, 256])
+def test_long_rows_of_few_tokens(capi, cuda, block_n):
+    # more K tiles than the ring has stages, several times over
+    _run(cuda, capi, 21, 784, 7168, [0, 1, 21], block_n=block_n)
 
 
 def test_one_row_of_a_wider_tensor(capi, cuda):
