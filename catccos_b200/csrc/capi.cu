@@ -24,6 +24,7 @@
 #include "mx_gemm_pair.cuh"
 #include "mx_gemm_small.cuh"
 #include "mx_grouped_gemm.cuh"
+#include "mx_grouped_pair.cuh"
 #include "mx_quant.cuh"
 #include "norm_quant.cuh"
 
@@ -1580,27 +1581,39 @@ int launch_matvec(cudaStream_t st, const MatvecParams& p, int num_sms)
                                            : launch_matvec_inst<kSets, false, __nv_bfloat16>(st, p, slabs, blocks, ctas));
 }
 
-// Width of a grouped launch's column tiles: the one that takes least by a fit to 260 drawn calls (1 to 16384 rows of 1 to 64
-// unevenly chosen experts, N and K to 7168; 8 % off).  A launch, then for each round of units a K tile's time, which grows with
-// the SMs that are busy, and the output.  The host does not know the experts' rows: it reckons with rows for nine in ten of the
-// experts that may have some, and seven in ten of those with a tile that is not full.  So chosen, a call takes 1 % more than with the best
-// width (26 % at worst); with the experts' true tiles it would be 0.1 %.
-uint32_t grouped_block_n(const RankCtx& rc, uint32_t rows, uint32_t experts, uint32_t n, uint32_t k)
+// A grouped launch's tiles: those that take least by a fit to 420 drawn calls (1 to 16384 rows of 1 to 64 unevenly chosen
+// experts, N and K to 7168; 8 to 11 % off).  A launch, then for each round of units a K tile's time, which grows with the SMs that are busy, and
+// the output.  The host does not know the experts' rows: it reckons with rows for nine in ten of the experts that may have some, and
+// seven in ten of those with a tile that is not full.  So chosen, a call takes 1.2 % more than with the best tiles (20 % at worst); with the
+// experts' true tiles it would be 0.6 %.  Without the pairs the 198 largest of these calls would take 9 % more.
+struct GroupedPlan {
+    uint32_t block_n;
+    bool pair;
+};
+
+GroupedPlan plan_grouped(const RankCtx& rc, uint32_t rows, uint32_t experts, uint32_t n, uint32_t k)
 {
     struct Cost {
-        uint32_t width;
+        uint32_t width, tile_rows, sms;
         double launch, k_tile, busy_k_tile, round;
     };
-    constexpr Cost costs[] = {{64, 2.99, 0.261, 0.033, 0.32}, {128, 3.18, 0.291, 0.075, 0.47}, {256, 3.57, 0.383, 0.207, 0.89}};
+    constexpr Cost costs[] = {{64, kGemmBlockM, 1, 3.08, 0.253, 0.042, 0.28},
+                              {128, kGemmBlockM, 1, 3.16, 0.285, 0.083, 0.46},
+                              {256, kGemmBlockM, 1, 3.46, 0.355, 0.207, 1.04},
+                              {kPairBlockN, kPairBlockM, 2, 4.34, 0.303, 0.125, 1.15}};
     const double active = std::min(rows, experts) < 2 ? 1.0 : 0.9 * std::min(rows, experts);
-    const double tiles = std::floor(std::max(active, rows / (double)kGemmBlockM + 0.7 * active) + 0.5);
-    uint32_t best = 0;
+    GroupedPlan best = {0, false};
     double least = 0;
     for (const Cost& c : costs) {
-        const double units = tiles * ((n + c.width - 1) / c.width), rounds = std::ceil(units / rc.num_sms);
-        const double time = c.launch + rounds * ((k / kGemmBlockK) * (c.k_tile + c.busy_k_tile * std::min(1.0, units / rc.num_sms)) + c.round);
-        if (best == 0 || time < least) {
-            best = c.width;
+        if ((g.cta_pair != 0 && (g.cta_pair == 1) != (c.sms == 2)) || (g.block_n != 0 && c.sms == 1 && (uint32_t)g.block_n != c.width)) {
+            continue;  // a test names the tiles
+        }
+        const double tiles = std::floor(std::max(active, rows / (double)c.tile_rows + 0.7 * active) + 0.5);
+        const double units = tiles * ((n + c.width - 1) / c.width), slots = rc.num_sms / c.sms;
+        const double time = c.launch + std::ceil(units / slots) *
+                                           ((k / kGemmBlockK) * (c.k_tile + c.busy_k_tile * std::min(1.0, units / slots)) + c.round);
+        if (best.block_n == 0 || time < least) {
+            best = {c.width, c.sms == 2};
             least = time;
         }
     }
@@ -1618,20 +1631,64 @@ int launch_grouped_inst(uint32_t grid, cudaStream_t st, const CUtensorMap& ta, c
     return 0;
 }
 
+// Maps of a grouped launch's rows (boxes of 128 and of 32) and of its weights (`columns` wide).
+int grouped_maps(CUtensorMap (&maps)[3], const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p, uint32_t columns)
+{
+    int rcode = encode_map_2d(&maps[0], a, p.K, p.rows, kGemmBlockK, kGemmBlockM, false, 1, a_row_bytes);
+    if (rcode == 0) rcode = encode_map_2d(&maps[1], a, p.K, p.rows, kGemmBlockK, 32, false, 1, a_row_bytes);
+    if (rcode == 0) rcode = encode_map_2d(&maps[2], b, p.N, (uint64_t)p.experts * p.K, columns, kGemmBlockK);
+    return rcode;
+}
+
+template <typename OutT>
+int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
+{
+    auto kern = mx_grouped_pair_kernel<OutT>;
+    static int resident[kMaxRanks * 2] = {};
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    int pairs = dev < kMaxRanks * 2 ? resident[dev] : 0;
+    if (pairs == 0) {
+        CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairSmem::kDynamicBytes));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)rc.num_sms / 2 * 2);
+        cfg.blockDim = dim3(kGemmThreads);
+        cfg.dynamicSmemBytes = PairSmem::kDynamicBytes;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs < 1) {
+            cudaGetLastError();
+            pairs = rc.num_sms / 2;
+        }
+        if (dev < kMaxRanks * 2) {
+            resident[dev] = pairs;
+        }
+    }
+    CUtensorMap maps[3];
+    int rcode = grouped_maps(maps, a, a_row_bytes, b, p, kGemmBlockM);
+    if (rcode != 0) return rcode;
+    const uint64_t units = (p.rows / kPairBlockM + std::min(p.rows, p.experts)) * (uint64_t)((p.N + kPairBlockN - 1) / kPairBlockN);
+    CUDA_TRY(launch_after(kern, dim3(2u * (unsigned)std::min<uint64_t>(units, (uint64_t)pairs)), kGemmThreads, PairSmem::kDynamicBytes, st,
+                          maps[0], maps[1], maps[2], p));
+    return 0;
+}
+
 template <uint32_t BLOCK_N>
 int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
 {
-    CUtensorMap ta, ta32, tb;
-    int rcode = encode_map_2d(&ta, a, p.K, p.rows, kGemmBlockK, kGemmBlockM, false, 1, a_row_bytes);
-    if (rcode == 0) rcode = encode_map_2d(&ta32, a, p.K, p.rows, kGemmBlockK, 32, false, 1, a_row_bytes);
-    if (rcode == 0) rcode = encode_map_2d(&tb, b, p.N, (uint64_t)p.experts * p.K, GemmSmem<BLOCK_N>::kBRow, kGemmBlockK);
+    CUtensorMap maps[3];
+    int rcode = grouped_maps(maps, a, a_row_bytes, b, p, GemmSmem<BLOCK_N>::kBRow);
     if (rcode != 0) return rcode;
     // at most one row tile that is not full for every expert that has rows
     const uint64_t tiles = p.rows / kGemmBlockM + std::min(p.rows, p.experts);
     const uint64_t units = tiles * ((p.N + BLOCK_N - 1) / BLOCK_N);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(units, (uint64_t)rc.num_sms);
-    return g.c_dtype == 1 ? launch_grouped_inst<BLOCK_N, __half>(grid, st, ta, ta32, tb, p)
-                          : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, ta, ta32, tb, p);
+    return g.c_dtype == 1 ? launch_grouped_inst<BLOCK_N, __half>(grid, st, maps[0], maps[1], maps[2], p)
+                          : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, maps[0], maps[1], maps[2], p);
 }
 
 }  // namespace
@@ -2527,10 +2584,15 @@ int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes
     p.b_fmt = g.b_dtype == 1 ? 1u : 0u;
     p.bar_timeout_ns = 2 * g.timeout_ns + 1000000000ull;
     p.status = rc.status;
-    const uint32_t bn = g.block_n != 0 ? (uint32_t)g.block_n : grouped_block_n(rc, rows, experts, n, k);
     cudaStream_t st = (cudaStream_t)stream;
-    return bn == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p)
-                    : (bn == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p) : launch_grouped<256>(rc, st, a, a_row_bytes, b, p));
+    const GroupedPlan plan = plan_grouped(rc, rows, experts, n, k);
+    if (plan.pair) {
+        return g.c_dtype == 1 ? launch_grouped_pair<__half>(rc, st, a, a_row_bytes, b, p)
+                              : launch_grouped_pair<__nv_bfloat16>(rc, st, a, a_row_bytes, b, p);
+    }
+    return plan.block_n == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p)
+                              : (plan.block_n == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p)
+                                                     : launch_grouped<256>(rc, st, a, a_row_bytes, b, p));
 }
 
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,

@@ -6,7 +6,7 @@
 //   B      8-bit codes [experts, K, N];  SFB E8M0 [experts, K/64, N, 2]
 //   C      bf16 or fp16 [rows, N]; rows outside the offsets are left as they are
 //
-// The tile, the shared-memory ring, the tensor-memory layout and the warps' roles are those of mx_gemm_kernel.  What differs
+// (mx_grouped_pair.cuh has the form for many rows an expert.)  The tile, the shared-memory ring, the tensor-memory layout and the warps' roles are those of mx_gemm_kernel.  What differs
 // is the list of work: every CTA reads the offsets, counts each expert's 128-row tiles and walks the (expert, row tile, column
 // tile) units blockIdx.x, blockIdx.x + gridDim.x, ... with the column tile running fastest, so that the CTAs that run at one
 // time share a few experts' weights and rows in L2.  The host knows an upper bound of the units only.
@@ -65,6 +65,36 @@ struct GroupedWalk {
     }
 };
 
+// One warp: the experts' rows, and how many tiles of tile_rows rows lie before each expert's (tiles[experts]: all of them).
+__device__ __forceinline__ void count_grouped_tiles(const GroupedParams& p, uint32_t tile_rows, uint32_t* tiles, uint32_t* row_begin,
+                                                    uint32_t* row_end, uint32_t lane)
+{
+    uint32_t before = 0;
+    for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
+        const uint32_t e = e0 + lane;
+        uint32_t begin = 0, end = 0;
+        if (e < p.experts) {
+            grouped_rows(__ldcg(p.offsets + e), __ldcg(p.offsets + e + 1u), p.rows, begin, end);
+            row_begin[e] = begin;
+            row_end[e] = end;
+        }
+        const uint32_t own = (end - begin + tile_rows - 1u) / tile_rows;
+        uint32_t incl = own;
+#pragma unroll
+        for (uint32_t d = 1; d < 32; d <<= 1) {
+            const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+            incl += lane >= d ? o : 0u;
+        }
+        if (e < p.experts) {
+            tiles[e] = before + incl - own;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, incl, 31);
+    }
+    if (lane == 0) {
+        tiles[p.experts] = before;
+    }
+}
+
 template <uint32_t BLOCK_N, typename OutT>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 mx_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
@@ -114,30 +144,7 @@ mx_grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
     grid_dep_wait();  // the offsets, the rows and their scales come from the kernels before this one
     if (warp == 0) {
-        uint32_t before = 0;
-        for (uint32_t e0 = 0; e0 < p.experts; e0 += 32u) {
-            const uint32_t e = e0 + lane;
-            uint32_t begin = 0, end = 0;
-            if (e < p.experts) {
-                grouped_rows(__ldcg(p.offsets + e), __ldcg(p.offsets + e + 1u), p.rows, begin, end);
-                row_begin[e] = begin;
-                row_end[e] = end;
-            }
-            uint32_t incl = (end - begin + kGemmBlockM - 1u) / kGemmBlockM;
-            const uint32_t own = incl;
-#pragma unroll
-            for (uint32_t d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, incl, d);
-                incl += lane >= d ? o : 0u;
-            }
-            if (e < p.experts) {
-                tiles[e] = before + incl - own;
-            }
-            before += __shfl_sync(0xFFFFFFFFu, incl, 31);
-        }
-        if (lane == 0) {
-            tiles[p.experts] = before;
-        }
+        count_grouped_tiles(p, kGemmBlockM, tiles, row_begin, row_end, lane);
     }
     tcgen05_fence_before();
     __syncthreads();

@@ -41,14 +41,14 @@ def _set(capi, options):
         capi.set_option(key, value)
 
 
-def _run(torch, capi, rows, n, k, offsets, a_dtype=0, out="bfloat16", packed=False, block_n=0, seed=0):
+def _run(torch, capi, rows, n, k, offsets, a_dtype=0, out="bfloat16", packed=False, block_n=0, cta_pair=0, seed=0):
     experts = len(offsets) - 1
     a, a_scales, b, b_scales = _operands(torch, capi, rows, n, k, experts, a_dtype, seed + rows + n + k)
     off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
     dtype = getattr(torch, out)
     c = torch.full((rows, n), 7.0, dtype=dtype, device="cuda")
     single = torch.full((rows, n), 7.0, dtype=dtype, device="cuda")
-    options = dict(a_dtype=a_dtype, c_dtype=1 if out == "float16" else 0, block_n=block_n)
+    options = dict(a_dtype=a_dtype, c_dtype=1 if out == "float16" else 0, block_n=block_n, cta_pair=cta_pair)
     _set(capi, options)
     try:
         assert capi.mx_grouped_gemm(*(_packed(torch, capi, a, a_scales) if packed else (a, a_scales)), b, b_scales, off, out=c) is c
@@ -72,50 +72,54 @@ def _run(torch, capi, rows, n, k, offsets, a_dtype=0, out="bfloat16", packed=Fal
             assert bool(((c[lo:hi].double() - want).abs() <= slack + half * (want.abs() + slack) + 2.0**-25).all()), e
 
 
-@pytest.mark.parametrize("block_n", [64, 128, 256])
+@pytest.mark.parametrize("block_n,cta_pair", [(64, 2), (128, 2), (256, 2), (0, 1)])
 @pytest.mark.parametrize("rows,n,k,offsets", [
     (1, 16, 128, [0, 1]),
     (9, 272, 256, [0, 1, 1, 4, 9]),                          # one row, none, a few
     (400, 528, 384, [3, 3, 35, 68, 197, 325, 325, 390]),     # 32, 33, 129, 128 rows; rows in front and behind that nobody has
     (700, 2320, 512, [0, 0, 0, 700]),                        # one expert has them all; the last tiles are ragged
     (130, 64, 1152, [0, 97, 130, 130]),
+    (1300, 784, 640, [0, 128, 129, 385, 642, 1300]),         # an end on each side of a pair's halves
 ])
-def test_rows_of_each_expert(capi, cuda, rows, n, k, offsets, block_n):
-    _run(cuda, capi, rows, n, k, offsets, block_n=block_n)
+def test_rows_of_each_expert(capi, cuda, rows, n, k, offsets, block_n, cta_pair):
+    _run(cuda, capi, rows, n, k, offsets, block_n=block_n, cta_pair=cta_pair)
 
 
+@pytest.mark.parametrize("cta_pair", [1, 2])
 @pytest.mark.parametrize("a_dtype,out,packed", [(0, "bfloat16", True), (1, "float16", False), (1, "bfloat16", True), (0, "float16", True)])
 @pytest.mark.parametrize("rows,n,k,offsets", [(300, 304, 640, [0, 20, 20, 160, 300]), (16, 1040, 1024, list(range(0, 17, 2)))])
-def test_types_and_packed_rows(capi, cuda, rows, n, k, offsets, a_dtype, out, packed):
-    _run(cuda, capi, rows, n, k, offsets, a_dtype, out, packed)
+def test_types_and_packed_rows(capi, cuda, rows, n, k, offsets, a_dtype, out, packed, cta_pair):
+    _run(cuda, capi, rows, n, k, offsets, a_dtype, out, packed, cta_pair=cta_pair)
 
 
-def test_many_experts(capi, cuda):
+@pytest.mark.parametrize("cta_pair", [1, 2])
+def test_many_experts(capi, cuda, cta_pair):
     # more experts than a warp counts at a time, most of them without rows; several rounds of units a CTA
     counts = [(i * 7919) % 5 if i % 3 == 0 else 0 for i in range(200)] + [150]
     offsets = [0]
     for v in counts:
         offsets.append(offsets[-1] + v)
-    _run(cuda, capi, offsets[-1] + 5, 336, 128, offsets)
+    _run(cuda, capi, offsets[-1] + 5, 336, 128, offsets, cta_pair=cta_pair)
 
 
-def test_as_many_experts_as_there_may_be(capi, cuda):
+@pytest.mark.parametrize("cta_pair", [1, 2])
+def test_as_many_experts_as_there_may_be(capi, cuda, cta_pair):
     counts = [(i * 7919) % 41 if i % 97 == 5 else 0 for i in range(1024)]
     offsets = [0]
     for v in counts:
         offsets.append(offsets[-1] + v)
-    _run(cuda, capi, offsets[-1], 32, 128, offsets)
+    _run(cuda, capi, offsets[-1], 32, 128, offsets, cta_pair=cta_pair)
 
 
-@pytest.mark.parametrize("block_n", [0, 64, 128])
-def test_several_rounds_of_tiles(capi, cuda, block_n):
-    _run(cuda, capi, 2500, 2304, 256, [0, 100, 612, 613, 1500, 2500], block_n=block_n)
+@pytest.mark.parametrize("block_n,cta_pair", [(0, 0), (64, 2), (128, 2), (0, 1)])
+def test_several_rounds_of_tiles(capi, cuda, block_n, cta_pair):
+    _run(cuda, capi, 2500, 2304, 256, [0, 100, 612, 613, 1500, 2500], block_n=block_n, cta_pair=cta_pair)
 
 
-@pytest.mark.parametrize("block_n", [64, 128, 256])
-def test_long_rows_of_few_tokens(capi, cuda, block_n):
+@pytest.mark.parametrize("block_n,cta_pair", [(64, 2), (128, 2), (256, 2), (0, 1)])
+def test_long_rows_of_few_tokens(capi, cuda, block_n, cta_pair):
     # more K tiles than the ring has stages, several times over
-    _run(cuda, capi, 21, 784, 7168, [0, 1, 21], block_n=block_n)
+    _run(cuda, capi, 21, 784, 7168, [0, 1, 21], block_n=block_n, cta_pair=cta_pair)
 
 
 def test_one_row_of_a_wider_tensor(capi, cuda):
@@ -127,17 +131,20 @@ def test_one_row_of_a_wider_tensor(capi, cuda):
     assert torch.equal(got, want)
 
 
-def test_offsets_that_are_none(capi, cuda):
+@pytest.mark.parametrize("cta_pair", [1, 2])
+def test_offsets_that_are_none(capi, cuda, cta_pair):
     # cut to the matrix in the kernel: unspecified results, no access outside; nothing at all is written where none is left
     torch = cuda
     a, a_scales, b, b_scales = _operands(torch, capi, 40, 64, 128, 3, 0, 2)
     guard = torch.full((42, 64), 7.0, dtype=torch.bfloat16, device="cuda")
     c = guard[:40]
+    capi.set_option("cta_pair", cta_pair)
     for bad in ([-5, -3, -1, -1], [40, 40, 40, 2**31 - 1], [50, 60, 70, 80]):
         capi.mx_grouped_gemm(a, a_scales, b, b_scales, torch.tensor(bad, dtype=torch.int32, device="cuda"), out=c)
         assert bool((guard == 7).all())
     for bad in ([0, 10, 5, 20], [-(2**31), 2**31 - 1, 2**31 - 1, 2**31 - 1], [30, 10, 2**31 - 1, 5]):
         capi.mx_grouped_gemm(a, a_scales, b, b_scales, torch.tensor(bad, dtype=torch.int32, device="cuda"), out=c)
+    capi.set_option("cta_pair", 0)
     assert bool((guard[40:] == 7).all())
     assert capi.last_status()[0] == 0
 
