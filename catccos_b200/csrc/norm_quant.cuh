@@ -20,6 +20,7 @@ constexpr uint32_t kNormColsPerWarp = 512;   // 32 lanes x 16 elements
 constexpr uint32_t kNormMaxWarps = 16;       // of one row
 constexpr uint32_t kNormMaxPasses = 4;
 constexpr uint32_t kNormMaxCols = kNormColsPerWarp * kNormMaxWarps * kNormMaxPasses;
+constexpr float kNormMinEps = 1e-30f;  // squares that fp32 holds as denormals do not count beside it
 
 struct NormQuantParams {
     const uint8_t* x;          // bf16 [rows, n]
@@ -71,6 +72,29 @@ __device__ __forceinline__ void store_half_block(void* p, const uint32_t (&v)[8]
     }
 }
 
+// The sum over the lanes of the warps that share a row, the same on all of them.
+__device__ __forceinline__ float row_sum(float sum, float* partial, uint32_t warps_per_row)
+{
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (uint32_t d = 16; d > 0; d >>= 1) {
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    }
+    if (warps_per_row > 1u) {
+        if (lane == 0) {
+            partial[warp] = sum;
+        }
+        __syncthreads();
+        sum = lane < warps_per_row ? partial[lane] : 0.0f;
+#pragma unroll
+        for (uint32_t d = 8; d > 0; d >>= 1) {
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        }
+        sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+    }
+    return sum;
+}
+
 // kPasses passes of warps_per_row x 512 columns cover a row; blockDim.x = 32 * warps_per_row * rows_per_cta.  With several rows
 // to a CTA each has one warp (rows_per_cta > 1 only then), and nothing crosses warps.
 template <uint32_t kPasses, bool kE5m2>
@@ -117,23 +141,24 @@ __global__ void __launch_bounds__(32 * kNormMaxWarps) add_rms_norm_mx_quant_kern
             store_half_block(p.residual_out + at, h[i]);
         }
     }
+    sum = row_sum(sum, partial, warps_per_row);
+    float inv = 1.0f / sqrtf(fmaf(sum, p.inv_n, p.eps));
+    if (isinf(sum)) {  // |h| beyond 1e16; the same on all warps of a row, and a CTA with several warps to a row has one row
+        sum = 0.0f;
 #pragma unroll
-    for (uint32_t d = 16; d > 0; d >>= 1) {
-        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    }
-    if (warps_per_row > 1u) {
-        if (lane == 0) {
-            partial[warp] = sum;
-        }
-        __syncthreads();
-        sum = lane < warps_per_row ? partial[lane] : 0.0f;
+        for (uint32_t i = 0; i < kPasses; ++i) {
 #pragma unroll
-        for (uint32_t d = 8; d > 0; d >>= 1) {
-            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            for (uint32_t j = 0; j < 8; ++j) {
+                const float2 f = bf16x2_to_f32(h[i][j]);
+                sum = fmaf(f.x * 0x1p-72f, f.x * 0x1p-72f, fmaf(f.y * 0x1p-72f, f.y * 0x1p-72f, sum));
+            }
         }
-        sum = __shfl_sync(0xFFFFFFFFu, sum, 0);
+        if (warps_per_row > 1u) {
+            __syncthreads();  // all have read partial
+        }
+        sum = row_sum(sum, partial, warps_per_row);
+        inv = 0x1p-72f / sqrtf(sum * p.inv_n);  // eps is nothing beside it
     }
-    const float inv = 1.0f / sqrtf(fmaf(sum, p.inv_n, p.eps));
 
 #pragma unroll
     for (uint32_t i = 0; i < kPasses; ++i) {

@@ -115,6 +115,22 @@ def test_rows_of_zeros_and_values_that_are_not_finite(capi, cuda):
     _check(torch, x[5:], None, weight, codes[5:], scales[5:], None, norm[5:], 0)
 
 
+@pytest.mark.parametrize("n", [96, 512, 2080, 16416])
+def test_squares_beyond_fp32(capi, cuda, n):
+    # 1 / rms may be as small as 2^-128, which fp32 holds to 2^-22: 4 * 2^-24 more, 2.8e-6 in all
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x, residual = (torch.randn((5, n), generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2))
+    x[0], x[2], x[3] = x[0] * 2.0**60, x[2] * 2.0**64, x[3] * 2.0**125  # sums of squares around 2^128 and far beyond
+    x[4, 3], x[1, n - 1] = 3e38, -1e20  # one large value among ordinary ones
+    residual[3], residual[4, 3] = 1e30, 0.0
+    weight = (1 + 0.2 * torch.randn(n, generator=gen, device="cuda")).to(torch.bfloat16)
+    h, norm = torch.empty_like(x), torch.empty_like(x)
+    assert bool(torch.isfinite(x.float() + residual.float()).all())
+    codes, scales = capi.add_rms_norm_mx_quant(x, residual, weight, EPS, residual_out=h, norm_out=norm)
+    _check(torch, x, residual, weight, codes, scales, h, norm, 0)
+
+
 def test_tiny_blocks_of_the_device_rule(capi, cuda):
     torch = cuda
     n = 256
