@@ -2390,8 +2390,9 @@ int catccos_b200_add_rms_norm_mx_quant(void* stream, const void* x_bf16, const v
                                        float eps, uint32_t rows, uint32_t n, void* residual_out, void* norm_out, void* codes,
                                        void* scales)
 {
-    if (n == 0 || n % 32 != 0 || n > kNormMaxCols || !(eps > 0.0f) || std::isinf(eps)) {
-        ERROR_LOG("add_rms_norm_mx_quant: n must be a multiple of 32 up to %u, eps positive (got n=%u eps=%g)", kNormMaxCols, n, eps);
+    if (n == 0 || n % 32 != 0 || n > kNormMaxCols || !(eps >= kNormMinEps) || std::isinf(eps) || rows > 0x7FFFFFFFu) {
+        ERROR_LOG("add_rms_norm_mx_quant: n must be a multiple of 32 up to %u, eps finite and at least 1e-30, rows below 2^31 (got n=%u eps=%g rows=%u)",
+                  kNormMaxCols, n, eps, rows);
         return CATCCOS_B200_EINVAL;
     }
     if (g.a_dtype == 2) {
@@ -2407,6 +2408,26 @@ int catccos_b200_add_rms_norm_mx_quant(void* stream, const void* x_bf16, const v
     if (misaligned(x_bf16, 16) || misaligned(residual_bf16, 16) || misaligned(weight_bf16, 16) || misaligned(residual_out, 16) ||
         misaligned(norm_out, 16) || misaligned(codes, 16) || (n % 128 == 0 && misaligned(scales, 4))) {
         return CATCCOS_B200_EINVAL;  // 16 bytes at a time; the GEMMs read the scales of such rows as 32-bit words
+    }
+    // A value's thread reads x and the residual before it writes there, so whole tensors may coincide; nothing else may overlap.
+    const size_t values = (size_t)rows * n;
+    auto astray = [](const void* out, size_t out_bytes, const void* in, size_t in_bytes, bool may_coincide) {
+        return out != nullptr && in != nullptr && share_memory(out, out_bytes, in, in_bytes) && !(may_coincide && out == in);
+    };
+    bool overlap = astray(norm_out, 2 * values, residual_out, 2 * values, false) || astray(scales, values / 32, codes, values, false);
+    for (const void* in : {x_bf16, residual_bf16}) {
+        overlap = overlap || astray(residual_out, 2 * values, in, 2 * values, true) || astray(norm_out, 2 * values, in, 2 * values, true);
+    }
+    for (const void* in : {x_bf16, residual_bf16, (const void*)residual_out, (const void*)norm_out}) {
+        overlap = overlap || astray(codes, values, in, 2 * values, false) || astray(scales, values / 32, in, 2 * values, false);
+    }
+    for (const void* out : {residual_out, norm_out}) {
+        overlap = overlap || astray(out, 2 * values, weight_bf16, 2 * (size_t)n, false);
+    }
+    overlap = overlap || astray(codes, values, weight_bf16, 2 * (size_t)n, false) || astray(scales, values / 32, weight_bf16, 2 * (size_t)n, false);
+    if (overlap) {
+        ERROR_LOG("add_rms_norm_mx_quant: only residual_out and norm_out may be x or residual, and not the same one");
+        return CATCCOS_B200_EINVAL;
     }
     int rcode = ensure_init();
     if (rcode != 0) return rcode;
@@ -2448,6 +2469,13 @@ int catccos_b200_moe_route(void* stream, const void* logits, int logits_bf16, co
         misaligned(weights, 4) || (uint64_t)tokens * top_k > 0x7FFFFFFFull) {
         return CATCCOS_B200_EINVAL;
     }
+    const size_t route_bytes = 4 * (size_t)tokens * top_k, logit_bytes = (size_t)tokens * experts * (logits_bf16 ? 2 : 4);
+    if (share_memory(ids, route_bytes, weights, route_bytes) || share_memory(ids, route_bytes, logits, logit_bytes) ||
+        share_memory(weights, route_bytes, logits, logit_bytes) ||
+        (bias && (share_memory(ids, route_bytes, bias, 4 * (size_t)experts) || share_memory(weights, route_bytes, bias, 4 * (size_t)experts)))) {
+        ERROR_LOG("moe_route: ids or weights overlap what is read");
+        return CATCCOS_B200_EINVAL;
+    }
     int rcode = ensure_init();
     if (rcode != 0) return rcode;
     RouteParams p = {};
@@ -2479,6 +2507,12 @@ int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes,
     if ((routes != 0 && (!ids || !row_index)) || !offsets || misaligned(ids, 4) || misaligned(row_index, 4) || misaligned(offsets, 4)) {
         return CATCCOS_B200_EINVAL;
     }
+    const size_t route_bytes = 4 * (size_t)routes, offset_bytes = 4 * (size_t)experts + 4;
+    if (routes != 0 && ((row_index != ids && share_memory(row_index, route_bytes, ids, route_bytes)) ||
+                        share_memory(offsets, offset_bytes, ids, route_bytes) || share_memory(offsets, offset_bytes, row_index, route_bytes))) {
+        ERROR_LOG("moe_row_plan: row_index may be ids, and nothing else overlaps");  // a warp reads its routes before it writes them
+        return CATCCOS_B200_EINVAL;
+    }
     int rcode = ensure_init();
     if (rcode != 0) return rcode;
     RowPlanParams p = {};
@@ -2505,6 +2539,12 @@ int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows
     if ((rows != 0 && !expert_out) || !row_index || !weights || !out || misaligned(expert_out, 16) || misaligned(shared_out, 16) ||
         misaligned(out, 16) || misaligned(row_index, 4) || misaligned(weights, 4) || rows > 0x7FFFFFFFu) {
         return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    const size_t out_bytes = 2 * (size_t)tokens * n;
+    if (share_memory(out, out_bytes, expert_out, 2 * (size_t)rows * n) || (out != shared_out && shared_out && share_memory(out, out_bytes, shared_out, out_bytes)) ||
+        share_memory(out, out_bytes, row_index, 4 * (size_t)tokens * top_k) || share_memory(out, out_bytes, weights, 4 * (size_t)tokens * top_k)) {
+        ERROR_LOG("moe_combine: out may be shared_out, and overlaps nothing else");
+        return CATCCOS_B200_EINVAL;
     }
     CombineParams p = {};
     p.y = static_cast<const uint8_t*>(expert_out);
@@ -2557,6 +2597,12 @@ int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes
         a_scale_row_bytes % 4 != 0 || misaligned(a, 16) || misaligned(b, 16) || misaligned(c, 32) || misaligned(a_scale, 4) ||
         misaligned(b_scale, 2) || misaligned(offsets, 4)) {
         ERROR_LOG("mx grouped gemm: a, b and the rows of a 16-byte aligned, c 32-byte, the rows of a_scale 4-byte, b_scale 2-byte");
+        return CATCCOS_B200_EINVAL;
+    }
+    const size_t c_bytes = 2 * (size_t)rows * n, weights = (size_t)experts * k * n;
+    if (share_memory(c, c_bytes, a, (rows - 1) * a_row_bytes + k) || share_memory(c, c_bytes, a_scale, (rows - 1) * a_scale_row_bytes + k / 32) ||
+        share_memory(c, c_bytes, b, weights) || share_memory(c, c_bytes, b_scale, weights / 32) || share_memory(c, c_bytes, offsets, 4 * (size_t)experts + 4)) {
+        ERROR_LOG("mx grouped gemm: c overlaps an operand (a tile's rows of a are read while other tiles of them are stored)");
         return CATCCOS_B200_EINVAL;
     }
     int rcode = ensure_init();
@@ -2612,6 +2658,12 @@ int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, 
     }
     if (!x_bf16 || !w || !w_scale || !out || misaligned(x_bf16, 16) || misaligned(w, 16) || misaligned(w_scale, 16) ||
         misaligned(ids, 4) || misaligned(out, 4)) {
+        return CATCCOS_B200_EINVAL;
+    }
+    const size_t out_bytes = 2 * (size_t)rows * n, weights = (size_t)experts * k * n;
+    if (share_memory(out, out_bytes, x_bf16, 2 * (size_t)x_rows * k) || share_memory(out, out_bytes, w, weights / 2) ||
+        share_memory(out, out_bytes, w_scale, weights / 32) || (ids && share_memory(out, out_bytes, ids, 4 * (size_t)rows))) {
+        ERROR_LOG("mx_fp4_matvec: out overlaps an operand");
         return CATCCOS_B200_EINVAL;
     }
     int rcode = ensure_init();

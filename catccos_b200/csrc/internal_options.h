@@ -3,13 +3,13 @@
 // kernel variant through the same C ABI the operators use; a caller never needs them.
 #pragma once
 
-// 0 = automatic, 64, 128 or 256: width of the single-CTA GEMM tile
+// 0 = automatic, 64, 128 or 256: width of the single-CTA GEMM tile (of the grouped GEMM too)
 #define CATCCOS_B200_OPT_BLOCK_N "block_n"
 // bit 0 = launch the producer half, bit 1 = launch the consumer half (default 3).  The harness that hosts
 // several ranks on ONE GPU runs every rank's producer before any consumer, because kernels of different
 // ranks must not wait on one another while they share a device.
 #define CATCCOS_B200_OPT_PHASE_MASK "phase_mask"
-// 0 = automatic, 1 = always run the GEMM on CTA pairs (256 x 256 tiles, cta_group::2), 2 = never
+// 0 = automatic, 1 = always run the GEMM on CTA pairs (256 x 256 tiles, cta_group::2), 2 = never; the grouped GEMM too
 #define CATCCOS_B200_OPT_CTA_PAIR "cta_pair"
 // -1 = automatic (3 with one rank, 6 with several);
 // 0 = quantise and pusher warps inside the GEMM kernel (one launch); 3 = one rank only: quantise kernel, then GEMM

@@ -155,8 +155,8 @@ int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, cons
  * expanded_row_idx and the activations from its caller) ------------------------------------------------------------------
  * None of these calls allocates, keeps anything from one call to the next or shares a scratch with another: calls on
  * different streams may overlap, and calls may be captured in CUDA graphs and replayed.  They run on the current device;
- * `stream` is one of its streams.  Inputs and outputs must not overlap except where a comment says so.  An empty batch
- * (no rows, tokens or routes) is CATCCOS_B200_OK. */
+ * `stream` is one of its streams.  Outputs overlap neither inputs nor one another except where a comment says so (else
+ * CATCCOS_B200_EINVAL).  An empty batch (no rows, tokens or routes) is CATCCOS_B200_OK. */
 
 /* Residual addition, root-mean-square norm and MX quantiser: the activations that catccos_b200_mx_gemm and the
  * AllGather-Matmuls read, in one pass.  With h = bf16(x + residual) (or x, without a residual):
@@ -164,8 +164,8 @@ int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, cons
  * x, residual, residual_out, norm_out bf16 [rows, n]; weight bf16 [n]; codes uint8 [rows, n]; scales uint8 [rows, n/32].
  * y stays in fp32 up to the codes (catccos_b200_mx_quant of norm_out would round twice); element type and small blocks
  * follow the options "a_dtype" (0 or 1) and "tiny_block_rule", blocks with an infinity or NaN get 0xFF / 0x7F.
- * residual and residual_out are both NULL or both given, norm_out may be NULL.  residual_out may be residual or x, norm_out
- * may be x or (with another residual_out) residual.  n % 32 == 0, n <= 32768; eps > 0; everything 16-byte aligned, scales
+ * residual and residual_out are both NULL or both given, norm_out may be NULL.  residual_out and norm_out
+ * may be x or residual, not the same one.  n % 32 == 0, n <= 32768; eps >= 1e-30; everything 16-byte aligned, scales
  * 4-byte where n % 128 == 0. */
 int catccos_b200_add_rms_norm_mx_quant(void* stream, const void* x_bf16, const void* residual_bf16, const void* weight_bf16,
                                        float eps, uint32_t rows, uint32_t n, void* residual_out, void* norm_out, void* codes,
@@ -188,7 +188,7 @@ int catccos_b200_moe_route(void* stream, const void* logits, int logits_bf16, co
  *   row_index int32 [routes] = a route's row, -1 where its id is outside [first_expert, first_expert + experts): the
  *                              expanded_row_idx of catccos_b200_mx_quant_scatter_packed
  *   offsets int32 [experts + 1]: rows [offsets[e], offsets[e + 1]) belong to expert first_expert + e
- * 1 <= experts <= 1024, first_expert >= 0. */
+ * 1 <= experts <= 1024, first_expert >= 0; row_index may be ids. */
 int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes, uint32_t experts, int32_t first_expert,
                               int32_t* row_index, int32_t* offsets);
 

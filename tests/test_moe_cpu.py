@@ -18,8 +18,11 @@ def test_norm_refuses(capi):
         return L.catccos_b200_add_rms_norm_mx_quant(None, x, residual, weight, eps, rows, n, residual_out, norm_out, codes, scales)
 
     for bad in (dict(x=None), dict(weight=None), dict(codes=None), dict(scales=None), dict(residual=None), dict(residual_out=None),
-                dict(n=0), dict(n=48), dict(n=32800), dict(eps=0.0), dict(eps=float("nan")), dict(x=A + 8), dict(residual=B + 2),
-                dict(weight=C + 4), dict(residual_out=B + 8), dict(norm_out=F + 8), dict(codes=D + 8), dict(scales=E + 2)):
+                dict(n=0), dict(n=48), dict(n=32800), dict(rows=2**31), dict(eps=0.0), dict(eps=1e-31), dict(eps=float("nan")), dict(x=A + 8), dict(residual=B + 2),
+                dict(weight=C + 4), dict(residual_out=B + 8), dict(norm_out=F + 8), dict(codes=D + 8), dict(scales=E + 2),
+                # overlaps: one output in another, or in what is read, other than the whole of x or residual
+                dict(norm_out=B), dict(norm_out=B + 16), dict(residual_out=A + 32), dict(residual_out=B + 1024), dict(norm_out=A + 1024),
+                dict(codes=A), dict(codes=B + 16), dict(scales=D + 512), dict(scales=C), dict(residual_out=C), dict(codes=F, norm_out=F)):
         assert call(**bad) == -1, bad
     assert call(rows=0) == 0  # an empty batch needs no addresses and no device
 
@@ -36,7 +39,7 @@ def test_route_refuses(capi):
                 dict(ids=C + 1), dict(weights=D + 2), dict(experts=0), dict(experts=1025), dict(top_k=0), dict(top_k=33), dict(groups=0),
                 dict(groups=7), dict(groups=64), dict(groups=8, top_groups=9), dict(top_groups=0), dict(groups=32, top_groups=1),
                 dict(group_best=0), dict(group_best=3), dict(score=2), dict(score=-1), dict(bf16=2), dict(scale=float("inf")),
-                dict(tokens=2**31)):
+                dict(tokens=2**31), dict(ids=D), dict(weights=C + 32), dict(ids=A + 64), dict(weights=B)):
         assert call(**bad) == -1, bad
     assert call(tokens=0) == 0
 
@@ -48,7 +51,8 @@ def test_row_plan_refuses(capi):
         return L.catccos_b200_moe_row_plan(None, ids, routes, experts, first, index, offsets)
 
     for bad in (dict(ids=None), dict(index=None), dict(offsets=None), dict(ids=A + 2), dict(index=B + 1), dict(offsets=C + 2),
-                dict(experts=0), dict(experts=1025), dict(first=-1), dict(routes=2**31)):
+                dict(experts=0), dict(experts=1025), dict(first=-1), dict(routes=2**31), dict(index=A + 4),
+                dict(offsets=A), dict(offsets=B + 16)):
         assert call(**bad) == -1, bad
 
 
@@ -59,7 +63,8 @@ def test_combine_refuses(capi):
         return L.catccos_b200_moe_combine(None, y, rows, index, weights, shared, out, tokens, n, top_k, f16)
 
     for bad in (dict(y=None), dict(index=None), dict(weights=None), dict(out=None), dict(y=A + 8), dict(shared=D + 8), dict(out=E + 8),
-                dict(index=B + 2), dict(weights=C + 2), dict(n=0), dict(n=12), dict(top_k=0), dict(f16=2), dict(rows=2**31)):
+                dict(index=B + 2), dict(weights=C + 2), dict(n=0), dict(n=12), dict(top_k=0), dict(f16=2), dict(rows=2**31),
+                dict(out=A), dict(out=D + 16), dict(out=B), dict(shared=None, out=A + 512), dict(weights=E)):
         assert call(**bad) == -1, bad
     assert call(tokens=0) == 0
 
@@ -73,7 +78,8 @@ def test_grouped_gemm_refuses(capi):
     for bad in (dict(a=None), dict(a_scale=None), dict(b=None), dict(b_scale=None), dict(offsets=None), dict(c=None), dict(a=A + 8),
                 dict(a_scale=B + 2), dict(b=C + 8), dict(b_scale=D + 1), dict(offsets=E + 2), dict(c=F + 16), dict(step=127),
                 dict(step=136), dict(scale_step=3), dict(scale_step=6), dict(n=0), dict(n=24), dict(k=0), dict(k=64), dict(experts=0),
-                dict(experts=1025), dict(experts=1024, k=2**22, step=2**22), dict(rows=2**31)):
+                dict(experts=1025), dict(experts=1024, k=2**22, step=2**22), dict(rows=2**31), dict(c=A), dict(c=A + 1024 - 128),
+                dict(c=C + 128 * 128 - 32), dict(a_scale=F), dict(b_scale=F + 32), dict(offsets=F + 1020)):
         assert call(**bad) == -1, bad
     assert call(rows=0) == 0
     for option in (b"a_dtype", b"b_dtype"):
@@ -90,7 +96,8 @@ def test_matvec_refuses(capi):
 
     for bad in (dict(x=None), dict(w=None), dict(w_scale=None), dict(out=None), dict(x=A + 8), dict(w=B + 8), dict(w_scale=C + 8),
                 dict(ids=D + 2), dict(out=E + 2), dict(n=0), dict(n=24), dict(k=0), dict(k=96), dict(experts=0), dict(x_rows=0),
-                dict(x_rows=3), dict(rows=65536, x_rows=65536), dict(ids=None), dict(ids=None, experts=1)):
+                dict(x_rows=3), dict(rows=65536, x_rows=65536), dict(ids=None), dict(ids=None, experts=1),
+                dict(out=A), dict(out=B + 64), dict(w_scale=E), dict(ids=E + 64)):
         assert call(**bad) == -1, bad
     assert call(rows=0) == 0
 

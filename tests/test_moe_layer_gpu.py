@@ -60,7 +60,7 @@ def _products(torch, a, a_scales, w64, offsets):
     return want, size
 
 
-@pytest.mark.parametrize("tokens", [1, 37, 300])
+@pytest.mark.parametrize("tokens", [1, 37, 300, 5000])
 def test_layer(capi, cuda, tokens):
     torch = cuda
     layer = Layer(torch, capi, tokens)
@@ -88,9 +88,9 @@ def test_layer(capi, cuda, tokens):
     assert bool(((out.double() - want).abs() <= slack + 2.0**-8 * (want.abs() + slack)).all())
 
 
-def test_layer_in_a_graph(capi, cuda):
+@pytest.mark.parametrize("tokens", [40, 4400])  # one CTA and a cluster of sixteen for the plan; single CTAs and pairs for the products
+def test_layer_in_a_graph(capi, cuda, tokens):
     torch = cuda
-    tokens = 40
     layer = Layer(torch, capi, 1)
     gen = torch.Generator(device="cuda").manual_seed(2)
     inputs = [tuple(torch.randn((tokens, HIDDEN), generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2)) for _ in range(3)]

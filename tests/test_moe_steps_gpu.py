@@ -209,6 +209,16 @@ def test_rows_of_the_dispatch(capi, cuda, routes, experts, first):
         np.testing.assert_array_equal(offsets.cpu().numpy(), want_offsets)
 
 
+@pytest.mark.parametrize("routes", [100, 70001])
+def test_row_plan_in_place(capi, cuda, routes):
+    torch = cuda
+    ids = torch.randint(-1, 40, (routes,), generator=torch.Generator(device="cuda").manual_seed(routes), device="cuda", dtype=torch.int32)
+    index, offsets = capi.moe_row_plan(ids, 30, first_expert=3)
+    other = torch.empty_like(offsets)
+    code = capi.load().catccos_b200_moe_row_plan(torch.cuda.current_stream().cuda_stream, ids.data_ptr(), routes, 30, 3, ids.data_ptr(), other.data_ptr())
+    assert code == 0 and torch.equal(ids, index) and torch.equal(other, offsets)
+
+
 def test_row_plan_refusals(capi, cuda):
     torch = cuda
     ids = torch.zeros((4, 2), dtype=torch.int32, device="cuda")
