@@ -648,11 +648,18 @@ __global__ void __launch_bounds__(kPlanThreads, 1) moe_row_plan_kernel(const Row
         __syncwarp();
         cluster_sync_all();
         if (e < p.experts) {
-            for (uint32_t c = 0; c < ctas; ++c) {
-                uint32_t v;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_to_cta(smem_u32(totals + e), c)) : "memory");
-                before += c < cta ? v : 0u;
-                all += v;
+            uint32_t v[kPlanMaxCluster];
+#pragma unroll
+            for (uint32_t c = 0; c < kPlanMaxCluster; ++c) {
+                v[c] = 0u;
+                if (c < ctas) {
+                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v[c]) : "r"(map_to_cta(smem_u32(totals + e), c)) : "memory");
+                }
+            }
+#pragma unroll
+            for (uint32_t c = 0; c < kPlanMaxCluster; ++c) {
+                before += c < cta ? v[c] : 0u;
+                all += v[c];
             }
         }
     } else if (e < p.experts) {
