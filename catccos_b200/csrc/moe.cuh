@@ -138,8 +138,9 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
         a = larger(a, v);
     };
     if (p.group_in_lanes != 0u) {
+        a = c[0];
 #pragma unroll
-        for (uint32_t i = 0; i < kVpl; ++i) {
+        for (uint32_t i = 1; i < kVpl; ++i) {
             take(c[i]);
         }
     } else {
@@ -159,15 +160,20 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
     }
     for (uint32_t d = p.group_lanes / 2u; d > 0; d >>= 1) {
         const Real oa = __shfl_xor_sync(kAll, a, d), ob = __shfl_xor_sync(kAll, b, d);
-        take(oa);
-        b = larger(b, ob);
+        b = larger(larger(b, ob), smaller(a, oa));
+        a = larger(a, oa);
     }
     const Real score = p.group_best == 1u || b == none ? a : a + b;
+    // the lanes of a group share the comparisons with the others (a group of no expert is below all)
     uint32_t rank = 0;
-#pragma unroll 4
-    for (uint32_t o = 0; o < p.groups; ++o) {
-        const Real other = __shfl_sync(kAll, score, o << p.group_shift);
-        rank += o < mine ? (other >= score ? 1u : 0u) : (other > score ? 1u : 0u);
+#pragma unroll 2
+    for (uint32_t o0 = 0; o0 < p.groups; o0 += p.group_lanes) {
+        const uint32_t o = o0 + (lane & (p.group_lanes - 1u));
+        const Real other = __shfl_sync(kAll, score, (o << p.group_shift) & 31u);
+        rank += o < p.groups && (other > score || (other == score && o < mine)) ? 1u : 0u;
+    }
+    for (uint32_t d = p.group_lanes / 2u; d > 0; d >>= 1) {
+        rank += __shfl_xor_sync(kAll, rank, d);
     }
     const bool taken = mine < p.groups && rank < p.top_groups && score > none;
     if (p.group_in_lanes != 0u) {
@@ -265,6 +271,7 @@ __device__ __forceinline__ uint32_t gather_candidates(const RouteParams& p, cons
     }
     const uint32_t wanted = p.top_k + (slack > 0.0f ? 1u : 0u);
     uint32_t key = ordered_bits(best), bound = 0;
+#pragma unroll 4
     for (uint32_t r = 0; r < wanted; ++r) {
         bound = __reduce_max_sync(kAll, key);
         key = key == bound ? 0u : key;
@@ -287,13 +294,15 @@ __device__ __forceinline__ uint32_t gather_candidates(const RouteParams& p, cons
     if (lane - count < 4u) {
         found[lane] = 0ull;  // the ranking reads four at a time
     }
-    uint32_t at = end - mine;
     if (mine != 0u && end <= 32u) {
+        uint32_t at = smem_u32(s.sorted + (end - mine));
 #pragma unroll
         for (uint32_t i = 0; i < kVpl; ++i) {
-            if (c[i] >= least) {
-                s.sorted[at++] = make_float2(c[i], __uint_as_float(lane * kVpl + i));
-            }
+            // a branch around each store took as long as the rest of this
+            asm volatile("{.reg .pred take; setp.ge.f32 take, %1, %2; @take st.shared.v2.b32 [%0], {%1, %3}; @take add.u32 %0, %0, 8;}"
+                         : "+r"(at)
+                         : "f"(c[i]), "f"(least), "f"(__uint_as_float(lane * kVpl + i))
+                         : "memory");
         }
     }
     __syncwarp();
@@ -371,9 +380,9 @@ __device__ __noinline__ int32_t choose_in_64_bits(const RouteParams& p, size_t a
 // are chosen by the logits themselves; the others are computed with the fast exponential and inverse, and where two neighbours
 // of the order are closer than such values can tell apart (one token in some hundred), the dozen candidates are computed and
 // ordered in fp64, one a lane; where groups are that close, everything is.
-// Bound by instructions at large batches (16384 tokens, 256 experts, top_k 8: 11.5 us by the logits, 16.8 with sigmoid, bias and
+// Bound by instructions at large batches (16384 tokens, 256 experts, top_k 8: 11.5 us by the logits, 15.8 with sigmoid, bias and
 // 4 of 8 groups; one expert a round of warp-wide reductions, scores by expf and IEEE divisions and everything again in fp64
-// where they were close took 17.7 and 38.7), by the chain of warp-wide steps at small ones (16 tokens: 2.3 and 3.1 us).
+// where they were close took 17.7 and 38.7), by the chain of warp-wide steps at small ones (16 tokens: 2.1 and 2.7 us).
 template <uint32_t kVpl, typename LogitT>
 __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const RouteParams p)
 {
@@ -403,10 +412,6 @@ __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const Route
             l[i] = e0 + i < p.experts ? load_logit<LogitT>(p.logits, at + e0 + i) : none;
         }
     }
-#pragma unroll
-    for (uint32_t i = 0; i < kVpl; ++i) {
-        l[i] = fmaxf(l[i], none);  // NaN becomes minus infinity
-    }
     float m = 0.0f, sum = 1.0f;  // of the softmax; the sum where the weights need it
     if (p.sigmoid == 0u) {
         m = none;
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const Route
     if (by_logit) {
 #pragma unroll
         for (uint32_t i = 0; i < kVpl; ++i) {
-            c[i] = l[i];
+            c[i] = fmaxf(l[i], none);  // NaN becomes minus infinity
         }
         if (p.top_groups < p.groups) {
             keep_best_groups<kVpl, float, false>(p, c, reinterpret_cast<float*>(row), lane, 0.0f);
