@@ -150,7 +150,7 @@ enum class Mode { kNone, kProcess, kLocal };
 
 struct State {
     std::mutex mu;
-    Mode mode = Mode::kNone;
+    std::atomic<Mode> mode{Mode::kNone};
     int world = 1;
     int rank = 0;  // acting rank
     std::vector<RankCtx> ranks;
@@ -242,6 +242,10 @@ int ensure_init()
 {
     if (g.mode != Mode::kNone) {
         return 0;
+    }
+    std::lock_guard<std::mutex> lock(g.mu);
+    if (g.mode != Mode::kNone) {
+        return 0;  // another thread's first call was faster
     }
     int dev = 0;
     CUDA_TRY(cudaGetDevice(&dev));

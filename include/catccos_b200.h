@@ -154,8 +154,9 @@ int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, cons
 /* ---- the steps around the matmuls of a mixture-of-experts layer (one GPU; no counterpart in the reference, which takes
  * expanded_row_idx and the activations from its caller) ------------------------------------------------------------------
  * None of these calls allocates, keeps anything from one call to the next or shares a scratch with another: calls on
- * different streams may overlap, and calls may be captured in CUDA graphs and replayed.  They run on the current device;
- * `stream` is one of its streams.  Outputs overlap neither inputs nor one another except where a comment says so (else
+ * different streams may overlap, and calls may be captured in CUDA graphs and replayed (the process's first call of the
+ * library, where catccos_b200_init did not come before it, sets the library up and has to stay outside of a capture).
+ * They run on the current device; `stream` is one of its streams.  Outputs overlap neither inputs nor one another except where a comment says so (else
  * CATCCOS_B200_EINVAL).  An empty batch (no rows, tokens or routes) is CATCCOS_B200_OK. */
 
 /* Residual addition, root-mean-square norm and MX quantiser: the activations that catccos_b200_mx_gemm and the
@@ -218,7 +219,8 @@ int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows
  *   ids int32 [rows]: out[r] = x[r / (rows / x_rows)] x dequant(w[ids[r]]) with w [experts, k, n/2] and w_scale
  *     [experts, k/64, n, 2]: rows == tokens * top_k with one row of x a token, or one a route.  A row whose id is negative or
  *     not below experts is zero.
- * The weight is read once for every eight rows (with ids, for every row): meant for decoding, where that is all the work.
+ * A weight is read once for every eight rows, with ids for every four that share it: meant for decoding, where that is all
+ * the work.
  * k % 64 == 0, n % 16 == 0, rows <= 65535; x, w and w_scale 16-byte aligned, out 4-byte. */
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
                                uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k);

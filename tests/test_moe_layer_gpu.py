@@ -1,10 +1,15 @@
 """GPU test of the mixture-of-experts steps run together, as a layer uses them: norm, routing, rows of the dispatch, packed scatter,
 the experts' products, the combination; and a token's way through FP4 experts.  Every stage is checked against its definition in
 64 bits on what the stage before wrote; the whole is captured in a CUDA graph and replayed, and run on two streams at once."""
+import os
+import subprocess
+import sys
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HIDDEN, INNER, EXPERTS, TOP_K = 512, 256, 12, 4
 EPS = 1e-5
 
@@ -174,3 +179,37 @@ def test_tokens_through_fp4_experts(capi, cuda):
     for _ in range(3):
         graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(captured, (ids, gate_up, inner, y, weights, out)))
+
+
+FIRST_CALLS = """
+import threading, torch
+from catccos_b200 import capi
+capi.load()
+gen = torch.Generator(device="cuda").manual_seed(4)
+logits = torch.randn((500, 64), generator=gen, device="cuda")
+x = torch.randn((33, 256), generator=gen, device="cuda").to(torch.bfloat16)
+weight = torch.ones(256, dtype=torch.bfloat16, device="cuda")
+torch.cuda.synchronize()
+start, out = threading.Barrier(16), [None] * 16
+
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        out[i] = capi.moe_route(logits, 6) if i % 2 else capi.add_rms_norm_mx_quant(x, None, weight, 1e-6)
+        torch.cuda.current_stream().synchronize()
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(16)]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+for i in range(2, 16):
+    assert all(torch.equal(a, b) for a, b in zip(out[i], out[i % 2])), i
+print("first calls ok")
+"""
+
+
+def test_first_calls_of_several_threads(capi, cuda):
+    # a process of their own: the calls that set the library up
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "first calls ok" in run.stdout, run.stdout + run.stderr
