@@ -39,8 +39,10 @@ EXPORTS = [
     "catccos_b200_moe_route",
     "catccos_b200_moe_row_plan",
     "catccos_b200_mx_grouped_gemm",
+    "catccos_b200_mx_grouped_gemm_typed",
     "catccos_b200_moe_combine",
     "catccos_b200_mx_fp4_matvec",
+    "catccos_b200_mx_fp4_matvec_typed",
     "catccos_b200_mx_quant_matmul_static",
     "catccos_b200_mx_quant_matmul_static_status",
     "catccos_b200_last_status",
@@ -107,8 +109,10 @@ def load() -> ctypes.CDLL:
     L.catccos_b200_moe_route.argtypes = [vp, vp, i32, vp, u32, u32, u32, u32, u32, u32, i32, i32, f32, vp, vp]
     L.catccos_b200_moe_row_plan.argtypes = [vp, vp, u32, u32, i32, vp, vp]
     L.catccos_b200_mx_grouped_gemm.argtypes = [vp, vp, sz, vp, sz, vp, vp, vp, vp, u32, u32, u32, u32]
+    L.catccos_b200_mx_grouped_gemm_typed.argtypes = [*L.catccos_b200_mx_grouped_gemm.argtypes, i32, i32, i32]
     L.catccos_b200_moe_combine.argtypes = [vp, vp, u32, vp, vp, vp, vp, u32, u32, u32, i32]
     L.catccos_b200_mx_fp4_matvec.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32]
+    L.catccos_b200_mx_fp4_matvec_typed.argtypes = [*L.catccos_b200_mx_fp4_matvec.argtypes, i32]
     L.catccos_b200_mx_quant_matmul_static.argtypes = [vp, vp, vp, vp, vp, u32, u32, u32]
     L.catccos_b200_last_status.argtypes = [ctypes.POINTER(u32)]
     L.catccos_b200_mx_quant_matmul_static_status.argtypes = [ctypes.POINTER(u32)]
@@ -341,8 +345,10 @@ def mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out=None, out_dtype
     """c [rows, N]: rows offsets[e] .. offsets[e + 1] are dequant(a) x dequant(b[e]); b [experts, K, N], b_scales [experts, K/64, N, 2].
 
     a_codes [rows, K] and a_scales [rows, K/32] may be columns of a wider tensor (packed[:, :K] and packed[:, K:K + K // 32] of
-    mx_quant_scatter_packed).  Rows outside the offsets stay as they are (of a tensor allocated here: unset)."""
-    code, out = (_calls or _load_calls()).mx_grouped_gemm(a_codes, a_scales, b, b_scales, offsets, out, out_dtype)
+    mx_quant_scatter_packed).  Rows outside the offsets stay as they are (of a tensor allocated here: unset).  out's type, or
+    out_dtype (bf16 without either), is the result's; codes of a float8 type are of that type, codes in uint8 of the options'
+    "a_dtype" and "b_dtype"."""
+    code, out = (_calls or _load_calls()).mx_grouped_gemm_typed(a_codes, a_scales, b, b_scales, offsets, out, out_dtype)
     if code:
         raise CatccosError("catccos_b200_mx_grouped_gemm", code)
     return out
@@ -360,8 +366,9 @@ def mx_fp4_matvec(x_bf16, w, w_scales, ids=None, out=None, out_dtype=None):
     """x [rows, K] x dequant(w): w packed E2M1 [K, N/2], w_scales [K/64, N, 2] -> [rows, N].
 
     With ids int32 (any shape, i values): w [experts, K, N/2], w_scales [experts, K/64, N, 2] -> [i, N], row r with weight ids[r]
-    and x's row r // (i // rows); a negative id gives a row of zeros."""
-    code, out = (_calls or _load_calls()).mx_fp4_matvec(x_bf16, w, w_scales, ids, out, out_dtype)
+    and x's row r // (i // rows); a negative id gives a row of zeros.  out's type, or out_dtype (bf16 without either), is the
+    result's."""
+    code, out = (_calls or _load_calls()).mx_fp4_matvec_typed(x_bf16, w, w_scales, ids, out, out_dtype)
     if code:
         raise CatccosError("catccos_b200_mx_fp4_matvec", code)
     return out

@@ -1573,16 +1573,16 @@ int launch_matvec_inst(cudaStream_t st, const MatvecParams& p, uint32_t slabs, u
 }
 
 template <uint32_t kSets>
-int launch_matvec(cudaStream_t st, const MatvecParams& p, int num_sms)
+int launch_matvec(cudaStream_t st, const MatvecParams& p, bool f16, int num_sms)
 {
     const uint32_t slabs = (p.n + kMatvecCols - 1) / kMatvecCols;
     const uint32_t blocks = p.ids != nullptr ? p.rows : (p.rows + 4 * kSets - 1) / (4 * kSets);
     const uint32_t ctas = matvec_ctas((uint64_t)slabs * blocks, p.k / kMatvecUnit, 0.53125e-6 * p.n * p.k * (p.ids ? p.rows : 1), num_sms);
     // rows of whole 16-byte chunks, where they also begin on such
-    return p.n % 32 == 0 ? (g.c_dtype == 1 ? launch_matvec_inst<kSets, true, __half>(st, p, slabs, blocks, ctas)
-                                           : launch_matvec_inst<kSets, true, __nv_bfloat16>(st, p, slabs, blocks, ctas))
-                         : (g.c_dtype == 1 ? launch_matvec_inst<kSets, false, __half>(st, p, slabs, blocks, ctas)
-                                           : launch_matvec_inst<kSets, false, __nv_bfloat16>(st, p, slabs, blocks, ctas));
+    return p.n % 32 == 0 ? (f16 ? launch_matvec_inst<kSets, true, __half>(st, p, slabs, blocks, ctas)
+                                : launch_matvec_inst<kSets, true, __nv_bfloat16>(st, p, slabs, blocks, ctas))
+                         : (f16 ? launch_matvec_inst<kSets, false, __half>(st, p, slabs, blocks, ctas)
+                                : launch_matvec_inst<kSets, false, __nv_bfloat16>(st, p, slabs, blocks, ctas));
 }
 
 // A grouped launch's tiles: those that take least by a fit to 420 drawn calls (1 to 16384 rows of 1 to 64 unevenly chosen
@@ -1682,7 +1682,7 @@ int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_
 }
 
 template <uint32_t BLOCK_N>
-int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
+int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p, bool f16)
 {
     CUtensorMap maps[3];
     int rcode = grouped_maps(maps, a, a_row_bytes, b, p, GemmSmem<BLOCK_N>::kBRow);
@@ -1691,8 +1691,8 @@ int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_b
     const uint64_t tiles = p.rows / kGemmBlockM + std::min(p.rows, p.experts);
     const uint64_t units = tiles * ((p.N + BLOCK_N - 1) / BLOCK_N);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(units, (uint64_t)rc.num_sms);
-    return g.c_dtype == 1 ? launch_grouped_inst<BLOCK_N, __half>(grid, st, maps[0], maps[1], maps[2], p)
-                          : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, maps[0], maps[1], maps[2], p);
+    return f16 ? launch_grouped_inst<BLOCK_N, __half>(grid, st, maps[0], maps[1], maps[2], p)
+               : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, maps[0], maps[1], maps[2], p);
 }
 
 }  // namespace
@@ -2581,14 +2581,25 @@ int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes
                                  const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows, uint32_t experts,
                                  uint32_t n, uint32_t k)
 {
+    return catccos_b200_mx_grouped_gemm_typed(stream, a, a_row_bytes, a_scale, a_scale_row_bytes, b, b_scale, offsets, c, rows, experts, n, k,
+                                              -1, -1, -1);
+}
+
+int catccos_b200_mx_grouped_gemm_typed(void* stream, const void* a, size_t a_row_bytes, const void* a_scale, size_t a_scale_row_bytes,
+                                       const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows,
+                                       uint32_t experts, uint32_t n, uint32_t k, int a_type, int b_type, int c_type)
+{
+    a_type = a_type == -1 ? g.a_dtype : a_type;
+    b_type = b_type == -1 ? g.b_dtype : b_type;
+    c_type = c_type == -1 ? g.c_dtype : c_type;
     if (n == 0 || n % 16 != 0 || k == 0 || k % kGemmBlockK != 0 || experts == 0 || experts > kGroupedMaxExperts ||
         (uint64_t)experts * k > 0x7FFFFFFFull || rows > 0x7FFFFFFFu) {
         ERROR_LOG("mx grouped gemm needs K %% 128 == 0, N %% 16 == 0 and 1 to %u experts (got N=%u K=%u experts=%u)", kGroupedMaxExperts, n,
                   k, experts);
         return CATCCOS_B200_EINVAL;
     }
-    if (g.a_dtype == 2 || g.b_dtype == 2) {
-        ERROR_LOG("mx grouped gemm takes 8-bit operands: a_dtype and b_dtype 0 or 1");
+    if (a_type < 0 || a_type > 1 || b_type < 0 || b_type > 1 || c_type < 0 || c_type > 1) {
+        ERROR_LOG("mx grouped gemm takes 8-bit operands and gives 16-bit floats: types 0 or 1 (got %d, %d, %d)", a_type, b_type, c_type);
         return CATCCOS_B200_EINVAL;
     }
     if (rows == 0) {
@@ -2630,26 +2641,34 @@ int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes
     p.experts = experts;
     p.N = n;
     p.K = k;
-    p.a_fmt = g.a_dtype == 1 ? 1u : 0u;
-    p.b_fmt = g.b_dtype == 1 ? 1u : 0u;
+    p.a_fmt = (uint32_t)a_type;
+    p.b_fmt = (uint32_t)b_type;
     p.bar_timeout_ns = 2 * g.timeout_ns + 1000000000ull;
     p.status = rc.status;
     cudaStream_t st = (cudaStream_t)stream;
+    const bool f16 = c_type == 1;
     const GroupedPlan plan = plan_grouped(rc, rows, experts, n, k);
     if (plan.pair) {
-        return g.c_dtype == 1 ? launch_grouped_pair<__half>(rc, st, a, a_row_bytes, b, p)
-                              : launch_grouped_pair<__nv_bfloat16>(rc, st, a, a_row_bytes, b, p);
+        return f16 ? launch_grouped_pair<__half>(rc, st, a, a_row_bytes, b, p) : launch_grouped_pair<__nv_bfloat16>(rc, st, a, a_row_bytes, b, p);
     }
-    return plan.block_n == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p)
-                              : (plan.block_n == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p)
-                                                     : launch_grouped<256>(rc, st, a, a_row_bytes, b, p));
+    return plan.block_n == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p, f16)
+                              : (plan.block_n == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p, f16)
+                                                     : launch_grouped<256>(rc, st, a, a_row_bytes, b, p, f16));
 }
 
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
                                uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k)
 {
-    if (n == 0 || n % 16 != 0 || k == 0 || k % kMatvecUnit != 0 || experts == 0) {
-        ERROR_LOG("mx_fp4_matvec needs K %% 64 == 0, N %% 16 == 0 and a weight (got N=%u K=%u experts=%u)", n, k, experts);
+    return catccos_b200_mx_fp4_matvec_typed(stream, x_bf16, w, w_scale, ids, out, rows, x_rows, experts, n, k, -1);
+}
+
+int catccos_b200_mx_fp4_matvec_typed(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
+                                     uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k, int c_type)
+{
+    c_type = c_type == -1 ? g.c_dtype : c_type;
+    if (n == 0 || n % 16 != 0 || k == 0 || k % kMatvecUnit != 0 || experts == 0 || c_type < 0 || c_type > 1) {
+        ERROR_LOG("mx_fp4_matvec needs K %% 64 == 0, N %% 16 == 0, a weight and a 16-bit type (got N=%u K=%u experts=%u type=%d)", n, k, experts,
+                  c_type);
         return CATCCOS_B200_EINVAL;
     }
     if (rows == 0) {
@@ -2683,8 +2702,8 @@ int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, 
     p.k = k;
     p.experts = experts;
     p.rows_per_x = rows / x_rows;
-    return ids != nullptr || rows <= 4 ? launch_matvec<1>((cudaStream_t)stream, p, cur().num_sms)
-                                       : launch_matvec<2>((cudaStream_t)stream, p, cur().num_sms);
+    return ids != nullptr || rows <= 4 ? launch_matvec<1>((cudaStream_t)stream, p, c_type == 1, cur().num_sms)
+                                       : launch_matvec<2>((cudaStream_t)stream, p, c_type == 1, cur().num_sms);
 }
 
 int catccos_b200_last_status(uint32_t out[4])

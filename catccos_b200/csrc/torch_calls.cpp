@@ -33,9 +33,9 @@ BOUND(mxfp8_matmul_reduce_scatter);
 BOUND(add_rms_norm_mx_quant);
 BOUND(moe_route);
 BOUND(moe_row_plan);
-BOUND(mx_grouped_gemm);
+BOUND(mx_grouped_gemm_typed);
 BOUND(moe_combine);
-BOUND(mx_fp4_matvec);
+BOUND(mx_fp4_matvec_typed);
 BOUND(mx_quant_matmul_static);
 BOUND(mx_quant_allgather);
 BOUND(mx_quant_allgather_matmul);
@@ -308,6 +308,12 @@ at::ScalarType half_type(PyObject* dtype)
     return type;
 }
 
+// The type of 8-bit codes as the C ABI numbers it, where the tensor says it: bytes may be either, the option tells (-1).
+int code_type(const at::Tensor& t)
+{
+    return t.scalar_type() == at::kFloat8_e4m3fn ? 0 : (t.scalar_type() == at::kFloat8_e5m2 ? 1 : -1);
+}
+
 PyObject* with_output(PyObject* code, PyObject* given, const at::Tensor& made)
 {
     PyObject* out = PyTuple_New(2);
@@ -499,7 +505,7 @@ CALL(moe_row_plan, 3)
 END_CALL
 
 // a, a_scales, b, b_scales, offsets, out, out_dtype
-CALL(mx_grouped_gemm, 7)
+CALL(mx_grouped_gemm_typed, 7)
     const auto codes = {kU8, at::kFloat8_e4m3fn, at::kFloat8_e5m2};
     const at::Tensor& x = plain(a[0], "a_codes", "a CUDA matrix of 8-bit codes, its columns next to one another", codes, 2, nullptr, false);
     const at::Tensor& xs = plain(a[1], "a_scales", "a CUDA matrix of bytes on a_codes' device, its columns next to one another",
@@ -520,10 +526,12 @@ CALL(mx_grouped_gemm, 7)
     const at::Tensor out = result(a[5], "a contiguous bf16 or fp16 matrix [rows, N] on a_codes' device", {kBf16, kF16}, x, rows, n, half_type(a[6]));
     // one row has no distance to the next
     const size_t step = rows > 1 ? (size_t)x.stride(0) : (size_t)(k + 15) / 16 * 16, scale_step = rows > 1 ? (size_t)xs.stride(0) : (size_t)(k / 32 + 3) / 4 * 4;
+    const int a_type = code_type(x), b_type = code_type(b), c_type = out.scalar_type() == kF16 ? 1 : 0;
     void *ac = x.data_ptr(), *as = xs.data_ptr(), *bc = b.data_ptr(), *bf = bs.data_ptr(), *o = offsets.data_ptr(), *c = out.data_ptr();
     return with_output(released([&] {
-                           return mx_grouped_gemm_fn(on.stream, ac, step, as, scale_step, bc, bf, (const int32_t*)o, c, (uint32_t)rows,
-                                                     (uint32_t)experts, (uint32_t)n, (uint32_t)k);
+                           return mx_grouped_gemm_typed_fn(on.stream, ac, step, as, scale_step, bc, bf, (const int32_t*)o, c,
+                                                           (uint32_t)rows, (uint32_t)experts, (uint32_t)n, (uint32_t)k, a_type, b_type,
+                                                           c_type);
                        }),
                        a[5], out);
 END_CALL
@@ -554,7 +562,7 @@ CALL(moe_combine, 5)
 END_CALL
 
 // x, w, w_scales, ids, out, out_dtype
-CALL(mx_fp4_matvec, 6)
+CALL(mx_fp4_matvec_typed, 6)
     const bool many = a[3] != Py_None;
     const at::Tensor& x = plain(a[0], "x", "a contiguous bf16 CUDA matrix", {kBf16}, 2);
     const at::Tensor& w = plain(a[1], "w", "contiguous packed codes [K, N / 2], with ids [experts, K, N / 2], on x's device", {kU8}, many ? 3 : 2, &x);
@@ -568,10 +576,11 @@ CALL(mx_fp4_matvec, 6)
     }
     const OnDevice on(x);
     const at::Tensor out = result(a[4], "a contiguous bf16 or fp16 matrix [rows or ids, N] on x's device", {kBf16, kF16}, x, rows, n, half_type(a[5]));
+    const int c_type = out.scalar_type() == kF16 ? 1 : 0;
     void *in = x.data_ptr(), *wp = w.data_ptr(), *sp = ws.data_ptr(), *i = data_or_null(a[3]), *o = out.data_ptr();
     return with_output(released([&] {
-                           return mx_fp4_matvec_fn(on.stream, in, wp, sp, (const int32_t*)i, o, (uint32_t)rows, (uint32_t)x_rows,
-                                                   (uint32_t)experts, (uint32_t)n, (uint32_t)k);
+                           return mx_fp4_matvec_typed_fn(on.stream, in, wp, sp, (const int32_t*)i, o, (uint32_t)rows, (uint32_t)x_rows,
+                                                         (uint32_t)experts, (uint32_t)n, (uint32_t)k, c_type);
                        }),
                        a[4], out);
 END_CALL
@@ -598,9 +607,9 @@ PyObject* bind(PyObject*, PyObject* args)
     BIND(add_rms_norm_mx_quant)
     BIND(moe_route)
     BIND(moe_row_plan)
-    BIND(mx_grouped_gemm)
+    BIND(mx_grouped_gemm_typed)
     BIND(moe_combine)
-    BIND(mx_fp4_matvec)
+    BIND(mx_fp4_matvec_typed)
     BIND(mx_quant_matmul_static)
     BIND(mx_quant_allgather)
     BIND(mx_quant_allgather_matmul)
@@ -621,9 +630,9 @@ PyMethodDef methods[] = {
     METHOD(add_rms_norm_mx_quant),
     METHOD(moe_route),
     METHOD(moe_row_plan),
-    METHOD(mx_grouped_gemm),
+    METHOD(mx_grouped_gemm_typed),
     METHOD(moe_combine),
-    METHOD(mx_fp4_matvec),
+    METHOD(mx_fp4_matvec_typed),
     METHOD(mx_quant_matmul_static),
     METHOD(mx_quant_allgather),
     METHOD(mx_quant_allgather_matmul),

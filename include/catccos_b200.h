@@ -206,6 +206,12 @@ int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes
                                  const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows, uint32_t experts,
                                  uint32_t n, uint32_t k);
 
+/* The same with the call's own element types, numbered as in the options "a_dtype", "b_dtype" and "c_dtype"; -1 takes the
+ * option.  capi.mx_grouped_gemm comes this way with its tensors' types: the options are the process's, a tensor's type is not. */
+int catccos_b200_mx_grouped_gemm_typed(void* stream, const void* a, size_t a_row_bytes, const void* a_scale, size_t a_scale_row_bytes,
+                                       const void* b, const void* b_scale, const int32_t* offsets, void* c, uint32_t rows,
+                                       uint32_t experts, uint32_t n, uint32_t k, int a_type, int b_type, int c_type);
+
 /* The end of the layer: out[t] = sum over r of weights[t, r] * expert_out[row_index[t, r]] (+ shared_out[t]), r ascending, in
  * fp32, rounded once.  expert_out [rows, n], shared_out (or NULL) and out [tokens, n]: bf16 (f16 0) or fp16 (f16 1); row_index
  * int32 and weights fp32 [tokens, top_k].  A route whose row is negative or not below rows adds nothing.  out may be
@@ -224,6 +230,10 @@ int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows
  * k % 64 == 0, n % 16 == 0, rows <= 65535; x, w and w_scale 16-byte aligned, out 4-byte. */
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
                                uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k);
+
+/* The same with the call's own type of out: 0 bf16, 1 fp16, -1 as the option "c_dtype" says. */
+int catccos_b200_mx_fp4_matvec_typed(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
+                                     uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k, int c_type);
 
 /* Quantise + matmul on one GPU that allocates nothing.  It has no counterpart in the reference.
  * c [m, n] = dequant(quantise(a_bf16 [m, k])) x dequant(b [k, n], b_scale [k/64, n, 2]): the same two

@@ -102,6 +102,27 @@ def test_matvec_refuses(capi):
     assert call(rows=0) == 0
 
 
+def test_typed_calls_refuse(capi):
+    L = capi.load()
+
+    def grouped(types, rows=8):
+        return L.catccos_b200_mx_grouped_gemm_typed(None, A, 128, B, 4, C, D, E, F, rows, 2, 64, 128, *types)
+
+    def matvec(c_type, rows=8):
+        return L.catccos_b200_mx_fp4_matvec_typed(None, A, B, C, D, E, rows, rows // 2, 2, 64, 128, c_type)
+
+    for bad in ((2, 0, 0), (-2, 0, 0), (0, 2, 0), (0, 0, 2), (0, 0, -2)):
+        assert grouped(bad) == -1, bad
+    assert matvec(2) == -1 and matvec(-2) == -1
+    for types in ((0, 1, 0), (1, 0, 1), (-1, -1, -1)):
+        assert grouped(types, rows=0) == 0
+    assert matvec(1, rows=0) == 0 and matvec(-1, rows=0) == 0
+    for option in (b"a_dtype", b"b_dtype"):  # an option counts only where the call leaves its type to it
+        L.catccos_b200_set_option(option, 2)
+        assert grouped((-1, -1, -1), rows=0) == -1 and grouped((0, 0, 0), rows=0) == 0
+        L.catccos_b200_set_option(option, 0)
+
+
 @pytest.mark.skipif(shutil.which("nvcc") is None, reason="needs nvcc")
 def test_rows_of_an_expert_stay_inside_the_matrix(tmp_path):
     exe = tmp_path / "grouped_rows_selftest"
