@@ -19,6 +19,7 @@
 #include "internal_options.h"
 #include "common.cuh"
 #include "fp4_matvec.cuh"
+#include "map_cache.hpp"
 #include "moe.cuh"
 #include "mx_gemm.cuh"
 #include "mx_gemm_pair.cuh"
@@ -443,30 +444,6 @@ int launch_quant_push_ordered(RankCtx& rc, cudaStream_t st, QuantPushParams& p, 
     return 0;
 }
 
-// Tensor maps depend on (address, extents, box) only; a decode loop calls with the same few buffers over and
-// over, and an encode costs about as much as the launch it precedes.  A small most-recently-used table keeps the
-// last maps (calls of one process are serialised by its callers: one host thread per rank).
-struct MapKey {
-    const void* base;
-    uint64_t inner, outer;
-    uint32_t box_inner, box_outer;
-    bool fp4;
-    uint32_t elem;
-    uint64_t pitch;
-    bool operator==(const MapKey& o) const
-    {
-        return base == o.base && inner == o.inner && outer == o.outer && box_inner == o.box_inner &&
-               box_outer == o.box_outer && fp4 == o.fp4 && elem == o.elem && pitch == o.pitch;
-    }
-};
-constexpr int kMapCacheSize = 16;
-struct MapCache {
-    MapKey key[kMapCacheSize] = {};
-    CUtensorMap map[kMapCacheSize];
-    uint64_t used[kMapCacheSize] = {};
-    uint64_t clock = 0;
-} g_maps;
-
 int encode_map_2d_uncached(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,
                            uint32_t box_outer, bool fp4, uint32_t elem, uint64_t pitch);
 
@@ -476,24 +453,9 @@ int encode_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t o
                   uint32_t box_outer, bool fp4 = false, uint32_t elem = 1, uint64_t pitch = 0)
 {
     const MapKey k{base, inner, outer, box_inner, box_outer, fp4, elem, pitch};
-    int victim = 0;
-    for (int i = 0; i < kMapCacheSize; ++i) {
-        if (g_maps.used[i] != 0 && g_maps.key[i] == k) {
-            g_maps.used[i] = ++g_maps.clock;
-            *map = g_maps.map[i];
-            return 0;
-        }
-        if (g_maps.used[i] < g_maps.used[victim]) {
-            victim = i;
-        }
-    }
-    int rc = encode_map_2d_uncached(map, base, inner, outer, box_inner, box_outer, fp4, elem, pitch);
-    if (rc == 0) {
-        g_maps.key[victim] = k;
-        g_maps.map[victim] = *map;
-        g_maps.used[victim] = ++g_maps.clock;
-    }
-    return rc;
+    return thread_maps<CUtensorMap>().get(k, map, [&](CUtensorMap* made) {
+        return encode_map_2d_uncached(made, base, inner, outer, box_inner, box_outer, fp4, elem, pitch);
+    });
 }
 
 int encode_map_2d_uncached(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_inner,

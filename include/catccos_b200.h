@@ -153,9 +153,11 @@ int catccos_b200_mx_quant_scatter_packed(void* stream, const void* in_bf16, cons
 
 /* ---- the steps around the matmuls of a mixture-of-experts layer (one GPU; no counterpart in the reference, which takes
  * expanded_row_idx and the activations from its caller) ------------------------------------------------------------------
- * None of these calls allocates, keeps anything from one call to the next or shares a scratch with another: calls on
- * different streams may overlap, and calls may be captured in CUDA graphs and replayed (the process's first call of the
- * library, where catccos_b200_init did not come before it, sets the library up and has to stay outside of a capture).
+ * None of these calls allocates device memory, keeps data from one call to the next or shares a scratch with another (a host thread
+ * keeps the tensor maps of its last operands, which depend on addresses and sizes alone): calls on different streams may
+ * overlap, several host threads may call at once (not beside set_option, init or finalize), and calls may be captured in CUDA
+ * graphs and replayed (the process's first call of the library, where catccos_b200_init did not come before it, sets the
+ * library up and has to stay outside of a capture).
  * They run on the current device; `stream` is one of its streams.  Outputs overlap neither inputs nor one another except where a comment says so (else
  * CATCCOS_B200_EINVAL).  An empty batch (no rows, tokens or routes) is CATCCOS_B200_OK. */
 

@@ -3,6 +3,8 @@ bit, against the single-CTA GEMM on the expert's operands (the same tile, the sa
 
 Against 64 bits a result may be off by K * 2^-23 of the sum of its products' magnitudes (K steps of an fp32 accumulator that
 truncates) and half a step of its type."""
+import threading
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -147,6 +149,39 @@ def test_offsets_that_are_none(capi, cuda, cta_pair):
     capi.set_option("cta_pair", 0)
     assert bool((guard[40:] == 7).all())
     assert capi.last_status()[0] == 0
+
+
+def test_calls_of_several_threads(capi, cuda):
+    # more operands than a table of tensor maps holds, other ones in every thread; each result as one thread alone gets it
+    torch = cuda
+    threads, sets, rounds = 8, 8, 40
+    work = []
+    for t in range(threads):
+        for i in range(sets):
+            rows, n, k = 33 + 40 * i + t, 64 + 16 * t, 128 * (1 + (i + t) % 3)
+            a, a_scales, b, b_scales = _operands(torch, capi, rows, n, k, 2, 0, t * sets + i)
+            offsets = torch.tensor([0, rows // 3, rows], dtype=torch.int32, device="cuda")
+            operands = (a, a_scales, b, b_scales, offsets)
+            work.append((operands, capi.mx_grouped_gemm(*operands)))
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(threads), [None] * threads
+
+    def run(t):
+        stream, bad = torch.cuda.Stream(), 0
+        with torch.cuda.stream(stream):
+            start.wait()
+            for r in range(rounds):
+                got = [capi.mx_grouped_gemm(*operands) for operands, _ in work[t * sets : (t + 1) * sets]]
+                bad += sum(not torch.equal(g, want) for g, (_, want) in zip(got, work[t * sets : (t + 1) * sets]))
+            stream.synchronize()
+        wrong[t] = bad
+
+    running = [threading.Thread(target=run, args=(t,)) for t in range(threads)]
+    for thread in running:
+        thread.start()
+    for thread in running:
+        thread.join()
+    assert wrong == [0] * threads and capi.last_status()[0] == 0
 
 
 def test_refusals(capi, cuda):
