@@ -28,6 +28,7 @@
 #include "mx_grouped_pair.cuh"
 #include "mx_quant.cuh"
 #include "norm_quant.cuh"
+#include "per_device.hpp"
 
 using namespace catccos;
 
@@ -72,7 +73,8 @@ struct Driver {
     decltype(&cuMemSetAccess) MemSetAccess = nullptr;
     decltype(&cuMemGetAllocationGranularity) MemGetGranularity = nullptr;
     decltype(&cuTensorMapEncodeTiled) TensorMapEncodeTiled = nullptr;
-    bool ok = false;
+    std::mutex mu;
+    std::atomic<bool> ok{false};  // every pointer above is there
 
     template <typename F>
     bool Get(const char* name, F& fn)
@@ -92,6 +94,7 @@ struct Driver {
         if (ok) {
             return true;
         }
+        std::lock_guard<std::mutex> lock(mu);
         ok = Get("cuMemCreate", MemCreate) && Get("cuMemRelease", MemRelease) &&
              Get("cuMemExportToShareableHandle", MemExport) && Get("cuMemImportFromShareableHandle", MemImport) &&
              Get("cuMemAddressReserve", MemAddressReserve) && Get("cuMemAddressFree", MemAddressFree) &&
@@ -1390,16 +1393,16 @@ cudaError_t launch_clusters_after(void (*kern)(KArgs...), dim3 grid, uint32_t cl
 
 // Kernels with more than 48 KB of shared memory say so once per device.
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kern, size_t bytes, bool (&done)[kMaxRanks * 2])
+cudaError_t allow_smem(Kernel kern, size_t bytes, PerDevice<bool, kMaxRanks * 2>& done)
 {
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
-    if (err != cudaSuccess || (dev < kMaxRanks * 2 && done[dev])) {
+    if (err != cudaSuccess || done.get(dev)) {
         return err;
     }
     err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (err == cudaSuccess && dev < kMaxRanks * 2) {
-        done[dev] = true;
+    if (err == cudaSuccess) {
+        done.set(dev, true);
     }
     return err;
 }
@@ -1464,10 +1467,10 @@ int launch_row_plan(cudaStream_t st, RowPlanParams p)
 {
     auto kern = moe_row_plan_kernel<kBits>;
     // clusters of sixteen are more than every device promises: asked once for each
-    static uint32_t most[kMaxRanks * 2] = {};
+    static PerDevice<uint32_t, kMaxRanks * 2> most;
     int dev = 0;
     CUDA_TRY(cudaGetDevice(&dev));
-    uint32_t limit = dev < kMaxRanks * 2 ? most[dev] : 0;
+    uint32_t limit = most.get(dev);
     if (limit == 0) {
         const size_t smem = row_plan_smem(kPlanMaxExperts);
         CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -1487,9 +1490,7 @@ int launch_row_plan(cudaStream_t st, RowPlanParams p)
             limit = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg) == cudaSuccess && clusters >= 1 ? kPlanMaxCluster : 8;
         }
         cudaGetLastError();
-        if (dev < kMaxRanks * 2) {
-            most[dev] = limit;
-        }
+        most.set(dev, limit);
     }
     const uint32_t ctas = plan_ctas(p.routes, limit);
     const uint64_t threads = (uint64_t)ctas * kPlanThreads;
@@ -1527,7 +1528,7 @@ uint32_t matvec_ctas(uint64_t blocks, uint32_t steps, double megabytes, int num_
 template <uint32_t kSets, bool kWhole, typename OutT>
 int launch_matvec_inst(cudaStream_t st, const MatvecParams& p, uint32_t slabs, uint32_t blocks, uint32_t ctas)
 {
-    static bool done[kMaxRanks * 2] = {};
+    static PerDevice<bool, kMaxRanks * 2> done;
     CUDA_TRY(allow_smem(fp4_matvec_kernel<kSets, kWhole, OutT>, kMatvecSmem<kSets>, done));
     CUDA_TRY(launch_clusters_after(fp4_matvec_kernel<kSets, kWhole, OutT>, dim3(slabs * ctas, blocks), ctas, kMatvecThreads,
                                    kMatvecSmem<kSets>, st, p));
@@ -1590,7 +1591,7 @@ template <uint32_t BLOCK_N, typename OutT>
 int launch_grouped_inst(uint32_t grid, cudaStream_t st, const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb,
                         const GroupedParams& p)
 {
-    static bool done[kMaxRanks * 2] = {};
+    static PerDevice<bool, kMaxRanks * 2> done;
     CUDA_TRY(allow_smem(mx_grouped_gemm_kernel<BLOCK_N, OutT>, GroupedSmem<BLOCK_N>::dynamic_bytes(kGroupedMaxExperts), done));
     CUDA_TRY(launch_after(mx_grouped_gemm_kernel<BLOCK_N, OutT>, dim3(grid), kGemmThreads, GroupedSmem<BLOCK_N>::dynamic_bytes(p.experts),
                           st, ta, ta32, tb, p));
@@ -1610,10 +1611,10 @@ template <typename OutT>
 int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
 {
     auto kern = mx_grouped_pair_kernel<OutT>;
-    static int resident[kMaxRanks * 2] = {};
+    static PerDevice<int, kMaxRanks * 2> resident;
     int dev = 0;
     CUDA_TRY(cudaGetDevice(&dev));
-    int pairs = dev < kMaxRanks * 2 ? resident[dev] : 0;
+    int pairs = resident.get(dev);
     if (pairs == 0) {
         CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairSmem::kDynamicBytes));
         cudaLaunchConfig_t cfg = {};
@@ -1630,9 +1631,7 @@ int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_
             cudaGetLastError();
             pairs = rc.num_sms / 2;
         }
-        if (dev < kMaxRanks * 2) {
-            resident[dev] = pairs;
-        }
+        resident.set(dev, pairs);
     }
     CUtensorMap maps[3];
     int rcode = grouped_maps(maps, a, a_row_bytes, b, p, kGemmBlockM);
