@@ -122,10 +122,19 @@ __device__ __forceinline__ float fast_inverse(float x)
     return y;
 }
 
+// Keys that order like the floats (minus zero and zero are one value).
+__device__ __forceinline__ uint32_t ordered_bits(float v)
+{
+    const uint32_t bits = __float_as_uint(v + 0.0f);
+    return (bits >> 31) != 0u ? ~bits : bits | 0x80000000u;
+}
+
+__device__ __forceinline__ float from_ordered_bits(uint32_t key) { return __uint_as_float((key >> 31) != 0u ? key & 0x7FFFFFFFu : ~key); }
+
 // Which of this lane's experts are in the top_groups best groups.  c[i] is the choice value of expert lane * kVpl + i, minus
 // infinity where it may not be chosen; the others are set to that.  `row`: experts values of this warp's shared memory, used
-// where groups are not whole lanes.  Returns false where kSlack and the border between the last group taken and the first left
-// out is closer than the values' errors.
+// where groups are not whole lanes.  Returns false where kSlack and a group that is left out may belong above one that is taken:
+// a score is off by the errors of its summands, which go by their own sizes (they may cancel), so every group has its own reach.
 template <uint32_t kVpl, typename Real, bool kSlack>
 __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)[kVpl], Real* row, uint32_t lane, float slack)
 {
@@ -163,7 +172,8 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
         b = larger(larger(b, ob), smaller(a, oa));
         a = larger(a, oa);
     }
-    const Real score = p.group_best == 1u || b == none ? a : a + b;
+    const bool two = p.group_best != 1u && b != none;
+    const Real score = two ? a + b : a;
     // the lanes of a group share the comparisons with the others (a group of no expert is below all)
     uint32_t rank = 0;
 #pragma unroll 2
@@ -192,21 +202,13 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
     if (!kSlack) {
         return true;
     }
-    // ranks are distinct: the last group taken and the first one left out
-    const uint32_t last = __ballot_sync(kAll, mine < p.groups && rank + 1u == p.top_groups);
-    const uint32_t first = __ballot_sync(kAll, mine < p.groups && rank == p.top_groups);
-    const float vl = __shfl_sync(kAll, (float)score, __ffs((int)last) - 1), vf = __shfl_sync(kAll, (float)score, __ffs((int)first) - 1);
-    return vf == minus_infinity<float>() || apart(vl * 0.5f, vf * 0.5f, slack);  // the error of a sum of two is twice as large
+    // Half of apart()'s slack for each of two groups, which covers two values there and four here: 84 or 11.7 units of 2^-23 against
+    // 42 or 10.8, and 5.9 units of the values' sizes against one (their additions and the sum).  Infinite sizes tell nothing apart.
+    const float reach = slack * (1.0f + (float)(two ? fabs(a) + fabs(b) : fabs(a)));
+    const uint32_t least = taken ? ordered_bits(fmaxf((float)score - reach, -3.402823466e38f)) : 0xFFFFFFFFu;
+    const uint32_t most = mine < p.groups && !taken && score > none ? ordered_bits(fminf((float)score + reach, 3.402823466e38f)) : 0u;
+    return __reduce_min_sync(kAll, least) > __reduce_max_sync(kAll, most);
 }
-
-// Keys that order like the floats (minus zero and zero are one value).
-__device__ __forceinline__ uint32_t ordered_bits(float v)
-{
-    const uint32_t bits = __float_as_uint(v + 0.0f);
-    return (bits >> 31) != 0u ? ~bits : bits | 0x80000000u;
-}
-
-__device__ __forceinline__ float from_ordered_bits(uint32_t key) { return __uint_as_float((key >> 31) != 0u ? key & 0x7FFFFFFFu : ~key); }
 
 // The top_k experts by value, descending, ties to the lower index: lane r gets the r-th (-1: none left).  One expert a round;
 // this is the way of 64-bit values, and of logits of which too many are near the border for gather_candidates().

@@ -148,6 +148,55 @@ def test_masked_experts(capi, cuda, score, with_bias, groups, top_groups, group_
     _check_route(capi, torch, logits, bias, 6, score, groups, top_groups, group_best, renormalize)
 
 
+def _choice(logits, bias, top_k, score, groups, top_groups):
+    """ids by the two best of each group, for finite logits and biases, in 64 bits; and how far apart the groups at the border are."""
+    l, b = logits.astype(np.float64), bias.astype(np.float64)
+    e = np.exp(l - l.max(1, keepdims=True))
+    choice = (e / e.sum(1, keepdims=True) if score == "softmax" else 1.0 / (1.0 + np.exp(-l))) + b
+    tokens, experts = l.shape
+    best = np.sort(choice.reshape(tokens, groups, -1), axis=2)[:, :, -2:].sum(axis=2)
+    order = np.argsort(-best, axis=1, kind="stable")
+    open_ = np.zeros((tokens, groups), bool)
+    np.put_along_axis(open_, order[:, :top_groups], True, 1)
+    choice[~np.repeat(open_, experts // groups, axis=1)] = -np.inf
+    ranked = np.take_along_axis(best, order, 1)
+    return np.argsort(-choice, axis=1, kind="stable")[:, :top_k].astype(np.int32), ranked[:, top_groups - 1] - ranked[:, top_groups]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("experts,groups,top_groups", [(32, 4, 2), (40, 5, 3)])  # whole lanes, and not
+@pytest.mark.parametrize("size", [64.0, 1000.0, 10000.0])
+def test_group_sums_that_cancel(capi, cuda, score, experts, groups, top_groups, size):
+    # one expert a group far up, the others far down: a group's two best add up to far less than either, whose rounding stays
+    torch = cuda
+    rng = np.random.default_rng(int(size) + experts)
+    logits = (0.2 + 1e-3 * rng.standard_normal((4096, experts))).astype(np.float32)
+    bias = np.full(experts, -size, np.float32)
+    bias[:: experts // groups] = size
+    want, apart = _choice(logits, bias, top_groups, score, groups, top_groups)
+    keep = apart > 64 * size * 2.0**-52  # where 64 bits themselves decide
+    assert keep.mean() > 0.99
+    ids, _ = capi.moe_route(torch.from_numpy(logits).cuda(), top_groups, bias=torch.from_numpy(bias).cuda(), score=score, groups=groups,
+                            top_groups=top_groups, group_best=2)
+    np.testing.assert_array_equal(ids.cpu().numpy()[keep], want[keep])
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_one_large_group_hides_no_close_pair(capi, cuda, score):
+    # the groups at the border are small and apart; a group further down is so large that its sum may belong above them
+    torch = cuda
+    rng = np.random.default_rng(5)
+    logits = (0.2 + 1e-3 * rng.standard_normal((4096, 32))).astype(np.float32)
+    bias = np.zeros(32, np.float32)
+    bias[8:16] = 0.001
+    bias[16:24], bias[16] = -20000.0, 20000.0
+    want, apart = _choice(logits, bias, 8, score, 4, 1)
+    keep = apart > 64 * 20000 * 2.0**-52
+    assert keep.mean() > 0.99
+    ids, _ = capi.moe_route(torch.from_numpy(logits).cuda(), 8, bias=torch.from_numpy(bias).cuda(), score=score, groups=4, group_best=2)
+    np.testing.assert_array_equal(ids.cpu().numpy()[keep], want[keep])
+
+
 def test_route_refusals_and_empty_batch(capi, cuda):
     torch = cuda
     l = torch.zeros((4, 32), device="cuda")
