@@ -185,7 +185,7 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
     for (uint32_t d = p.group_lanes / 2u; d > 0; d >>= 1) {
         rank += __shfl_xor_sync(kAll, rank, d);
     }
-    const bool taken = mine < p.groups && rank < p.top_groups && score > none;
+    const bool taken = mine < p.groups && rank < p.top_groups && a > none;  // a sum in fp32 may pass its range
     if (p.group_in_lanes != 0u) {
 #pragma unroll
         for (uint32_t i = 0; i < kVpl; ++i) {
@@ -206,7 +206,7 @@ __device__ __forceinline__ bool keep_best_groups(const RouteParams& p, Real (&c)
     // 42 or 10.8, and 5.9 units of the values' sizes against one (their additions and the sum).  Infinite sizes tell nothing apart.
     const float reach = slack * (1.0f + (float)(two ? fabs(a) + fabs(b) : fabs(a)));
     const uint32_t least = taken ? ordered_bits(fmaxf((float)score - reach, -3.402823466e38f)) : 0xFFFFFFFFu;
-    const uint32_t most = mine < p.groups && !taken && score > none ? ordered_bits(fminf((float)score + reach, 3.402823466e38f)) : 0u;
+    const uint32_t most = mine < p.groups && !taken && a > none ? ordered_bits(fminf((float)score + reach, 3.402823466e38f)) : 0u;
     return __reduce_min_sync(kAll, least) > __reduce_max_sync(kAll, most);
 }
 

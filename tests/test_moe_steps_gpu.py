@@ -197,6 +197,22 @@ def test_one_large_group_hides_no_close_pair(capi, cuda, score):
     np.testing.assert_array_equal(ids.cpu().numpy()[keep], want[keep])
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("group_best", [1, 2])
+@pytest.mark.parametrize("experts,groups", [(32, 4), (60, 5)])  # whole lanes, and not
+def test_groups_masked_by_the_lowest_value(capi, cuda, score, group_best, experts, groups):
+    # the type's lowest value is a value: the sum of two of them passes fp32's range, and the group still counts as one with experts
+    torch = cuda
+    low = torch.finfo(torch.float32).min
+    logits = torch.randn((33, experts), generator=torch.Generator(device="cuda").manual_seed(experts), device="cuda")
+    bias = torch.full((experts,), low, device="cuda")
+    bias[experts // groups : 2 * (experts // groups)] = 0.0
+    _check_route(capi, torch, logits, bias, experts // groups + 2, score, groups, 2, group_best)
+    bias[: experts // groups] = float("-inf")  # and comes before one that has none
+    _check_route(capi, torch, logits, bias, experts // groups + 2, score, groups, 2, group_best)
+    _check_route(capi, torch, logits, -bias.clamp(min=low), 5, score, groups, 2, group_best)  # as far up
+
+
 def test_route_refusals_and_empty_batch(capi, cuda):
     torch = cuda
     l = torch.zeros((4, 32), device="cuda")
