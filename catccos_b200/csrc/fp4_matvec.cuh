@@ -13,7 +13,11 @@
 //
 // x goes in as f16 after a power of two per token and 64 k that brings its largest magnitude to 2^14 .. 2^15: every bf16
 // within 2^-29 of the largest stays exact, smaller ones are off by at most 2^-40 of it, far below the fp32 sums' rounding.
-// Sums of 32 products share a weight scale, which is applied to them in fp32.
+// Sums of 32 products share a weight scale, which is applied to them in fp32, after the power of two is undone: what lies between
+// may be larger than what comes out.  A sum of 32 is below 2^22.6 (values to 2^15, weights to 6), and for the largest bf16 2^113 is
+// to be undone, so all sums are held at 2^-8 of their size up to the end and no step of a result that bf16 holds leaves fp32's
+// range.  The additions of results near fp32's lowest normal number are off by up to 2^-142 for that, a 512th of bf16's lowest.
+// (Deciding step by step costs 1 to 5 % with a branch, 7 % with a multiplication more.)
 //
 // Every warp has a ring of its own in shared memory, filled by asynchronous copies, two steps (10 KB) ahead; 150 KB an SM.  One
 // token and a weight of 330 MB run at 5.5 TB/s; small ones are some 5 us of launch, first and last step around that (one token,
@@ -34,6 +38,7 @@ constexpr uint32_t kMatvecCols = 128;  // of a CTA: 8 lane groups x 16
 constexpr uint32_t kMatvecUnit = 64;   // k of a warp's step: the two scale groups that lie together
 constexpr uint32_t kMatvecDepth = 2;   // steps of a warp's ring
 constexpr uint32_t kMatvecMaxCluster = 8;
+constexpr int kMatvecHeadroom = 8;     // sums are held at 2^-8 of their size
 constexpr uint32_t kMatvecPartRow = kMatvecCols + 8;
 constexpr uint32_t kMatvecWindow = 1024;  // routes among which a weight's rows find one another
 
@@ -282,10 +287,10 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
             }
             top = max(top, __shfl_xor_sync(kAll, top, 1));
             top = max(top, __shfl_xor_sync(kAll, top, 2));
-            const int up = min(141 - (int)(top >> 7), 126);
+            const int up = min(141 - (int)(top >> 7), 118);
             const float mul = __uint_as_float((uint32_t)(127 + up) << 23);
             // this lane's sums belong to token tig of the set
-            back[t] = __uint_as_float((uint32_t)(127 - __shfl_sync(kAll, up, tig * 8u)) << 23);
+            back[t] = __uint_as_float((uint32_t)(127 - kMatvecHeadroom - __shfl_sync(kAll, up, tig * 8u)) << 23);
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
                 const uint32_t a[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
@@ -393,7 +398,8 @@ __global__ void __launch_bounds__(kMatvecThreads, 2) fp4_matvec_kernel(const Mat
             row = token == t ? rows[t] : row;
         }
         if (c < p.n) {
-            *reinterpret_cast<uint32_t*>(p.out + ((size_t)row * p.n + c) * 2u) = pack2<OutT>(a, b);
+            constexpr float kSize = (float)(1 << kMatvecHeadroom);
+            *reinterpret_cast<uint32_t*>(p.out + ((size_t)row * p.n + c) * 2u) = pack2<OutT>(a * kSize, b * kSize);
         }
     }
     if (ctas > 1u) {

@@ -113,6 +113,30 @@ def test_scales_at_their_ends(capi, cuda):
     assert bool(torch.isnan(out[:, 2]).all())  # a scale of 0xFF is NaN, whatever it scales
 
 
+@pytest.mark.parametrize("rows", [1, 5])  # one and two sets of four tokens
+def test_large_values_with_small_scales(capi, cuda, rows):
+    # the activations' power of two is undone before the weights' scale is applied: what lies between stays in range
+    torch = cuda
+    k, n = 256, 32
+    w = torch.zeros((k, n // 2), dtype=torch.uint8, device="cuda")
+    w[0], w[64] = 0x76, 0xE2  # 4 and 6; 1 and -4
+    s = torch.full((k // 64, n, 2), 107, dtype=torch.uint8, device="cuda")
+    s[:, 2:4], s[:, 4] = 0, 254
+    x = torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = torch.tensor([2.0**127, 2.0**115, 2.0**113, 2.0**-100, 1.0][:rows])
+    x[:, 64] = torch.tensor([-(2.0**126), 2.0**127, 1.0, 2.0**127, 2.0**-133][:rows])
+    want = x.double() @ _dequantised(torch, w, s)
+    got = capi.mx_fp4_matvec(x, w, s).double()
+    inside = want.abs() < 2.0**127
+    # two products, exact in the tensor core, and one sum of theirs in fp32: two roundings of 2^-24 and half a step of bf16
+    assert bool(((got - want).abs() <= (2.0**-8 + 2.0**-22) * want.abs())[inside].all())
+    assert bool(inside[:, :4].all()) and not bool(inside[:, 4].any())
+    # column 4: a product of 2^129 and more is infinite in the fp32 sums; row 0 has one of either sign (2^256 - 2^253), and no sum
+    w64 = _dequantised(torch, w, s)
+    sums = (x[:, :1].double() * w64[0]).float() + (x[:, 64:65].double() * w64[64]).float()
+    assert torch.equal(torch.nan_to_num(got[:, 4], nan=-1.0), torch.nan_to_num(sums[:, 4].double(), nan=-1.0))
+
+
 def test_values_that_are_not_finite(capi, cuda):
     torch = cuda
     k, n = 192, 32
