@@ -12,7 +12,8 @@
 // other operand and the second slot in the next, with a zero beside it: eight columns of it are four tokens.
 //
 // x goes in as f16 after a power of two per token and 64 k that brings its largest magnitude to 2^14 .. 2^15: every bf16
-// within 2^-29 of the largest stays exact, smaller ones are off by at most 2^-40 of it, far below the fp32 sums' rounding.
+// within 2^-29 of the largest stays exact, smaller ones are off by at most 2^-39 of it (half a step of f16's denormals, 2^-25, of
+// 2^14), far below the fp32 sums' rounding.
 // Sums of 32 products share a weight scale, which is applied to them in fp32, after the power of two is undone: what lies between
 // may be larger than what comes out.  A sum of 32 is below 2^22.6 (values to 2^15, weights to 6), and for the largest bf16 2^113 is
 // to be undone, so all sums are held at 2^-8 of their size up to the end and no step of a result that bf16 holds leaves fp32's
