@@ -69,6 +69,30 @@ def test_experts(capi, cuda, tokens, top_k, experts, n, k, per_route):
             assert bool((out[r] == 0).all())
 
 
+@pytest.mark.parametrize("routes,experts,top_k,n,k", [(1023, 1, 1, 16, 64), (1025, 5, 1, 48, 128), (1500, 7, 4, 144, 64), (2049, 700, 1, 16, 128),
+                                                      (65535, 3, 1, 16, 64)])
+@pytest.mark.parametrize("kind", ["random", "one expert", "mostly dropped"])
+def test_more_routes_than_a_window(capi, cuda, routes, experts, top_k, n, k, kind):
+    # rows that share a weight find one another among 1024 routes: here they go on in the next ones
+    torch = cuda
+    gen = torch.Generator(device="cuda").manual_seed(routes + experts)
+    w, s = _weights(torch, gen, (experts,), k, n)
+    ids = torch.randint(-1, experts + 1, (routes,), generator=gen, device="cuda", dtype=torch.int32)
+    if kind == "one expert":
+        ids[:] = experts - 1
+    elif kind == "mostly dropped":
+        ids[torch.rand(routes, generator=gen, device="cuda") < 7 / 8] = -1
+    x = torch.randn((routes // top_k, k), generator=gen, device="cuda").to(torch.bfloat16)
+    guard = torch.full((routes + 1, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = capi.mx_fp4_matvec(x, w, s, ids=ids, out=guard[:routes])
+    w64, x_row = _dequantised(torch, w, s), torch.arange(routes, device="cuda") // top_k
+    for e in range(experts):
+        rows = (ids == e).nonzero().flatten()
+        if rows.numel():
+            _compare(torch, out[rows], x[x_row[rows]], w64[e], k)
+    assert bool((out[(ids < 0) | (ids >= experts)] == 0).all()) and bool((guard[routes:] == 7).all())
+
+
 def test_every_code_at_every_place(capi, cuda):
     # weights read back one k at a time: unit vectors give the weight itself
     torch = cuda

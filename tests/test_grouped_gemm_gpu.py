@@ -124,6 +124,14 @@ def test_long_rows_of_few_tokens(capi, cuda, block_n, cta_pair):
     _run(cuda, capi, 21, 784, 7168, [0, 1, 21], block_n=block_n, cta_pair=cta_pair)
 
 
+@pytest.mark.parametrize("cta_pair", [0, 1, 2])
+@pytest.mark.parametrize("live", [0, 1, 500, 4096])
+def test_rows_that_nobody_has(capi, cuda, live, cta_pair):
+    # a rank with some of the experts hands over room for every route and uses a part: the rest stays as it is
+    offsets = [0, live // 8, live // 8, live // 2, live // 2 + live % 3, live, live, live, live]
+    _run(cuda, capi, 4096, 1056, 512, offsets, cta_pair=cta_pair)
+
+
 def test_one_row_of_a_wider_tensor(capi, cuda):
     torch = cuda
     a, a_scales, b, b_scales = _operands(torch, capi, 1, 32, 128, 2, 0, 1)
