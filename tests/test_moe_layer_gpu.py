@@ -213,3 +213,46 @@ def test_first_calls_of_several_threads(capi, cuda):
     # a process of their own: the calls that set the library up
     run = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "first calls ok" in run.stdout, run.stdout + run.stderr
+
+
+FIRST_PRODUCTS = """
+import threading, torch
+from catccos_b200 import capi
+capi.load()
+gen = torch.Generator(device="cuda").manual_seed(4)
+n, k, experts = 256, 256, 2
+codes = lambda *shape: torch.randint(0, 120, shape, generator=gen, device="cuda", dtype=torch.uint8)
+scales = lambda *shape: torch.randint(118, 122, shape, generator=gen, device="cuda", dtype=torch.uint8)
+small = (codes(40, k), scales(40, k // 32), codes(experts, k, n), scales(experts, k // 64, n, 2), torch.tensor([0, 9, 40], dtype=torch.int32, device="cuda"))
+large = (codes(9000, k), scales(9000, k // 32), *small[2:4], torch.tensor([0, 9, 9000], dtype=torch.int32, device="cuda"))
+ids = torch.randint(-1, 9, (9000, 2), generator=gen, device="cuda", dtype=torch.int32)
+x = torch.randn((6, k), generator=gen, device="cuda").to(torch.bfloat16)
+w, w_scales = codes(k, n // 2), scales(k // 64, n, 2)
+calls = [lambda: capi.mx_grouped_gemm(*small), lambda: capi.mx_grouped_gemm(*large), lambda: capi.moe_row_plan(ids, 9),
+         lambda: capi.mx_fp4_matvec(x, w, w_scales)]
+torch.cuda.synchronize()
+start, out = threading.Barrier(16), [None] * 16
+
+def work(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        got = calls[i % 4]()
+        out[i] = got if isinstance(got, tuple) else (got,)
+        torch.cuda.current_stream().synchronize()
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(16)]
+for t in threads:
+    t.start()
+for t in threads:
+    t.join()
+for i in range(4, 16):
+    assert all(torch.equal(a, b) for a, b in zip(out[i], out[i % 4])), i
+assert all(bool(torch.isfinite(o[0]).all()) for o in out) and capi.last_status()[0] == 0
+print("first products ok")
+"""
+
+
+def test_first_products_of_several_threads(capi, cuda):
+    # the entry points of the driver, what kernels may use and the tensor maps are found out by threads that call at once
+    run = subprocess.run([sys.executable, "-c", FIRST_PRODUCTS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "first products ok" in run.stdout, run.stdout + run.stderr
