@@ -43,6 +43,12 @@ EXPORTS = [
     "catccos_b200_moe_combine",
     "catccos_b200_mx_fp4_matvec",
     "catccos_b200_mx_fp4_matvec_typed",
+    "catccos_b200_block_quant",
+    "catccos_b200_block_gemm",
+    "catccos_b200_block_grouped_gemm",
+    "catccos_b200_moe_dispatch",
+    "catccos_b200_moe_dispatch_grad",
+    "catccos_b200_moe_combine_grad",
     "catccos_b200_mx_quant_matmul_static",
     "catccos_b200_mx_quant_matmul_static_status",
     "catccos_b200_last_status",
@@ -61,6 +67,14 @@ class Tiling(ctypes.Structure):
             "commDataSplit", "commBlockM", "rankSize", "epSize", "expertNum", "topK",
         )
     ]
+
+
+class BlockOperand(ctypes.Structure):
+    """catccos_b200_block_operand_t: a matrix of codes and the fp32 scales of its blocks."""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("line_bytes", ctypes.c_size_t), ("matrix_bytes", ctypes.c_size_t), ("scales", ctypes.c_void_p),
+                ("scale_row", ctypes.c_size_t), ("scale_col", ctypes.c_size_t), ("scale_matrix", ctypes.c_size_t),
+                ("transposed", ctypes.c_int), ("per_column", ctypes.c_int), ("type", ctypes.c_int)]
 
 
 class CatccosError(RuntimeError):
@@ -113,6 +127,13 @@ def load() -> ctypes.CDLL:
     L.catccos_b200_moe_combine.argtypes = [vp, vp, u32, vp, vp, vp, vp, u32, u32, u32, i32]
     L.catccos_b200_mx_fp4_matvec.argtypes = [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32]
     L.catccos_b200_mx_fp4_matvec_typed.argtypes = [*L.catccos_b200_mx_fp4_matvec.argtypes, i32]
+    op = ctypes.POINTER(BlockOperand)
+    L.catccos_b200_block_quant.argtypes = [vp, vp, i32, sz, u32, u32, i32, i32, vp, u32, u32, vp, vp]
+    L.catccos_b200_block_gemm.argtypes = [vp, op, op, vp, u32, u32, u32, i32]
+    L.catccos_b200_block_grouped_gemm.argtypes = [vp, op, op, vp, vp, u32, u32, u32, u32, i32]
+    L.catccos_b200_moe_dispatch.argtypes = [vp, vp, vp, vp, u32, u32, u32, u32]
+    L.catccos_b200_moe_dispatch_grad.argtypes = [vp, vp, u32, vp, vp, vp, u32, u32, u32, i32]
+    L.catccos_b200_moe_combine_grad.argtypes = [vp, vp, vp, u32, vp, vp, vp, vp, u32, u32, u32, i32]
     L.catccos_b200_mx_quant_matmul_static.argtypes = [vp, vp, vp, vp, vp, u32, u32, u32]
     L.catccos_b200_last_status.argtypes = [ctypes.POINTER(u32)]
     L.catccos_b200_mx_quant_matmul_static_status.argtypes = [ctypes.POINTER(u32)]
@@ -372,6 +393,81 @@ def mx_fp4_matvec(x_bf16, w, w_scales, ids=None, out=None, out_dtype=None):
     if code:
         raise CatccosError("catccos_b200_mx_fp4_matvec", code)
     return out
+
+
+_BLOCKS = {"row": 0, "column": 1, "square": 2}
+
+
+def block_quant(x, dtype=None, block: str = "row", row_index=None, rows=None, out=None):
+    """x [rows, K] (bf16, fp16 or fp32) -> codes [rows, K] of dtype (torch.float8_e4m3fn or e5m2, by default the first) and fp32 scales.
+
+    A scale for each block of 128 values of a row ("row": [rows, ceil(K / 128)]), of a column ("column": [ceil(rows / 128), K]) or of
+    128 x 128 ("square": [ceil(rows / 128), ceil(K / 128)]); a code stands for code * scale.  With row_index int32 [rows, top_k] (blocks
+    of rows) token t's codes and scales are written to the rows row_index[t], of `rows` (by default rows * top_k); rows that it does not
+    name stay as they are (unset, where they are allocated here).  out: the pair (codes, scales) to write to."""
+    import torch
+
+    if block not in _BLOCKS:
+        raise ValueError(f"block is one of {sorted(_BLOCKS)}, got {block!r}")
+    codes, scales = (None, None) if out is None else out
+    code, codes, scales = (_calls or _load_calls()).block_quant(x, torch.float8_e4m3fn if dtype is None else dtype, _BLOCKS[block], row_index,
+                                                                rows, codes, scales)
+    if code:
+        raise CatccosError("catccos_b200_block_quant", code)
+    return codes, scales
+
+
+def block_gemm(a, a_scales, b, b_scales, out=None, out_dtype=None):
+    """c [M, N] = dequant(a [M, K]) x dequant(b [K, N]), fp32 scales for blocks of 128 along K.
+
+    a_scales [M, ceil(K / 128)]; b_scales [ceil(K / 128), ceil(N / 128)], or [ceil(K / 128), N], one for each column.  a and b may be
+    transposed views: x W is block_gemm(x, xs, w, ws), with a checkpoint's [N, K] weight (x, xs, w.t(), ws.t()); the gradient of x
+    is (dy, dys, w.t(), ws.t()); that of w (x.t(), xs.t(), dy, dys) with x and dy quantised in blocks of columns.  Codes of a float8
+    type are of that type, uint8 of the options' "a_dtype" and "b_dtype"; out (or out_dtype) is bf16, fp16 or fp32, bf16 without
+    either."""
+    code, out = (_calls or _load_calls()).block_gemm(a, a_scales, b, b_scales, out, out_dtype)
+    if code:
+        raise CatccosError("catccos_b200_block_gemm", code)
+    return out
+
+
+def block_grouped_gemm(a, a_scales, b, b_scales, offsets, out=None, out_dtype=None):
+    """c [rows, N]: rows offsets[e] .. offsets[e + 1] are dequant(a) x dequant(b[e]); b [experts, K, N] or a transposed view of
+    [experts, N, K], b_scales [experts, ceil(K / 128), ceil(N / 128)].  Otherwise as block_gemm and mx_grouped_gemm: rows outside the
+    offsets stay as they are (of a tensor allocated here: unset)."""
+    code, out = (_calls or _load_calls()).block_grouped_gemm(a, a_scales, b, b_scales, offsets, out, out_dtype)
+    if code:
+        raise CatccosError("catccos_b200_block_grouped_gemm", code)
+    return out
+
+
+def moe_dispatch(x, row_index, rows=None, out=None):
+    """out [rows, n] with out[row_index[t, r]] = x[t], the rows of a token's routes; x bf16 or fp16 [tokens, n], row_index of moe_row_plan.
+
+    rows is by default tokens * top_k; rows that row_index does not name stay as they are (of a tensor allocated here: unset)."""
+    code, out = (_calls or _load_calls()).moe_dispatch(x, row_index, rows, out)
+    if code:
+        raise CatccosError("catccos_b200_moe_dispatch", code)
+    return out
+
+
+def moe_dispatch_grad(d_rows, row_index, shared=None, out=None):
+    """The gradient of moe_dispatch: out [tokens, n] = sum over r of d_rows[row_index[t, r]] (+ shared[t]), in fp32, rounded once."""
+    code, out = (_calls or _load_calls()).moe_dispatch_grad(d_rows, row_index, shared, out)
+    if code:
+        raise CatccosError("catccos_b200_moe_dispatch_grad", code)
+    return out
+
+
+def moe_combine_grad(d_out, expert_out, row_index, weights, out=None):
+    """The gradients of moe_combine: (d_expert_out [rows, n], d_weights fp32 [tokens, top_k]); that of its `shared` is d_out itself.
+
+    d_expert_out[row_index[t, r]] = weights[t, r] * d_out[t], into out if given (it may be expert_out); rows that row_index does not name
+    stay as they are (unset, without out).  d_weights[t, r] is d_out[t] times the route's row, 0 for a dropped one."""
+    code, d_expert_out, d_weights = (_calls or _load_calls()).moe_combine_grad(d_out, expert_out, row_index, weights, out)
+    if code:
+        raise CatccosError("catccos_b200_moe_combine_grad", code)
+    return d_expert_out, d_weights
 
 
 def mxfp8_matmul_reduce_scatter(a_codes, a_scales, b, b_scales, d, symm: int, world: int) -> None:

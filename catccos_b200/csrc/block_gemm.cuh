@@ -1,0 +1,405 @@
+// Products of 8-bit codes with one fp32 scale for each block of 128, for sm_100a, dense and per expert:
+//   C[i, j] = sum over blocks t of K:  sa[i, t] * sb[t, j / 128] * (sum over k in block t of A[i, k] B[k, j])
+// (or sb[t, j]: B scaled by column, a weight's gradient).  With offsets [experts + 1] on the device, rows offsets[e] ..
+// offsets[e + 1] of A meet expert e's B.
+//
+// The scales are no powers of two, so the tensor core cannot apply them: every block's products are a tensor-memory tile of
+// their own, which the promotion warps read, scale and add to sums in registers while the next block is multiplied into the
+// other tile.  128 columns of K are four tcgen05.mma kind::f8f6f4 (K = 32).
+//
+// Either operand may be stored with K or with its other axis running fastest: both are operand layouts of the tensor core, so
+// that x W, dy W^T and x^T dy read the same codes without a transposed copy.  K need not be a multiple of 128: TMA fills the
+// last block with zeros.
+//
+// 320 threads: warps 0-7 promotion and output (warp w: lane quarter w % 4, column half w / 4), warp 8 TMA, warp 9 MMA.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "mx_grouped_gemm.cuh"
+
+namespace catccos {
+
+constexpr uint32_t kBlockGemmThreads = 320;
+constexpr uint32_t kBlockGemmM = 128;
+constexpr uint32_t kBlockGemmMaxParts = 8;
+
+struct BlockGemmParams {
+    const float* a_scales;
+    size_t a_scale_row, a_scale_block;                     // floats from one row's (block's) scale to the next
+    const float* b_scales;
+    size_t b_scale_block, b_scale_col, b_scale_matrix;     // from one block of K, of columns (by column: 1), one expert to the next
+    const int32_t* offsets;                                // nullptr: one matrix
+    void* c;
+    uint32_t rows, experts, N, K;
+    uint32_t a_fmt, b_fmt;                                 // 0 = E4M3, 1 = E5M2
+    uint32_t a_cols, b_rows;                               // 1: A is stored [K, rows]; B [N, K]
+    uint32_t parts;                                        // CTAs of a cluster that share K (a power of two)
+    uint64_t bar_timeout_ns;
+    StatusBlock* status;
+};
+
+// Instruction descriptor of kind::f8f6f4 with fp32 accumulators: make_idesc_mxf8's fields without the scales' (bits 4, 5: fp32)
+__host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t M, uint32_t N, uint32_t a_fmt, uint32_t b_fmt, bool a_mn, bool b_mn)
+{
+    return (1u << 4) | (a_fmt << 7) | (b_fmt << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                        uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns -> 16 registers per thread; they hold the values behind tmem_ld_fence of them
+__device__ __forceinline__ void tmem_ld_16(uint32_t taddr, float (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Waits for this thread's tensor-memory loads; nothing that reads r moves in front of it.
+__device__ __forceinline__ void tmem_ld_fence(float (&r)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                   "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
+                 :
+                 : "memory");
+}
+
+// Sixteen columns of a row to global memory; p is aligned to their size or 32 bytes
+template <typename OutT>
+__device__ __forceinline__ void store_16(OutT* p, const float (&v)[16])
+{
+    if constexpr (sizeof(OutT) == 4) {
+        uint32_t o[2][8];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            o[i / 8][i % 8] = __float_as_uint(v[i]);
+        }
+        st_global_v8(p, o[0]);
+        st_global_v8(p + 8, o[1]);
+    } else {
+        uint32_t o[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            o[i] = pack2<OutT>(v[2 * i], v[2 * i + 1]);
+        }
+        st_global_v8(p, o);
+    }
+}
+
+// The scales of one row (or of one block of columns) along K, read ahead of the products: with the blocks next to one another
+// and 16-byte aligned rows four at a time, the next four while these are used.
+struct ScaleReader {
+    const float* at;
+    size_t step;
+    uint32_t left;  // blocks not yet requested
+    bool wide;
+    float4 cur, nxt;
+
+    __device__ __forceinline__ float4 fetch()
+    {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (wide && left >= 4u) {
+            v = __ldcg(reinterpret_cast<const float4*>(at));
+        } else {
+            if (left > 0u) v.x = __ldcg(at);
+            if (left > 1u) v.y = __ldcg(at + step);
+            if (left > 2u) v.z = __ldcg(at + 2 * step);
+            if (left > 3u) v.w = __ldcg(at + 3 * step);
+        }
+        at += 4 * step;
+        left -= min(left, 4u);
+        return v;
+    }
+    // blocks [first, first + count) of the line that starts at `line`
+    __device__ __forceinline__ void start(const float* line, size_t block_step, uint32_t first, uint32_t count)
+    {
+        at = line + first * block_step;
+        step = block_step;
+        left = count;
+        wide = block_step == 1 && ((uintptr_t)at & 15u) == 0u;
+        cur = fetch();
+        nxt = fetch();
+    }
+    // the i-th of them, i ascending by one
+    __device__ __forceinline__ float get(uint32_t i)
+    {
+        if (i != 0u && (i & 3u) == 0u) {
+            cur = nxt;
+            nxt = fetch();
+        }
+        const uint32_t j = i & 3u;
+        return j == 0u ? cur.x : (j == 1u ? cur.y : (j == 2u ? cur.z : cur.w));
+    }
+};
+
+// One warp: where each expert's rows and row tiles begin (count_grouped_tiles), or the one matrix without offsets.
+__device__ __forceinline__ void count_block_tiles(const BlockGemmParams& p, uint32_t tile_rows, uint32_t* tiles, uint32_t* row_begin,
+                                                  uint32_t* row_end, uint32_t lane)
+{
+    if (p.offsets != nullptr) {
+        GroupedParams g = {};
+        g.offsets = p.offsets;
+        g.rows = p.rows;
+        g.experts = p.experts;
+        count_grouped_tiles(g, tile_rows, tiles, row_begin, row_end, lane);
+    } else if (lane == 0) {
+        tiles[0] = 0;
+        tiles[1] = (p.rows + tile_rows - 1u) / tile_rows;
+        row_begin[0] = 0;
+        row_end[0] = p.rows;
+    }
+}
+
+template <uint32_t BLOCK_N>
+struct BlockGemmSmem {
+    static constexpr uint32_t kStages = BLOCK_N == 64 ? 4 : 3;  // two CTAs to an SM
+    static constexpr uint32_t kABytes = kBlockGemmM * 128;
+    static constexpr uint32_t kBBytes = BLOCK_N * 128;
+    static constexpr uint32_t kOffA = 0;
+    static constexpr uint32_t kOffB = kOffA + kStages * kABytes;
+    // by column: a slot is free again when the product two steps behind its stage's next is multiplied (see the producer)
+    static constexpr uint32_t kScaleSlots = kStages + 2;
+    static constexpr uint32_t kOffScale = kOffB + kStages * kBBytes;
+    static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * BLOCK_N * 4;
+    static constexpr uint32_t kNumBars = 2 * kStages + 4;  // full[S], empty[S], tmem_full[2], tmem_empty[2]
+    static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
+    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
+    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
+    static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
+    // the parts' sums meet in the ring: [part][128 rows][a part's columns, four more]
+    static_assert(kBlockGemmM * (BLOCK_N + 4 * kBlockGemmMaxParts) * 4 <= kOffScale, "the sums of all parts fit the ring");
+};
+
+template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
+__global__ void __launch_bounds__(kBlockGemmThreads, 2)
+block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
+                  const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ BlockGemmParams p)
+{
+    using S = BlockGemmSmem<BLOCK_N>;
+    constexpr uint32_t kStages = S::kStages, kCols = BLOCK_N / 2;  // columns of a promotion warp
+    constexpr uint32_t kTmemCols = 2 * BLOCK_N;
+
+    grid_dep_launch();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
+    uint64_t* empty = full + kStages;
+    uint64_t* tmem_full = empty + kStages;
+    uint64_t* tmem_empty = tmem_full + 2;
+    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
+    uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
+    uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
+    uint32_t* row_begin = tiles + p.experts + 1u;
+    uint32_t* row_end = row_begin + p.experts;
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
+    const uint32_t k_blocks = (p.K + 127u) / 128u;
+    const uint32_t part = blockIdx.x & (p.parts - 1u), first_unit = blockIdx.x / p.parts, stride = gridDim.x / p.parts;
+    const uint32_t kb0 = (uint32_t)((uint64_t)part * k_blocks / p.parts), kb1 = (uint32_t)((uint64_t)(part + 1u) * k_blocks / p.parts);
+    const uint32_t steps = kb1 - kb0;  // blocks of K that this CTA multiplies of a unit
+    const uint64_t bar_ns = p.bar_timeout_ns;
+
+    if (threadIdx.x == 256) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(&tmem_full[a], 1);
+            mbar_init(&tmem_empty[a], 8);
+        }
+        *dead = 0u;
+        mbar_fence_init();
+        tma_prefetch_desc(&tmap_a);
+        tma_prefetch_desc(&tmap_a32);
+        tma_prefetch_desc(&tmap_b);
+    }
+    if (warp == 9) {
+        tmem_alloc(tmem_ptr_smem, kTmemCols);
+        tmem_relinquish();
+    }
+    grid_dep_wait();
+    if (warp == 0) {
+        count_block_tiles(p, kBlockGemmM, tiles, row_begin, row_end, lane);
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = *tmem_ptr_smem;
+    const uint32_t num_units = tiles[p.experts] * n_tiles;
+    bool alive = true;  // false once a wait of this role has given up
+    GroupedWalk walk;
+
+    if (warp == 8) {
+        // ------------------------------- TMA producer -------------------------------------
+        uint32_t it = 0;
+        for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
+            const TileCoord tc = walk.seek(tiles, n_tiles, unit);
+            const uint32_t m0 = row_begin[walk.e] + tc.m_tile * kBlockGemmM, n0 = tc.n_tile * BLOCK_N;
+            const uint32_t boxes = (min(row_end[walk.e] - m0, kBlockGemmM) + 31u) / 32u;  // of 32 rows
+            const uint32_t scale_bytes = kByColumn ? min(p.N - n0, BLOCK_N) * 4u : 0u;
+            const uint32_t tx_bytes = (p.a_cols ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes + scale_bytes;
+            for (uint32_t kb = kb0; alive && kb < kb1; ++kb, ++it) {
+                const uint32_t s = it % kStages;
+                alive = mbar_wait_warp(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 400, s, bar_ns);
+                if (!alive) {
+                    break;
+                }
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&full[s], tx_bytes);
+                    const int32_t k = (int32_t)(kb * 128u);
+                    tma_load_3d(smem + S::kOffB + s * S::kBBytes, &tmap_b, &full[s], p.b_rows ? k : (int32_t)n0,
+                                p.b_rows ? (int32_t)n0 : k, (int32_t)walk.e);
+                    uint8_t* a = smem + S::kOffA + s * S::kABytes;
+                    if (p.a_cols) {
+                        tma_load_2d(a, &tmap_a, &full[s], (int32_t)m0, k);
+                    } else if (boxes == 4u) {
+                        tma_load_2d(a, &tmap_a, &full[s], k, (int32_t)m0);
+                    } else {
+                        for (uint32_t i = 0; i < boxes; ++i) {
+                            tma_load_2d(a + i * (32u * 128u), &tmap_a32, &full[s], k, (int32_t)(m0 + i * 32u));
+                        }
+                    }
+                    if (kByColumn) {
+                        // Step `it` may overwrite the scales of step it - kStages - 2: the product of it - kStages has been
+                        // multiplied (empty[s]), for which the tile of it - kStages - 2 had to be promoted (tmem_empty).
+                        bulk_load(smem + S::kOffScale + (it % S::kScaleSlots) * (BLOCK_N * 4u),
+                                  p.b_scales + (size_t)walk.e * p.b_scale_matrix + kb * p.b_scale_block + n0, scale_bytes, &full[s]);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------- MMA issuer ---------------------------------------
+        const uint32_t idesc0 = make_idesc_f8(kBlockGemmM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
+        const uint64_t desc_a = p.a_cols ? make_smem_desc(0, 16384, 1024, 2) : make_smem_desc(0, 16, 1024, 2);
+        const uint64_t desc_b = p.b_rows ? make_smem_desc(0, 16, 1024, 2)
+                                         : make_smem_desc(0, 16384, 8 * BLOCK_N, BLOCK_N == 64 ? 4 : 2);
+        const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
+        const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
+        const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4);
+        const uint32_t step_a = (p.a_cols ? 32u * 128u : 32u) >> 4, step_b = (p.b_rows ? 32u : 32u * BLOCK_N) >> 4;
+        uint32_t it = 0;
+        for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
+            // a ragged last column of tiles is multiplied as wide as it is (a multiple of 16)
+            const uint32_t idesc = idesc0 | ((min(p.N - unit % n_tiles * BLOCK_N, BLOCK_N) >> 3) << 17);
+            for (uint32_t i = 0; alive && i < steps; ++i, ++it) {
+                const uint32_t s = it % kStages, buf = it & 1u;
+                alive = mbar_wait_warp(&tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, buf, bar_ns) &&
+                        mbar_wait_warp(&full[s], (it / kStages) & 1u, p.status, 403, s, bar_ns);
+                if (!alive) {
+                    break;  // nothing is issued, and no tile reported, after a wait has given up
+                }
+                tcgen05_fence_after();
+                if (elect_one()) {
+                    const uint32_t a_lo = a_lo0 + s * (S::kABytes >> 4), b_lo = b_lo0 + s * (S::kBBytes >> 4);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        umma_f8(tmem_base + buf * BLOCK_N, a_lo + j * step_a, hi_a, b_lo + j * step_b, hi_b, idesc, j);
+                    }
+                    tcgen05_commit(&empty[s]);
+                    tcgen05_commit(&tmem_full[buf]);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ------------------------------- promotion and output -----------------------------
+        const uint32_t q = warp & 3u, half = warp >> 2;
+        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + half * kCols;
+        uint32_t it = 0;
+        for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
+            const TileCoord tc = walk.seek(tiles, n_tiles, unit);
+            const uint32_t first = row_begin[walk.e] + tc.m_tile * kBlockGemmM, end = row_end[walk.e];
+            const uint32_t row0 = first + q * 32u, row = row0 + lane, n0 = tc.n_tile * BLOCK_N;
+            const bool live = row0 < end && n0 + half * kCols < p.N;  // else there is nothing to fetch
+            float acc[kCols] = {};
+            ScaleReader sa, sb;
+            sa.start(p.a_scales + min(row, end - 1u) * p.a_scale_row, p.a_scale_block, kb0, steps);
+            sb.start(p.b_scales + walk.e * p.b_scale_matrix + (n0 / 128u) * p.b_scale_col, p.b_scale_block, kb0, kByColumn ? 0u : steps);
+            for (uint32_t i = 0; i < steps; ++i, ++it) {
+                const uint32_t buf = it & 1u;
+                const float f = kByColumn ? sa.get(i) : sa.get(i) * sb.get(i);
+                alive = mbar_wait_warp(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
+                if (!alive) {
+                    break;  // a tile that never filled is not written out
+                }
+                tcgen05_fence_after();
+                if (live) {
+                    const float* scale = reinterpret_cast<const float*>(smem + S::kOffScale) + (it % S::kScaleSlots) * BLOCK_N + half * kCols;
+#pragma unroll
+                    for (uint32_t c = 0; c < kCols; c += 16) {
+                        float r[16];
+                        tmem_ld_16(tmem + buf * BLOCK_N + c, r);
+                        tmem_ld_fence(r);
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) {
+                            acc[c + j] = fmaf(r[j], kByColumn ? f * scale[c + j] : f, acc[c + j]);
+                        }
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tmem_empty[buf]);
+                }
+            }
+            if (p.parts == 1u && alive && row < end) {
+                OutT* dst = static_cast<OutT*>(p.c) + (size_t)row * p.N + n0 + half * kCols;
+#pragma unroll
+                for (uint32_t c = 0; c < kCols; c += 16) {
+                    if (n0 + half * kCols + c < p.N) {
+                        float v[16];
+#pragma unroll
+                        for (uint32_t j = 0; j < 16; ++j) {
+                            v[j] = acc[c + j];
+                        }
+                        store_16(dst + c, v);
+                    }
+                }
+            }
+        }
+    }
+
+    tcgen05_fence_before();
+    if (__syncthreads_or(alive ? 0 : 1)) {
+        drain_after_abort(p.status);
+    }
+    if (warp == 9) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+}  // namespace catccos

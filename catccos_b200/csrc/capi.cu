@@ -15,6 +15,8 @@
 #include <vector>
 
 #include "../../include/catccos_b200.h"
+#include "block_gemm.cuh"
+#include "block_quant.cuh"
 #include "bootstrap.hpp"
 #include "internal_options.h"
 #include "common.cuh"
@@ -1656,6 +1658,231 @@ int launch_grouped(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_b
                : launch_grouped_inst<BLOCK_N, __nv_bfloat16>(grid, st, maps[0], maps[1], maps[2], p);
 }
 
+// The sum of a token's rows, with weights (the combination) or without (the dispatch backwards).
+int moe_sum(const char* name, void* stream, const void* expert_out, uint32_t rows, const int32_t* row_index, const float* weights,
+            const void* shared_out, void* out, uint32_t tokens, uint32_t n, uint32_t top_k, int f16)
+{
+    if (n == 0 || n % 8 != 0 || top_k == 0 || f16 < 0 || f16 > 1) {
+        ERROR_LOG("%s: n must be a multiple of 8 (got %u), top_k at least 1 (got %u)", name, n, top_k);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if ((rows != 0 && !expert_out) || !row_index || !out || misaligned(expert_out, 16) || misaligned(shared_out, 16) ||
+        misaligned(out, 16) || misaligned(row_index, 4) || misaligned(weights, 4) || rows > 0x7FFFFFFFu) {
+        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    const size_t out_bytes = 2 * (size_t)tokens * n;
+    if (share_memory(out, out_bytes, expert_out, 2 * (size_t)rows * n) || (out != shared_out && shared_out && share_memory(out, out_bytes, shared_out, out_bytes)) ||
+        share_memory(out, out_bytes, row_index, 4 * (size_t)tokens * top_k) || (weights && share_memory(out, out_bytes, weights, 4 * (size_t)tokens * top_k))) {
+        ERROR_LOG("%s: out may be shared_out, and overlaps nothing else", name);
+        return CATCCOS_B200_EINVAL;
+    }
+    CombineParams p = {};
+    p.y = static_cast<const uint8_t*>(expert_out);
+    p.row_index = row_index;
+    p.weights = weights;
+    p.shared_out = static_cast<const uint8_t*>(shared_out);
+    p.out = static_cast<uint8_t*>(out);
+    p.tokens = tokens;
+    p.rows = rows;
+    p.n = n;
+    p.top_k = top_k;
+    const bool wide = n % 16 == 0 && !misaligned(expert_out, 32) && !misaligned(shared_out, 32) && !misaligned(out, 32) &&
+                      combine_wide(tokens, n, top_k);
+    p.vectors = wide ? n / 16 : n / 8;
+    p.slabs = p.vectors >= kCombineThreads ? (p.vectors + kCombineThreads - 1) / kCombineThreads : 0;
+    const uint64_t per_cta = p.slabs ? 1 : kCombineThreads / p.vectors;
+    const uint64_t grid = p.slabs ? (uint64_t)tokens * p.slabs : (tokens + per_cta - 1) / per_cta;
+    if (grid > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    auto kern = f16 ? (wide ? moe_combine_kernel<__half, true> : moe_combine_kernel<__half, false>)
+                    : (wide ? moe_combine_kernel<__nv_bfloat16, true> : moe_combine_kernel<__nv_bfloat16, false>);
+    if (weights == nullptr) {
+        kern = f16 ? (wide ? moe_combine_kernel<__half, true, false> : moe_combine_kernel<__half, false, false>)
+                   : (wide ? moe_combine_kernel<__nv_bfloat16, true, false> : moe_combine_kernel<__nv_bfloat16, false, false>);
+    }
+    CUDA_TRY(launch_after(kern, dim3((unsigned)grid), kCombineThreads, 0, (cudaStream_t)stream, p));
+    return 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// blocks of 128 with fp32 scales
+// ---------------------------------------------------------------------------------------------
+// `depth` matrices of 8-bit codes, `plane` bytes apart; inner, outer, box and pitch as in encode_map_2d.
+int encode_map_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t depth, uint32_t box_inner, uint32_t box_outer,
+                  uint64_t pitch, uint64_t plane)
+{
+    const MapKey k{base, inner, outer, box_inner, box_outer, false, 1, pitch, depth, plane};
+    return thread_maps<CUtensorMap>().get(k, map, [&](CUtensorMap* made) -> int {
+        cuuint64_t dims[3] = {inner, outer, depth};
+        cuuint64_t strides[2] = {pitch, plane};
+        cuuint32_t box[3] = {box_inner, box_outer, 1};
+        cuuint32_t estr[3] = {1, 1, 1};
+        CU_TRY(g.drv.TensorMapEncodeTiled(made, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
+        return 0;
+    });
+}
+
+template <typename T, bool kE5m2>
+int launch_block_quant(cudaStream_t st, const BlockQuantParams& p, int block)
+{
+    const uint64_t grid = block == 0 ? (p.units + kBlockQuantThreads / 8 - 1) / (kBlockQuantThreads / 8)
+                                     : (uint64_t)((p.rows + kBlockSize - 1) / kBlockSize) * p.blocks;
+    if (grid > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    CUDA_TRY(launch_after(block == 0 ? block_quant_rows_kernel<T, kE5m2>
+                                     : (block == 1 ? block_quant_tiles_kernel<T, kE5m2, false> : block_quant_tiles_kernel<T, kE5m2, true>),
+                          dim3((unsigned)grid), kBlockQuantThreads, 0, st, p));
+    return 0;
+}
+
+// The operands of a block-scaled product as the kernels take them.
+struct BlockOperands {
+    const catccos_b200_block_operand_t *a, *b;
+};
+
+// Maps of the rows of a (boxes of a_box and of 32 rows; stored by column: boxes of 128 x 128) and of b (`columns` wide).
+int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmParams& p, uint32_t columns)
+{
+    const void* a = o.a->codes;
+    const uint64_t lda = o.a->line_bytes, ldb = o.b->line_bytes;
+    int rcode = p.a_cols ? encode_map_2d(&maps[0], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[0], a, p.K, p.rows, 128, 128, false, 1, lda);
+    if (rcode == 0) rcode = p.a_cols ? encode_map_2d(&maps[1], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[1], a, p.K, p.rows, 128, 32, false, 1, lda);
+    if (rcode != 0) return rcode;
+    const uint64_t plane = p.experts > 1 ? o.b->matrix_bytes : ldb * (p.b_rows ? p.N : p.K);
+    return p.b_rows ? encode_map_3d(&maps[2], o.b->codes, p.K, p.N, p.experts, 128, columns, ldb, plane)
+                    : encode_map_3d(&maps[2], o.b->codes, p.N, p.K, p.experts, columns, 128, ldb, plane);
+}
+
+template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
+int launch_block_gemm_inst(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
+{
+    using S = BlockGemmSmem<BLOCK_N>;
+    static PerDevice<bool, kMaxRanks * 2> done;
+    CUDA_TRY(allow_smem(block_gemm_kernel<BLOCK_N, OutT, kByColumn>, S::dynamic_bytes(kGroupedMaxExperts), done));
+    CUtensorMap maps[3];
+    int rcode = block_maps(maps, o, p, BLOCK_N);
+    if (rcode != 0) return rcode;
+    // at most one row tile that is not full for every expert that has rows
+    const uint64_t tiles = p.offsets ? p.rows / kBlockGemmM + std::min(p.rows, p.experts) : (p.rows + kBlockGemmM - 1) / kBlockGemmM;
+    const uint64_t units = tiles * ((p.N + BLOCK_N - 1) / BLOCK_N);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(units, 2 * (uint64_t)rc.num_sms);
+    CUDA_TRY(launch_after(block_gemm_kernel<BLOCK_N, OutT, kByColumn>, dim3(grid), kBlockGemmThreads, S::dynamic_bytes(p.experts), st, maps[0],
+                          maps[1], maps[2], p));
+    return 0;
+}
+
+template <typename OutT>
+int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
+{
+    if (o.b->per_column) {
+        return launch_block_gemm_inst<128, OutT, true>(rc, st, o, p);
+    }
+    return g.block_n == 64 ? launch_block_gemm_inst<64, OutT, false>(rc, st, o, p) : launch_block_gemm_inst<128, OutT, false>(rc, st, o, p);
+}
+
+// Common part of the two products.
+int block_product(const char* name, void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b,
+                  const int32_t* offsets, bool grouped, void* c, uint32_t rows, uint32_t experts, uint32_t n, uint32_t k, int c_type)
+{
+    if (!a || !b) {
+        return CATCCOS_B200_EINVAL;
+    }
+    const int a_type = a->type == -1 ? g.a_dtype : a->type, b_type = b->type == -1 ? g.b_dtype : b->type;
+    c_type = c_type == -1 ? g.c_dtype : c_type;
+    constexpr uint32_t kMost = 0x7FFFFF00u;  // with a tile behind it, still an int
+    if (n == 0 || n % 16 != 0 || k == 0 || k % 16 != 0 || n > kMost || k > kMost || rows > kMost || experts == 0 || experts > kGroupedMaxExperts) {
+        ERROR_LOG("%s needs K %% 16 == 0, N %% 16 == 0, sizes below 2^31 and 1 to %u experts (got rows=%u N=%u K=%u experts=%u)", name,
+                  kGroupedMaxExperts, rows, n, k, experts);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (a_type < 0 || a_type > 1 || b_type < 0 || b_type > 1 || c_type < 0 || c_type > 2) {
+        ERROR_LOG("%s takes 8-bit operands (types 0, 1) and gives bf16, fp16 or fp32 (0 to 2); got %d, %d, %d", name, a_type, b_type, c_type);
+        return CATCCOS_B200_EINVAL;
+    }
+    if ((a->transposed | b->transposed | a->per_column | b->per_column) & ~1 || a->per_column || (grouped && (a->transposed || b->per_column)) ||
+        (a->transposed && rows % 16 != 0)) {
+        ERROR_LOG("%s: a stored by column has a multiple of 16 rows (got %u); only a dense b is scaled by column, and rows of experts are stored by row",
+                  name, rows);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (rows == 0) {
+        return 0;
+    }
+    const uint64_t a_inner = a->transposed ? rows : k, a_outer = a->transposed ? k : rows;
+    const uint64_t b_inner = b->transposed ? k : n, b_outer = b->transposed ? n : k;
+    if (!a->codes || !a->scales || !b->codes || !b->scales || !c || (grouped && !offsets) || misaligned(a->codes, 16) || misaligned(b->codes, 16) ||
+        misaligned(a->scales, 4) || misaligned(b->scales, 4) || misaligned(c, 32) || misaligned(offsets, 4)) {
+        return CATCCOS_B200_EINVAL;
+    }
+    constexpr uint64_t kFar = 1ull << 40;
+    if (a->line_bytes < a_inner || b->line_bytes < b_inner || a->line_bytes % 16 != 0 || b->line_bytes % 16 != 0 || a->line_bytes >= kFar ||
+        b->line_bytes >= kFar || a->scale_row >= kFar || a->scale_col >= kFar || b->scale_row >= kFar || b->scale_col >= kFar ||
+        (experts > 1 && (b->matrix_bytes % 16 != 0 || b->matrix_bytes < b->line_bytes * (b_outer - 1) + b_inner || b->matrix_bytes >= kFar ||
+                         b->scale_matrix >= kFar))) {
+        ERROR_LOG("%s: rows, columns and matrices of codes are apart by multiples of 16 bytes and do not overlap", name);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (b->per_column && (b->scale_col != 1 || b->scale_row % 4 != 0 || misaligned(b->scales, 16))) {
+        ERROR_LOG("%s: scales by column lie next to one another, their rows 16-byte aligned", name);
+        return CATCCOS_B200_EINVAL;
+    }
+    const size_t k_blocks = (k + 127u) / 128u, n_scales = b->per_column ? n : (n + 127u) / 128u;
+    const size_t c_bytes = (size_t)rows * n * (c_type == 2 ? 4 : 2);
+    if (share_memory(c, c_bytes, a->codes, (a_outer - 1) * a->line_bytes + a_inner) ||
+        share_memory(c, c_bytes, a->scales, 4 * ((rows - 1) * a->scale_row + (k_blocks - 1) * a->scale_col + 1)) ||
+        share_memory(c, c_bytes, b->codes, (experts - 1) * b->matrix_bytes + (b_outer - 1) * b->line_bytes + b_inner) ||
+        share_memory(c, c_bytes, b->scales, 4 * ((experts - 1) * b->scale_matrix + (k_blocks - 1) * b->scale_row + (n_scales - 1) * b->scale_col + 1)) ||
+        (offsets && share_memory(c, c_bytes, offsets, 4 * (size_t)experts + 4))) {
+        ERROR_LOG("%s: c overlaps an operand", name);
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    if (!g.drv.Load()) {
+        return CATCCOS_B200_ECUDA;
+    }
+    RankCtx& rc = cur();
+    int dev = 0;
+    CUDA_TRY(cudaGetDevice(&dev));
+    if (dev != rc.device) {
+        return CATCCOS_B200_ESTATE;  // the record of its waits is on the rank's device
+    }
+    BlockGemmParams p = {};
+    p.a_scales = a->scales;
+    p.a_scale_row = a->scale_row;
+    p.a_scale_block = a->scale_col;
+    p.b_scales = b->scales;
+    p.b_scale_block = b->scale_row;
+    p.b_scale_col = b->scale_col;
+    p.b_scale_matrix = experts > 1 ? b->scale_matrix : 0;
+    p.offsets = offsets;
+    p.c = c;
+    p.rows = rows;
+    p.experts = experts;
+    p.N = n;
+    p.K = k;
+    p.a_fmt = (uint32_t)a_type;
+    p.b_fmt = (uint32_t)b_type;
+    p.a_cols = (uint32_t)a->transposed;
+    p.b_rows = (uint32_t)b->transposed;
+    p.parts = 1;
+    p.bar_timeout_ns = 2 * g.timeout_ns + 1000000000ull;
+    p.status = rc.status;
+    const BlockOperands o = {a, b};
+    cudaStream_t st = (cudaStream_t)stream;
+    return c_type == 2 ? launch_block_gemm<float>(rc, st, o, p)
+                       : (c_type == 1 ? launch_block_gemm<__half>(rc, st, o, p) : launch_block_gemm<__nv_bfloat16>(rc, st, o, p));
+}
+
 }  // namespace
 
 // =============================================================================================
@@ -2494,48 +2721,10 @@ int catccos_b200_moe_row_plan(void* stream, const int32_t* ids, uint32_t routes,
 int catccos_b200_moe_combine(void* stream, const void* expert_out, uint32_t rows, const int32_t* row_index, const float* weights,
                              const void* shared_out, void* out, uint32_t tokens, uint32_t n, uint32_t top_k, int f16)
 {
-    if (n == 0 || n % 8 != 0 || top_k == 0 || f16 < 0 || f16 > 1) {
-        ERROR_LOG("moe_combine: n must be a multiple of 8 (got %u), top_k at least 1 (got %u)", n, top_k);
+    if (!weights && tokens != 0) {
         return CATCCOS_B200_EINVAL;
     }
-    if (tokens == 0) {
-        return 0;
-    }
-    if ((rows != 0 && !expert_out) || !row_index || !weights || !out || misaligned(expert_out, 16) || misaligned(shared_out, 16) ||
-        misaligned(out, 16) || misaligned(row_index, 4) || misaligned(weights, 4) || rows > 0x7FFFFFFFu) {
-        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
-    }
-    const size_t out_bytes = 2 * (size_t)tokens * n;
-    if (share_memory(out, out_bytes, expert_out, 2 * (size_t)rows * n) || (out != shared_out && shared_out && share_memory(out, out_bytes, shared_out, out_bytes)) ||
-        share_memory(out, out_bytes, row_index, 4 * (size_t)tokens * top_k) || share_memory(out, out_bytes, weights, 4 * (size_t)tokens * top_k)) {
-        ERROR_LOG("moe_combine: out may be shared_out, and overlaps nothing else");
-        return CATCCOS_B200_EINVAL;
-    }
-    CombineParams p = {};
-    p.y = static_cast<const uint8_t*>(expert_out);
-    p.row_index = row_index;
-    p.weights = weights;
-    p.shared_out = static_cast<const uint8_t*>(shared_out);
-    p.out = static_cast<uint8_t*>(out);
-    p.tokens = tokens;
-    p.rows = rows;
-    p.n = n;
-    p.top_k = top_k;
-    const bool wide = n % 16 == 0 && !misaligned(expert_out, 32) && !misaligned(shared_out, 32) && !misaligned(out, 32) &&
-                      combine_wide(tokens, n, top_k);
-    p.vectors = wide ? n / 16 : n / 8;
-    p.slabs = p.vectors >= kCombineThreads ? (p.vectors + kCombineThreads - 1) / kCombineThreads : 0;
-    const uint64_t per_cta = p.slabs ? 1 : kCombineThreads / p.vectors;
-    const uint64_t grid = p.slabs ? (uint64_t)tokens * p.slabs : (tokens + per_cta - 1) / per_cta;
-    if (grid > 0x7FFFFFFFull) {
-        return CATCCOS_B200_EINVAL;
-    }
-    int rcode = ensure_init();
-    if (rcode != 0) return rcode;
-    CUDA_TRY(launch_after(f16 ? (wide ? moe_combine_kernel<__half, true> : moe_combine_kernel<__half, false>)
-                              : (wide ? moe_combine_kernel<__nv_bfloat16, true> : moe_combine_kernel<__nv_bfloat16, false>),
-                          dim3((unsigned)grid), kCombineThreads, 0, (cudaStream_t)stream, p));
-    return 0;
+    return moe_sum("moe_combine", stream, expert_out, rows, row_index, weights, shared_out, out, tokens, n, top_k, f16);
 }
 
 int catccos_b200_mx_grouped_gemm(void* stream, const void* a, size_t a_row_bytes, const void* a_scale, size_t a_scale_row_bytes,
@@ -2615,6 +2804,168 @@ int catccos_b200_mx_grouped_gemm_typed(void* stream, const void* a, size_t a_row
     return plan.block_n == 64 ? launch_grouped<64>(rc, st, a, a_row_bytes, b, p, f16)
                               : (plan.block_n == 128 ? launch_grouped<128>(rc, st, a, a_row_bytes, b, p, f16)
                                                      : launch_grouped<256>(rc, st, a, a_row_bytes, b, p, f16));
+}
+
+int catccos_b200_block_quant(void* stream, const void* x, int x_type, size_t x_row_bytes, uint32_t rows, uint32_t k, int block, int code_type,
+                             const int32_t* row_index, uint32_t top_k, uint32_t out_rows, void* codes, float* scales)
+{
+    code_type = code_type == -1 ? g.a_dtype : code_type;
+    if (k == 0 || k % 16 != 0 || x_type < 0 || x_type > 2 || block < 0 || block > 2 || code_type < 0 || code_type > 1 || rows > 0x7FFFFFFFu ||
+        out_rows > 0x7FFFFFFFu || k > 0x7FFFFF00u) {
+        ERROR_LOG("block_quant: K must be a multiple of 16, x bf16, fp16 or fp32 (0 to 2), blocks of rows, columns or squares (0 to 2), codes of type "
+                  "0 or 1 (got K=%u x=%d block=%d codes=%d)", k, x_type, block, code_type);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (row_index != nullptr && (block != 0 || top_k == 0)) {
+        ERROR_LOG("block_quant: row_index goes with blocks of rows and at least one route a token");
+        return CATCCOS_B200_EINVAL;
+    }
+    if (rows == 0 || (row_index != nullptr && out_rows == 0)) {
+        return 0;
+    }
+    const size_t bytes = x_type == 2 ? 4 : 2;
+    if (!x || !codes || !scales || misaligned(x, 16) || misaligned(codes, 16) || misaligned(scales, 4) || misaligned(row_index, 4) ||
+        x_row_bytes < k * bytes || x_row_bytes % 16 != 0 || x_row_bytes >= (1ull << 40)) {
+        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    const uint32_t blocks = (k + kBlockSize - 1) / kBlockSize, row_blocks = (rows + kBlockSize - 1) / kBlockSize;
+    const size_t to_rows = row_index ? out_rows : rows;
+    const size_t x_bytes = (rows - 1) * x_row_bytes + k * bytes, code_bytes = to_rows * k;
+    const size_t scale_bytes = 4 * (block == 0 ? to_rows * blocks : (size_t)row_blocks * (block == 1 ? k : blocks));
+    const size_t index_bytes = row_index ? 4 * (size_t)rows * top_k : 0;
+    if (share_memory(codes, code_bytes, x, x_bytes) || share_memory(scales, scale_bytes, x, x_bytes) || share_memory(codes, code_bytes, scales, scale_bytes) ||
+        (row_index && (share_memory(codes, code_bytes, row_index, index_bytes) || share_memory(scales, scale_bytes, row_index, index_bytes)))) {
+        ERROR_LOG("block_quant: an output overlaps an input or the other output");
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    BlockQuantParams p = {};
+    p.x = static_cast<const uint8_t*>(x);
+    p.x_row_bytes = x_row_bytes;
+    p.row_index = row_index;
+    p.codes = static_cast<uint8_t*>(codes);
+    p.scales = scales;
+    p.rows = rows;
+    p.k = k;
+    p.blocks = blocks;
+    p.top_k = top_k;
+    p.out_rows = out_rows;
+    p.units = (uint64_t)rows * blocks;
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool e5m2 = code_type == 1;
+    return x_type == 2 ? (e5m2 ? launch_block_quant<float, true>(st, p, block) : launch_block_quant<float, false>(st, p, block))
+                       : (x_type == 1 ? (e5m2 ? launch_block_quant<__half, true>(st, p, block) : launch_block_quant<__half, false>(st, p, block))
+                                      : (e5m2 ? launch_block_quant<__nv_bfloat16, true>(st, p, block) : launch_block_quant<__nv_bfloat16, false>(st, p, block)));
+}
+
+int catccos_b200_block_gemm(void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b, void* c, uint32_t m,
+                            uint32_t n, uint32_t k, int c_type)
+{
+    return block_product("block_gemm", stream, a, b, nullptr, false, c, m, 1, n, k, c_type);
+}
+
+int catccos_b200_block_grouped_gemm(void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b,
+                                    const int32_t* offsets, void* c, uint32_t rows, uint32_t experts, uint32_t n, uint32_t k, int c_type)
+{
+    return block_product("block_grouped_gemm", stream, a, b, offsets, true, c, rows, experts, n, k, c_type);
+}
+
+int catccos_b200_moe_dispatch(void* stream, const void* x, const int32_t* row_index, void* out, uint32_t tokens, uint32_t rows, uint32_t n,
+                              uint32_t top_k)
+{
+    if (n == 0 || n % 8 != 0 || top_k == 0 || rows > 0x7FFFFFFFu) {
+        ERROR_LOG("moe_dispatch: n must be a multiple of 8 (got %u), top_k at least 1 (got %u), rows below 2^31", n, top_k);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (tokens == 0 || rows == 0) {
+        return 0;
+    }
+    if (!x || !row_index || !out || misaligned(x, 16) || misaligned(out, 16) || misaligned(row_index, 4)) {
+        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    const size_t out_bytes = 2 * (size_t)rows * n;
+    if (share_memory(out, out_bytes, x, 2 * (size_t)tokens * n) || share_memory(out, out_bytes, row_index, 4 * (size_t)tokens * top_k)) {
+        ERROR_LOG("moe_dispatch: out overlaps an input");
+        return CATCCOS_B200_EINVAL;
+    }
+    DispatchParams p = {};
+    p.x = static_cast<const uint8_t*>(x);
+    p.row_index = row_index;
+    p.out = static_cast<uint8_t*>(out);
+    p.tokens = tokens;
+    p.rows = rows;
+    p.top_k = top_k;
+    p.vectors = n / 8;
+    p.slabs = p.vectors >= kCombineThreads ? (p.vectors + kCombineThreads - 1) / kCombineThreads : 0;
+    const uint64_t per_cta = p.slabs ? 1 : kCombineThreads / p.vectors;
+    const uint64_t grid = p.slabs ? (uint64_t)tokens * p.slabs : (tokens + per_cta - 1) / per_cta;
+    if (grid > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    CUDA_TRY(launch_after(moe_dispatch_kernel, dim3((unsigned)grid), kCombineThreads, 0, (cudaStream_t)stream, p));
+    return 0;
+}
+
+int catccos_b200_moe_dispatch_grad(void* stream, const void* d_rows, uint32_t rows, const int32_t* row_index, const void* shared, void* out,
+                                   uint32_t tokens, uint32_t n, uint32_t top_k, int f16)
+{
+    return moe_sum("moe_dispatch_grad", stream, d_rows, rows, row_index, nullptr, shared, out, tokens, n, top_k, f16);
+}
+
+int catccos_b200_moe_combine_grad(void* stream, const void* d_out, const void* expert_out, uint32_t rows, const int32_t* row_index,
+                                  const float* weights, void* d_expert_out, float* d_weights, uint32_t tokens, uint32_t n, uint32_t top_k, int f16)
+{
+    if (n == 0 || n % 8 != 0 || top_k == 0 || f16 < 0 || f16 > 1 || rows > 0x7FFFFFFFu) {
+        ERROR_LOG("moe_combine_grad: n must be a multiple of 8 (got %u), top_k at least 1 (got %u), rows below 2^31", n, top_k);
+        return CATCCOS_B200_EINVAL;
+    }
+    if (tokens == 0) {
+        return 0;
+    }
+    if (!d_out || (rows != 0 && (!expert_out || !d_expert_out)) || !row_index || !weights || !d_weights || misaligned(d_out, 16) ||
+        misaligned(expert_out, 16) || misaligned(d_expert_out, 16) || misaligned(row_index, 4) || misaligned(weights, 4) || misaligned(d_weights, 4)) {
+        return CATCCOS_B200_EINVAL;  // rows are read and written 16 bytes at a time
+    }
+    const size_t row_bytes = 2 * (size_t)rows * n, token_bytes = 2 * (size_t)tokens * n, route_bytes = 4 * (size_t)tokens * top_k;
+    const void* ins[4] = {d_out, expert_out, row_index, weights};
+    const size_t in_bytes[4] = {token_bytes, row_bytes, route_bytes, route_bytes};
+    bool overlap = share_memory(d_expert_out, row_bytes, d_weights, route_bytes);
+    for (int i = 0; i < 4; ++i) {
+        // a value's thread reads expert_out before it writes there, and nobody else does either
+        overlap = overlap || (share_memory(d_expert_out, row_bytes, ins[i], in_bytes[i]) && !(i == 1 && d_expert_out == expert_out)) ||
+                  share_memory(d_weights, route_bytes, ins[i], in_bytes[i]);
+    }
+    if (overlap) {
+        ERROR_LOG("moe_combine_grad: d_expert_out may be expert_out; otherwise an output overlaps nothing");
+        return CATCCOS_B200_EINVAL;
+    }
+    CombineGradParams p = {};
+    p.d_out = static_cast<const uint8_t*>(d_out);
+    p.y = static_cast<const uint8_t*>(expert_out);
+    p.row_index = row_index;
+    p.weights = weights;
+    p.d_y = static_cast<uint8_t*>(d_expert_out);
+    p.d_weights = d_weights;
+    p.tokens = tokens;
+    p.rows = rows;
+    p.top_k = top_k;
+    p.vectors = n / 8;
+    p.chunks = (top_k + kCombineGradRoutes - 1) / kCombineGradRoutes;
+    const uint64_t grid = (uint64_t)tokens * p.chunks;
+    if (grid > 0x7FFFFFFFull) {
+        return CATCCOS_B200_EINVAL;
+    }
+    int rcode = ensure_init();
+    if (rcode != 0) return rcode;
+    // threads that all have as many pieces of a row, at most one less
+    const uint32_t rounds = (p.vectors + kCombineGradThreads - 1) / kCombineGradThreads;
+    const uint32_t threads = ((p.vectors + rounds - 1) / rounds + 31) / 32 * 32;
+    CUDA_TRY(launch_after(f16 ? moe_combine_grad_kernel<__half> : moe_combine_grad_kernel<__nv_bfloat16>, dim3((unsigned)grid), threads, 0,
+                          (cudaStream_t)stream, p));
+    return 0;
 }
 
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,

@@ -17,10 +17,12 @@ struct MapKey {
     bool fp4;
     uint32_t elem;
     uint64_t pitch;
+    uint32_t depth = 0;  // matrices of a map with three axes, 0: two axes
+    uint64_t plane = 0;  // bytes from one of them to the next
     bool operator==(const MapKey& o) const
     {
         return base == o.base && inner == o.inner && outer == o.outer && box_inner == o.box_inner &&
-               box_outer == o.box_outer && fp4 == o.fp4 && elem == o.elem && pitch == o.pitch;
+               box_outer == o.box_outer && fp4 == o.fp4 && elem == o.elem && pitch == o.pitch && depth == o.depth && plane == o.plane;
     }
 };
 

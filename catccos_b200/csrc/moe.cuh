@@ -1,6 +1,7 @@
 // The mixture-of-experts steps around the experts' products: scores to experts and weights (moe_route_kernel), the rows of the
 // dispatch (moe_row_plan_kernel: the expanded_row_idx that mx_quant_scatter_packed_kernel takes, and where each expert's rows
-// begin), and the weighted sum of a token's expert rows (moe_combine_kernel).
+// begin), and the weighted sum of a token's expert rows (moe_combine_kernel).  The rows there in 16 bits (moe_dispatch_kernel) and
+// the gradients of both ways.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -768,7 +769,10 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v)
 // Bound by memory: every live row once, 2 n bytes, and the result.  A lane owns eight columns of a token and has up to eight
 // rows on their way before it adds the first, or (wide) sixteen columns, a whole sector a load, and four rows.  4095 tokens x 8
 // rows of 7168 columns: 79 us wide (6.5 TB/s), 97 to 106 narrow; 16 tokens, where one round trip counts: see combine_wide().
-template <typename T, bool kWide>
+//
+// Without weights (kWeighted false) the rows are added as they are: the gradient of the dispatch, which copies a token's row to each
+// of its routes.
+template <typename T, bool kWide, bool kWeighted = true>
 __global__ void __launch_bounds__(kCombineThreads, kWide ? 7 : 1) moe_combine_kernel(const CombineParams p)
 {
     constexpr uint32_t kWords = kWide ? 8 : 4, kInFlight = kWide ? 4 : 8;
@@ -811,7 +815,7 @@ __global__ void __launch_bounds__(kCombineThreads, kWide ? 7 : 1) moe_combine_ke
         for (uint32_t j = 0; j < kInFlight; ++j) {
             const size_t at = (size_t)token * p.top_k + min(r0 + j, p.top_k - 1u);
             index[j] = (uint32_t)__ldcg(p.row_index + at);
-            w[j] = __ldcg(p.weights + at);
+            w[j] = kWeighted ? __ldcg(p.weights + at) : 1.0f;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kInFlight; ++j) {
@@ -856,6 +860,132 @@ __global__ void __launch_bounds__(kCombineThreads, kWide ? 7 : 1) moe_combine_ke
         st_global_v8(dst, o);
     } else {
         *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// dispatch, and the combination backwards
+// ------------------------------------------------------------------------------------------
+struct DispatchParams {
+    const uint8_t* x;          // [tokens, n], 16-bit values
+    const int32_t* row_index;  // [tokens, top_k]
+    uint8_t* out;              // [rows, n]
+    uint32_t tokens, rows, top_k;
+    uint32_t vectors;          // 16-byte pieces of a row
+    uint32_t slabs;            // as in CombineParams
+};
+
+// out[row_index[t, r]] = x[t].  Bound by memory: a token's row is read once and stored once for every live route.
+__global__ void __launch_bounds__(kCombineThreads) moe_dispatch_kernel(const DispatchParams p)
+{
+    grid_dep_wait();
+    grid_dep_launch();
+    uint32_t token, v;
+    if (p.slabs != 0u) {
+        token = blockIdx.x / p.slabs;
+        v = (blockIdx.x - token * p.slabs) * kCombineThreads + threadIdx.x;
+    } else {
+        const uint32_t in_cta = threadIdx.x / p.vectors;
+        token = blockIdx.x * (kCombineThreads / p.vectors) + in_cta;
+        v = threadIdx.x - in_cta * p.vectors;
+        if (in_cta >= kCombineThreads / p.vectors) {
+            return;
+        }
+    }
+    if (token >= p.tokens || v >= p.vectors) {
+        return;
+    }
+    const uint4 x = __ldcs(reinterpret_cast<const uint4*>(p.x) + (size_t)token * p.vectors + v);
+    for (uint32_t r = 0; r < p.top_k; ++r) {
+        const uint32_t to = (uint32_t)__ldcg(p.row_index + (size_t)token * p.top_k + r);
+        if (to < p.rows) {  // a dropped route is negative: above any row
+            reinterpret_cast<uint4*>(p.out)[(size_t)to * p.vectors + v] = x;
+        }
+    }
+}
+
+constexpr uint32_t kCombineGradThreads = 256, kCombineGradRoutes = 4;
+
+struct CombineGradParams {
+    const uint8_t* d_out;      // [tokens, n], 16-bit floats
+    const uint8_t* y;          // [rows, n]
+    const int32_t* row_index;  // [tokens, top_k]
+    const float* weights;      // [tokens, top_k]
+    uint8_t* d_y;              // [rows, n]
+    float* d_weights;          // [tokens, top_k]
+    uint32_t tokens, rows, top_k;
+    uint32_t vectors;          // 16-byte pieces of a row
+    uint32_t chunks;           // CTAs of a token: its routes in groups of kCombineGradRoutes
+};
+
+// out[t] = sum over r of weights[t, r] * y[row_index[t, r]] backwards:
+//   d_y[row_index[t, r]] = weights[t, r] * d_out[t];   d_weights[t, r] = sum over columns of d_out[t] * y[row_index[t, r]]
+// A CTA has a token and four of its routes.  Bound by memory: d_out once, a row read and a row written for every live route.  The
+// sums are fp32, a thread's columns ascending, then lanes and warps in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(kCombineGradThreads) moe_combine_grad_kernel(const CombineGradParams p)
+{
+    __shared__ float partial[kCombineGradThreads / 32][kCombineGradRoutes];
+    grid_dep_wait();
+    grid_dep_launch();
+    const uint32_t token = blockIdx.x / p.chunks, r0 = (blockIdx.x - token * p.chunks) * kCombineGradRoutes;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint32_t index[kCombineGradRoutes];
+    float w[kCombineGradRoutes], sum[kCombineGradRoutes] = {};
+#pragma unroll
+    for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+        const size_t at = (size_t)token * p.top_k + min(r0 + j, p.top_k - 1u);
+        index[j] = r0 + j < p.top_k ? (uint32_t)__ldcg(p.row_index + at) : 0xFFFFFFFFu;  // a dropped route is negative: above any row
+        w[j] = __ldcg(p.weights + at);
+    }
+    for (uint32_t v = threadIdx.x; v < p.vectors; v += blockDim.x) {
+        const uint4 d4 = __ldcg(reinterpret_cast<const uint4*>(p.d_out) + (size_t)token * p.vectors + v);
+        uint4 y4[kCombineGradRoutes];
+#pragma unroll
+        for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+            y4[j] = make_uint4(0, 0, 0, 0);
+            if (index[j] < p.rows) {
+                y4[j] = __ldcs(reinterpret_cast<const uint4*>(p.y) + (size_t)index[j] * p.vectors + v);
+            }
+        }
+        const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
+        float2 d[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            d[i] = unpack2<T>(dw[i]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+            if (index[j] < p.rows) {
+                const uint32_t yw[4] = {y4[j].x, y4[j].y, y4[j].z, y4[j].w};
+                uint32_t o[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float2 f = unpack2<T>(yw[i]);
+                    sum[j] = fmaf(d[i].x, f.x, fmaf(d[i].y, f.y, sum[j]));
+                    o[i] = pack2<T>(w[j] * d[i].x, w[j] * d[i].y);
+                }
+                __stcs(reinterpret_cast<uint4*>(p.d_y) + (size_t)index[j] * p.vectors + v, make_uint4(o[0], o[1], o[2], o[3]));
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+#pragma unroll
+        for (uint32_t d = 16; d > 0; d >>= 1) {
+            sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], d);
+        }
+        if (lane == 0) {
+            partial[warp][j] = sum[j];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < kCombineGradRoutes && r0 + threadIdx.x < p.top_k) {
+        float s = 0.0f;
+        for (uint32_t i = 0; i < blockDim.x / 32; ++i) {
+            s += partial[i][threadIdx.x];
+        }
+        p.d_weights[(size_t)token * p.top_k + r0 + threadIdx.x] = s;
     }
 }
 

@@ -36,6 +36,12 @@ BOUND(moe_row_plan);
 BOUND(mx_grouped_gemm_typed);
 BOUND(moe_combine);
 BOUND(mx_fp4_matvec_typed);
+BOUND(block_quant);
+BOUND(block_gemm);
+BOUND(block_grouped_gemm);
+BOUND(moe_dispatch);
+BOUND(moe_dispatch_grad);
+BOUND(moe_combine_grad);
 BOUND(mx_quant_matmul_static);
 BOUND(mx_quant_allgather);
 BOUND(mx_quant_allgather_matmul);
@@ -561,6 +567,217 @@ CALL(moe_combine, 5)
                        a[4], out);
 END_CALL
 
+// torch.float8_e4m3fn, torch.float8_e5m2
+at::ScalarType code_dtype(PyObject* dtype)
+{
+    const at::ScalarType type = THPDtype_Check(dtype) ? reinterpret_cast<THPDtype*>(dtype)->scalar_type : at::kFloat;
+    if (type != at::kFloat8_e4m3fn && type != at::kFloat8_e5m2) {
+        refuse("dtype", "torch.float8_e4m3fn or torch.float8_e5m2");
+    }
+    return type;
+}
+
+// x, dtype, block, row_index, rows, codes, scales
+CALL(block_quant, 7)
+    const at::Tensor& x = plain(a[0], "x", "a bf16, fp16 or fp32 CUDA matrix, its columns next to one another", {kBf16, kF16, kF32}, 2, nullptr, false);
+    const at::ScalarType type = code_dtype(a[1]);
+    const int64_t m = x.size(0), k = x.size(1), block = whole(a[2], "block"), blocks = (k + 127) / 128, row_blocks = (m + 127) / 128;
+    if (k > 1 && x.stride(1) != 1) {
+        refuse("x", "columns next to one another");
+    }
+    int64_t top_k = 0, rows = m;
+    if (a[3] != Py_None) {
+        const at::Tensor& index = plain(a[3], "row_index", "a contiguous int32 matrix on x's device", {kI32}, 2, &x);
+        if (index.size(0) != m) {
+            refuse("row_index", "a row for each row of x");
+        }
+        top_k = index.size(1);
+        rows = a[5] != Py_None ? tensor(a[5]).size(0) : (a[4] != Py_None ? whole(a[4], "rows") : m * top_k);
+    } else if (a[4] != Py_None) {
+        refuse("rows", "None without row_index");
+    }
+    const int64_t scale_rows = block == 0 ? rows : row_blocks, scale_cols = block == 1 ? k : blocks;
+    const OnDevice on(x);
+    at::Tensor codes, scales;
+    if (a[5] != Py_None) {
+        codes = plain(a[5], "out", "contiguous codes of dtype on x's device", {type}, 2, &x);
+        scales = plain(a[6], "out", "contiguous fp32 scales on x's device", {kF32}, 2, &x);
+        if (codes.size(0) != rows || codes.size(1) != k || scales.size(0) != scale_rows || scales.size(1) != scale_cols) {
+            refuse("out", "codes and scales as the call would allocate them");
+        }
+    } else {
+        const Pair out(x, {rows, k}, type, {scale_rows, scale_cols}, kF32);
+        codes = out.first;
+        scales = out.second;
+    }
+    const int x_type = x.scalar_type() == kF32 ? 2 : (x.scalar_type() == kF16 ? 1 : 0), code = type == at::kFloat8_e5m2 ? 1 : 0;
+    const size_t row_bytes = (size_t)(m > 1 ? x.stride(0) : (k + 15) / 16 * 16) * x.element_size();  // one row has no distance to the next
+    void *in = x.data_ptr(), *i = data_or_null(a[3]), *c = codes.data_ptr(), *s = scales.data_ptr();
+    return with_outputs(released([&] {
+                            return block_quant_fn(on.stream, in, x_type, row_bytes, (uint32_t)m, (uint32_t)k, (int)block, code,
+                                                  (const int32_t*)i, (uint32_t)top_k, (uint32_t)rows, c, (float*)s);
+                        }),
+                        codes, scales);
+END_CALL
+
+// The last two axes of a tensor of codes: rows, columns, and which of them is stored next to one another.
+struct Matrix {
+    int64_t rows, cols;
+    catccos_b200_block_operand_t op;
+    Matrix(const at::Tensor& t, const char* what)
+    {
+        rows = t.size(-2), cols = t.size(-1);
+        op = {};
+        const bool by_row = cols <= 1 || t.stride(-1) == 1, by_col = rows <= 1 || t.stride(-2) == 1;
+        if (!by_row && !by_col) {
+            refuse(what, "rows or columns of codes next to one another");
+        }
+        op.transposed = by_row ? 0 : 1;
+        const int64_t inner = by_row ? cols : rows, outer = by_row ? rows : cols, step = t.stride(by_row ? -2 : -1);
+        op.line_bytes = (size_t)(outer > 1 ? step : (inner + 15) / 16 * 16);  // one line has no distance to the next
+        op.codes = t.data_ptr();
+        op.type = code_type(t);
+    }
+    void scales(const at::Tensor& s)
+    {
+        op.scales = static_cast<const float*>(s.data_ptr());
+        op.scale_row = (size_t)s.stride(-2);
+        op.scale_col = (size_t)s.stride(-1);
+    }
+};
+
+// torch.bfloat16, torch.float16, torch.float32, or None for the first
+at::ScalarType float_type(PyObject* dtype)
+{
+    if (dtype == Py_None) {
+        return kBf16;
+    }
+    const at::ScalarType type = THPDtype_Check(dtype) ? reinterpret_cast<THPDtype*>(dtype)->scalar_type : at::kInt;
+    if (type != kBf16 && type != kF16 && type != kF32) {
+        refuse("out_dtype", "torch.bfloat16, torch.float16 or torch.float32");
+    }
+    return type;
+}
+
+int float_code(at::ScalarType type) { return type == kF32 ? 2 : (type == kF16 ? 1 : 0); }
+
+// a, a_scales, b, b_scales, out, out_dtype
+CALL(block_gemm, 6)
+    const auto codes = {kU8, at::kFloat8_e4m3fn, at::kFloat8_e5m2};
+    const at::Tensor& x = plain(a[0], "a", "a CUDA matrix of 8-bit codes", codes, 2, nullptr, false);
+    const at::Tensor& xs = plain(a[1], "a_scales", "a matrix of fp32 scales on a's device", {kF32}, 2, &x, false);
+    const at::Tensor& b = plain(a[2], "b", "a matrix of 8-bit codes on a's device", codes, 2, &x, false);
+    const at::Tensor& bs = plain(a[3], "b_scales", "a matrix of fp32 scales on a's device", {kF32}, 2, &x, false);
+    Matrix am(x, "a"), bm(b, "b");
+    const int64_t m = am.rows, k = am.cols, n = bm.cols, blocks = (k + 127) / 128, columns = (n + 127) / 128;
+    if (bm.rows != k || xs.size(0) != m || xs.size(1) != blocks || bs.size(0) != blocks || (bs.size(1) != columns && bs.size(1) != n)) {
+        refuse("block_gemm", "a [M, K], a_scales [M, ceil(K / 128)], b [K, N], b_scales [ceil(K / 128), ceil(N / 128)] or [ceil(K / 128), N]");
+    }
+    am.scales(xs);
+    bm.scales(bs);
+    bm.op.per_column = bs.size(1) != columns ? 1 : 0;
+    if (bm.op.per_column && blocks <= 1) {
+        bm.op.scale_row = (size_t)(n + 3) / 4 * 4;
+    }
+    const OnDevice on(x);
+    const at::Tensor out = result(a[4], "a contiguous bf16, fp16 or fp32 matrix [M, N] on a's device", {kBf16, kF16, kF32}, x, m, n, float_type(a[5]));
+    const int c_type = float_code(out.scalar_type());
+    void* c = out.data_ptr();
+    return with_output(released([&] { return block_gemm_fn(on.stream, &am.op, &bm.op, c, (uint32_t)m, (uint32_t)n, (uint32_t)k, c_type); }), a[4], out);
+END_CALL
+
+// a, a_scales, b, b_scales, offsets, out, out_dtype
+CALL(block_grouped_gemm, 7)
+    const auto codes = {kU8, at::kFloat8_e4m3fn, at::kFloat8_e5m2};
+    const at::Tensor& x = plain(a[0], "a", "a CUDA matrix of 8-bit codes", codes, 2, nullptr, false);
+    const at::Tensor& xs = plain(a[1], "a_scales", "a matrix of fp32 scales on a's device", {kF32}, 2, &x, false);
+    const at::Tensor& b = plain(a[2], "b", "8-bit codes [experts, K, N] on a's device", codes, 3, &x, false);
+    const at::Tensor& bs = plain(a[3], "b_scales", "fp32 scales [experts, ceil(K / 128), ceil(N / 128)] on a's device", {kF32}, 3, &x, false);
+    const at::Tensor& offsets = plain(a[4], "offsets", "a contiguous int32 vector on a's device", {kI32}, 1, &x);
+    Matrix am(x, "a"), bm(b, "b");
+    const int64_t rows = am.rows, k = am.cols, experts = b.size(0), n = bm.cols, blocks = (k + 127) / 128, columns = (n + 127) / 128;
+    if (bm.rows != k || xs.size(0) != rows || xs.size(1) != blocks || bs.size(0) != experts || bs.size(1) != blocks || bs.size(2) != columns ||
+        offsets.size(0) != experts + 1) {
+        refuse("block_grouped_gemm", "a [rows, K], a_scales [rows, ceil(K / 128)], b [experts, K, N], b_scales [experts, ceil(K / 128), "
+                                     "ceil(N / 128)], offsets [experts + 1]");
+    }
+    am.scales(xs);
+    bm.scales(bs);
+    bm.op.matrix_bytes = (size_t)b.stride(0);
+    bm.op.scale_matrix = (size_t)bs.stride(0);
+    const OnDevice on(x);
+    const at::Tensor out = result(a[5], "a contiguous bf16, fp16 or fp32 matrix [rows, N] on a's device", {kBf16, kF16, kF32}, x, rows, n, float_type(a[6]));
+    const int c_type = float_code(out.scalar_type());
+    void *o = offsets.data_ptr(), *c = out.data_ptr();
+    return with_output(released([&] {
+                           return block_grouped_gemm_fn(on.stream, &am.op, &bm.op, (const int32_t*)o, c, (uint32_t)rows, (uint32_t)experts,
+                                                        (uint32_t)n, (uint32_t)k, c_type);
+                       }),
+                       a[5], out);
+END_CALL
+
+// x, row_index, rows, out
+CALL(moe_dispatch, 4)
+    const at::Tensor& x = plain(a[0], "x", "a contiguous bf16 or fp16 CUDA matrix", {kBf16, kF16}, 2);
+    const at::Tensor& index = plain(a[1], "row_index", "a contiguous int32 matrix on x's device", {kI32}, 2, &x);
+    const int64_t tokens = x.size(0), n = x.size(1), top_k = index.size(1);
+    if (index.size(0) != tokens) {
+        refuse("row_index", "a row for each row of x");
+    }
+    const int64_t rows = a[3] != Py_None ? tensor(a[3]).size(0) : (a[2] != Py_None ? whole(a[2], "rows") : tokens * top_k);
+    const OnDevice on(x);
+    const at::Tensor out = result(a[3], "a contiguous matrix [rows, n] of x's type and device", {x.scalar_type()}, x, rows, n, x.scalar_type());
+    void *in = x.data_ptr(), *i = index.data_ptr(), *o = out.data_ptr();
+    return with_output(released([&] {
+                           return moe_dispatch_fn(on.stream, in, (const int32_t*)i, o, (uint32_t)tokens, (uint32_t)rows, (uint32_t)n, (uint32_t)top_k);
+                       }),
+                       a[3], out);
+END_CALL
+
+// d_rows, row_index, shared, out
+CALL(moe_dispatch_grad, 4)
+    const at::Tensor& y = plain(a[0], "d_rows", "a contiguous bf16 or fp16 CUDA matrix", {kBf16, kF16}, 2);
+    const at::ScalarType type = y.scalar_type();
+    const at::Tensor& index = plain(a[1], "row_index", "a contiguous int32 matrix on d_rows' device", {kI32}, 2, &y);
+    const int64_t tokens = index.size(0), n = y.size(1);
+    const char* wanted = "a contiguous matrix [tokens, n] of d_rows' type and device";
+    const OnDevice on(y);
+    const at::Tensor out = result(a[3], wanted, {type}, y, tokens, n, type);
+    if (a[2] != Py_None && plain(a[2], "shared", wanted, {type}, 2, &y).sizes() != out.sizes()) {
+        refuse("shared", wanted);
+    }
+    void *in = y.data_ptr(), *i = index.data_ptr(), *s = data_or_null(a[2]), *o = out.data_ptr();
+    const uint32_t top_k = (uint32_t)index.size(1), rows = (uint32_t)y.size(0);
+    return with_output(released([&] {
+                           return moe_dispatch_grad_fn(on.stream, in, rows, (const int32_t*)i, s, o, (uint32_t)tokens, (uint32_t)n, top_k,
+                                                       type == kF16 ? 1 : 0);
+                       }),
+                       a[3], out);
+END_CALL
+
+// d_out, expert_out, row_index, weights, out
+CALL(moe_combine_grad, 5)
+    const at::Tensor& d = plain(a[0], "d_out", "a contiguous bf16 or fp16 CUDA matrix", {kBf16, kF16}, 2);
+    const at::ScalarType type = d.scalar_type();
+    const at::Tensor& y = plain(a[1], "expert_out", "a contiguous matrix [rows, n] of d_out's type and device", {type}, 2, &d);
+    const at::Tensor& index = plain(a[2], "row_index", "a contiguous int32 matrix on d_out's device", {kI32}, 2, &d);
+    const at::Tensor& w = plain(a[3], "weights", "a contiguous fp32 matrix on d_out's device", {kF32}, 2, &d);
+    const int64_t tokens = d.size(0), n = d.size(1);
+    if (index.size(0) != tokens || w.sizes() != index.sizes() || y.size(1) != n) {
+        refuse("moe_combine_grad", "d_out [tokens, n], expert_out [rows, n], row_index and weights [tokens, top_k]");
+    }
+    const OnDevice on(d);
+    const at::Tensor dy = result(a[4], "a contiguous matrix of expert_out's shape, type and device", {type}, d, y.size(0), n, type);
+    const at::Tensor dw = at::detail::empty_cuda(w.sizes(), kF32, d.device(), std::nullopt);
+    void *in = d.data_ptr(), *e = y.data_ptr(), *i = index.data_ptr(), *g = w.data_ptr(), *o = dy.data_ptr(), *ow = dw.data_ptr();
+    const uint32_t top_k = (uint32_t)index.size(1), rows = (uint32_t)y.size(0);
+    return with_outputs(released([&] {
+                            return moe_combine_grad_fn(on.stream, in, e, rows, (const int32_t*)i, (const float*)g, o, (float*)ow, (uint32_t)tokens,
+                                                       (uint32_t)n, top_k, type == kF16 ? 1 : 0);
+                        }),
+                        dy, dw);
+END_CALL
+
 // x, w, w_scales, ids, out, out_dtype
 CALL(mx_fp4_matvec_typed, 6)
     const bool many = a[3] != Py_None;
@@ -610,6 +827,12 @@ PyObject* bind(PyObject*, PyObject* args)
     BIND(mx_grouped_gemm_typed)
     BIND(moe_combine)
     BIND(mx_fp4_matvec_typed)
+    BIND(block_quant)
+    BIND(block_gemm)
+    BIND(block_grouped_gemm)
+    BIND(moe_dispatch)
+    BIND(moe_dispatch_grad)
+    BIND(moe_combine_grad)
     BIND(mx_quant_matmul_static)
     BIND(mx_quant_allgather)
     BIND(mx_quant_allgather_matmul)
@@ -633,6 +856,12 @@ PyMethodDef methods[] = {
     METHOD(mx_grouped_gemm_typed),
     METHOD(moe_combine),
     METHOD(mx_fp4_matvec_typed),
+    METHOD(block_quant),
+    METHOD(block_gemm),
+    METHOD(block_grouped_gemm),
+    METHOD(moe_dispatch),
+    METHOD(moe_dispatch_grad),
+    METHOD(moe_combine_grad),
     METHOD(mx_quant_matmul_static),
     METHOD(mx_quant_allgather),
     METHOD(mx_quant_allgather_matmul),

@@ -237,6 +237,81 @@ int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, 
 int catccos_b200_mx_fp4_matvec_typed(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,
                                      uint32_t rows, uint32_t x_rows, uint32_t experts, uint32_t n, uint32_t k, int c_type);
 
+/* ---- blocks of 128 with fp32 scales (one GPU; no counterpart in the reference) ------------------------------------------
+ * The other 8-bit format that checkpoints and training recipes use: E4M3 or E5M2 codes with one fp32 scale for each block of 128
+ * values, activations in blocks of 1 x 128 along the axis that is summed over, weights in blocks of 128 x 128.  As the calls of
+ * the mixture-of-experts layer above these allocate nothing, keep nothing and share no scratch, may be captured and replayed,
+ * check everything before a launch and take an empty batch.  The products run on the acting rank's device.  Element types: 0 =
+ * E4M3, 1 = E5M2, -1 = as the option "a_dtype" (the quantiser's codes, a) or "b_dtype" (b) says. */
+
+/* Quantiser.  For every block, at the edges of what is there: top = max(largest |x|, 2^-100), F = 448 (E4M3) or 57344 (E5M2),
+ *   scale = top / F;   code = RNE, saturating, of x * (F / top)
+ * A block with an infinity or a NaN: scale and codes NaN.  x [rows, k], rows x_row_bytes apart, bf16 (x_type 0), fp16 (1) or fp32
+ * (2); codes [rows, k]; scales fp32
+ *   block 0: [rows, ceil(k / 128)]               1 x 128
+ *   block 1: [ceil(rows / 128), k]               128 x 1
+ *   block 2: [ceil(rows / 128), ceil(k / 128)]   128 x 128
+ * With row_index int32 [rows, top_k] (block 0; else NULL, and top_k and out_rows do not count): codes [out_rows, k] and scales
+ * [out_rows, ceil(k / 128)], and row row_index[t, r] of both is token t's: the dispatch of an expert layer.  Places outside
+ * [0, out_rows) are skipped, rows that no place names stay as they are; a row is named at most once.
+ * k % 16 == 0; x, its rows and codes 16-byte aligned, scales and row_index 4-byte; outputs overlap nothing. */
+int catccos_b200_block_quant(void* stream, const void* x, int x_type, size_t x_row_bytes, uint32_t rows, uint32_t k, int block, int code_type,
+                             const int32_t* row_index, uint32_t top_k, uint32_t out_rows, void* codes, float* scales);
+
+/* A matrix of codes (of several experts: matrices) and its scales.  With [rows, cols] the matrix's shape as the product below has
+ * it, codes are stored row by row, line_bytes >= cols from one row to the next (transposed 0), or column by column, line_bytes >=
+ * rows from one column to the next (transposed 1); 16-byte aligned in all of this.  Scales fp32, any distances (in floats), for
+ * one row or column at a time or for 128: see the calls. */
+typedef struct catccos_b200_block_operand {
+    const void* codes;
+    size_t line_bytes;
+    size_t matrix_bytes;  /* from one expert's codes to the next (the grouped call's b, with more than one expert) */
+    const float* scales;
+    size_t scale_row;     /* from a row's scale (b: of a block of 128 rows) to the next one's */
+    size_t scale_col;     /* from the scale of a block of 128 columns (per_column: of a column) to the next */
+    size_t scale_matrix;  /* from one expert's scales to the next */
+    int transposed;
+    int per_column;       /* b of catccos_b200_block_gemm: one scale for each column of a block of 128 rows */
+    int type;
+} catccos_b200_block_operand_t;
+
+/* c [m, n] = dequant(a [m, k]) x dequant(b [k, n]), c bf16 (c_type 0), fp16 (1), fp32 (2) or, -1, as the option "c_dtype" says.
+ * a has a scale for every row and block of 128 columns; b for every block of 128 x 128, or of 128 rows and one column
+ * (per_column: scale_col 1, scale_row a multiple of 4, 16-byte aligned).  So one call is
+ *   x W       x in blocks 1 x 128, W [k, n] in blocks 128 x 128 (or the checkpoint's [n, k], transposed)
+ *   dy W^T    the same W, transposed the other way
+ *   x^T dy    both in blocks 128 x 1, x transposed, dy per_column
+ * The products of a block are summed by the tensor core, the blocks in fp32, in a fixed order.  n % 16 == 0, k % 16 == 0, a
+ * transposed: m % 16 == 0; c 32-byte aligned, overlapping nothing. */
+int catccos_b200_block_gemm(void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b, void* c, uint32_t m,
+                            uint32_t n, uint32_t k, int c_type);
+
+/* The same for every expert on its own rows: c[offsets[e] .. offsets[e + 1]) = dequant(a rows) x dequant(b[e]), offsets as in
+ * catccos_b200_mx_grouped_gemm.  a not transposed, b not per_column; experts <= 1024. */
+int catccos_b200_block_grouped_gemm(void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b,
+                                    const int32_t* offsets, void* c, uint32_t rows, uint32_t experts, uint32_t n, uint32_t k, int c_type);
+
+/* ---- the rows of an expert layer in 16 bits, and the gradients of their ways there and back -----------------------------------
+ * row_index int32 [tokens, top_k] as catccos_b200_moe_row_plan writes it: places outside [0, rows) are dropped routes, a row is
+ * named at most once (where a row is written), rows that no place names stay as they are.  n % 8 == 0, rows 16-byte aligned. */
+
+/* out[row_index[t, r]] = x[t]: x [tokens, n], out [rows, n], any 16-bit type. */
+int catccos_b200_moe_dispatch(void* stream, const void* x, const int32_t* row_index, void* out, uint32_t tokens, uint32_t rows, uint32_t n,
+                              uint32_t top_k);
+
+/* Its gradient: out[t] = sum over r of d_rows[row_index[t, r]] (+ shared[t]), r ascending, in fp32, rounded once; bf16 (f16 0) or
+ * fp16 (1).  shared (or NULL) [tokens, n]: the gradient that reaches x another way; out may be shared. */
+int catccos_b200_moe_dispatch_grad(void* stream, const void* d_rows, uint32_t rows, const int32_t* row_index, const void* shared, void* out,
+                                   uint32_t tokens, uint32_t n, uint32_t top_k, int f16);
+
+/* The gradient of catccos_b200_moe_combine (that of its shared_out is d_out itself):
+ *   d_expert_out[row_index[t, r]] = weights[t, r] * d_out[t], rounded once
+ *   d_weights[t, r] = sum over columns of d_out[t] * expert_out[row_index[t, r]], in fp32; 0 for a dropped route
+ * d_out [tokens, n], expert_out and d_expert_out [rows, n]: bf16 (f16 0) or fp16 (1); weights and d_weights fp32 [tokens, top_k].
+ * d_expert_out may be expert_out. */
+int catccos_b200_moe_combine_grad(void* stream, const void* d_out, const void* expert_out, uint32_t rows, const int32_t* row_index,
+                                  const float* weights, void* d_expert_out, float* d_weights, uint32_t tokens, uint32_t n, uint32_t top_k, int f16);
+
 /* Quantise + matmul on one GPU that allocates nothing.  It has no counterpart in the reference.
  * c [m, n] = dequant(quantise(a_bf16 [m, k])) x dequant(b [k, n], b_scale [k/64, n, 2]): the same two
  * stages as catccos_b200_mx_quant_allgather_matmul at rankSize 1, but the quantised copy of A
