@@ -95,7 +95,7 @@ __device__ __forceinline__ void tmem_ld_fence(float (&r)[16])
 
 // Sixteen columns of a row to global memory; p is aligned to their size or 32 bytes
 template <typename OutT>
-__device__ __forceinline__ void store_16(OutT* p, const float (&v)[16])
+__device__ __forceinline__ void store_16(OutT* p, const float* v)
 {
     if constexpr (sizeof(OutT) == 4) {
         uint32_t o[2][8];
@@ -112,6 +112,27 @@ __device__ __forceinline__ void store_16(OutT* p, const float (&v)[16])
             o[i] = pack2<OutT>(v[2 * i], v[2 * i + 1]);
         }
         st_global_v8(p, o);
+    }
+}
+
+// sums += f * the tile's kCols columns of this lane's row; by column: f * scale[column] * it.  The next sixteen columns are on
+// their way while these are added.
+template <uint32_t kCols, bool kByColumn>
+__device__ __forceinline__ void promote(float (&acc)[kCols], uint32_t tmem, float f, const float* scale)
+{
+    float r[2][16];
+    tmem_ld_16(tmem, r[0]);
+#pragma unroll
+    for (uint32_t c = 0; c < kCols; c += 16) {
+        float (&v)[16] = r[(c / 16) & 1];
+        tmem_ld_fence(v);
+        if (c + 16 < kCols) {
+            tmem_ld_16(tmem + c + 16, r[(c / 16 + 1) & 1]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+            acc[c + j] = fmaf(v[j], kByColumn ? f * scale[c + j] : f, acc[c + j]);
+        }
     }
 }
 
@@ -190,7 +211,7 @@ struct BlockGemmSmem {
     static constexpr uint32_t kScaleSlots = kStages + 2;
     static constexpr uint32_t kOffScale = kOffB + kStages * kBBytes;
     static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * BLOCK_N * 4;
-    static constexpr uint32_t kNumBars = 2 * kStages + 4;  // full[S], empty[S], tmem_full[2], tmem_empty[2]
+    static constexpr uint32_t kNumBars = 2 * kStages + 4 + kScaleSlots;  // full[S], empty[S], tmem_full[2], tmem_empty[2], scale_full[]
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
     static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
@@ -215,6 +236,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     uint64_t* empty = full + kStages;
     uint64_t* tmem_full = empty + kStages;
     uint64_t* tmem_empty = tmem_full + 2;
+    uint64_t* scale_full = tmem_empty + 2;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
@@ -237,6 +259,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         for (uint32_t a = 0; a < 2; ++a) {
             mbar_init(&tmem_full[a], 1);
             mbar_init(&tmem_empty[a], 8);
+        }
+        for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
+            mbar_init(&scale_full[i], 1);
         }
         *dead = 0u;
         mbar_fence_init();
@@ -267,8 +292,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
             const uint32_t m0 = row_begin[walk.e] + tc.m_tile * kBlockGemmM, n0 = tc.n_tile * BLOCK_N;
             const uint32_t boxes = (min(row_end[walk.e] - m0, kBlockGemmM) + 31u) / 32u;  // of 32 rows
-            const uint32_t scale_bytes = kByColumn ? min(p.N - n0, BLOCK_N) * 4u : 0u;
-            const uint32_t tx_bytes = (p.a_cols ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes + scale_bytes;
+            const uint32_t scale_bytes = min(p.N - n0, BLOCK_N) * 4u;
+            const uint32_t tx_bytes = (p.a_cols ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes;
             for (uint32_t kb = kb0; alive && kb < kb1; ++kb, ++it) {
                 const uint32_t s = it % kStages;
                 alive = mbar_wait_warp(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 400, s, bar_ns);
@@ -293,8 +318,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                     if (kByColumn) {
                         // Step `it` may overwrite the scales of step it - kStages - 2: the product of it - kStages has been
                         // multiplied (empty[s]), for which the tile of it - kStages - 2 had to be promoted (tmem_empty).
-                        bulk_load(smem + S::kOffScale + (it % S::kScaleSlots) * (BLOCK_N * 4u),
-                                  p.b_scales + (size_t)walk.e * p.b_scale_matrix + kb * p.b_scale_block + n0, scale_bytes, &full[s]);
+                        const uint32_t slot = it % S::kScaleSlots;
+                        mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
+                        bulk_load(smem + S::kOffScale + slot * (BLOCK_N * 4u), p.b_scales + kb * p.b_scale_block + n0, scale_bytes, &scale_full[slot]);
                     }
                 }
                 __syncwarp();
@@ -352,22 +378,17 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 const uint32_t buf = it & 1u;
                 const float f = kByColumn ? sa.get(i) : sa.get(i) * sb.get(i);
                 alive = mbar_wait_warp(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
+                const uint32_t slot = it % S::kScaleSlots;
+                if (kByColumn && alive) {
+                    alive = mbar_wait_warp(&scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 407, slot, bar_ns);
+                }
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
                 tcgen05_fence_after();
                 if (live) {
-                    const float* scale = reinterpret_cast<const float*>(smem + S::kOffScale) + (it % S::kScaleSlots) * BLOCK_N + half * kCols;
-#pragma unroll
-                    for (uint32_t c = 0; c < kCols; c += 16) {
-                        float r[16];
-                        tmem_ld_16(tmem + buf * BLOCK_N + c, r);
-                        tmem_ld_fence(r);
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) {
-                            acc[c + j] = fmaf(r[j], kByColumn ? f * scale[c + j] : f, acc[c + j]);
-                        }
-                    }
+                    promote<kCols, kByColumn>(acc, tmem + buf * BLOCK_N, f,
+                                              reinterpret_cast<const float*>(smem + S::kOffScale) + slot * BLOCK_N + half * kCols);
                 }
                 tcgen05_fence_before();
                 __syncwarp();
@@ -380,12 +401,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #pragma unroll
                 for (uint32_t c = 0; c < kCols; c += 16) {
                     if (n0 + half * kCols + c < p.N) {
-                        float v[16];
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j) {
-                            v[j] = acc[c + j];
-                        }
-                        store_16(dst + c, v);
+                        store_16(dst + c, &acc[c]);
                     }
                 }
             }

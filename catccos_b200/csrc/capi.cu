@@ -16,6 +16,7 @@
 
 #include "../../include/catccos_b200.h"
 #include "block_gemm.cuh"
+#include "block_gemm_pair.cuh"
 #include "block_quant.cuh"
 #include "bootstrap.hpp"
 #include "internal_options.h"
@@ -1609,32 +1610,47 @@ int grouped_maps(CUtensorMap (&maps)[3], const void* a, uint64_t a_row_bytes, co
     return rcode;
 }
 
-template <typename OutT>
-int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
+// How many CTA pairs of a kernel (with clusters of two in its declaration) run at one time on the current device, asked once.
+template <typename Kernel>
+cudaError_t resident_clusters_of_two(const RankCtx& rc, Kernel kern, uint32_t threads, size_t smem, PerDevice<int, kMaxRanks * 2>& resident, int* pairs)
 {
-    auto kern = mx_grouped_pair_kernel<OutT>;
-    static PerDevice<int, kMaxRanks * 2> resident;
     int dev = 0;
-    CUDA_TRY(cudaGetDevice(&dev));
-    int pairs = resident.get(dev);
-    if (pairs == 0) {
-        CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PairSmem::kDynamicBytes));
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) {
+        return err;
+    }
+    *pairs = resident.get(dev);
+    if (*pairs == 0) {
+        err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) {
+            return err;
+        }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)rc.num_sms / 2 * 2);
-        cfg.blockDim = dim3(kGemmThreads);
-        cfg.dynamicSmemBytes = PairSmem::kDynamicBytes;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 2;
         attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs < 1) {
+        if (cudaOccupancyMaxActiveClusters(pairs, kern, &cfg) != cudaSuccess || *pairs < 1) {
             cudaGetLastError();
-            pairs = rc.num_sms / 2;
+            *pairs = rc.num_sms / 2;
         }
-        resident.set(dev, pairs);
+        resident.set(dev, *pairs);
     }
+    return cudaSuccess;
+}
+
+template <typename OutT>
+int launch_grouped_pair(RankCtx& rc, cudaStream_t st, const void* a, uint64_t a_row_bytes, const void* b, const GroupedParams& p)
+{
+    auto kern = mx_grouped_pair_kernel<OutT>;
+    static PerDevice<int, kMaxRanks * 2> resident;
+    int pairs = 0;
+    CUDA_TRY(resident_clusters_of_two(rc, kern, kGemmThreads, PairSmem::kDynamicBytes, resident, &pairs));
     CUtensorMap maps[3];
     int rcode = grouped_maps(maps, a, a_row_bytes, b, p, kGemmBlockM);
     if (rcode != 0) return rcode;
@@ -1780,9 +1796,41 @@ int launch_block_gemm_inst(RankCtx& rc, cudaStream_t st, const BlockOperands& o,
     return 0;
 }
 
+template <typename OutT, bool kByColumn>
+int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
+{
+    using S = BlockPairSmem;
+    auto kern = block_gemm_pair_kernel<OutT, kByColumn>;
+    static PerDevice<int, kMaxRanks * 2> resident;
+    int pairs = 0;
+    CUDA_TRY(resident_clusters_of_two(rc, kern, kBlockPairThreads, S::dynamic_bytes(kGroupedMaxExperts), resident, &pairs));
+    static PerDevice<bool, kMaxRanks * 2> checked;
+    if (!checked.get(rc.device)) {
+        // the kernel's warps hand registers on: they wait for more than it was launched with for ever
+        cudaFuncAttributes attr;
+        CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
+        if ((uint32_t)attr.numRegs != kBlockPairRegs) {
+            ERROR_LOG("block_gemm_pair_kernel was built with %d registers a thread, not %u", attr.numRegs, kBlockPairRegs);
+            return CATCCOS_B200_ESTATE;
+        }
+        checked.set(rc.device, true);
+    }
+    CUtensorMap maps[3];
+    int rcode = block_maps(maps, o, p, 128);
+    if (rcode != 0) return rcode;
+    const uint64_t tiles = p.offsets ? p.rows / kPairBlockM + std::min(p.rows, p.experts) : (p.rows + kPairBlockM - 1) / kPairBlockM;
+    const uint64_t units = tiles * ((p.N + kPairBlockN - 1) / kPairBlockN);
+    CUDA_TRY(launch_after(kern, dim3(2u * (unsigned)std::min<uint64_t>(units, (uint64_t)pairs)), kBlockPairThreads, S::dynamic_bytes(p.experts), st,
+                          maps[0], maps[1], maps[2], p));
+    return 0;
+}
+
 template <typename OutT>
 int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
 {
+    if (g.cta_pair == 1 || (g.cta_pair == 0 && p.rows >= 1024)) {
+        return o.b->per_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
+    }
     if (o.b->per_column) {
         return launch_block_gemm_inst<128, OutT, true>(rc, st, o, p);
     }
