@@ -41,6 +41,19 @@ struct BlockGemmParams {
     StatusBlock* status;
 };
 
+// mbar_wait_warp whose first polls do not look at the clock: reading it takes longer than what these barriers are waited for (a
+// tile's way from the tensor core to the promotion and back counts in every block of K).
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, StatusBlock* st, uint32_t id, uint32_t stage, uint64_t limit_ns)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; i < 4096u; ++i) {
+        if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) {
+            return true;
+        }
+    }
+    return mbar_wait_warp(bar, parity, st, id, stage, limit_ns);
+}
+
 // Instruction descriptor of kind::f8f6f4 with fp32 accumulators: make_idesc_mxf8's fields without the scales' (bits 4, 5: fp32)
 __host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t M, uint32_t N, uint32_t a_fmt, uint32_t b_fmt, bool a_mn, bool b_mn)
 {
@@ -93,6 +106,17 @@ __device__ __forceinline__ void tmem_ld_fence(float (&r)[16])
                  : "memory");
 }
 
+// Thirty-two columns, there when it returns
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float (&r)[32])
+{
+    float (&lo)[16] = *reinterpret_cast<float (*)[16]>(&r[0]);
+    float (&hi)[16] = *reinterpret_cast<float (*)[16]>(&r[16]);
+    tmem_ld_16(taddr, lo);
+    tmem_ld_16(taddr + 16u, hi);
+    tmem_ld_fence(lo);
+    tmem_ld_fence(hi);
+}
+
 // Sixteen columns of a row to global memory; p is aligned to their size or 32 bytes
 template <typename OutT>
 __device__ __forceinline__ void store_16(OutT* p, const float* v)
@@ -115,8 +139,23 @@ __device__ __forceinline__ void store_16(OutT* p, const float* v)
     }
 }
 
-// sums += f * the tile's kCols columns of this lane's row; by column: f * scale[column] * it.  The next sixteen columns are on
-// their way while these are added.
+// (a0, a1) += (x0, x1) * (y0, y1), each rounded once, in one instruction
+__device__ __forceinline__ void fma_2(float& a0, float& a1, float x0, float x1, float y0, float y1)
+{
+    asm("{\n\t"
+        ".reg .b64 a, x, y;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 y, {%4, %5};\n\t"
+        "fma.rn.f32x2 a, x, y, a;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t"
+        "}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+
+// sums += f * the tile's kCols columns of this lane's row; by column: f * scale[column] * it.  The next sixteen columns
+// are on their way while these are added.
 template <uint32_t kCols, bool kByColumn>
 __device__ __forceinline__ void promote(float (&acc)[kCols], uint32_t tmem, float f, const float* scale)
 {
@@ -130,8 +169,23 @@ __device__ __forceinline__ void promote(float (&acc)[kCols], uint32_t tmem, floa
             tmem_ld_16(tmem + c + 16, r[(c / 16 + 1) & 1]);
         }
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) {
-            acc[c + j] = fmaf(v[j], kByColumn ? f * scale[c + j] : f, acc[c + j]);
+        for (uint32_t j = 0; j < 16; j += 2) {
+            fma_2(acc[c + j], acc[c + j + 1], v[j], v[j + 1], kByColumn ? f * scale[c + j] : f, kByColumn ? f * scale[c + j + 1] : f);
+        }
+    }
+}
+
+// A line's scales of blocks kb .. kb + 3 of K (those behind the last: 0); they are `step` floats apart.
+__device__ __forceinline__ void load_scales(const float* line, size_t step, uint32_t kb, uint32_t blocks, float (&v)[4])
+{
+    const float* at = line + kb * step;
+    if (step == 1 && kb + 4u <= blocks && ((uintptr_t)at & 15u) == 0u) {
+        const float4 w = __ldcg(reinterpret_cast<const float4*>(at));
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            v[j] = kb + j < blocks ? __ldcg(at + j * step) : 0.0f;
         }
     }
 }
@@ -296,7 +350,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const uint32_t tx_bytes = (p.a_cols ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes;
             for (uint32_t kb = kb0; alive && kb < kb1; ++kb, ++it) {
                 const uint32_t s = it % kStages;
-                alive = mbar_wait_warp(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 400, s, bar_ns);
+                alive = mbar_wait_soon(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 400, s, bar_ns);
                 if (!alive) {
                     break;
                 }
@@ -342,8 +396,8 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const uint32_t idesc = idesc0 | ((min(p.N - unit % n_tiles * BLOCK_N, BLOCK_N) >> 3) << 17);
             for (uint32_t i = 0; alive && i < steps; ++i, ++it) {
                 const uint32_t s = it % kStages, buf = it & 1u;
-                alive = mbar_wait_warp(&tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, buf, bar_ns) &&
-                        mbar_wait_warp(&full[s], (it / kStages) & 1u, p.status, 403, s, bar_ns);
+                alive = mbar_wait_soon(&tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, buf, bar_ns) &&
+                        mbar_wait_soon(&full[s], (it / kStages) & 1u, p.status, 403, s, bar_ns);
                 if (!alive) {
                     break;  // nothing is issued, and no tile reported, after a wait has given up
                 }
@@ -377,10 +431,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             for (uint32_t i = 0; i < steps; ++i, ++it) {
                 const uint32_t buf = it & 1u;
                 const float f = kByColumn ? sa.get(i) : sa.get(i) * sb.get(i);
-                alive = mbar_wait_warp(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
+                alive = mbar_wait_soon(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
                 const uint32_t slot = it % S::kScaleSlots;
                 if (kByColumn && alive) {
-                    alive = mbar_wait_warp(&scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 407, slot, bar_ns);
+                    alive = mbar_wait_soon(&scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 407, slot, bar_ns);
                 }
                 if (!alive) {
                     break;  // a tile that never filled is not written out

@@ -1,17 +1,24 @@
 // The products of block_gemm.cuh on CTA pairs (clusters of two SMs, tcgen05 cta_group::2), for calls that fill the GPU with 256 x 256
 // tiles.
 //
-// CTA r of a pair loads rows [128 r, +128) of A and columns [128 r, +128) of B (of a ragged last column of tiles, its half) with
-// plain TMA, 32 KB a block of K where a 128 x 256 tile on one SM takes 48; the leader issues the products of both, and each CTA
-// has the tile of its own 128 rows and all 256 columns in its own tensor memory.  Two such tiles fill tensor memory: one is
-// multiplied while the sixteen promotion warps (row = lane, 64 columns each) scale the other and add it to their sums.
+// CTA r of a pair loads rows [128 r, +128) of A and columns [128 r, +128) of B with plain TMA, 32 KB a block of K where a 128 x 256
+// tile on one SM takes 48; the leader issues the products of both, and each CTA has the results for its own 128 rows and all 256
+// columns in its own tensor memory.
 //
-//   full[s], tmem_empty[b]     live in the leader; both CTAs' TMA bytes, and promotion warps, go there
-//   empty[s], tmem_full[b]     live in each CTA; the leader's tcgen05.commit arrives on both copies
+// A block's way from the tensor core through the promotion and back takes longer than its products: about 1000 cycles until a
+// finished product is seen, 300 for the promotion, 200 back, against 512.  Two tiles of 256 columns (all that tensor memory
+// holds) would leave the tensor core waiting half of the time, so the columns are two halves, each with two tiles of its own,
+// multiplied one after the other: half h has columns 64 h to 64 h + 63 of each CTA's B.
+//
+//   full[s], tmem_empty[h][b]   live in the leader; both CTAs' TMA bytes, and a warp of each CTA's promotion, go there
+//   empty[s], tmem_full[h][b]   live in each CTA; the leader's tcgen05.commit arrives on both copies
 //   scale_full[i], scale_empty[i]  live in each CTA: the factors of its rows (and, by column, of the columns) for one block of K
 //
-// 640 threads: warps 0-15 promotion and output (warp w: lane quarter w % 4, columns 64 (w / 4)), warp 16 TMA, 17 MMA, 18 and 19
-// the factors: a row's scale times that of each half of the columns.  The promotion warps take registers from the other four.
+// 640 threads: warps 0-15 promotion and output (warp w: half w / 8, lane quarter w % 4, the half's columns of CTA (w / 4) % 2's B),
+// warp 16 TMA, 17 and 18 the products of a half each, 19 the factors: a row's scale times that of each CTA's columns.  The
+// promotion warps take registers from the other four.  A look at a barrier in shared memory takes some 150 cycles, so no warp of
+// the promotion makes two in a row: of a half's eight warps one waits for the tile, one for the factors of the next block, which all
+// fetch ahead, one gives the tile back and one the factors, and named barriers join them.
 #pragma once
 
 #include "block_gemm.cuh"
@@ -32,30 +39,55 @@ struct BlockPairSmem {
     static constexpr uint32_t kBBytes = 128 * 128;  // this CTA's columns
     static constexpr uint32_t kOffA = 0;
     static constexpr uint32_t kOffB = kOffA + kStages * kABytes;
-    static constexpr uint32_t kScaleSlots = 4;
+    static constexpr uint32_t kScaleSlots = 8;
     static constexpr uint32_t kOffScale = kOffB + kStages * kBBytes;               // by column: 256 scales a slot
-    static constexpr uint32_t kOffFactor = kOffScale + kScaleSlots * kPairBlockN * 4;  // [half][128 rows] a slot
+    static constexpr uint32_t kOffFactor = kOffScale + kScaleSlots * kPairBlockN * 4;  // [CTA whose columns][128 rows] a slot
     static constexpr uint32_t kOffBar = kOffFactor + kScaleSlots * 256 * 4;
-    static constexpr uint32_t kNumBars = 2 * kStages + 4 + 2 * kScaleSlots;
+    static constexpr uint32_t kNumBars = 2 * kStages + 8 + 2 * kScaleSlots;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
     static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
 };
 static_assert(BlockPairSmem::dynamic_bytes(kGroupedMaxExperts) <= 232448, "one CTA's shared memory");
 
-__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                             uint32_t accumulate)
+// One block of K: four products (K = 32) into the tile at tmem_d, then arrivals on both CTAs' `done` and `empty` when
+// they are finished.  Called by a converged warp, of which one lane issues everything: a branch on the lane around each instruction would
+// cost more than the instruction, and the next block's way through the promotion waits for this one.
+__device__ __forceinline__ void umma_f8_pair_block(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t a_step, uint32_t b_lo, uint32_t b_hi,
+                                                   uint32_t b_step, uint32_t idesc, uint64_t* done, uint64_t* empty)
 {
     asm volatile(
         "{\n\t"
-        ".reg .pred p;\n\t"
+        ".reg .pred one, add;\n\t"
         ".reg .b64 da, db;\n\t"
+        ".reg .b32 a, b;\n\t"
+        ".reg .b16 both;\n\t"
+        "mov.b16 both, 3;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "setp.ne.b32 add, 0, 0;\n\t"
         "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %5, p;\n\t"
+        "mov.b64 db, {%4, %5};\n\t"
+        "@one tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "setp.eq.b32 add, 0, 0;\n\t"
+        "add.u32 a, %1, %3;\n\t"
+        "add.u32 b, %4, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "add.u32 a, a, %3;\n\t"
+        "add.u32 b, b, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "add.u32 a, a, %3;\n\t"
+        "add.u32 b, b, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "@one tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%8], both;\n\t"
+        "@one tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%9], both;\n\t"
         "}"
-        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(a_step), "r"(b_lo), "r"(b_hi), "r"(b_step), "r"(idesc), "r"(smem_u32(done)), "r"(smem_u32(empty))
         : "memory");
 }
 
@@ -65,6 +97,23 @@ __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tma
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
         ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
         : "memory");
+}
+
+// Of the eight warps of a CTA that promote a half: true on all if all say so.
+__device__ __forceinline__ bool promoters_agree(uint32_t barrier, bool ok)
+{
+    uint32_t bad;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t"
+        "}"
+        : "=r"(bad)
+        : "r"(ok ? 0u : 1u), "r"(barrier), "n"(16 * kBlockPairPromoters)
+        : "memory");
+    return bad == 0u;
 }
 
 template <typename OutT, bool kByColumn>
@@ -81,8 +130,8 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
     uint64_t* empty = full + kStages;
     uint64_t* tmem_full = empty + kStages;
-    uint64_t* tmem_empty = tmem_full + 2;
-    uint64_t* scale_full = tmem_empty + 2;
+    uint64_t* tmem_empty = tmem_full + 4;  // [half][tile]
+    uint64_t* scale_full = tmem_empty + 4;
     uint64_t* scale_empty = scale_full + S::kScaleSlots;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
@@ -99,15 +148,15 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     if (threadIdx.x == 32 * kBlockPairPromoters) {
         for (uint32_t s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 2);  // both CTAs' producers (expect_tx)
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], 2);  // the products of both halves
         }
-        for (uint32_t b = 0; b < 2; ++b) {
+        for (uint32_t b = 0; b < 4; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], 2 * kBlockPairPromoters);  // of both CTAs
+            mbar_init(&tmem_empty[b], 2);  // a warp of each CTA, for all that promote the half
         }
         for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
-            mbar_init(&scale_full[i], kByColumn ? 3 : 2);  // warps 18 and 19 (and the columns' bytes)
-            mbar_init(&scale_empty[i], kBlockPairPromoters);
+            mbar_init(&scale_full[i], kByColumn ? 2 : 1);  // the rows' factors (and the columns' bytes)
+            mbar_init(&scale_empty[i], 2);  // a warp of each half
         }
         mbar_fence_init();
         tma_prefetch_desc(&tmap_a);
@@ -131,14 +180,12 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     bool alive = true;  // false once a wait of this role has given up
 
     struct Unit {
-        uint32_t e, m0, end, n0, width;  // expert; first row of the pair's tile, end of the expert's rows; first column, columns multiplied
+        uint32_t e, m0, end, n0;  // expert; first row of the pair's tile, end of the expert's rows; first column
     };
     GroupedWalk walk;
     auto unit_at = [&](uint32_t unit) {
         const TileCoord tc = walk.seek(tiles, n_tiles, unit);
-        const uint32_t left = p.N - tc.n_tile * kPairBlockN;
-        return Unit{walk.e, row_begin[walk.e] + tc.m_tile * kPairBlockM, row_end[walk.e], tc.n_tile * kPairBlockN,
-                    left < kPairBlockN ? (left + 31u) / 32u * 32u : kPairBlockN};
+        return Unit{walk.e, row_begin[walk.e] + tc.m_tile * kPairBlockM, row_end[walk.e], tc.n_tile * kPairBlockN};
     };
 
     // The changes of registers belong into the branches: code behind one is built for as many as the branch then has, and code
@@ -153,11 +200,11 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 const uint32_t m0 = u.m0 + cta * 128u;
                 const uint32_t boxes = m0 < u.end ? (min(u.end - m0, 128u) + 31u) / 32u : 0u;  // of 32 rows
                 const uint32_t tx_bytes = (p.a_cols && boxes ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes;
-                const int32_t n = (int32_t)(u.n0 + cta * (u.width / 2u));
+                const int32_t n = (int32_t)(u.n0 + cta * 128u);
                 for (uint32_t kb = 0; alive && kb < k_blocks; ++kb, ++it) {
                     const uint32_t s = it % kStages;
                     const uint32_t leader_bar = map_to_cta(smem_u32(&full[s]), 0);
-                    alive = mbar_wait_warp(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 500, s, bar_ns);
+                    alive = mbar_wait_soon(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 500, s, bar_ns);
                     if (!alive) {
                         break;
                     }
@@ -181,83 +228,88 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     __syncwarp();
                 }
             }
-        } else if (warp == 17) {
-            // ------------------------------- MMA issuer (leader CTA only) ---------------------
+        } else if (warp < 19) {
+            // ------------------------------- MMA issuers (leader CTA only) --------------------
             if (cta == 0) {
+                const uint32_t half = warp - 17u;
                 const uint32_t idesc0 = make_idesc_f8(kPairBlockM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
                 const uint64_t desc_k = make_smem_desc(0, 16, 1024, 2), desc_mn = make_smem_desc(0, 16384, 1024, 2);
                 const uint64_t desc_a = p.a_cols ? desc_mn : desc_k, desc_b = p.b_rows ? desc_k : desc_mn;
                 const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
                 const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
-                const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4);
+                const uint32_t b_lo0 = ((uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4)) + half * ((p.b_rows ? 64u * 128u : 64u) >> 4);
                 const uint32_t step_a = (p.a_cols ? 4096u : 32u) >> 4, step_b = (p.b_rows ? 32u : 4096u) >> 4;
+                uint64_t* const tile_full = tmem_full + 2u * half;
+                uint64_t* const tile_empty = tmem_empty + 2u * half;
                 uint32_t s = 0, ph = 0, it = 0;
                 for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
-                    const uint32_t idesc = idesc0 | ((unit_at(unit).width >> 3) << 17);
+                    // of a ragged last column of tiles as much is multiplied as the leader's columns need (the other CTA's are
+                    // fewer), at least the smallest product
+                    const uint32_t left = p.N - unit_at(unit).n0;
+                    const uint32_t columns = min(max(left, 64u * half + 16u) - 64u * half, 64u);
+                    const uint32_t idesc = idesc0 | (((columns + 15u) / 16u * 32u >> 3) << 17);
                     for (uint32_t i = 0; alive && i < k_blocks; ++i, ++it) {
                         const uint32_t buf = it & 1u;
-                        alive = mbar_wait_warp(&tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 501, buf, bar_ns) &&
-                                mbar_wait_warp(&full[s], ph, p.status, 503, s, bar_ns);
+                        // the operands are there before the tile is free, as a rule: what is waited for last is what counts
+                        alive = mbar_wait_soon(&full[s], ph, p.status, 503, s, bar_ns) &&
+                                mbar_wait_soon(&tile_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 501 + half, buf, bar_ns);
                         if (!alive) {
                             break;  // nothing is issued, and no tile reported, after a wait has given up
                         }
                         tcgen05_fence_after();
-                        if (elect_one()) {
-                            const uint32_t a_lo = a_lo0 + s * (S::kABytes >> 4), b_lo = b_lo0 + s * (S::kBBytes >> 4);
-#pragma unroll
-                            for (uint32_t j = 0; j < 4; ++j) {
-                                umma_f8_pair(tmem_base + buf * kPairBlockN, a_lo + j * step_a, hi_a, b_lo + j * step_b, hi_b, idesc, j);
-                            }
-                            tcgen05_commit_pair(&empty[s], 3);
-                            tcgen05_commit_pair(&tmem_full[buf], 3);
-                        }
-                        __syncwarp();
+                        umma_f8_pair_block(tmem_base + half * 256u + buf * 128u, a_lo0 + s * (S::kABytes >> 4), hi_a, step_a,
+                                           b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b, idesc, &tile_full[buf], &empty[s]);
                         s = (s + 1 == kStages) ? 0u : s + 1;
                         ph ^= s == 0u ? 1u : 0u;
                     }
                 }
             }
-        } else if (warp >= 18) {
+        } else {
             // ------------------------------- factors (both CTAs, own 128 rows) ----------------
-            const uint32_t r0 = (warp - 18u) * 64u + lane;  // this lane's rows: r0 and r0 + 32
             uint32_t it = 0;
             for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
                 const Unit u = unit_at(unit);
-                const uint32_t row = u.m0 + cta * 128u + r0;
+                const uint32_t row = u.m0 + cta * 128u + lane;
                 const uint32_t scale_bytes = min(p.N - u.n0, kPairBlockN) * 4u;
                 const float* b_scales = p.b_scales + u.e * p.b_scale_matrix + (u.n0 / 128u) * p.b_scale_col;
-                ScaleReader sa[2], sb[2];
+                const size_t b_next = u.n0 + 128u < p.N ? p.b_scale_col : 0u;
+                for (uint32_t kb0 = 0; alive && kb0 < k_blocks; kb0 += 4u) {
+                    float a[4][4], b[2][4];  // of four blocks
 #pragma unroll
-                for (uint32_t i = 0; i < 2; ++i) {
-                    sa[i].start(p.a_scales + min(row + 32u * i, u.end - 1u) * p.a_scale_row, p.a_scale_block, 0, k_blocks);
-                    sb[i].start(b_scales + (u.n0 + 128u * i < p.N ? i : 0u) * p.b_scale_col, p.b_scale_block, 0, kByColumn ? 0u : k_blocks);
-                }
-                for (uint32_t kb = 0; alive && kb < k_blocks; ++kb, ++it) {
-                    const uint32_t slot = it % S::kScaleSlots;
-                    float a[2], b[2];
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        load_scales(p.a_scales + min(row + 32u * i, u.end - 1u) * p.a_scale_row, p.a_scale_block, kb0, k_blocks, a[i]);
+                    }
+                    if (!kByColumn) {
+                        load_scales(b_scales, p.b_scale_block, kb0, k_blocks, b[0]);
+                        load_scales(b_scales + b_next, p.b_scale_block, kb0, k_blocks, b[1]);
+                    }
 #pragma unroll
-                    for (uint32_t i = 0; i < 2; ++i) {
-                        a[i] = sa[i].get(kb);
-                        b[i] = kByColumn ? 1.0f : sb[i].get(kb);
-                    }
-                    alive = mbar_wait_warp(&scale_empty[slot], ((it / S::kScaleSlots) & 1u) ^ 1u, p.status, 505, slot, bar_ns);
-                    if (!alive) {
-                        break;
-                    }
-                    if (kByColumn && warp == 18 && elect_one()) {
-                        mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
-                        bulk_load(smem + S::kOffScale + slot * (kPairBlockN * 4u), p.b_scales + kb * p.b_scale_block + u.n0, scale_bytes,
-                                  &scale_full[slot]);
-                    }
-                    __syncwarp();
-                    float* factor = reinterpret_cast<float*>(smem + S::kOffFactor) + slot * 256u + r0;
-                    factor[0] = a[0] * b[0];
-                    factor[32] = a[1] * b[0];
-                    factor[128] = a[0] * b[1];
-                    factor[160] = a[1] * b[1];
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(&scale_full[slot]);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        if (kb0 + j >= k_blocks || !alive) {
+                            break;
+                        }
+                        const uint32_t slot = it % S::kScaleSlots;
+                        alive = mbar_wait_soon(&scale_empty[slot], ((it / S::kScaleSlots) & 1u) ^ 1u, p.status, 505, slot, bar_ns);
+                        if (!alive) {
+                            break;
+                        }
+                        if (kByColumn && elect_one()) {
+                            mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
+                            bulk_load(smem + S::kOffScale + slot * (kPairBlockN * 4u), p.b_scales + (kb0 + j) * p.b_scale_block + u.n0, scale_bytes,
+                                      &scale_full[slot]);
+                        }
+                        __syncwarp();
+                        float* factor = reinterpret_cast<float*>(smem + S::kOffFactor) + slot * 256u + lane;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            factor[32u * i] = kByColumn ? a[i][j] : a[i][j] * b[0][j];
+                            factor[128u + 32u * i] = kByColumn ? a[i][j] : a[i][j] * b[1][j];
+                        }
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&scale_full[slot]);
+                        }
+                        ++it;
                     }
                 }
             }
@@ -267,10 +319,19 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBlockPairPromoteRegs));
         // ------------------------------- promotion and output (both CTAs, own 128 rows) ---
-        const uint32_t q = warp & 3u, col = (warp >> 2) * kCols;
-        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + col;
-        const uint32_t free_bar0 = map_to_cta(smem_u32(&tmem_empty[0]), 0), free_bar1 = map_to_cta(smem_u32(&tmem_empty[1]), 0);
+        const uint32_t q = warp & 3u, half = warp >> 3, from = (warp >> 2) & 1u, col = from * 128u + half * kCols;
+        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + half * 256u + from * kCols, w8 = warp & 7u;
+        const float* factors = reinterpret_cast<const float*>(smem + S::kOffFactor) + from * 128u + q * 32u + lane;
+        const uint32_t free_bar0 = map_to_cta(smem_u32(&tmem_empty[2u * half]), 0), free_bar1 = map_to_cta(smem_u32(&tmem_empty[2u * half + 1u]), 0);
         uint32_t it = 0;
+        float next = 0.0f;  // the next block's factor
+        if (pair < num_units) {
+            if (w8 == 1u) {
+                alive = mbar_wait_soon(&scale_full[0], 0, p.status, 508, 0, bar_ns);
+            }
+            alive = promoters_agree(1u + half, alive);
+            next = factors[0];
+        }
         for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
             const Unit u = unit_at(unit);
             const uint32_t row0 = u.m0 + cta * 128u + q * 32u, row = row0 + lane, col0 = u.n0 + col;
@@ -278,21 +339,35 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             float acc[kCols] = {};
             for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
                 const uint32_t buf = it & 1u, slot = it % S::kScaleSlots;
-                alive = mbar_wait_warp(&scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 507, slot, bar_ns) &&
-                        mbar_wait_warp(&tmem_full[buf], (it >> 1) & 1u, p.status, 506, buf, bar_ns);
+                if (w8 == 0u) {
+                    alive = mbar_wait_soon(&tmem_full[2u * half + buf], (it >> 1) & 1u, p.status, 506, buf, bar_ns);
+                } else if (w8 == 1u && (i + 1u < k_blocks || unit + num_pairs < num_units)) {
+                    const uint32_t nt = it + 1u;
+                    alive = mbar_wait_soon(&scale_full[nt % S::kScaleSlots], (nt / S::kScaleSlots) & 1u, p.status, 507, nt % S::kScaleSlots, bar_ns);
+                }
+                alive = promoters_agree(1u + half, alive);
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
                 tcgen05_fence_after();
+                const float f = next;
+                next = factors[(it + 1u) % S::kScaleSlots * 256u];  // behind the last block: whatever is there
                 if (live) {
-                    const float f = reinterpret_cast<const float*>(smem + S::kOffFactor)[slot * 256u + (col & 128u) + q * 32u + lane];
-                    promote<kCols, kByColumn>(acc, tmem + buf * kPairBlockN, f, reinterpret_cast<const float*>(smem + S::kOffScale) + slot * kPairBlockN + col);
+                    promote<kCols, kByColumn>(acc, tmem + buf * 128u, f, reinterpret_cast<const float*>(smem + S::kOffScale) + slot * kPairBlockN + col);
                 }
                 tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive_cluster(buf ? free_bar1 : free_bar0);
-                    mbar_arrive(&scale_empty[slot]);
+                if (w8 == 2u || w8 == 3u) {
+                    asm volatile("barrier.cta.sync %0, %1;" ::"r"(3u + half), "n"(16 * kBlockPairPromoters) : "memory");
+                    if (lane == 0) {
+                        if (w8 == 2u) {
+                            mbar_arrive_cluster(buf ? free_bar1 : free_bar0);
+                        } else {
+                            mbar_arrive(&scale_empty[slot]);
+                        }
+                    }
+                    __syncwarp();
+                } else {
+                    asm volatile("barrier.cta.arrive %0, %1;" ::"r"(3u + half), "n"(16 * kBlockPairPromoters) : "memory");
                 }
             }
             if (alive && row < u.end) {
