@@ -106,17 +106,6 @@ __device__ __forceinline__ void tmem_ld_fence(float (&r)[16])
                  : "memory");
 }
 
-// Thirty-two columns, there when it returns
-__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, float (&r)[32])
-{
-    float (&lo)[16] = *reinterpret_cast<float (*)[16]>(&r[0]);
-    float (&hi)[16] = *reinterpret_cast<float (*)[16]>(&r[16]);
-    tmem_ld_16(taddr, lo);
-    tmem_ld_16(taddr + 16u, hi);
-    tmem_ld_fence(lo);
-    tmem_ld_fence(hi);
-}
-
 // Sixteen columns of a row to global memory; p is aligned to their size or 32 bytes
 template <typename OutT>
 __device__ __forceinline__ void store_16(OutT* p, const float* v)
@@ -152,6 +141,42 @@ __device__ __forceinline__ void fma_2(float& a0, float& a1, float x0, float x1, 
         "}"
         : "+f"(a0), "+f"(a1)
         : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+
+// sixteen sums += f * the columns of this lane's row; by column: f * scale[column] * them (scale 16-byte aligned)
+template <bool kByColumn>
+__device__ __forceinline__ void add_scaled(float* acc, const float (&v)[16], float f, const float* scale)
+{
+#pragma unroll
+    for (uint32_t c = 0; c < 16; c += 4) {
+        float4 g = make_float4(f, f, f, f);
+        if (kByColumn) {
+            const float4 s = *reinterpret_cast<const float4*>(scale + c);
+            g = make_float4(f * s.x, f * s.y, f * s.z, f * s.w);
+        }
+        fma_2(acc[c], acc[c + 1], v[c], v[c + 1], g.x, g.y);
+        fma_2(acc[c + 2], acc[c + 3], v[c + 2], v[c + 3], g.z, g.w);
+    }
+}
+
+// 32 columns of row `lane` to a box of 32 rows in shared memory that TMA stores: 16-byte pieces in its swizzle of 64 (16-bit types) or
+// 128 bytes.
+template <typename OutT>
+__device__ __forceinline__ void stage_out(uint8_t* box, uint32_t lane, const float* v)
+{
+    constexpr uint32_t kPieces = 2 * sizeof(OutT), kPer = 32 / kPieces;  // of a row; values of one
+    const uint32_t turn = sizeof(OutT) == 4 ? lane & 7u : (lane >> 1) & 3u;
+#pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i) {
+        uint4 o;
+        if constexpr (sizeof(OutT) == 4) {
+            o = make_uint4(__float_as_uint(v[i * kPer]), __float_as_uint(v[i * kPer + 1]), __float_as_uint(v[i * kPer + 2]), __float_as_uint(v[i * kPer + 3]));
+        } else {
+            o = make_uint4(pack2<OutT>(v[i * kPer], v[i * kPer + 1]), pack2<OutT>(v[i * kPer + 2], v[i * kPer + 3]),
+                           pack2<OutT>(v[i * kPer + 4], v[i * kPer + 5]), pack2<OutT>(v[i * kPer + 6], v[i * kPer + 7]));
+        }
+        *reinterpret_cast<uint4*>(box + lane * (32u * sizeof(OutT)) + ((i ^ turn) << 4)) = o;
+    }
 }
 
 // sums += f * the tile's kCols columns of this lane's row; by column: f * scale[column] * it.  The next sixteen columns

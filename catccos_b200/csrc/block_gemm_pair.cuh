@@ -1,24 +1,25 @@
-// The products of block_gemm.cuh on CTA pairs (clusters of two SMs, tcgen05 cta_group::2), for calls that fill the GPU with 256 x 256
+// The products of block_gemm.cuh on CTA pairs (clusters of two SMs, tcgen05 cta_group::2), for calls that fill the GPU with 256 x 128
 // tiles.
 //
-// CTA r of a pair loads rows [128 r, +128) of A and columns [128 r, +128) of B with plain TMA, 32 KB a block of K where a 128 x 256
-// tile on one SM takes 48; the leader issues the products of both, and each CTA has the results for its own 128 rows and all 256
-// columns in its own tensor memory.
+// CTA r of a pair loads rows [128 r, +128) of A and columns [64 r, +64) of B with plain TMA; the leader issues the products of both,
+// and each CTA has the results for its own 128 rows and all 128 columns in its own tensor memory.
 //
-// A block's way from the tensor core through the promotion and back takes longer than its products: about 1000 cycles until a
-// finished product is seen, 300 for the promotion, 200 back, against 512.  Two tiles of 256 columns (all that tensor memory
-// holds) would leave the tensor core waiting half of the time, so the columns are two halves, each with two tiles of its own,
-// multiplied one after the other: half h has columns 64 h to 64 h + 63 of each CTA's B.
+// A block's way from the tensor core through the promotion and back is far longer than its products (256 cycles at best): some 1000
+// cycles until a finished product is seen, 300 to load the tile, 300 until the issuer knows that it is free again.  So four tiles
+// take turns (all that tensor memory holds), a tile goes back as soon as it is in registers, and no warp that promotes looks at a
+// barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: two other warps do, and named
+// barriers join them.  256 x 256 tiles, which read less of A and B, have room for two tiles only: 8192 x 2304 x 7168 took 153 us.
 //
-//   full[s], tmem_empty[h][b]   live in the leader; both CTAs' TMA bytes, and a warp of each CTA's promotion, go there
-//   empty[s], tmem_full[h][b]   live in each CTA; the leader's tcgen05.commit arrives on both copies
-//   scale_full[i], scale_empty[i]  live in each CTA: the factors of its rows (and, by column, of the columns) for one block of K
+//   full[s], tmem_empty[b]    live in the leader; both CTAs' TMA bytes, and the other CTA's word that it has read a tile, go there
+//   empty[s], tmem_full[b]    live in each CTA; the leader's tcgen05.commit arrives on both copies
+//   scale_full[i], scale_empty[i]   live in each CTA: the factors of its rows (and, by column, of the columns) for a group of four
+//                             blocks of K (every unit begins with a group of its own)
+//   named barriers 1 + b, 5 + b   tile b may be read; tile b has been read
 //
-// 640 threads: warps 0-15 promotion and output (warp w: half w / 8, lane quarter w % 4, the half's columns of CTA (w / 4) % 2's B),
-// warp 16 TMA, 17 and 18 the products of a half each, 19 the factors: a row's scale times that of each CTA's columns.  The
-// promotion warps take registers from the other four.  A look at a barrier in shared memory takes some 150 cycles, so no warp of
-// the promotion makes two in a row: of a half's eight warps one waits for the tile, one for the factors of the next block, which all
-// fetch ahead, one gives the tile back and one the factors, and named barriers join them.
+// A role takes 300 to 600 cycles for a block whatever its size (a look at a barrier, then instructions of one lane), hence so many of
+// them.  448 threads: warps 0-7 promotion and output (warp w: lane quarter w % 4, columns 64 (w / 4)), 8 and 9 TMA for A and B, 10
+// and 11 MMA, each every second block (in the other CTA they pass on that tiles have been read), 12 tells the promotion of tiles
+// and factors, 13 makes the factors, a row's scale times the columns'.
 #pragma once
 
 #include "block_gemm.cuh"
@@ -26,29 +27,32 @@
 
 namespace catccos {
 
-constexpr uint32_t kBlockPairThreads = 640;
-constexpr uint32_t kBlockPairPromoters = 16;                           // warps
-constexpr uint32_t kBlockPairRegs = 96;                                // of a thread at launch
-constexpr uint32_t kBlockPairPromoteRegs = 104, kBlockPairOtherRegs = 64;
-static_assert(32 * kBlockPairPromoters * kBlockPairPromoteRegs + (kBlockPairThreads - 32 * kBlockPairPromoters) * kBlockPairOtherRegs <=
-                  kBlockPairThreads * kBlockPairRegs, "the warpgroups' shares are what the block was launched with");
+constexpr uint32_t kBlockPairThreads = 448;
+constexpr uint32_t kBlockPairPromoters = 8;  // warps
+constexpr uint32_t kBlockPairM = 256, kBlockPairN = 128;
 
+template <typename OutT>
 struct BlockPairSmem {
-    static constexpr uint32_t kStages = 6;
+    static constexpr uint32_t kStages = sizeof(OutT) == 4 ? 5 : 6;
+    static constexpr uint32_t kTiles = 4;           // in tensor memory
     static constexpr uint32_t kABytes = 128 * 128;  // this CTA's rows
-    static constexpr uint32_t kBBytes = 128 * 128;  // this CTA's columns
+    static constexpr uint32_t kBBytes = 64 * 128;   // this CTA's columns
+    static constexpr uint32_t kOutBytes = 32 * 64 * sizeof(OutT);  // of a warp
+    static constexpr uint32_t kScaleSlots = 4;                     // groups of four blocks
     static constexpr uint32_t kOffA = 0;
     static constexpr uint32_t kOffB = kOffA + kStages * kABytes;
-    static constexpr uint32_t kScaleSlots = 8;
-    static constexpr uint32_t kOffScale = kOffB + kStages * kBBytes;               // by column: 256 scales a slot
-    static constexpr uint32_t kOffFactor = kOffScale + kScaleSlots * kPairBlockN * 4;  // [CTA whose columns][128 rows] a slot
-    static constexpr uint32_t kOffBar = kOffFactor + kScaleSlots * 256 * 4;
-    static constexpr uint32_t kNumBars = 2 * kStages + 8 + 2 * kScaleSlots;
+    static constexpr uint32_t kOffOut = kOffB + kStages * kBBytes;
+    static constexpr uint32_t kOffFactor = kOffOut + kBlockPairPromoters * kOutBytes;  // [128 rows][4 blocks] a slot
+    static constexpr uint32_t kOffScale = kOffFactor + kScaleSlots * 128 * 16;         // by column: [4 blocks][128 columns] a slot
+    static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * kBlockPairN * 16;
+    static constexpr uint32_t kNumBars = 2 * kStages + 2 * kTiles + 2 * kScaleSlots;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
+    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // the step (counted from 1) whose wait has given up
     static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
     static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
 };
-static_assert(BlockPairSmem::dynamic_bytes(kGroupedMaxExperts) <= 232448, "one CTA's shared memory");
+static_assert(BlockPairSmem<float>::dynamic_bytes(kGroupedMaxExperts) <= 232448 && BlockPairSmem<__half>::dynamic_bytes(kGroupedMaxExperts) <= 232448,
+              "one CTA's shared memory");
 
 // One block of K: four products (K = 32) into the tile at tmem_d, then arrivals on both CTAs' `done` and `empty` when
 // they are finished.  Called by a converged warp, of which one lane issues everything: a branch on the lane around each instruction would
@@ -91,37 +95,67 @@ __device__ __forceinline__ void umma_f8_pair_block(uint32_t tmem_d, uint32_t a_l
         : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int32_t x, int32_t y, int32_t z)
+// A pair's tile load with the announcement of its bytes, by one lane of a converged warp (as umma_f8_pair_block).
+__device__ __forceinline__ void tma_expect_and_load_2d(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+        "{\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%2], %5;\n\t"
+        "@one cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t"
+        "}"
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(bytes)
         : "memory");
 }
 
-// Of the eight warps of a CTA that promote a half: true on all if all say so.
-__device__ __forceinline__ bool promoters_agree(uint32_t barrier, bool ok)
+__device__ __forceinline__ void tma_expect_and_load_3d(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y,
+                                                       uint32_t z)
 {
-    uint32_t bad;
     asm volatile(
         "{\n\t"
-        ".reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%2], %6;\n\t"
+        "@one cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t"
         "}"
-        : "=r"(bad)
-        : "r"(ok ? 0u : 1u), "r"(barrier), "n"(16 * kBlockPairPromoters)
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z), "r"(bytes)
         : "memory");
-    return bad == 0u;
+}
+
+// Both barriers, looked at together.
+__device__ __forceinline__ bool mbar_wait_both(uint64_t* bar1, uint32_t parity1, uint64_t* bar2, uint32_t parity2, StatusBlock* st, uint32_t id,
+                                               uint32_t stage, uint64_t limit_ns)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; i < 4096u; ++i) {
+        const bool first = mbar_try_wait(bar1, parity1), second = mbar_try_wait(bar2, parity2);
+        if (__all_sync(0xFFFFFFFFu, first && second)) {
+            return true;
+        }
+    }
+    return mbar_wait_warp(bar1, parity1, st, id, stage, limit_ns) && mbar_wait_warp(bar2, parity2, st, id + 1u, stage, limit_ns);
+}
+
+constexpr uint32_t kBlockPairJoined = 32 * (kBlockPairPromoters + 1);  // threads of a named barrier
+
+__device__ __forceinline__ void named_sync(uint32_t id)
+{
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(kBlockPairJoined) : "memory");
+}
+
+__device__ __forceinline__ void named_arrive(uint32_t id)
+{
+    asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(kBlockPairJoined) : "memory");
 }
 
 template <typename OutT, bool kByColumn>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBlockPairThreads, 1)
 block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
-                       const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ BlockGemmParams p)
+                       const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_c,
+                       const __grid_constant__ BlockGemmParams p)
 {
-    using S = BlockPairSmem;
+    using S = BlockPairSmem<OutT>;
     constexpr uint32_t kStages = S::kStages, kCols = 64;  // columns of a promotion warp
 
     grid_dep_launch();
@@ -130,10 +164,11 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
     uint64_t* empty = full + kStages;
     uint64_t* tmem_full = empty + kStages;
-    uint64_t* tmem_empty = tmem_full + 4;  // [half][tile]
-    uint64_t* scale_full = tmem_empty + 4;
+    uint64_t* tmem_empty = tmem_full + S::kTiles;
+    uint64_t* scale_full = tmem_empty + S::kTiles;
     uint64_t* scale_empty = scale_full + S::kScaleSlots;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
+    volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + S::kOffDead);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
@@ -141,35 +176,37 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const uint32_t cta = cluster_ctarank();  // 0 = leader
     const uint32_t pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
-    const uint32_t n_tiles = (p.N + kPairBlockN - 1) / kPairBlockN;
+    const uint32_t n_tiles = (p.N + kBlockPairN - 1) / kBlockPairN;
     const uint32_t k_blocks = (p.K + 127u) / 128u;
     const uint64_t bar_ns = p.bar_timeout_ns;
 
     if (threadIdx.x == 32 * kBlockPairPromoters) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            mbar_init(&full[s], 2);  // both CTAs' producers (expect_tx)
-            mbar_init(&empty[s], 2);  // the products of both halves
+            mbar_init(&full[s], 4);  // both CTAs' producers (expect_tx)
+            mbar_init(&empty[s], 1);
         }
-        for (uint32_t b = 0; b < 4; ++b) {
+        for (uint32_t b = 0; b < S::kTiles; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], 2);  // a warp of each CTA, for all that promote the half
+            mbar_init(&tmem_empty[b], 1);  // of the other CTA
         }
         for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
             mbar_init(&scale_full[i], kByColumn ? 2 : 1);  // the rows' factors (and the columns' bytes)
-            mbar_init(&scale_empty[i], 2);  // a warp of each half
+            mbar_init(&scale_empty[i], 1);
         }
+        *dead = 0u;
         mbar_fence_init();
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_a32);
         tma_prefetch_desc(&tmap_b);
+        tma_prefetch_desc(&tmap_c);
     }
-    if (warp == 17) {
+    if (warp == 10) {
         tmem_alloc_pair(tmem_ptr_smem, 512);
         tmem_relinquish_pair();
     }
     grid_dep_wait();
     if (warp == 0) {
-        count_block_tiles(p, kPairBlockM, tiles, row_begin, row_end, lane);
+        count_block_tiles(p, kBlockPairM, tiles, row_begin, row_end, lane);
     }
     tcgen05_fence_before();
     __syncthreads();
@@ -177,211 +214,271 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_ptr_smem;
     const uint32_t num_units = tiles[p.experts] * n_tiles;
+    const uint32_t my_units = num_units > pair ? (num_units - pair + num_pairs - 1u) / num_pairs : 0u;
+    const uint32_t steps = my_units * k_blocks;  // blocks of K, over all units of this pair
     bool alive = true;  // false once a wait of this role has given up
 
     struct Unit {
         uint32_t e, m0, end, n0;  // expert; first row of the pair's tile, end of the expert's rows; first column
     };
-    GroupedWalk walk;
-    auto unit_at = [&](uint32_t unit) {
+    GroupedWalk own_walk;
+    auto find = [&](GroupedWalk& walk, uint32_t unit) {
         const TileCoord tc = walk.seek(tiles, n_tiles, unit);
-        return Unit{walk.e, row_begin[walk.e] + tc.m_tile * kPairBlockM, row_end[walk.e], tc.n_tile * kPairBlockN};
+        return Unit{walk.e, row_begin[walk.e] + tc.m_tile * kBlockPairM, row_end[walk.e], tc.n_tile * kBlockPairN};
     };
+    auto unit_at = [&](uint32_t unit) { return find(own_walk, unit); };
 
-    // The changes of registers belong into the branches: code behind one is built for as many as the branch then has, and code
-    // that all run again has what the block was launched with.
-    if (warp >= kBlockPairPromoters) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBlockPairOtherRegs));
-        if (warp == 16) {
-            // ------------------------------- TMA producer (both CTAs) -------------------------
-            uint32_t it = 0;
-            for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
-                const Unit u = unit_at(unit);
-                const uint32_t m0 = u.m0 + cta * 128u;
-                const uint32_t boxes = m0 < u.end ? (min(u.end - m0, 128u) + 31u) / 32u : 0u;  // of 32 rows
-                const uint32_t tx_bytes = (p.a_cols && boxes ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes;
-                const int32_t n = (int32_t)(u.n0 + cta * 128u);
-                for (uint32_t kb = 0; alive && kb < k_blocks; ++kb, ++it) {
-                    const uint32_t s = it % kStages;
-                    const uint32_t leader_bar = map_to_cta(smem_u32(&full[s]), 0);
-                    alive = mbar_wait_soon(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 500, s, bar_ns);
-                    if (!alive) {
-                        break;
-                    }
-                    if (elect_one()) {
-                        mbar_arrive_expect_tx_cluster(leader_bar, tx_bytes);
-                        const int32_t k = (int32_t)(kb * 128u);
-                        tma_load_3d_pair(smem + S::kOffB + s * S::kBBytes, &tmap_b, leader_bar, p.b_rows ? k : n, p.b_rows ? n : k, (int32_t)u.e);
-                        uint8_t* a = smem + S::kOffA + s * S::kABytes;
-                        if (p.a_cols) {
-                            if (boxes) {
-                                tma_load_2d_pair(a, &tmap_a, leader_bar, (int32_t)m0, k);
-                            }
-                        } else if (boxes == 4u) {
-                            tma_load_2d_pair(a, &tmap_a, leader_bar, k, (int32_t)m0);
-                        } else {
-                            for (uint32_t i = 0; i < boxes; ++i) {
-                                tma_load_2d_pair(a + i * (32u * 128u), &tmap_a32, leader_bar, k, (int32_t)(m0 + i * 32u));
-                            }
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-        } else if (warp < 19) {
-            // ------------------------------- MMA issuers (leader CTA only) --------------------
-            if (cta == 0) {
-                const uint32_t half = warp - 17u;
-                const uint32_t idesc0 = make_idesc_f8(kPairBlockM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
-                const uint64_t desc_k = make_smem_desc(0, 16, 1024, 2), desc_mn = make_smem_desc(0, 16384, 1024, 2);
-                const uint64_t desc_a = p.a_cols ? desc_mn : desc_k, desc_b = p.b_rows ? desc_k : desc_mn;
-                const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
-                const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
-                const uint32_t b_lo0 = ((uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4)) + half * ((p.b_rows ? 64u * 128u : 64u) >> 4);
-                const uint32_t step_a = (p.a_cols ? 4096u : 32u) >> 4, step_b = (p.b_rows ? 32u : 4096u) >> 4;
-                uint64_t* const tile_full = tmem_full + 2u * half;
-                uint64_t* const tile_empty = tmem_empty + 2u * half;
-                uint32_t s = 0, ph = 0, it = 0;
-                for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
-                    // of a ragged last column of tiles as much is multiplied as the leader's columns need (the other CTA's are
-                    // fewer), at least the smallest product
-                    const uint32_t left = p.N - unit_at(unit).n0;
-                    const uint32_t columns = min(max(left, 64u * half + 16u) - 64u * half, 64u);
-                    const uint32_t idesc = idesc0 | (((columns + 15u) / 16u * 32u >> 3) << 17);
-                    for (uint32_t i = 0; alive && i < k_blocks; ++i, ++it) {
-                        const uint32_t buf = it & 1u;
-                        // the operands are there before the tile is free, as a rule: what is waited for last is what counts
-                        alive = mbar_wait_soon(&full[s], ph, p.status, 503, s, bar_ns) &&
-                                mbar_wait_soon(&tile_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 501 + half, buf, bar_ns);
-                        if (!alive) {
-                            break;  // nothing is issued, and no tile reported, after a wait has given up
-                        }
-                        tcgen05_fence_after();
-                        umma_f8_pair_block(tmem_base + half * 256u + buf * 128u, a_lo0 + s * (S::kABytes >> 4), hi_a, step_a,
-                                           b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b, idesc, &tile_full[buf], &empty[s]);
-                        s = (s + 1 == kStages) ? 0u : s + 1;
-                        ph ^= s == 0u ? 1u : 0u;
-                    }
-                }
-            }
-        } else {
-            // ------------------------------- factors (both CTAs, own 128 rows) ----------------
-            uint32_t it = 0;
-            for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
-                const Unit u = unit_at(unit);
-                const uint32_t row = u.m0 + cta * 128u + lane;
-                const uint32_t scale_bytes = min(p.N - u.n0, kPairBlockN) * 4u;
-                const float* b_scales = p.b_scales + u.e * p.b_scale_matrix + (u.n0 / 128u) * p.b_scale_col;
-                const size_t b_next = u.n0 + 128u < p.N ? p.b_scale_col : 0u;
-                for (uint32_t kb0 = 0; alive && kb0 < k_blocks; kb0 += 4u) {
-                    float a[4][4], b[2][4];  // of four blocks
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        load_scales(p.a_scales + min(row + 32u * i, u.end - 1u) * p.a_scale_row, p.a_scale_block, kb0, k_blocks, a[i]);
-                    }
-                    if (!kByColumn) {
-                        load_scales(b_scales, p.b_scale_block, kb0, k_blocks, b[0]);
-                        load_scales(b_scales + b_next, p.b_scale_block, kb0, k_blocks, b[1]);
-                    }
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        if (kb0 + j >= k_blocks || !alive) {
-                            break;
-                        }
-                        const uint32_t slot = it % S::kScaleSlots;
-                        alive = mbar_wait_soon(&scale_empty[slot], ((it / S::kScaleSlots) & 1u) ^ 1u, p.status, 505, slot, bar_ns);
-                        if (!alive) {
-                            break;
-                        }
-                        if (kByColumn && elect_one()) {
-                            mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
-                            bulk_load(smem + S::kOffScale + slot * (kPairBlockN * 4u), p.b_scales + (kb0 + j) * p.b_scale_block + u.n0, scale_bytes,
-                                      &scale_full[slot]);
-                        }
-                        __syncwarp();
-                        float* factor = reinterpret_cast<float*>(smem + S::kOffFactor) + slot * 256u + lane;
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            factor[32u * i] = kByColumn ? a[i][j] : a[i][j] * b[0][j];
-                            factor[128u + 32u * i] = kByColumn ? a[i][j] : a[i][j] * b[1][j];
-                        }
-                        __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive(&scale_full[slot]);
-                        }
-                        ++it;
-                    }
-                }
-            }
-        }
-        __syncwarp();
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBlockPairRegs));
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBlockPairPromoteRegs));
-        // ------------------------------- promotion and output (both CTAs, own 128 rows) ---
-        const uint32_t q = warp & 3u, half = warp >> 3, from = (warp >> 2) & 1u, col = from * 128u + half * kCols;
-        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + half * 256u + from * kCols, w8 = warp & 7u;
-        const float* factors = reinterpret_cast<const float*>(smem + S::kOffFactor) + from * 128u + q * 32u + lane;
-        const uint32_t free_bar0 = map_to_cta(smem_u32(&tmem_empty[2u * half]), 0), free_bar1 = map_to_cta(smem_u32(&tmem_empty[2u * half + 1u]), 0);
+    if (warp == 8 || warp == 9) {
+        // ------------------------------- TMA producers (both CTAs) ------------------------
+        const bool rows = warp == 8;
         uint32_t it = 0;
-        float next = 0.0f;  // the next block's factor
-        if (pair < num_units) {
-            if (w8 == 1u) {
-                alive = mbar_wait_soon(&scale_full[0], 0, p.status, 508, 0, bar_ns);
-            }
-            alive = promoters_agree(1u + half, alive);
-            next = factors[0];
-        }
         for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
             const Unit u = unit_at(unit);
-            const uint32_t row0 = u.m0 + cta * 128u + q * 32u, row = row0 + lane, col0 = u.n0 + col;
-            const bool live = row0 < u.end && col0 < p.N;  // else there is nothing to fetch
-            float acc[kCols] = {};
-            for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
-                const uint32_t buf = it & 1u, slot = it % S::kScaleSlots;
-                if (w8 == 0u) {
-                    alive = mbar_wait_soon(&tmem_full[2u * half + buf], (it >> 1) & 1u, p.status, 506, buf, bar_ns);
-                } else if (w8 == 1u && (i + 1u < k_blocks || unit + num_pairs < num_units)) {
-                    const uint32_t nt = it + 1u;
-                    alive = mbar_wait_soon(&scale_full[nt % S::kScaleSlots], (nt / S::kScaleSlots) & 1u, p.status, 507, nt % S::kScaleSlots, bar_ns);
-                }
-                alive = promoters_agree(1u + half, alive);
+            const uint32_t m0 = u.m0 + cta * 128u;
+            const uint32_t boxes = m0 < u.end ? (min(u.end - m0, 128u) + 31u) / 32u : 0u;  // of 32 rows
+            const uint32_t n = u.n0 + cta * 64u;
+            for (uint32_t kb = 0; alive && kb < k_blocks; ++kb, ++it) {
+                const uint32_t s = it % kStages, k = kb * 128u;
+                const uint32_t leader_bar = map_to_cta(smem_u32(&full[s]), 0);
+                alive = mbar_wait_soon(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 500, s, bar_ns);
                 if (!alive) {
-                    break;  // a tile that never filled is not written out
+                    break;
                 }
-                tcgen05_fence_after();
-                const float f = next;
-                next = factors[(it + 1u) % S::kScaleSlots * 256u];  // behind the last block: whatever is there
-                if (live) {
-                    promote<kCols, kByColumn>(acc, tmem + buf * 128u, f, reinterpret_cast<const float*>(smem + S::kOffScale) + slot * kPairBlockN + col);
-                }
-                tcgen05_fence_before();
-                if (w8 == 2u || w8 == 3u) {
-                    asm volatile("barrier.cta.sync %0, %1;" ::"r"(3u + half), "n"(16 * kBlockPairPromoters) : "memory");
-                    if (lane == 0) {
-                        if (w8 == 2u) {
-                            mbar_arrive_cluster(buf ? free_bar1 : free_bar0);
-                        } else {
-                            mbar_arrive(&scale_empty[slot]);
+                if (!rows) {
+                    tma_expect_and_load_3d(smem + S::kOffB + s * S::kBBytes, &tmap_b, leader_bar, S::kBBytes, p.b_rows ? k : n, p.b_rows ? n : k, u.e);
+                } else if (boxes == 4u || (p.a_cols && boxes)) {
+                    tma_expect_and_load_2d(smem + S::kOffA + s * S::kABytes, &tmap_a, leader_bar, S::kABytes, p.a_cols ? m0 : k, p.a_cols ? k : m0);
+                } else {
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx_cluster(leader_bar, boxes * (32u * 128u));
+                        for (uint32_t i = 0; i < boxes; ++i) {
+                            tma_load_2d_pair(smem + S::kOffA + s * S::kABytes + i * (32u * 128u), &tmap_a32, leader_bar, (int32_t)k, (int32_t)(m0 + i * 32u));
                         }
                     }
                     __syncwarp();
-                } else {
-                    asm volatile("barrier.cta.arrive %0, %1;" ::"r"(3u + half), "n"(16 * kBlockPairPromoters) : "memory");
                 }
             }
-            if (alive && row < u.end) {
-                OutT* dst = static_cast<OutT*>(p.c) + (size_t)row * p.N + col0;
+        }
+    } else if (warp == 13) {
+        // ------------------------------- factors (both CTAs, own 128 rows) ----------------
+        uint32_t group = 0;
+        for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
+            const Unit u = unit_at(unit);
+            const uint32_t row = u.m0 + cta * 128u + lane;
+            const float* b_scales = p.b_scales + u.e * p.b_scale_matrix + (u.n0 / 128u) * p.b_scale_col;
+            for (uint32_t kb = 0; alive && kb < k_blocks; kb += 4u, ++group) {
+                float a[4][4], b[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // of four rows (and the columns) four blocks
 #pragma unroll
-                for (uint32_t c = 0; c < kCols; c += 16) {
-                    if (col0 + c < p.N) {
-                        store_16(dst + c, &acc[c]);
+                for (uint32_t i = 0; i < 4; ++i) {
+                    load_scales(p.a_scales + min(row + 32u * i, u.end - 1u) * p.a_scale_row, p.a_scale_block, kb, k_blocks, a[i]);
+                }
+                if (!kByColumn) {
+                    load_scales(b_scales, p.b_scale_block, kb, k_blocks, b);
+                }
+                const uint32_t slot = group % S::kScaleSlots;
+                alive = mbar_wait_soon(&scale_empty[slot], ((group / S::kScaleSlots) & 1u) ^ 1u, p.status, 505, slot, bar_ns);
+                if (!alive) {
+                    break;
+                }
+                if (kByColumn && elect_one()) {
+                    const uint32_t bytes = min(p.N - u.n0, kBlockPairN) * 4u, blocks = min(k_blocks - kb, 4u);
+                    mbar_arrive_expect_tx(&scale_full[slot], blocks * bytes);
+                    for (uint32_t j = 0; j < blocks; ++j) {
+                        bulk_load(smem + S::kOffScale + (slot * 4u + j) * (kBlockPairN * 4u), p.b_scales + (kb + j) * p.b_scale_block + u.n0, bytes,
+                                  &scale_full[slot]);
+                    }
+                }
+                __syncwarp();
+                float4* factor = reinterpret_cast<float4*>(smem + S::kOffFactor) + slot * 128u + lane;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    factor[32u * i] = make_float4(a[i][0] * b[0], a[i][1] * b[1], a[i][2] * b[2], a[i][3] * b[3]);
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&scale_full[slot]);
+                }
+            }
+        }
+    } else if (warp == 10 || warp == 11) {
+        // ------------------------------- MMA issuers (leader), tiles given back -----------
+        const uint32_t mine = warp - 10u;  // steps of this parity
+        // Hears that all promotion warps of this CTA have read the tile of step `it`, of whose unit it is the i-th, and tells the
+        // makers of factors when that was the first step of a group (the group before is done with); false once the promotion has ended.
+        uint32_t read = mine, read_i = 0, group = 0;
+        auto skip = [&] {  // a step of the other warp's, or of this one
+            group += (read_i & 3u) == 0u ? 1u : 0u;
+            read_i = read_i + 1u == k_blocks ? 0u : read_i + 1u;
+        };
+        if (mine) {
+            skip();
+        }
+        auto hear = [&] {
+            named_sync(5u + (read & 3u));
+            if (*dead == read + 1u) {
+                alive = false;
+                return;
+            }
+            if ((read_i & 3u) == 0u && group != 0u && lane == 0) {
+                mbar_arrive(&scale_empty[(group - 1u) % S::kScaleSlots]);
+            }
+            skip();
+            skip();
+            read += 2u;
+        };
+        if (cta == 0) {
+            const uint32_t idesc0 = make_idesc_f8(kBlockPairM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
+            const uint64_t desc_k = make_smem_desc(0, 16, 1024, 2);
+            const uint64_t desc_a = p.a_cols ? make_smem_desc(0, 16384, 1024, 2) : desc_k, desc_b = p.b_rows ? desc_k : make_smem_desc(0, 16384, 512, 4);
+            const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
+            const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
+            const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4);
+            const uint32_t step_a = (p.a_cols ? 4096u : 32u) >> 4, step_b = (p.b_rows ? 32u : 2048u) >> 4;
+            uint32_t unit = pair, i = mine;  // of step `it`: its unit, the how manieth there
+            uint32_t idesc = 0, of_unit = 0xFFFFFFFFu;
+            for (uint32_t it = mine; it < steps; it += 2u, i += 2u) {
+                while (i >= k_blocks) {
+                    i -= k_blocks;
+                    unit += num_pairs;
+                }
+                if (unit != of_unit) {
+                    // of a ragged last column of tiles as much is multiplied as the leader's columns need: the other CTA's are fewer
+                    const uint32_t columns = (min(p.N - unit_at(unit).n0, 64u) + 15u) / 16u * 16u;
+                    idesc = idesc0 | ((2u * columns >> 3) << 17);
+                    of_unit = unit;
+                }
+                const uint32_t b = it & 3u, s = it % kStages;
+                if (it >= S::kTiles) {
+                    hear();
+                }
+                alive = alive && mbar_wait_both(&full[s], (it / kStages) & 1u, &tmem_empty[b], ((it >> 2) & 1u) ^ 1u, p.status, 501, b, bar_ns);
+                if (!alive) {
+                    break;  // nothing is issued, and no tile reported, after a wait has given up
+                }
+                tcgen05_fence_after();
+                umma_f8_pair_block(tmem_base + b * kBlockPairN, a_lo0 + s * (S::kABytes >> 4), hi_a, step_a, b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b,
+                                   idesc, &tmem_full[b], &empty[s]);
+            }
+            while (alive && read < steps) {
+                hear();
+            }
+        } else {
+            const uint32_t free_bar = map_to_cta(smem_u32(&tmem_empty[0]), 0);
+            while (alive && read < steps) {
+                const uint32_t b = read & 3u;
+                hear();
+                if (alive && lane == 0) {
+                    mbar_arrive_cluster(free_bar + b * 8u);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 12) {
+        // ------------------------------- tells of tiles and factors -----------------------
+        // It is never two turns ahead on a named barrier: tile b is filled again after all have read it.  When a wait gives up, the
+        // promotion and warps 10 and 11 are told with that step and end with it.
+        uint32_t i = 0, group = 0;
+        for (uint32_t it = 0; alive && it < steps; ++it) {
+            const uint32_t b = it & 3u, slot = group % S::kScaleSlots;
+            if ((i & 3u) == 0u) {
+                alive = mbar_wait_both(&tmem_full[b], (it >> 2) & 1u, &scale_full[slot], (group / S::kScaleSlots) & 1u, p.status, 506, b, bar_ns);
+                ++group;
+            } else {
+                alive = mbar_wait_soon(&tmem_full[b], (it >> 2) & 1u, p.status, 506, b, bar_ns);
+            }
+            i = i + 1u == k_blocks ? 0u : i + 1u;
+            if (!alive && lane == 0) {
+                *dead = it + 1u;
+            }
+            __syncwarp();
+            tcgen05_fence_after();
+            tcgen05_fence_before();
+            named_arrive(1u + b);
+        }
+    } else {
+        // ------------------------------- promotion and output (both CTAs, own 128 rows) ---
+        const uint32_t q = warp & 3u, col = (warp >> 2) * kCols;
+        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + col;
+        const float4* factors = reinterpret_cast<const float4*>(smem + S::kOffFactor) + q * 32u + lane;
+        uint8_t* out = smem + S::kOffOut + warp * S::kOutBytes;
+        uint32_t it = 0, group = 0;
+        float4 f4 = {};  // the factors of a group
+        for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
+            const Unit u = unit_at(unit);
+            const uint32_t row0 = u.m0 + cta * 128u + q * 32u, col0 = u.n0 + col;
+            const bool live = row0 < u.end && col0 < p.N;  // else there is nothing to fetch
+            float acc[kCols] = {};
+            // Sixteen columns are added while the next are on their way, a step's last while the next step's first are; a tile goes
+            // back when its last are in registers.
+            float v[2][16], f = 0.0f;
+            const float* scale = nullptr;
+            for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
+                const uint32_t b = it & 3u, j = i & 3u;
+                named_sync(1u + b);
+                tcgen05_fence_after();
+                const uint32_t dead_step = *dead;
+                if (live) {
+                    const uint32_t tile = tmem + b * kBlockPairN;
+                    tmem_ld_16(tile, v[0]);
+                    if (j == 0u) {
+                        f4 = factors[group % S::kScaleSlots * 128u];
+                    }
+                    if (i != 0u) {
+                        add_scaled<kByColumn>(&acc[48], v[1], f, scale + 48);
+                    }
+                    f = j == 0u ? f4.x : (j == 1u ? f4.y : (j == 2u ? f4.z : f4.w));
+                    scale = reinterpret_cast<const float*>(smem + S::kOffScale) + (group % S::kScaleSlots * 4u + j) * kBlockPairN + col;
+                    tmem_ld_fence(v[0]);
+#pragma unroll
+                    for (uint32_t c = 0; c < 3; ++c) {
+                        tmem_ld_16(tile + 16u * c + 16u, v[(c + 1) & 1]);
+                        add_scaled<kByColumn>(&acc[16 * c], v[c & 1], f, scale + 16 * c);
+                        tmem_ld_fence(v[(c + 1) & 1]);
+                    }
+                }
+                tcgen05_fence_before();
+                named_arrive(5u + b);
+                if (dead_step == it + 1u) {
+                    alive = false;  // a tile that never filled is not written out
+                    break;
+                }
+                group += j == 3u || i + 1u == k_blocks ? 1u : 0u;
+            }
+            if (live) {
+                add_scaled<kByColumn>(&acc[48], v[1], f, scale + 48);
+            }
+            if (live && alive) {
+                if (row0 + 32u <= u.end || p.offsets == nullptr) {
+                    // twice 32 rows of 32 columns, in the order that TMA reads with its swizzle; what lies outside the matrix is not written
+                    if (lane == 0) {
+                        bulk_store_wait_read();
+                    }
+                    __syncwarp();
+                    stage_out<OutT>(out, lane, &acc[0]);
+                    stage_out<OutT>(out + S::kOutBytes / 2u, lane, &acc[32]);
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&tmap_c, out, (int32_t)col0, (int32_t)row0);
+                        if (col0 + 32u < p.N) {
+                            tma_store_2d(&tmap_c, out + S::kOutBytes / 2u, (int32_t)(col0 + 32u), (int32_t)row0);
+                        }
+                        bulk_store_commit();
+                    }
+                } else if (row0 + lane < u.end) {
+                    OutT* dst = static_cast<OutT*>(p.c) + (size_t)(row0 + lane) * p.N + col0;
+#pragma unroll
+                    for (uint32_t c = 0; c < kCols; c += 16) {
+                        if (col0 + c < p.N) {
+                            store_16(dst + c, &acc[c]);
+                        }
                     }
                 }
             }
         }
-        __syncwarp();
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBlockPairRegs));
+        if (lane == 0) {
+            bulk_store_wait_all();
+        }
     }
 
     tcgen05_fence_before();
@@ -389,7 +486,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         drain_after_abort(p.status);  // both CTAs stay while loads that report to the other's barriers may be in flight
     }
     cluster_sync_all();  // nobody leaves while the other CTA may still arrive on its barriers
-    if (warp == 17) {
+    if (warp == 10) {
         tcgen05_fence_after();
         tmem_dealloc_pair(tmem_base, 512);
     }

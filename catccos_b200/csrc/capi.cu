@@ -474,7 +474,8 @@ int encode_map_2d_uncached(CUtensorMap* map, const void* base, uint64_t inner, u
     // packed 4-bit values land in shared memory sixteen to a 16-byte chunk (8 bytes of values, 8 bytes of gap):
     // the same 128 bytes per 128 values as the 8-bit types, so boxes, swizzle and descriptors stay as they are
     const CUtensorMapDataType dt = fp4 ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B
-                                       : (elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8);
+                                       : (elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32
+                                                     : (elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8));
     CU_TRY(g.drv.TensorMapEncodeTiled(map, dt, 2, const_cast<void*>(base), dims, strides, box,
                                       estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                       !fp4 && box_inner * elem == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1799,29 +1800,19 @@ int launch_block_gemm_inst(RankCtx& rc, cudaStream_t st, const BlockOperands& o,
 template <typename OutT, bool kByColumn>
 int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
 {
-    using S = BlockPairSmem;
+    using S = BlockPairSmem<OutT>;
     auto kern = block_gemm_pair_kernel<OutT, kByColumn>;
     static PerDevice<int, kMaxRanks * 2> resident;
     int pairs = 0;
     CUDA_TRY(resident_clusters_of_two(rc, kern, kBlockPairThreads, S::dynamic_bytes(kGroupedMaxExperts), resident, &pairs));
-    static PerDevice<bool, kMaxRanks * 2> checked;
-    if (!checked.get(rc.device)) {
-        // the kernel's warps hand registers on: they wait for more than it was launched with for ever
-        cudaFuncAttributes attr;
-        CUDA_TRY(cudaFuncGetAttributes(&attr, kern));
-        if ((uint32_t)attr.numRegs != kBlockPairRegs) {
-            ERROR_LOG("block_gemm_pair_kernel was built with %d registers a thread, not %u", attr.numRegs, kBlockPairRegs);
-            return CATCCOS_B200_ESTATE;
-        }
-        checked.set(rc.device, true);
-    }
-    CUtensorMap maps[3];
-    int rcode = block_maps(maps, o, p, 128);
+    CUtensorMap maps[3], out;
+    int rcode = block_maps(maps, o, p, 64);
+    if (rcode == 0) rcode = encode_map_2d(&out, p.c, p.N, p.rows, 32, 32, false, sizeof(OutT));
     if (rcode != 0) return rcode;
-    const uint64_t tiles = p.offsets ? p.rows / kPairBlockM + std::min(p.rows, p.experts) : (p.rows + kPairBlockM - 1) / kPairBlockM;
-    const uint64_t units = tiles * ((p.N + kPairBlockN - 1) / kPairBlockN);
+    const uint64_t tiles = p.offsets ? p.rows / kBlockPairM + std::min(p.rows, p.experts) : (p.rows + kBlockPairM - 1) / kBlockPairM;
+    const uint64_t units = tiles * ((p.N + kBlockPairN - 1) / kBlockPairN);
     CUDA_TRY(launch_after(kern, dim3(2u * (unsigned)std::min<uint64_t>(units, (uint64_t)pairs)), kBlockPairThreads, S::dynamic_bytes(p.experts), st,
-                          maps[0], maps[1], maps[2], p));
+                          maps[0], maps[1], maps[2], out, p));
     return 0;
 }
 
