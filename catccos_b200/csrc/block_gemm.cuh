@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "mx_gemm_small.cuh"
 #include "mx_grouped_gemm.cuh"
 
 namespace catccos {
@@ -37,6 +38,7 @@ struct BlockGemmParams {
     uint32_t a_fmt, b_fmt;                                 // 0 = E4M3, 1 = E5M2
     uint32_t a_cols, b_rows;                               // 1: A is stored [K, rows]; B [N, K]
     uint32_t parts;                                        // CTAs of a cluster that share K (a power of two)
+    uint32_t stages, a_stage_rows, ring_bytes;             // of block_gemm_kernel's ring (BlockGemmSmem)
     uint64_t bar_timeout_ns;
     StatusBlock* status;
 };
@@ -58,22 +60,6 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, S
 __host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t M, uint32_t N, uint32_t a_fmt, uint32_t b_fmt, bool a_mn, bool b_mn)
 {
     return (1u << 4) | (a_fmt << 7) | (b_fmt << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
-}
-
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                        uint32_t accumulate)
-{
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        ".reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %2};\n\t"
-        "mov.b64 db, {%3, %4};\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t"
-        "}"
-        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
-        : "memory");
 }
 
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z)
@@ -179,27 +165,6 @@ __device__ __forceinline__ void stage_out(uint8_t* box, uint32_t lane, const flo
     }
 }
 
-// sums += f * the tile's kCols columns of this lane's row; by column: f * scale[column] * it.  The next sixteen columns
-// are on their way while these are added.
-template <uint32_t kCols, bool kByColumn>
-__device__ __forceinline__ void promote(float (&acc)[kCols], uint32_t tmem, float f, const float* scale)
-{
-    float r[2][16];
-    tmem_ld_16(tmem, r[0]);
-#pragma unroll
-    for (uint32_t c = 0; c < kCols; c += 16) {
-        float (&v)[16] = r[(c / 16) & 1];
-        tmem_ld_fence(v);
-        if (c + 16 < kCols) {
-            tmem_ld_16(tmem + c + 16, r[(c / 16 + 1) & 1]);
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 16; j += 2) {
-            fma_2(acc[c + j], acc[c + j + 1], v[j], v[j + 1], kByColumn ? f * scale[c + j] : f, kByColumn ? f * scale[c + j + 1] : f);
-        }
-    }
-}
-
 // A line's scales of blocks kb .. kb + 3 of K (those behind the last: 0); they are `step` floats apart.
 __device__ __forceinline__ void load_scales(const float* line, size_t step, uint32_t kb, uint32_t blocks, float (&v)[4])
 {
@@ -214,52 +179,6 @@ __device__ __forceinline__ void load_scales(const float* line, size_t step, uint
         }
     }
 }
-
-// The scales of one row (or of one block of columns) along K, read ahead of the products: with the blocks next to one another
-// and 16-byte aligned rows four at a time, the next four while these are used.
-struct ScaleReader {
-    const float* at;
-    size_t step;
-    uint32_t left;  // blocks not yet requested
-    bool wide;
-    float4 cur, nxt;
-
-    __device__ __forceinline__ float4 fetch()
-    {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (wide && left >= 4u) {
-            v = __ldcg(reinterpret_cast<const float4*>(at));
-        } else {
-            if (left > 0u) v.x = __ldcg(at);
-            if (left > 1u) v.y = __ldcg(at + step);
-            if (left > 2u) v.z = __ldcg(at + 2 * step);
-            if (left > 3u) v.w = __ldcg(at + 3 * step);
-        }
-        at += 4 * step;
-        left -= min(left, 4u);
-        return v;
-    }
-    // blocks [first, first + count) of the line that starts at `line`
-    __device__ __forceinline__ void start(const float* line, size_t block_step, uint32_t first, uint32_t count)
-    {
-        at = line + first * block_step;
-        step = block_step;
-        left = count;
-        wide = block_step == 1 && ((uintptr_t)at & 15u) == 0u;
-        cur = fetch();
-        nxt = fetch();
-    }
-    // the i-th of them, i ascending by one
-    __device__ __forceinline__ float get(uint32_t i)
-    {
-        if (i != 0u && (i & 3u) == 0u) {
-            cur = nxt;
-            nxt = fetch();
-        }
-        const uint32_t j = i & 3u;
-        return j == 0u ? cur.x : (j == 1u ? cur.y : (j == 2u ? cur.z : cur.w));
-    }
-};
 
 // One warp: where each expert's rows and row tiles begin (count_grouped_tiles), or the one matrix without offsets.
 __device__ __forceinline__ void count_block_tiles(const BlockGemmParams& p, uint32_t tile_rows, uint32_t* tiles, uint32_t* row_begin,
@@ -279,46 +198,102 @@ __device__ __forceinline__ void count_block_tiles(const BlockGemmParams& p, uint
     }
 }
 
+// One block of K: four products (K = 32) into the tile at tmem_d, then arrivals on `done` and `empty` when they are finished.  Called
+// by a converged warp, of which one lane issues everything: with a branch on the lane it takes three times as long.
+__device__ __forceinline__ void umma_f8_block(uint32_t tmem_d, uint32_t a_lo, uint32_t a_hi, uint32_t a_step, uint32_t b_lo, uint32_t b_hi,
+                                              uint32_t b_step, uint32_t idesc, uint64_t* done, uint64_t* empty)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred one, add;\n\t"
+        ".reg .b64 da, db;\n\t"
+        ".reg .b32 a, b;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "setp.ne.b32 add, 0, 0;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%4, %5};\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "setp.eq.b32 add, 0, 0;\n\t"
+        "add.u32 a, %1, %3;\n\t"
+        "add.u32 b, %4, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "add.u32 a, a, %3;\n\t"
+        "add.u32 b, b, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "add.u32 a, a, %3;\n\t"
+        "add.u32 b, b, %6;\n\t"
+        "mov.b64 da, {a, %2};\n\t"
+        "mov.b64 db, {b, %5};\n\t"
+        "@one tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %7, add;\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t"
+        "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%9];\n\t"
+        "}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(a_hi), "r"(a_step), "r"(b_lo), "r"(b_hi), "r"(b_step), "r"(idesc), "r"(smem_u32(done)), "r"(smem_u32(empty))
+        : "memory");
+}
+
+// Both barriers, looked at together.
+__device__ __forceinline__ bool mbar_wait_both(uint64_t* bar1, uint32_t parity1, uint64_t* bar2, uint32_t parity2, StatusBlock* st, uint32_t id,
+                                               uint32_t stage, uint64_t limit_ns)
+{
+#pragma unroll 1
+    for (uint32_t i = 0; i < 4096u; ++i) {
+        const bool first = mbar_try_wait(bar1, parity1), second = mbar_try_wait(bar2, parity2);
+        if (__all_sync(0xFFFFFFFFu, first && second)) {
+            return true;
+        }
+    }
+    return mbar_wait_warp(bar1, parity1, st, id, stage, limit_ns) && mbar_wait_warp(bar2, parity2, st, id + 1u, stage, limit_ns);
+}
+
+// Shared memory of block_gemm_kernel.  How many rows of A a stage holds, and with it how many stages there are, is the launch's
+// choice: few rows leave more room for B on its way.  (The tensor core reads 128 rows whatever a stage holds; the others' products
+// are not looked at.)
 template <uint32_t BLOCK_N>
 struct BlockGemmSmem {
-    static constexpr uint32_t kStages = BLOCK_N == 64 ? 4 : 3;  // two CTAs to an SM
-    static constexpr uint32_t kABytes = kBlockGemmM * 128;
+    static constexpr uint32_t kMaxStages = 8;
     static constexpr uint32_t kBBytes = BLOCK_N * 128;
-    static constexpr uint32_t kOffA = 0;
-    static constexpr uint32_t kOffB = kOffA + kStages * kABytes;
-    // by column: a slot is free again when the product two steps behind its stage's next is multiplied (see the producer)
-    static constexpr uint32_t kScaleSlots = kStages + 2;
-    static constexpr uint32_t kOffScale = kOffB + kStages * kBBytes;
-    static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * BLOCK_N * 4;
-    static constexpr uint32_t kNumBars = 2 * kStages + 4 + kScaleSlots;  // full[S], empty[S], tmem_full[2], tmem_empty[2], scale_full[]
-    static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
-    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
-    static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
+    static constexpr uint32_t kScaleSlots = 4;                                                  // by column: scales of a block
+    static constexpr uint32_t kScaleBytes = kScaleSlots * BLOCK_N * 4;
+    static constexpr uint32_t kNumBars = 2 * kMaxStages + 4 + 2 * kScaleSlots;                  // full[], empty[], tmem_full[2], tmem_empty[2], scale_full[], scale_empty[]
+    static constexpr uint32_t kRest = kScaleBytes + kNumBars * 8 + 16;                          // behind the ring
+    static constexpr uint32_t dynamic_bytes(uint32_t ring, uint32_t experts) { return ring + kRest + (3u * experts + 1u) * 4u + 1024u; }
+    static constexpr uint32_t kRing = 106496;  // at most: two CTAs to an SM
     // the parts' sums meet in the ring: [part][128 rows][a part's columns, four more]
-    static_assert(kBlockGemmM * (BLOCK_N + 4 * kBlockGemmMaxParts) * 4 <= kOffScale, "the sums of all parts fit the ring");
+    static constexpr uint32_t sum_bytes(uint32_t parts) { return kBlockGemmM * (BLOCK_N + 4u * parts) * 4u; }
 };
 
+// K may be cut over the CTAs of a cluster (p.parts: 1, 2, 4 or 8), so that calls of few tiles stream their weights with every SM.
+// Their sums meet in distributed shared memory: part d owns BLOCK_N / parts of the columns, the others push theirs into its idle
+// ring, and it adds them in ascending order of the parts.  A launch with parts has a cluster for every unit there may be.
 template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
 __global__ void __launch_bounds__(kBlockGemmThreads, 2)
 block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
                   const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ BlockGemmParams p)
 {
     using S = BlockGemmSmem<BLOCK_N>;
-    constexpr uint32_t kStages = S::kStages, kCols = BLOCK_N / 2;  // columns of a promotion warp
+    constexpr uint32_t kCols = BLOCK_N / 2;  // of a promotion warp
     constexpr uint32_t kTmemCols = 2 * BLOCK_N;
 
     grid_dep_launch();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
-    uint64_t* empty = full + kStages;
-    uint64_t* tmem_full = empty + kStages;
+    const uint32_t stages = p.stages, a_bytes = p.a_stage_rows * 128u;
+    uint8_t* smem_b = smem + stages * a_bytes;
+    float* scales = reinterpret_cast<float*>(smem + p.ring_bytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.ring_bytes + S::kScaleBytes);
+    uint64_t* empty = full + S::kMaxStages;
+    uint64_t* tmem_full = empty + S::kMaxStages;
     uint64_t* tmem_empty = tmem_full + 2;
     uint64_t* scale_full = tmem_empty + 2;
-    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
-    uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
-    uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
+    uint64_t* scale_empty = scale_full + S::kScaleSlots;
+    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(scale_empty + S::kScaleSlots);
+    uint32_t* dead = tmem_ptr_smem + 1;  // a part of this cluster has given up
+    uint32_t* tiles = tmem_ptr_smem + 4;
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
 
@@ -327,11 +302,10 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     const uint32_t k_blocks = (p.K + 127u) / 128u;
     const uint32_t part = blockIdx.x & (p.parts - 1u), first_unit = blockIdx.x / p.parts, stride = gridDim.x / p.parts;
     const uint32_t kb0 = (uint32_t)((uint64_t)part * k_blocks / p.parts), kb1 = (uint32_t)((uint64_t)(part + 1u) * k_blocks / p.parts);
-    const uint32_t steps = kb1 - kb0;  // blocks of K that this CTA multiplies of a unit
     const uint64_t bar_ns = p.bar_timeout_ns;
 
     if (threadIdx.x == 256) {
-        for (uint32_t s = 0; s < kStages; ++s) {
+        for (uint32_t s = 0; s < stages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -341,6 +315,7 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         }
         for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
             mbar_init(&scale_full[i], 1);
+            mbar_init(&scale_empty[i], 8);
         }
         *dead = 0u;
         mbar_fence_init();
@@ -366,25 +341,23 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 
     if (warp == 8) {
         // ------------------------------- TMA producer -------------------------------------
-        uint32_t it = 0;
+        uint32_t it = 0, s = 0, ph = 1;
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
             const uint32_t m0 = row_begin[walk.e] + tc.m_tile * kBlockGemmM, n0 = tc.n_tile * BLOCK_N;
             const uint32_t boxes = (min(row_end[walk.e] - m0, kBlockGemmM) + 31u) / 32u;  // of 32 rows
             const uint32_t scale_bytes = min(p.N - n0, BLOCK_N) * 4u;
-            const uint32_t tx_bytes = (p.a_cols ? S::kABytes : boxes * (32u * 128u)) + S::kBBytes;
+            const uint32_t tx_bytes = (p.a_cols ? kBlockGemmM * 128u : boxes * (32u * 128u)) + S::kBBytes;
             for (uint32_t kb = kb0; alive && kb < kb1; ++kb, ++it) {
-                const uint32_t s = it % kStages;
-                alive = mbar_wait_soon(&empty[s], ((it / kStages) & 1u) ^ 1u, p.status, 400, s, bar_ns);
+                alive = mbar_wait_soon(&empty[s], ph, p.status, 400, s, bar_ns);
                 if (!alive) {
                     break;
                 }
                 if (elect_one()) {
                     mbar_arrive_expect_tx(&full[s], tx_bytes);
                     const int32_t k = (int32_t)(kb * 128u);
-                    tma_load_3d(smem + S::kOffB + s * S::kBBytes, &tmap_b, &full[s], p.b_rows ? k : (int32_t)n0,
-                                p.b_rows ? (int32_t)n0 : k, (int32_t)walk.e);
-                    uint8_t* a = smem + S::kOffA + s * S::kABytes;
+                    tma_load_3d(smem_b + s * S::kBBytes, &tmap_b, &full[s], p.b_rows ? k : (int32_t)n0, p.b_rows ? (int32_t)n0 : k, (int32_t)walk.e);
+                    uint8_t* a = smem + s * a_bytes;
                     if (p.a_cols) {
                         tma_load_2d(a, &tmap_a, &full[s], (int32_t)m0, k);
                     } else if (boxes == 4u) {
@@ -394,15 +367,19 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                             tma_load_2d(a + i * (32u * 128u), &tmap_a32, &full[s], k, (int32_t)(m0 + i * 32u));
                         }
                     }
-                    if (kByColumn) {
-                        // Step `it` may overwrite the scales of step it - kStages - 2: the product of it - kStages has been
-                        // multiplied (empty[s]), for which the tile of it - kStages - 2 had to be promoted (tmem_empty).
-                        const uint32_t slot = it % S::kScaleSlots;
-                        mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
-                        bulk_load(smem + S::kOffScale + slot * (BLOCK_N * 4u), p.b_scales + kb * p.b_scale_block + n0, scale_bytes, &scale_full[slot]);
-                    }
                 }
                 __syncwarp();
+                if (kByColumn) {
+                    const uint32_t slot = it % S::kScaleSlots;
+                    alive = mbar_wait_soon(&scale_empty[slot], ((it / S::kScaleSlots) & 1u) ^ 1u, p.status, 405, slot, bar_ns);
+                    if (alive && elect_one()) {
+                        mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
+                        bulk_load(scales + slot * BLOCK_N, p.b_scales + (size_t)walk.e * p.b_scale_matrix + kb * p.b_scale_block + n0, scale_bytes, &scale_full[slot]);
+                    }
+                    __syncwarp();
+                }
+                s = s + 1u == stages ? 0u : s + 1u;
+                ph ^= s == 0u ? 1u : 0u;
             }
         }
     } else if (warp == 9) {
@@ -412,31 +389,24 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
         const uint64_t desc_b = p.b_rows ? make_smem_desc(0, 16, 1024, 2)
                                          : make_smem_desc(0, 16384, 8 * BLOCK_N, BLOCK_N == 64 ? 4 : 2);
         const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
-        const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
-        const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4);
+        const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem) >> 4);
+        const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem_b) >> 4);
         const uint32_t step_a = (p.a_cols ? 32u * 128u : 32u) >> 4, step_b = (p.b_rows ? 32u : 32u * BLOCK_N) >> 4;
-        uint32_t it = 0;
+        uint32_t it = 0, s = 0, ph = 0;
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             // a ragged last column of tiles is multiplied as wide as it is (a multiple of 16)
             const uint32_t idesc = idesc0 | ((min(p.N - unit % n_tiles * BLOCK_N, BLOCK_N) >> 3) << 17);
-            for (uint32_t i = 0; alive && i < steps; ++i, ++it) {
-                const uint32_t s = it % kStages, buf = it & 1u;
-                alive = mbar_wait_soon(&tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, buf, bar_ns) &&
-                        mbar_wait_soon(&full[s], (it / kStages) & 1u, p.status, 403, s, bar_ns);
+            for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t buf = it & 1u;
+                alive = mbar_wait_both(&full[s], ph, &tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, s, bar_ns);
                 if (!alive) {
                     break;  // nothing is issued, and no tile reported, after a wait has given up
                 }
                 tcgen05_fence_after();
-                if (elect_one()) {
-                    const uint32_t a_lo = a_lo0 + s * (S::kABytes >> 4), b_lo = b_lo0 + s * (S::kBBytes >> 4);
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        umma_f8(tmem_base + buf * BLOCK_N, a_lo + j * step_a, hi_a, b_lo + j * step_b, hi_b, idesc, j);
-                    }
-                    tcgen05_commit(&empty[s]);
-                    tcgen05_commit(&tmem_full[buf]);
-                }
-                __syncwarp();
+                umma_f8_block(tmem_base + buf * BLOCK_N, a_lo0 + s * (a_bytes >> 4), hi_a, step_a, b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b, idesc,
+                              &tmem_full[buf], &empty[s]);
+                s = s + 1u == stages ? 0u : s + 1u;
+                ph ^= s == 0u ? 1u : 0u;
             }
         }
     } else {
@@ -449,42 +419,112 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             const uint32_t first = row_begin[walk.e] + tc.m_tile * kBlockGemmM, end = row_end[walk.e];
             const uint32_t row0 = first + q * 32u, row = row0 + lane, n0 = tc.n_tile * BLOCK_N;
             const bool live = row0 < end && n0 + half * kCols < p.N;  // else there is nothing to fetch
+            const float* a_line = p.a_scales + min(row, end - 1u) * p.a_scale_row;
+            const float* b_line = p.b_scales + walk.e * p.b_scale_matrix + (n0 / 128u) * p.b_scale_col;
             float acc[kCols] = {};
-            ScaleReader sa, sb;
-            sa.start(p.a_scales + min(row, end - 1u) * p.a_scale_row, p.a_scale_block, kb0, steps);
-            sb.start(p.b_scales + walk.e * p.b_scale_matrix + (n0 / 128u) * p.b_scale_col, p.b_scale_block, kb0, kByColumn ? 0u : steps);
-            for (uint32_t i = 0; i < steps; ++i, ++it) {
-                const uint32_t buf = it & 1u;
-                const float f = kByColumn ? sa.get(i) : sa.get(i) * sb.get(i);
-                alive = mbar_wait_soon(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
-                const uint32_t slot = it % S::kScaleSlots;
-                if (kByColumn && alive) {
-                    alive = mbar_wait_soon(&scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 407, slot, bar_ns);
+            float a4[4], b4[4];  // scales of four blocks
+            auto fetch = [&](uint32_t kb) {
+                if (live) {
+                    load_scales(a_line, p.a_scale_block, kb, kb1, a4);
+                    if (!kByColumn) {
+                        load_scales(b_line, p.b_scale_block, kb, kb1, b4);
+                    }
                 }
+            };
+            fetch(kb0);
+            for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t buf = it & 1u, slot = it % S::kScaleSlots, j = (kb - kb0) & 3u;
+                alive = kByColumn ? mbar_wait_both(&tmem_full[buf], (it >> 1) & 1u, &scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 406, buf, bar_ns)
+                                  : mbar_wait_soon(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
                 tcgen05_fence_after();
                 if (live) {
-                    promote<kCols, kByColumn>(acc, tmem + buf * BLOCK_N, f,
-                                              reinterpret_cast<const float*>(smem + S::kOffScale) + slot * BLOCK_N + half * kCols);
+                    auto pick = [&](const float (&v)[4]) { return j == 0u ? v[0] : (j == 1u ? v[1] : (j == 2u ? v[2] : v[3])); };
+                    const float f = kByColumn ? pick(a4) : pick(a4) * pick(b4);
+                    if (j == 3u) {
+                        fetch(kb + 1u);  // the next four, while this block is added
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < kCols; c += 16) {
+                        float v[16];
+                        tmem_ld_16(tmem + buf * BLOCK_N + c, v);
+                        tmem_ld_fence(v);
+                        add_scaled<kByColumn>(&acc[c], v, f, scales + slot * BLOCK_N + half * kCols + c);
+                    }
                 }
                 tcgen05_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(&tmem_empty[buf]);
+                    if (kByColumn) {
+                        mbar_arrive(&scale_empty[slot]);
+                    }
                 }
             }
-            if (p.parts == 1u && alive && row < end) {
-                OutT* dst = static_cast<OutT*>(p.c) + (size_t)row * p.N + n0 + half * kCols;
+            if (p.parts == 1u) {
+                if (alive && row < end) {
+                    OutT* dst = static_cast<OutT*>(p.c) + (size_t)row * p.N + n0 + half * kCols;
 #pragma unroll
-                for (uint32_t c = 0; c < kCols; c += 16) {
-                    if (n0 + half * kCols + c < p.N) {
-                        store_16(dst + c, &acc[c]);
+                    for (uint32_t c = 0; c < kCols; c += 16) {
+                        if (n0 + half * kCols + c < p.N) {
+                            store_16(dst + c, &acc[c]);
+                        }
+                    }
+                }
+                continue;
+            }
+            // The sums of all parts.  Every CTA of the cluster has multiplied its last block: the rings are idle.
+            const uint32_t cols = BLOCK_N / p.parts, shift = __ffs(cols) - 1, pitch = cols + 4u;  // a part's columns; four more keep lanes off one bank
+            cluster_sync_all();
+            if (!alive && lane == 0) {
+                for (uint32_t d = 0; d < p.parts; ++d) {
+                    st_shared_cluster_u32(map_to_cta(smem_u32(dead), d), 1u);
+                }
+            }
+            __syncwarp();
+            if (alive && row < end) {
+                const uint32_t line = smem_u32(smem) + (part * 128u + q * 32u + lane) * pitch * 4u;
+#pragma unroll
+                for (uint32_t c = 0; c < kCols; c += 4) {
+                    const uint32_t col = half * kCols + c, d = col >> shift;
+                    st_shared_cluster_v4(map_to_cta(line + (col - (d << shift)) * 4u, d), __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]),
+                                         __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+                }
+            }
+            __syncwarp();
+            cluster_sync_all();
+            if (*reinterpret_cast<volatile uint32_t*>(dead) != 0u) {
+                alive = false;
+            }
+            const uint32_t rows = min(end - first, kBlockGemmM);
+            for (uint32_t i = threadIdx.x; alive && i < rows << (shift - 2u); i += 256u) {
+                const uint32_t r = i >> (shift - 2u), c = (i & ((1u << (shift - 2u)) - 1u)) * 4u, n = n0 + part * cols + c;
+                const float* at = reinterpret_cast<const float*>(smem) + r * pitch + c;
+                float4 sum = *reinterpret_cast<const float4*>(at);
+                for (uint32_t src = 1; src < p.parts; ++src) {
+                    const float4 x = *reinterpret_cast<const float4*>(at + src * 128u * pitch);
+                    sum.x += x.x;
+                    sum.y += x.y;
+                    sum.z += x.z;
+                    sum.w += x.w;
+                }
+                if (n < p.N) {
+                    OutT* dst = static_cast<OutT*>(p.c) + (size_t)(first + r) * p.N + n;
+                    if constexpr (sizeof(OutT) == 4) {
+                        *reinterpret_cast<float4*>(dst) = sum;
+                    } else {
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<OutT>(sum.x, sum.y), pack2<OutT>(sum.z, sum.w));
                     }
                 }
             }
         }
+    }
+    if (warp >= 8 && p.parts > 1u && first_unit < num_units) {
+        __syncwarp();
+        cluster_sync_all();  // the two meetings of the promotion warps
+        cluster_sync_all();
     }
 
     tcgen05_fence_before();

@@ -123,20 +123,6 @@ __device__ __forceinline__ void tma_expect_and_load_3d(void* smem_dst, const voi
         : "memory");
 }
 
-// Both barriers, looked at together.
-__device__ __forceinline__ bool mbar_wait_both(uint64_t* bar1, uint32_t parity1, uint64_t* bar2, uint32_t parity2, StatusBlock* st, uint32_t id,
-                                               uint32_t stage, uint64_t limit_ns)
-{
-#pragma unroll 1
-    for (uint32_t i = 0; i < 4096u; ++i) {
-        const bool first = mbar_try_wait(bar1, parity1), second = mbar_try_wait(bar2, parity2);
-        if (__all_sync(0xFFFFFFFFu, first && second)) {
-            return true;
-        }
-    }
-    return mbar_wait_warp(bar1, parity1, st, id, stage, limit_ns) && mbar_wait_warp(bar2, parity2, st, id + 1u, stage, limit_ns);
-}
-
 constexpr uint32_t kBlockPairJoined = 32 * (kBlockPairPromoters + 1);  // threads of a named barrier
 
 __device__ __forceinline__ void named_sync(uint32_t id)

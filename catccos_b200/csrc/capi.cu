@@ -1779,21 +1779,39 @@ int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmPa
                     : encode_map_3d(&maps[2], o.b->codes, p.N, p.K, p.experts, columns, 128, ldb, plane);
 }
 
+// Units of a launch of single CTAs (with offsets: as many as there may be, one row tile that is not full for every expert with rows).
+uint64_t block_units(const BlockGemmParams& p, uint32_t tile_rows, uint32_t tile_columns)
+{
+    const uint64_t tiles = p.offsets ? p.rows / tile_rows + std::min(p.rows, p.experts) : (p.rows + tile_rows - 1) / tile_rows;
+    return tiles * ((p.N + tile_columns - 1) / tile_columns);
+}
+
 template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
 int launch_block_gemm_inst(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
 {
     using S = BlockGemmSmem<BLOCK_N>;
+    auto kern = block_gemm_kernel<BLOCK_N, OutT, kByColumn>;
     static PerDevice<bool, kMaxRanks * 2> done;
-    CUDA_TRY(allow_smem(block_gemm_kernel<BLOCK_N, OutT, kByColumn>, S::dynamic_bytes(kGroupedMaxExperts), done));
+    CUDA_TRY(allow_smem(kern, S::dynamic_bytes(S::kRing, kGroupedMaxExperts), done));
     CUtensorMap maps[3];
     int rcode = block_maps(maps, o, p, BLOCK_N);
     if (rcode != 0) return rcode;
-    // at most one row tile that is not full for every expert that has rows
-    const uint64_t tiles = p.offsets ? p.rows / kBlockGemmM + std::min(p.rows, p.experts) : (p.rows + kBlockGemmM - 1) / kBlockGemmM;
-    const uint64_t units = tiles * ((p.N + BLOCK_N - 1) / BLOCK_N);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(units, 2 * (uint64_t)rc.num_sms);
-    CUDA_TRY(launch_after(block_gemm_kernel<BLOCK_N, OutT, kByColumn>, dim3(grid), kBlockGemmThreads, S::dynamic_bytes(p.experts), st, maps[0],
-                          maps[1], maps[2], p));
+    // the list of experts, where it is long, takes its room from the ring (a CTA of two on an SM has 113 KB)
+    const uint32_t rest = S::dynamic_bytes(0, p.experts), ring = std::min(S::kRing, 113u * 1024u - rest);
+    p.a_stage_rows = p.a_cols ? kBlockGemmM : (std::min(p.rows, kBlockGemmM) + 31u) / 32u * 32u;
+    p.stages = std::min(ring / (p.a_stage_rows * 128u + S::kBBytes), S::kMaxStages);
+    p.ring_bytes = std::max(p.stages * (p.a_stage_rows * 128u + S::kBBytes), p.parts > 1 ? S::sum_bytes(p.parts) : 0u);
+    // the tensor core reads 128 rows of the last stage
+    p.ring_bytes = std::max(p.ring_bytes, (p.stages - 1u) * p.a_stage_rows * 128u + kBlockGemmM * 128u);
+    p.ring_bytes = (p.ring_bytes + 1023u) / 1024u * 1024u;
+    const uint64_t units = block_units(p, kBlockGemmM, BLOCK_N);
+    const uint32_t smem = S::dynamic_bytes(p.ring_bytes, p.experts);
+    if (p.parts > 1) {
+        CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockGemmThreads, smem, st, maps[0], maps[1], maps[2], p));
+    } else {
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(units, 2 * (uint64_t)rc.num_sms);
+        CUDA_TRY(launch_after(kern, dim3(grid), kBlockGemmThreads, smem, st, maps[0], maps[1], maps[2], p));
+    }
     return 0;
 }
 
@@ -1809,23 +1827,50 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     int rcode = block_maps(maps, o, p, 64);
     if (rcode == 0) rcode = encode_map_2d(&out, p.c, p.N, p.rows, 32, 32, false, sizeof(OutT));
     if (rcode != 0) return rcode;
-    const uint64_t tiles = p.offsets ? p.rows / kBlockPairM + std::min(p.rows, p.experts) : (p.rows + kBlockPairM - 1) / kBlockPairM;
-    const uint64_t units = tiles * ((p.N + kBlockPairN - 1) / kBlockPairN);
+    const uint64_t units = block_units(p, kBlockPairM, kBlockPairN);
     CUDA_TRY(launch_after(kern, dim3(2u * (unsigned)std::min<uint64_t>(units, (uint64_t)pairs)), kBlockPairThreads, S::dynamic_bytes(p.experts), st,
                           maps[0], maps[1], maps[2], out, p));
     return 0;
 }
 
-template <typename OutT>
-int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
+// A launch's tiles and in how many parts K is cut.
+struct BlockPlan {
+    uint32_t block_n, parts;
+    bool pair;
+};
+
+BlockPlan plan_block_gemm(const RankCtx& rc, const BlockGemmParams& p, bool by_column)
 {
-    if (g.cta_pair == 1 || (g.cta_pair == 0 && p.rows >= 1024)) {
-        return o.b->per_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
+    const uint32_t k_blocks = (p.K + 127u) / 128u;
+    auto most_parts = [&](uint32_t width) {
+        const uint64_t units = block_units(p, kBlockGemmM, width);
+        uint32_t parts = 1;
+        while (parts < kBlockGemmMaxParts && units * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
+               (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
+            parts *= 2;
+        }
+        return parts;
+    };
+    if (g.cta_pair == 1 || (g.cta_pair == 0 && p.rows >= 512)) {
+        return {kBlockPairN, 1, true};
     }
-    if (o.b->per_column) {
+    const uint32_t width = by_column || g.block_n == 128 ? 128u : 64u;
+    return {width, most_parts(width), false};
+}
+
+template <typename OutT>
+int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
+{
+    const bool by_column = o.b->per_column != 0;
+    const BlockPlan plan = plan_block_gemm(rc, p, by_column);
+    p.parts = plan.parts;
+    if (plan.pair) {
+        return by_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
+    }
+    if (by_column) {
         return launch_block_gemm_inst<128, OutT, true>(rc, st, o, p);
     }
-    return g.block_n == 64 ? launch_block_gemm_inst<64, OutT, false>(rc, st, o, p) : launch_block_gemm_inst<128, OutT, false>(rc, st, o, p);
+    return plan.block_n == 64 ? launch_block_gemm_inst<64, OutT, false>(rc, st, o, p) : launch_block_gemm_inst<128, OutT, false>(rc, st, o, p);
 }
 
 // Common part of the two products.
