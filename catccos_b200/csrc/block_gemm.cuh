@@ -11,7 +11,7 @@
 // that x W, dy W^T and x^T dy read the same codes without a transposed copy.  K need not be a multiple of 128: TMA fills the
 // last block with zeros.
 //
-// 320 threads: warps 0-7 promotion and output (warp w: lane quarter w % 4, column half w / 4), warp 8 TMA, warp 9 MMA.
+// This file: what the two forms share, and the one for few rows (an expert); block_gemm_pair.cuh: the one for many.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -23,9 +23,9 @@
 
 namespace catccos {
 
-constexpr uint32_t kBlockGemmThreads = 320;
-constexpr uint32_t kBlockGemmM = 128;
-constexpr uint32_t kBlockGemmMaxParts = 8;
+constexpr uint32_t kBlockFewThreads = 256;
+constexpr uint32_t kBlockFewColumns = 128;  // of the weight, to a tile
+constexpr uint32_t kBlockFewMaxParts = 8;
 
 struct BlockGemmParams {
     const float* a_scales;
@@ -37,8 +37,7 @@ struct BlockGemmParams {
     uint32_t rows, experts, N, K;
     uint32_t a_fmt, b_fmt;                                 // 0 = E4M3, 1 = E5M2
     uint32_t a_cols, b_rows;                               // 1: A is stored [K, rows]; B [N, K]
-    uint32_t parts;                                        // CTAs of a cluster that share K (a power of two)
-    uint32_t stages, a_stage_rows, ring_bytes;             // of block_gemm_kernel's ring (BlockGemmSmem)
+    uint32_t parts;                                        // few rows: CTAs of a cluster that share K (a power of two)
     uint64_t bar_timeout_ns;
     StatusBlock* status;
 };
@@ -62,11 +61,31 @@ __host__ __device__ constexpr uint32_t make_idesc_f8(uint32_t M, uint32_t N, uin
     return (1u << 4) | (a_fmt << 7) | (b_fmt << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
 
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z)
+// A tile load with the announcement of its bytes, by one lane of a converged warp: with a branch on the lane such instructions take
+// several times as long to issue.
+__device__ __forceinline__ void tma_expect_and_load_2d(void* smem_dst, const void* tmap, uint64_t* bar, uint32_t bytes, uint32_t x, uint32_t y)
 {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        "{\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one mbarrier.arrive.expect_tx.shared::cta.b64 _, [%2], %5;\n\t"
+        "@one cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t"
+        "}"
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(bytes)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_expect_and_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, uint32_t bytes, uint32_t x, uint32_t y, uint32_t z)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred one;\n\t"
+        "elect.sync _|one, 0xffffffff;\n\t"
+        "@one mbarrier.arrive.expect_tx.shared::cta.b64 _, [%2], %6;\n\t"
+        "@one cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t"
+        "}"
+        ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(bytes)
         : "memory");
 }
 
@@ -250,233 +269,240 @@ __device__ __forceinline__ bool mbar_wait_both(uint64_t* bar1, uint32_t parity1,
     return mbar_wait_warp(bar1, parity1, st, id, stage, limit_ns) && mbar_wait_warp(bar2, parity2, st, id + 1u, stage, limit_ns);
 }
 
-// Shared memory of block_gemm_kernel.  How many rows of A a stage holds, and with it how many stages there are, is the launch's
-// choice: few rows leave more room for B on its way.  (The tensor core reads 128 rows whatever a stage holds; the others' products
-// are not looked at.)
-template <uint32_t BLOCK_N>
-struct BlockGemmSmem {
-    static constexpr uint32_t kMaxStages = 8;
-    static constexpr uint32_t kBBytes = BLOCK_N * 128;
-    static constexpr uint32_t kScaleSlots = 4;                                                  // by column: scales of a block
-    static constexpr uint32_t kScaleBytes = kScaleSlots * BLOCK_N * 4;
-    static constexpr uint32_t kNumBars = 2 * kMaxStages + 4 + 2 * kScaleSlots;                  // full[], empty[], tmem_full[2], tmem_empty[2], scale_full[], scale_empty[]
-    static constexpr uint32_t kRest = kScaleBytes + kNumBars * 8 + 16;                          // behind the ring
-    static constexpr uint32_t dynamic_bytes(uint32_t ring, uint32_t experts) { return ring + kRest + (3u * experts + 1u) * 4u + 1024u; }
-    static constexpr uint32_t kRing = 106496;  // at most: two CTAs to an SM
-    // the parts' sums meet in the ring: [part][128 rows][a part's columns, four more]
-    static constexpr uint32_t sum_bytes(uint32_t parts) { return kBlockGemmM * (BLOCK_N + 4u * parts) * 4u; }
+// ------------------------------------------------------------------------------------------
+// few rows
+// ------------------------------------------------------------------------------------------
+// Up to 64 rows (of an expert) are bound by streaming the weights and by latencies, so the operands change sides: 128 columns of the
+// weight are the rows of a tile, kRows rows of A its columns.  A lane then has one weight column and kRows sums, and every warp of
+// the promotion has work however few the rows are.  (With the rows of A on the lanes the one warp that has 16 rows took 600 cycles a
+// block and 16 x 4096 x 7168 12.9 us.)
+//
+// K may be cut over the CTAs of a cluster (p.parts: 1, 2, 4 or 8), so that calls of few tiles stream their weights with every SM.
+// Their sums meet in distributed shared memory: part d owns 128 / parts of the weight columns, the others push theirs into its idle
+// ring, and it adds them in ascending order of the parts.  A launch with parts has a cluster for every unit there may be.
+//
+// 256 threads, two CTAs to an SM: warps 0-3 promotion and output (lane quarter = warp), 4 and 5 TMA for B and A, 6 MMA, 7 the factors:
+// the scales of the rows times the weight's, for groups of four blocks of K (every unit begins with a group of its own).
+template <uint32_t kRows>
+struct BlockFewSmem {
+    static constexpr uint32_t kStages = kRows == 64 ? 4 : 5;
+    static constexpr uint32_t kWBytes = kBlockFewColumns * 128, kXBytes = kRows * 128;
+    static constexpr uint32_t kTiles = 4, kTmemCols = kTiles * kRows;
+    static constexpr uint32_t kGroups = 4;  // of factors, on their way
+    static constexpr uint32_t kOffW = 0;
+    static constexpr uint32_t kOffX = kOffW + kStages * kWBytes;
+    static constexpr uint32_t kOffFactor = kOffX + kStages * kXBytes;  // [4 blocks][kRows] a group
+    static constexpr uint32_t kOffBar = kOffFactor + kGroups * 4 * kRows * 4;
+    static constexpr uint32_t kNumBars = 2 * kStages + 2 * kTiles + 2 * kGroups;
+    static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
+    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
+    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
+    static constexpr uint32_t kPitch = kRows + 4;  // floats of a weight column's sums in the exchange
+    static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
+    static_assert(kBlockFewColumns * kPitch * 4 <= kOffX, "the sums of all parts fit the idle ring");
 };
 
-// K may be cut over the CTAs of a cluster (p.parts: 1, 2, 4 or 8), so that calls of few tiles stream their weights with every SM.
-// Their sums meet in distributed shared memory: part d owns BLOCK_N / parts of the columns, the others push theirs into its idle
-// ring, and it adds them in ascending order of the parts.  A launch with parts has a cluster for every unit there may be.
-template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
-__global__ void __launch_bounds__(kBlockGemmThreads, 2)
-block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
-                  const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ BlockGemmParams p)
+template <uint32_t kRows, typename OutT>
+__global__ void __launch_bounds__(kBlockFewThreads, 2)
+block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ BlockGemmParams p)
 {
-    using S = BlockGemmSmem<BLOCK_N>;
-    constexpr uint32_t kCols = BLOCK_N / 2;  // of a promotion warp
-    constexpr uint32_t kTmemCols = 2 * BLOCK_N;
+    using S = BlockFewSmem<kRows>;
+    constexpr uint32_t kStages = S::kStages, kTiles = S::kTiles;
 
     grid_dep_launch();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const uint32_t stages = p.stages, a_bytes = p.a_stage_rows * 128u;
-    uint8_t* smem_b = smem + stages * a_bytes;
-    float* scales = reinterpret_cast<float*>(smem + p.ring_bytes);
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + p.ring_bytes + S::kScaleBytes);
-    uint64_t* empty = full + S::kMaxStages;
-    uint64_t* tmem_full = empty + S::kMaxStages;
-    uint64_t* tmem_empty = tmem_full + 2;
-    uint64_t* scale_full = tmem_empty + 2;
-    uint64_t* scale_empty = scale_full + S::kScaleSlots;
-    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(scale_empty + S::kScaleSlots);
-    uint32_t* dead = tmem_ptr_smem + 1;  // a part of this cluster has given up
-    uint32_t* tiles = tmem_ptr_smem + 4;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kOffBar);
+    uint64_t* empty = full + kStages;
+    uint64_t* tmem_full = empty + kStages;
+    uint64_t* tmem_empty = tmem_full + kTiles;
+    uint64_t* scale_full = tmem_empty + kTiles;
+    uint64_t* scale_empty = scale_full + S::kGroups;
+    uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
+    uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
+    uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t n_tiles = (p.N + BLOCK_N - 1) / BLOCK_N;
+    const uint32_t n_tiles = (p.N + kBlockFewColumns - 1) / kBlockFewColumns;
     const uint32_t k_blocks = (p.K + 127u) / 128u;
     const uint32_t part = blockIdx.x & (p.parts - 1u), first_unit = blockIdx.x / p.parts, stride = gridDim.x / p.parts;
     const uint32_t kb0 = (uint32_t)((uint64_t)part * k_blocks / p.parts), kb1 = (uint32_t)((uint64_t)(part + 1u) * k_blocks / p.parts);
     const uint64_t bar_ns = p.bar_timeout_ns;
 
-    if (threadIdx.x == 256) {
-        for (uint32_t s = 0; s < stages; ++s) {
-            mbar_init(&full[s], 1);
+    if (threadIdx.x == 128) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 2);  // both producers (expect_tx)
             mbar_init(&empty[s], 1);
         }
-        for (uint32_t a = 0; a < 2; ++a) {
-            mbar_init(&tmem_full[a], 1);
-            mbar_init(&tmem_empty[a], 8);
+        for (uint32_t b = 0; b < kTiles; ++b) {
+            mbar_init(&tmem_full[b], 1);
+            mbar_init(&tmem_empty[b], 4);
         }
-        for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
+        for (uint32_t i = 0; i < S::kGroups; ++i) {
             mbar_init(&scale_full[i], 1);
-            mbar_init(&scale_empty[i], 8);
+            mbar_init(&scale_empty[i], 4);
         }
         *dead = 0u;
         mbar_fence_init();
-        tma_prefetch_desc(&tmap_a);
-        tma_prefetch_desc(&tmap_a32);
-        tma_prefetch_desc(&tmap_b);
+        tma_prefetch_desc(&tmap_x);
+        tma_prefetch_desc(&tmap_w);
     }
-    if (warp == 9) {
-        tmem_alloc(tmem_ptr_smem, kTmemCols);
+    if (warp == 6) {
+        tmem_alloc(tmem_ptr_smem, S::kTmemCols);
         tmem_relinquish();
     }
     grid_dep_wait();
     if (warp == 0) {
-        count_block_tiles(p, kBlockGemmM, tiles, row_begin, row_end, lane);
+        count_block_tiles(p, kRows, tiles, row_begin, row_end, lane);
     }
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_ptr_smem;
-    const uint32_t num_units = tiles[p.experts] * n_tiles;
+    // Offsets that do not ascend may give more units than the host reckoned with: with parts a cluster meets for one unit, no more.
+    const uint32_t num_units = p.parts > 1u ? min(tiles[p.experts] * n_tiles, stride) : tiles[p.experts] * n_tiles;
     bool alive = true;  // false once a wait of this role has given up
     GroupedWalk walk;
 
-    if (warp == 8) {
-        // ------------------------------- TMA producer -------------------------------------
-        uint32_t it = 0, s = 0, ph = 1;
+    if (warp == 4 || warp == 5) {
+        // ------------------------------- TMA producers ------------------------------------
+        uint32_t s = 0, ph = 1;
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
-            const uint32_t m0 = row_begin[walk.e] + tc.m_tile * kBlockGemmM, n0 = tc.n_tile * BLOCK_N;
-            const uint32_t boxes = (min(row_end[walk.e] - m0, kBlockGemmM) + 31u) / 32u;  // of 32 rows
-            const uint32_t scale_bytes = min(p.N - n0, BLOCK_N) * 4u;
-            const uint32_t tx_bytes = (p.a_cols ? kBlockGemmM * 128u : boxes * (32u * 128u)) + S::kBBytes;
-            for (uint32_t kb = kb0; alive && kb < kb1; ++kb, ++it) {
+            const uint32_t m0 = row_begin[walk.e] + tc.m_tile * kRows, n0 = tc.n_tile * kBlockFewColumns;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                const uint32_t k = kb * 128u;
                 alive = mbar_wait_soon(&empty[s], ph, p.status, 400, s, bar_ns);
                 if (!alive) {
                     break;
                 }
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(&full[s], tx_bytes);
-                    const int32_t k = (int32_t)(kb * 128u);
-                    tma_load_3d(smem_b + s * S::kBBytes, &tmap_b, &full[s], p.b_rows ? k : (int32_t)n0, p.b_rows ? (int32_t)n0 : k, (int32_t)walk.e);
-                    uint8_t* a = smem + s * a_bytes;
-                    if (p.a_cols) {
-                        tma_load_2d(a, &tmap_a, &full[s], (int32_t)m0, k);
-                    } else if (boxes == 4u) {
-                        tma_load_2d(a, &tmap_a, &full[s], k, (int32_t)m0);
-                    } else {
-                        for (uint32_t i = 0; i < boxes; ++i) {
-                            tma_load_2d(a + i * (32u * 128u), &tmap_a32, &full[s], k, (int32_t)(m0 + i * 32u));
-                        }
-                    }
+                if (warp == 4) {
+                    tma_expect_and_load_3d(smem + S::kOffW + s * S::kWBytes, &tmap_w, &full[s], S::kWBytes, p.b_rows ? k : n0, p.b_rows ? n0 : k, walk.e);
+                } else {  // rows behind the expert's last come along: their products are not looked at
+                    tma_expect_and_load_2d(smem + S::kOffX + s * S::kXBytes, &tmap_x, &full[s], S::kXBytes, k, m0);
                 }
-                __syncwarp();
-                if (kByColumn) {
-                    const uint32_t slot = it % S::kScaleSlots;
-                    alive = mbar_wait_soon(&scale_empty[slot], ((it / S::kScaleSlots) & 1u) ^ 1u, p.status, 405, slot, bar_ns);
-                    if (alive && elect_one()) {
-                        mbar_arrive_expect_tx(&scale_full[slot], scale_bytes);
-                        bulk_load(scales + slot * BLOCK_N, p.b_scales + (size_t)walk.e * p.b_scale_matrix + kb * p.b_scale_block + n0, scale_bytes, &scale_full[slot]);
-                    }
-                    __syncwarp();
-                }
-                s = s + 1u == stages ? 0u : s + 1u;
+                s = s + 1u == kStages ? 0u : s + 1u;
                 ph ^= s == 0u ? 1u : 0u;
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == 6) {
         // ------------------------------- MMA issuer ---------------------------------------
-        const uint32_t idesc0 = make_idesc_f8(kBlockGemmM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
-        const uint64_t desc_a = p.a_cols ? make_smem_desc(0, 16384, 1024, 2) : make_smem_desc(0, 16, 1024, 2);
-        const uint64_t desc_b = p.b_rows ? make_smem_desc(0, 16, 1024, 2)
-                                         : make_smem_desc(0, 16384, 8 * BLOCK_N, BLOCK_N == 64 ? 4 : 2);
-        const uint32_t hi_a = (uint32_t)(desc_a >> 32), hi_b = (uint32_t)(desc_b >> 32);
-        const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem) >> 4);
-        const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem_b) >> 4);
-        const uint32_t step_a = (p.a_cols ? 32u * 128u : 32u) >> 4, step_b = (p.b_rows ? 32u : 32u * BLOCK_N) >> 4;
+        const uint32_t idesc = make_idesc_f8(kBlockFewColumns, kRows, p.b_fmt, p.a_fmt, p.b_rows == 0u, false);
+        const uint64_t desc_k = make_smem_desc(0, 16, 1024, 2), desc_w = p.b_rows ? desc_k : make_smem_desc(0, 16384, 1024, 2);
+        const uint32_t hi_w = (uint32_t)(desc_w >> 32), hi_x = (uint32_t)(desc_k >> 32);
+        const uint32_t w_lo0 = (uint32_t)desc_w | (smem_u32(smem + S::kOffW) >> 4);
+        const uint32_t x_lo0 = (uint32_t)desc_k | (smem_u32(smem + S::kOffX) >> 4);
+        const uint32_t step_w = (p.b_rows ? 32u : 4096u) >> 4;
         uint32_t it = 0, s = 0, ph = 0;
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
-            // a ragged last column of tiles is multiplied as wide as it is (a multiple of 16)
-            const uint32_t idesc = idesc0 | ((min(p.N - unit % n_tiles * BLOCK_N, BLOCK_N) >> 3) << 17);
             for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t buf = it & 1u;
-                alive = mbar_wait_both(&full[s], ph, &tmem_empty[buf], ((it >> 1) & 1u) ^ 1u, p.status, 401, s, bar_ns);
+                const uint32_t b = it % kTiles;
+                alive = mbar_wait_both(&full[s], ph, &tmem_empty[b], ((it / kTiles) & 1u) ^ 1u, p.status, 401, s, bar_ns);
                 if (!alive) {
                     break;  // nothing is issued, and no tile reported, after a wait has given up
                 }
                 tcgen05_fence_after();
-                umma_f8_block(tmem_base + buf * BLOCK_N, a_lo0 + s * (a_bytes >> 4), hi_a, step_a, b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b, idesc,
-                              &tmem_full[buf], &empty[s]);
-                s = s + 1u == stages ? 0u : s + 1u;
+                umma_f8_block(tmem_base + b * kRows, w_lo0 + s * (S::kWBytes >> 4), hi_w, step_w, x_lo0 + s * (S::kXBytes >> 4), hi_x, 32u >> 4, idesc,
+                              &tmem_full[b], &empty[s]);
+                s = s + 1u == kStages ? 0u : s + 1u;
                 ph ^= s == 0u ? 1u : 0u;
+            }
+        }
+    } else if (warp == 7) {
+        // ------------------------------- factors ------------------------------------------
+        constexpr uint32_t kPerLane = (kRows + 31) / 32;
+        uint32_t group = 0;
+        for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
+            const TileCoord tc = walk.seek(tiles, n_tiles, unit);
+            const uint32_t row = row_begin[walk.e] + tc.m_tile * kRows + lane, end = row_end[walk.e];
+            const float* w_scales = p.b_scales + walk.e * p.b_scale_matrix + tc.n_tile * p.b_scale_col;
+            for (uint32_t kb = kb0; kb < kb1; kb += 4u, ++group) {
+                float x[kPerLane][4], w[4];
+                load_scales(w_scales, p.b_scale_block, kb, kb1, w);
+#pragma unroll
+                for (uint32_t i = 0; i < kPerLane; ++i) {
+                    load_scales(p.a_scales + min(row + 32u * i, end - 1u) * p.a_scale_row, p.a_scale_block, kb, kb1, x[i]);
+                }
+                const uint32_t slot = group % S::kGroups;
+                alive = mbar_wait_soon(&scale_empty[slot], ((group / S::kGroups) & 1u) ^ 1u, p.status, 405, slot, bar_ns);
+                if (!alive) {
+                    break;
+                }
+                float* factor = reinterpret_cast<float*>(smem + S::kOffFactor) + slot * (4u * kRows) + lane;
+                if (lane < kRows) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kPerLane; ++i) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            factor[j * kRows + 32u * i] = x[i][j] * w[j];
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&scale_full[slot]);
+                }
             }
         }
     } else {
         // ------------------------------- promotion and output -----------------------------
-        const uint32_t q = warp & 3u, half = warp >> 2;
-        const uint32_t tmem = tmem_base + ((q * 32u) << 16) + half * kCols;
-        uint32_t it = 0;
+        const uint32_t tmem = tmem_base + ((warp * 32u) << 16), column = warp * 32u + lane;
+        uint32_t it = 0, group = 0;
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
-            const uint32_t first = row_begin[walk.e] + tc.m_tile * kBlockGemmM, end = row_end[walk.e];
-            const uint32_t row0 = first + q * 32u, row = row0 + lane, n0 = tc.n_tile * BLOCK_N;
-            const bool live = row0 < end && n0 + half * kCols < p.N;  // else there is nothing to fetch
-            const float* a_line = p.a_scales + min(row, end - 1u) * p.a_scale_row;
-            const float* b_line = p.b_scales + walk.e * p.b_scale_matrix + (n0 / 128u) * p.b_scale_col;
-            float acc[kCols] = {};
-            float a4[4], b4[4];  // scales of four blocks
-            auto fetch = [&](uint32_t kb) {
-                if (live) {
-                    load_scales(a_line, p.a_scale_block, kb, kb1, a4);
-                    if (!kByColumn) {
-                        load_scales(b_line, p.b_scale_block, kb, kb1, b4);
-                    }
-                }
-            };
-            fetch(kb0);
+            const uint32_t first = row_begin[walk.e] + tc.m_tile * kRows, rows = min(row_end[walk.e] - first, kRows);
+            const uint32_t n0 = tc.n_tile * kBlockFewColumns;
+            float acc[kRows] = {};
             for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t buf = it & 1u, slot = it % S::kScaleSlots, j = (kb - kb0) & 3u;
-                alive = kByColumn ? mbar_wait_both(&tmem_full[buf], (it >> 1) & 1u, &scale_full[slot], (it / S::kScaleSlots) & 1u, p.status, 406, buf, bar_ns)
-                                  : mbar_wait_soon(&tmem_full[buf], (it >> 1) & 1u, p.status, 406, buf, bar_ns);
+                const uint32_t b = it % kTiles, slot = group % S::kGroups, j = (kb - kb0) & 3u;
+                alive = j == 0u ? mbar_wait_both(&tmem_full[b], (it / kTiles) & 1u, &scale_full[slot], (group / S::kGroups) & 1u, p.status, 406, b, bar_ns)
+                                : mbar_wait_soon(&tmem_full[b], (it / kTiles) & 1u, p.status, 406, b, bar_ns);
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
                 tcgen05_fence_after();
-                if (live) {
-                    auto pick = [&](const float (&v)[4]) { return j == 0u ? v[0] : (j == 1u ? v[1] : (j == 2u ? v[2] : v[3])); };
-                    const float f = kByColumn ? pick(a4) : pick(a4) * pick(b4);
-                    if (j == 3u) {
-                        fetch(kb + 1u);  // the next four, while this block is added
-                    }
+                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (slot * 4u + j) * (kRows / 4);
 #pragma unroll
-                    for (uint32_t c = 0; c < kCols; c += 16) {
+                for (uint32_t c = 0; c < kRows; c += 16) {
+                    if (c < rows) {
                         float v[16];
-                        tmem_ld_16(tmem + buf * BLOCK_N + c, v);
+                        tmem_ld_16(tmem + b * kRows + c, v);
                         tmem_ld_fence(v);
-                        add_scaled<kByColumn>(&acc[c], v, f, scales + slot * BLOCK_N + half * kCols + c);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i += 4) {
+                            const float4 f = factor[(c + i) / 4];
+                            fma_2(acc[c + i], acc[c + i + 1], v[i], v[i + 1], f.x, f.y);
+                            fma_2(acc[c + i + 2], acc[c + i + 3], v[i + 2], v[i + 3], f.z, f.w);
+                        }
                     }
                 }
                 tcgen05_fence_before();
                 __syncwarp();
+                const bool group_end = j == 3u || kb + 1u == kb1;
                 if (lane == 0) {
-                    mbar_arrive(&tmem_empty[buf]);
-                    if (kByColumn) {
+                    mbar_arrive(&tmem_empty[b]);
+                    if (group_end) {
                         mbar_arrive(&scale_empty[slot]);
                     }
                 }
+                group += group_end ? 1u : 0u;
             }
+            OutT* out = static_cast<OutT*>(p.c) + (size_t)first * p.N + n0;
             if (p.parts == 1u) {
-                if (alive && row < end) {
-                    OutT* dst = static_cast<OutT*>(p.c) + (size_t)row * p.N + n0 + half * kCols;
+                if (alive && n0 + column < p.N) {
 #pragma unroll
-                    for (uint32_t c = 0; c < kCols; c += 16) {
-                        if (n0 + half * kCols + c < p.N) {
-                            store_16(dst + c, &acc[c]);
+                    for (uint32_t t = 0; t < kRows; ++t) {
+                        if (t < rows) {
+                            out[(size_t)t * p.N + column] = static_cast<OutT>(acc[t]);
                         }
                     }
                 }
                 continue;
             }
             // The sums of all parts.  Every CTA of the cluster has multiplied its last block: the rings are idle.
-            const uint32_t cols = BLOCK_N / p.parts, shift = __ffs(cols) - 1, pitch = cols + 4u;  // a part's columns; four more keep lanes off one bank
+            const uint32_t shift = __ffs(kBlockFewColumns / p.parts) - 1;  // of a part's columns
             cluster_sync_all();
             if (!alive && lane == 0) {
                 for (uint32_t d = 0; d < p.parts; ++d) {
@@ -484,13 +510,15 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
                 }
             }
             __syncwarp();
-            if (alive && row < end) {
-                const uint32_t line = smem_u32(smem) + (part * 128u + q * 32u + lane) * pitch * 4u;
+            if (alive) {
+                const uint32_t to = column >> shift, line = (part << shift) + (column - (to << shift));
+                const uint32_t at = map_to_cta(smem_u32(smem) + line * (S::kPitch * 4u), to);
 #pragma unroll
-                for (uint32_t c = 0; c < kCols; c += 4) {
-                    const uint32_t col = half * kCols + c, d = col >> shift;
-                    st_shared_cluster_v4(map_to_cta(line + (col - (d << shift)) * 4u, d), __float_as_uint(acc[c]), __float_as_uint(acc[c + 1]),
-                                         __float_as_uint(acc[c + 2]), __float_as_uint(acc[c + 3]));
+                for (uint32_t t = 0; t < kRows; t += 4) {
+                    if (t < rows) {
+                        st_shared_cluster_v4(at + t * 4u, __float_as_uint(acc[t]), __float_as_uint(acc[t + 1]), __float_as_uint(acc[t + 2]),
+                                             __float_as_uint(acc[t + 3]));
+                    }
                 }
             }
             __syncwarp();
@@ -498,30 +526,20 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
             if (*reinterpret_cast<volatile uint32_t*>(dead) != 0u) {
                 alive = false;
             }
-            const uint32_t rows = min(end - first, kBlockGemmM);
-            for (uint32_t i = threadIdx.x; alive && i < rows << (shift - 2u); i += 256u) {
-                const uint32_t r = i >> (shift - 2u), c = (i & ((1u << (shift - 2u)) - 1u)) * 4u, n = n0 + part * cols + c;
-                const float* at = reinterpret_cast<const float*>(smem) + r * pitch + c;
-                float4 sum = *reinterpret_cast<const float4*>(at);
+            for (uint32_t i = threadIdx.x; alive && i < rows << shift; i += 128u) {
+                const uint32_t t = i >> shift, c = i - (t << shift), n = (part << shift) + c;
+                const float* at = reinterpret_cast<const float*>(smem) + c * S::kPitch + t;
+                float sum = *at;
                 for (uint32_t src = 1; src < p.parts; ++src) {
-                    const float4 x = *reinterpret_cast<const float4*>(at + src * 128u * pitch);
-                    sum.x += x.x;
-                    sum.y += x.y;
-                    sum.z += x.z;
-                    sum.w += x.w;
+                    sum += at[(src << shift) * S::kPitch];
                 }
-                if (n < p.N) {
-                    OutT* dst = static_cast<OutT*>(p.c) + (size_t)(first + r) * p.N + n;
-                    if constexpr (sizeof(OutT) == 4) {
-                        *reinterpret_cast<float4*>(dst) = sum;
-                    } else {
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<OutT>(sum.x, sum.y), pack2<OutT>(sum.z, sum.w));
-                    }
+                if (n0 + n < p.N) {
+                    out[(size_t)t * p.N + n] = static_cast<OutT>(sum);
                 }
             }
         }
     }
-    if (warp >= 8 && p.parts > 1u && first_unit < num_units) {
+    if (warp >= 4 && p.parts > 1u && first_unit < num_units) {
         __syncwarp();
         cluster_sync_all();  // the two meetings of the promotion warps
         cluster_sync_all();
@@ -531,9 +549,9 @@ block_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
     if (__syncthreads_or(alive ? 0 : 1)) {
         drain_after_abort(p.status);
     }
-    if (warp == 9) {
+    if (warp == 6) {
         tcgen05_fence_after();
-        tmem_dealloc(tmem_base, kTmemCols);
+        tmem_dealloc(tmem_base, S::kTmemCols);
     }
 }
 

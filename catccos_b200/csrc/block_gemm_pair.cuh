@@ -96,7 +96,7 @@ __device__ __forceinline__ void umma_f8_pair_block(uint32_t tmem_d, uint32_t a_l
 }
 
 // A pair's tile load with the announcement of its bytes, by one lane of a converged warp (as umma_f8_pair_block).
-__device__ __forceinline__ void tma_expect_and_load_2d(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y)
+__device__ __forceinline__ void tma_expect_and_load_2d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y)
 {
     asm volatile(
         "{\n\t"
@@ -109,7 +109,7 @@ __device__ __forceinline__ void tma_expect_and_load_2d(void* smem_dst, const voi
         : "memory");
 }
 
-__device__ __forceinline__ void tma_expect_and_load_3d(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y,
+__device__ __forceinline__ void tma_expect_and_load_3d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, uint32_t bytes, uint32_t x, uint32_t y,
                                                        uint32_t z)
 {
     asm volatile(
@@ -231,9 +231,9 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     break;
                 }
                 if (!rows) {
-                    tma_expect_and_load_3d(smem + S::kOffB + s * S::kBBytes, &tmap_b, leader_bar, S::kBBytes, p.b_rows ? k : n, p.b_rows ? n : k, u.e);
+                    tma_expect_and_load_3d_pair(smem + S::kOffB + s * S::kBBytes, &tmap_b, leader_bar, S::kBBytes, p.b_rows ? k : n, p.b_rows ? n : k, u.e);
                 } else if (boxes == 4u || (p.a_cols && boxes)) {
-                    tma_expect_and_load_2d(smem + S::kOffA + s * S::kABytes, &tmap_a, leader_bar, S::kABytes, p.a_cols ? m0 : k, p.a_cols ? k : m0);
+                    tma_expect_and_load_2d_pair(smem + S::kOffA + s * S::kABytes, &tmap_a, leader_bar, S::kABytes, p.a_cols ? m0 : k, p.a_cols ? k : m0);
                 } else {
                     if (elect_one()) {
                         mbar_arrive_expect_tx_cluster(leader_bar, boxes * (32u * 128u));

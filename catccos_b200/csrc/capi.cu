@@ -177,6 +177,7 @@ struct State {
     int a_dtype = 0;         // element type of the A codes (what the quantiser writes, what the GEMM reads): 0 = E4M3, 1 = E5M2
     int b_dtype = 0;         // element type of the B codes the caller passes
     int split_k = 0;         // 0 = automatic, 1 = never split K, 2..8 = split K in that many parts when it fits
+    int block_rows = 0;      // products of blocks of 128: 0 = automatic, 16, 32, 64 = tiles of so many rows
     int b_lsu = 0;           // 0 = automatic, 1 = B through the load/store units, 2 = through TMA
     int small_tile = 0;      // 0 = automatic, 1 = always the small-tile kernel where it can run, 2 = never
     int small_quant = 0;     // 0 = automatic, 1 = the small-tile kernel quantises a fused call itself, 2 = never
@@ -1766,13 +1767,14 @@ struct BlockOperands {
     const catccos_b200_block_operand_t *a, *b;
 };
 
-// Maps of the rows of a (boxes of a_box and of 32 rows; stored by column: boxes of 128 x 128) and of b (`columns` wide).
-int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmParams& p, uint32_t columns)
+// Maps of the rows of a (boxes of `most` and, in maps[1], of `few` rows; stored by column: boxes of 128 x 128) and of b (`columns`
+// wide).
+int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmParams& p, uint32_t few, uint32_t columns)
 {
     const void* a = o.a->codes;
     const uint64_t lda = o.a->line_bytes, ldb = o.b->line_bytes;
     int rcode = p.a_cols ? encode_map_2d(&maps[0], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[0], a, p.K, p.rows, 128, 128, false, 1, lda);
-    if (rcode == 0) rcode = p.a_cols ? encode_map_2d(&maps[1], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[1], a, p.K, p.rows, 128, 32, false, 1, lda);
+    if (rcode == 0) rcode = p.a_cols ? encode_map_2d(&maps[1], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[1], a, p.K, p.rows, 128, few, false, 1, lda);
     if (rcode != 0) return rcode;
     const uint64_t plane = p.experts > 1 ? o.b->matrix_bytes : ldb * (p.b_rows ? p.N : p.K);
     return p.b_rows ? encode_map_3d(&maps[2], o.b->codes, p.K, p.N, p.experts, 128, columns, ldb, plane)
@@ -1786,31 +1788,23 @@ uint64_t block_units(const BlockGemmParams& p, uint32_t tile_rows, uint32_t tile
     return tiles * ((p.N + tile_columns - 1) / tile_columns);
 }
 
-template <uint32_t BLOCK_N, typename OutT, bool kByColumn>
-int launch_block_gemm_inst(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
+template <uint32_t kRows, typename OutT>
+int launch_block_few(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
 {
-    using S = BlockGemmSmem<BLOCK_N>;
-    auto kern = block_gemm_kernel<BLOCK_N, OutT, kByColumn>;
+    using S = BlockFewSmem<kRows>;
+    auto kern = block_gemm_few_kernel<kRows, OutT>;
     static PerDevice<bool, kMaxRanks * 2> done;
-    CUDA_TRY(allow_smem(kern, S::dynamic_bytes(S::kRing, kGroupedMaxExperts), done));
+    CUDA_TRY(allow_smem(kern, S::dynamic_bytes(kGroupedMaxExperts), done));
     CUtensorMap maps[3];
-    int rcode = block_maps(maps, o, p, BLOCK_N);
+    int rcode = block_maps(maps, o, p, kRows, kBlockFewColumns);
     if (rcode != 0) return rcode;
-    // the list of experts, where it is long, takes its room from the ring (a CTA of two on an SM has 113 KB)
-    const uint32_t rest = S::dynamic_bytes(0, p.experts), ring = std::min(S::kRing, 113u * 1024u - rest);
-    p.a_stage_rows = p.a_cols ? kBlockGemmM : (std::min(p.rows, kBlockGemmM) + 31u) / 32u * 32u;
-    p.stages = std::min(ring / (p.a_stage_rows * 128u + S::kBBytes), S::kMaxStages);
-    p.ring_bytes = std::max(p.stages * (p.a_stage_rows * 128u + S::kBBytes), p.parts > 1 ? S::sum_bytes(p.parts) : 0u);
-    // the tensor core reads 128 rows of the last stage
-    p.ring_bytes = std::max(p.ring_bytes, (p.stages - 1u) * p.a_stage_rows * 128u + kBlockGemmM * 128u);
-    p.ring_bytes = (p.ring_bytes + 1023u) / 1024u * 1024u;
-    const uint64_t units = block_units(p, kBlockGemmM, BLOCK_N);
-    const uint32_t smem = S::dynamic_bytes(p.ring_bytes, p.experts);
+    const uint64_t units = block_units(p, kRows, kBlockFewColumns);
+    const uint32_t smem = S::dynamic_bytes(p.experts);
     if (p.parts > 1) {
-        CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockGemmThreads, smem, st, maps[0], maps[1], maps[2], p));
+        CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockFewThreads, smem, st, maps[1], maps[2], p));
     } else {
         const uint32_t grid = (uint32_t)std::min<uint64_t>(units, 2 * (uint64_t)rc.num_sms);
-        CUDA_TRY(launch_after(kern, dim3(grid), kBlockGemmThreads, smem, st, maps[0], maps[1], maps[2], p));
+        CUDA_TRY(launch_after(kern, dim3(grid), kBlockFewThreads, smem, st, maps[1], maps[2], p));
     }
     return 0;
 }
@@ -1824,7 +1818,7 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     int pairs = 0;
     CUDA_TRY(resident_clusters_of_two(rc, kern, kBlockPairThreads, S::dynamic_bytes(kGroupedMaxExperts), resident, &pairs));
     CUtensorMap maps[3], out;
-    int rcode = block_maps(maps, o, p, 64);
+    int rcode = block_maps(maps, o, p, 32, 64);
     if (rcode == 0) rcode = encode_map_2d(&out, p.c, p.N, p.rows, 32, 32, false, sizeof(OutT));
     if (rcode != 0) return rcode;
     const uint64_t units = block_units(p, kBlockPairM, kBlockPairN);
@@ -1833,29 +1827,29 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     return 0;
 }
 
-// A launch's tiles and in how many parts K is cut.
+// Which form a launch takes: CTA pairs (rows 0), or tiles of so many rows with K in so many parts.
 struct BlockPlan {
-    uint32_t block_n, parts;
-    bool pair;
+    uint32_t rows, parts;
 };
 
 BlockPlan plan_block_gemm(const RankCtx& rc, const BlockGemmParams& p, bool by_column)
 {
-    const uint32_t k_blocks = (p.K + 127u) / 128u;
-    auto most_parts = [&](uint32_t width) {
-        const uint64_t units = block_units(p, kBlockGemmM, width);
-        uint32_t parts = 1;
-        while (parts < kBlockGemmMaxParts && units * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
-               (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
-            parts *= 2;
-        }
-        return parts;
-    };
-    if (g.cta_pair == 1 || (g.cta_pair == 0 && p.rows >= 512)) {
-        return {kBlockPairN, 1, true};
+    if (p.a_cols || by_column || g.cta_pair == 1) {
+        return {0, 1};
     }
-    const uint32_t width = by_column || g.block_n == 128 ? 128u : 64u;
-    return {width, most_parts(width), false};
+    const uint32_t per_expert = (p.rows + p.experts - 1) / p.experts;
+    const uint32_t rows = g.block_rows ? (uint32_t)g.block_rows : (per_expert <= 16 ? 16u : (per_expert <= 32 ? 32u : 64u));
+    if (g.block_rows == 0 && per_expert > 128) {
+        return {0, 1};
+    }
+    const uint32_t k_blocks = (p.K + 127u) / 128u;
+    const uint64_t units = block_units(p, rows, kBlockFewColumns);
+    uint32_t parts = 1;
+    while (parts < kBlockFewMaxParts && units * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
+           (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
+        parts *= 2;
+    }
+    return {rows, parts};
 }
 
 template <typename OutT>
@@ -1864,13 +1858,12 @@ int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, Bloc
     const bool by_column = o.b->per_column != 0;
     const BlockPlan plan = plan_block_gemm(rc, p, by_column);
     p.parts = plan.parts;
-    if (plan.pair) {
-        return by_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
+    switch (plan.rows) {
+        case 0: return by_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
+        case 16: return launch_block_few<16, OutT>(rc, st, o, p);
+        case 32: return launch_block_few<32, OutT>(rc, st, o, p);
+        default: return launch_block_few<64, OutT>(rc, st, o, p);
     }
-    if (by_column) {
-        return launch_block_gemm_inst<128, OutT, true>(rc, st, o, p);
-    }
-    return plan.block_n == 64 ? launch_block_gemm_inst<64, OutT, false>(rc, st, o, p) : launch_block_gemm_inst<128, OutT, false>(rc, st, o, p);
 }
 
 // Common part of the two products.
@@ -3149,6 +3142,8 @@ int catccos_b200_set_option(const char* key, int64_t value)
         g.fuse_mode = (int)value;
     } else if (k == CATCCOS_B200_OPT_SPLIT_K && value >= 0 && value <= 8) {
         g.split_k = (int)value;
+    } else if (k == CATCCOS_B200_OPT_BLOCK_ROWS && (value == 0 || value == 16 || value == 32 || value == 64)) {
+        g.block_rows = (int)value;
     } else if (k == CATCCOS_B200_OPT_B_LSU && value >= 0 && value <= 2) {
         g.b_lsu = (int)value;
     } else if (k == CATCCOS_B200_OPT_SMALL_TILE && value >= 0 && value <= 2) {

@@ -31,3 +31,6 @@
 // order in which a flag-gated GEMM visits its row tiles: -1 = automatic (follows fuse_mode), 1 = this rank's own
 // shard first, then the peers slice by slice, 0 = slice by slice over all ranks, own slice leading
 #define CATCCOS_B200_OPT_TILE_ORDER "tile_order"
+// products of blocks of 128: 0 = automatic, 16, 32 or 64 = the form for few rows with tiles of so many, where it can run ("cta_pair"
+// 1 = CTA pairs; "split_k" bounds the parts of K there)
+#define CATCCOS_B200_OPT_BLOCK_ROWS "block_rows"

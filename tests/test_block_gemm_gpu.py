@@ -10,13 +10,12 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
-# the kernels' forms: single CTAs of 64 and 128 columns, K cut over CTAs, pairs of CTAs, and what the library chooses
-FORMS = [dict(block_n=64, cta_pair=2, split_k=1), dict(block_n=128, cta_pair=2, split_k=1), dict(block_n=64, cta_pair=2, split_k=8),
-         dict(block_n=128, cta_pair=2, split_k=4), dict(cta_pair=1), dict()]
-IDS = ["64", "128", "64x8", "128x4", "pair", "auto"]
+# the kernels' forms: tiles of 16, 32 and 64 rows, K cut over CTAs, pairs of CTAs, and what the library chooses
+FORMS = [dict(block_rows=16, split_k=1), dict(block_rows=32, split_k=1), dict(block_rows=64, split_k=1), dict(block_rows=16, split_k=8),
+         dict(block_rows=32, split_k=2), dict(block_rows=64, split_k=4), dict(cta_pair=1), dict()]
+IDS = ["16", "32", "64", "16x8", "32x2", "64x4", "pair", "auto"]
 HALF = {"bfloat16": 2.0**-8, "float16": 2.0**-11, "float32": 2.0**-24}
 LEAST = {"bfloat16": 0.0, "float16": 2.0**-25, "float32": 0.0}
-ALL_OPTIONS = ("block_n", "cta_pair", "split_k")
 
 
 class Options:
