@@ -31,16 +31,14 @@ struct BlockQuantParams {
     uint64_t units;            // row form: blocks of the matrix
 };
 
-// kValues (a multiple of 8) consecutive values as fp32; p is 16-byte aligned
-template <typename T, uint32_t kValues>
-__device__ __forceinline__ void load_values(const uint8_t* p, float (&v)[kValues])
+// kChunks consecutive 16-byte pieces; p is 16-byte aligned
+template <uint32_t kChunks>
+__device__ __forceinline__ void load_pieces(const uint8_t* p, uint4 (&w)[kChunks])
 {
-    constexpr uint32_t kChunks = kValues * sizeof(T) / 16, kPer = 16 / sizeof(T);
-    uint4 w[kChunks];
     if (kChunks >= 2 && ((uintptr_t)p & 31u) == 0u) {
 #pragma unroll
-        for (uint32_t i = 0; i < kChunks / 2; ++i) {
-            ld_global_stream_v8(p + 32u * i, w[2 * i], w[2 * i + 1]);
+        for (uint32_t i = 0; i + 1 < kChunks; i += 2) {
+            ld_global_stream_v8(p + 16u * i, w[i], w[i + 1]);
         }
     } else {
 #pragma unroll
@@ -48,6 +46,13 @@ __device__ __forceinline__ void load_values(const uint8_t* p, float (&v)[kValues
             w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
         }
     }
+}
+
+// Their values as fp32
+template <typename T, uint32_t kChunks>
+__device__ __forceinline__ void values_of(const uint4 (&w)[kChunks], float (&v)[kChunks * 16 / sizeof(T)])
+{
+    constexpr uint32_t kPer = 16 / sizeof(T);
 #pragma unroll
     for (uint32_t i = 0; i < kChunks; ++i) {
         const uint32_t b[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
@@ -103,7 +108,9 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_rows_kernel(co
     const bool live = unit < p.units, inside = live && col < p.k;
     float v[16] = {};
     if (inside) {
-        load_values<T, 16>(p.x + (size_t)row * p.x_row_bytes + (size_t)col * sizeof(T), v);
+        uint4 w[sizeof(T)];
+        load_pieces(p.x + (size_t)row * p.x_row_bytes + (size_t)col * sizeof(T), w);
+        values_of<T>(w, v);
     }
     uint32_t top = 0;
 #pragma unroll
@@ -140,35 +147,38 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_rows_kernel(co
     }
 }
 
-// Blocks of 128 x 1 and of 128 x 128: a CTA has 128 rows of 128 columns in registers, a thread 8 columns of every 16th row.
+// Blocks of 128 x 1 and of 128 x 128: a CTA has 128 rows of 128 columns in registers, as they are stored (as fp32 the 16-bit types
+// would leave room for half as many CTAs: 8190 x 2304 by column 20.0 us), a thread 8 columns of every 16th row.
 template <typename T, bool kE5m2, bool kSquare>
 __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_tiles_kernel(const BlockQuantParams p)
 {
-    __shared__ uint32_t tops[kBlockQuantThreads / 32][kBlockSize];
+    __shared__ __align__(16) uint32_t tops[kBlockQuantThreads / 32][kBlockSize];
     grid_dep_wait();
     grid_dep_launch();
     const uint32_t tx = threadIdx.x & 15u, ty = threadIdx.x >> 4, warp = threadIdx.x >> 5;
     const uint32_t row0 = (uint32_t)(blockIdx.x / p.blocks) * kBlockSize, block = blockIdx.x % p.blocks;
     const uint32_t col = block * kBlockSize + tx * 8u;
-    float v[8][8];
-    uint32_t top[8] = {};
+    uint4 w[8][sizeof(T) / 2];
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         const uint32_t row = row0 + ty + 16u * i;
         if (row < p.rows && col < p.k) {
-            load_values<T, 8>(p.x + (size_t)row * p.x_row_bytes + (size_t)col * sizeof(T), v[i]);
+            load_pieces(p.x + (size_t)row * p.x_row_bytes + (size_t)col * sizeof(T), w[i]);
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                v[i][j] = 0.0f;
+            for (uint32_t c = 0; c < sizeof(T) / 2; ++c) {
+                w[i][c] = make_uint4(0, 0, 0, 0);
             }
         }
     }
+    uint32_t top[8] = {};
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
+        float v[8];
+        values_of<T>(w[i], v);
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
-            top[j] = max(top[j], abs_bits(v[i][j]));
+            top[j] = max(top[j], abs_bits(v[j]));
         }
     }
     if (kSquare) {
@@ -183,24 +193,31 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_tiles_kernel(c
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t w = 0; w < kBlockQuantThreads / 32; ++w) {
-            all = max(all, tops[w][0]);
+        for (uint32_t i = 0; i < kBlockQuantThreads / 32; ++i) {
+            all = max(all, tops[i][0]);
         }
         top[0] = all;
     } else {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
             top[j] = max(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], 16));
-            if ((threadIdx.x & 16u) == 0u) {
-                tops[warp][tx * 8u + j] = top[j];
+        }
+        if ((threadIdx.x & 16u) == 0u) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                *reinterpret_cast<uint4*>(&tops[warp][tx * 8u + 4u * h]) = make_uint4(top[4 * h], top[4 * h + 1], top[4 * h + 2], top[4 * h + 3]);
             }
         }
         __syncthreads();
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
+        for (uint32_t i = 0; i < kBlockQuantThreads / 32; ++i) {
 #pragma unroll
-            for (uint32_t w = 0; w < kBlockQuantThreads / 32; ++w) {
-                top[j] = max(top[j], tops[w][tx * 8u + j]);
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint4 o = *reinterpret_cast<const uint4*>(&tops[i][tx * 8u + 4u * h]);
+                top[4 * h] = max(top[4 * h], o.x);
+                top[4 * h + 1] = max(top[4 * h + 1], o.y);
+                top[4 * h + 2] = max(top[4 * h + 2], o.z);
+                top[4 * h + 3] = max(top[4 * h + 3], o.w);
             }
         }
     }
@@ -223,11 +240,13 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_tiles_kernel(c
     for (uint32_t i = 0; i < 8; ++i) {
         const uint32_t row = row0 + ty + 16u * i;
         if (row < p.rows && col < p.k) {
+            float v[8];
+            values_of<T>(w[i], v);
             uint32_t o[2];
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
-                o[h] = encode_4<kE5m2>(v[i][4 * h] * mul[kSquare ? 0 : 4 * h], v[i][4 * h + 1] * mul[kSquare ? 0 : 4 * h + 1],
-                                       v[i][4 * h + 2] * mul[kSquare ? 0 : 4 * h + 2], v[i][4 * h + 3] * mul[kSquare ? 0 : 4 * h + 3]);
+                o[h] = encode_4<kE5m2>(v[4 * h] * mul[kSquare ? 0 : 4 * h], v[4 * h + 1] * mul[kSquare ? 0 : 4 * h + 1],
+                                       v[4 * h + 2] * mul[kSquare ? 0 : 4 * h + 2], v[4 * h + 3] * mul[kSquare ? 0 : 4 * h + 3]);
             }
             *reinterpret_cast<uint2*>(p.codes + (size_t)row * p.k + col) = make_uint2(o[0], o[1]);
         }

@@ -1728,6 +1728,28 @@ int moe_sum(const char* name, void* stream, const void* expert_out, uint32_t row
     return 0;
 }
 
+uint32_t combine_grad_routes(uint32_t tokens, uint32_t top_k)
+{
+    return top_k <= 1 || (uint64_t)tokens * top_k <= 512 ? 1 : (top_k <= 2 || (uint64_t)tokens * top_k <= 2048 ? 2 : 4);
+}
+
+template <typename T, bool kWide>
+int launch_combine_grad(cudaStream_t st, const CombineGradParams& p, uint32_t routes, unsigned grid)
+{
+    // threads that all have as many pieces of a row, at most one less
+    const uint32_t rounds = (p.vectors + kCombineGradThreads - 1) / kCombineGradThreads;
+    const uint32_t threads = ((p.vectors + rounds - 1) / rounds + 31) / 32 * 32;
+    auto kern = routes == 1 ? moe_combine_grad_kernel<T, 1, kWide> : (routes == 2 ? moe_combine_grad_kernel<T, 2, kWide> : moe_combine_grad_kernel<T, 4, kWide>);
+    CUDA_TRY(launch_after(kern, dim3(grid), threads, 0, st, p));
+    return 0;
+}
+
+template <typename T>
+int launch_combine_grad(cudaStream_t st, const CombineGradParams& p, uint32_t routes, bool wide, unsigned grid)
+{
+    return wide ? launch_combine_grad<T, true>(st, p, routes, grid) : launch_combine_grad<T, false>(st, p, routes, grid);
+}
+
 // ---------------------------------------------------------------------------------------------
 // blocks of 128 with fp32 scales
 // ---------------------------------------------------------------------------------------------
@@ -1827,30 +1849,52 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     return 0;
 }
 
-// Which form a launch takes: CTA pairs (rows 0), or tiles of so many rows with K in so many parts.
+// Which form a launch takes: CTA pairs (rows 0), or tiles of so many rows with K in so many parts.  The one that takes least by a fit
+// to 600 measured calls (dense with 1 to 1024 rows, experts with 1 to 512 rows each; 14 to 22 % off): a launch, then for each round of
+// units a block of K, which takes longer the more SMs are busy, and the output; the meeting of the parts.  So chosen, a call takes
+// 2.4 % more than in the best form; by the rows alone (16, 32, 64, pairs above 128 rows an expert) it would be 13 %.  An expert's rows are
+// reckoned with as in plan_grouped.
 struct BlockPlan {
     uint32_t rows, parts;
 };
 
 BlockPlan plan_block_gemm(const RankCtx& rc, const BlockGemmParams& p, bool by_column)
 {
+    struct Cost {
+        uint32_t rows;
+        double launch, block, busy_block, round, meeting;
+    };
+    constexpr Cost costs[] = {{0, 4.28, 0.299, 0.053, 0.50, 0}, {16, 3.71, 0.219, 0.205, 0.28, 1.29}, {32, 3.82, 0.241, 0.235, 0.56, 1.96}, {64, 5.06, 0.286, 0.360, 0.72, 2.37}};
     if (p.a_cols || by_column || g.cta_pair == 1) {
-        return {0, 1};
-    }
-    const uint32_t per_expert = (p.rows + p.experts - 1) / p.experts;
-    const uint32_t rows = g.block_rows ? (uint32_t)g.block_rows : (per_expert <= 16 ? 16u : (per_expert <= 32 ? 32u : 64u));
-    if (g.block_rows == 0 && per_expert > 128) {
-        return {0, 1};
+        return {0, 1};  // the form for few rows has neither
     }
     const uint32_t k_blocks = (p.K + 127u) / 128u;
-    const uint64_t units = block_units(p, rows, kBlockFewColumns);
-    uint32_t parts = 1;
-    while (parts < kBlockFewMaxParts && units * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
-           (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
-        parts *= 2;
+    const double active = std::min(p.rows, p.experts) < 2 ? 1.0 : 0.9 * std::min(p.rows, p.experts);
+    BlockPlan best = {0, 0};
+    double least = 0;
+    for (const Cost& c : costs) {
+        if ((g.block_rows != 0 && (uint32_t)g.block_rows != c.rows) || (g.block_rows == 0 && g.cta_pair == 2 && c.rows == 0)) {
+            continue;  // a test names the form
+        }
+        const uint32_t tile_rows = c.rows ? c.rows : kBlockPairM;
+        uint32_t parts = 1;
+        const uint64_t most = block_units(p, tile_rows, kBlockFewColumns);
+        while (c.rows != 0 && parts < kBlockFewMaxParts && most * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
+               (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
+            parts *= 2;
+        }
+        const double tiles = p.offsets ? std::max(active, p.rows / (double)tile_rows + 0.7 * active) : std::ceil(p.rows / (double)tile_rows);
+        const double units = tiles * ((p.N + kBlockFewColumns - 1) / kBlockFewColumns) * parts, slots = c.rows ? 2 * rc.num_sms : rc.num_sms / 2;
+        const double time = c.launch + (parts > 1 ? c.meeting : 0) +
+                            std::ceil(units / slots) * ((k_blocks + parts - 1) / parts * (c.block + c.busy_block * std::min(1.0, units / slots)) + c.round);
+        if (best.parts == 0 || time < least) {
+            best = {c.rows, parts};
+            least = time;
+        }
     }
-    return {rows, parts};
+    return best;
 }
+static_assert(kBlockPairN == kBlockFewColumns, "the plan counts columns of tiles alike");
 
 template <typename OutT>
 int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
@@ -3029,20 +3073,19 @@ int catccos_b200_moe_combine_grad(void* stream, const void* d_out, const void* e
     p.tokens = tokens;
     p.rows = rows;
     p.top_k = top_k;
-    p.vectors = n / 8;
-    p.chunks = (top_k + kCombineGradRoutes - 1) / kCombineGradRoutes;
+    const bool wide = n % 16 == 0 && !misaligned(d_out, 32) && !misaligned(expert_out, 32) && !misaligned(d_expert_out, 32);
+    p.vectors = wide ? n / 16 : n / 8;
+    // four routes a CTA read a token's gradient less often; with few tokens one or two spread the rows over the SMs
+    const uint32_t routes = combine_grad_routes(tokens, top_k);
+    p.chunks = (top_k + routes - 1) / routes;
     const uint64_t grid = (uint64_t)tokens * p.chunks;
     if (grid > 0x7FFFFFFFull) {
         return CATCCOS_B200_EINVAL;
     }
     int rcode = ensure_init();
     if (rcode != 0) return rcode;
-    // threads that all have as many pieces of a row, at most one less
-    const uint32_t rounds = (p.vectors + kCombineGradThreads - 1) / kCombineGradThreads;
-    const uint32_t threads = ((p.vectors + rounds - 1) / rounds + 31) / 32 * 32;
-    CUDA_TRY(launch_after(f16 ? moe_combine_grad_kernel<__half> : moe_combine_grad_kernel<__nv_bfloat16>, dim3((unsigned)grid), threads, 0,
-                          (cudaStream_t)stream, p));
-    return 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    return f16 ? launch_combine_grad<__half>(st, p, routes, wide, (unsigned)grid) : launch_combine_grad<__nv_bfloat16>(st, p, routes, wide, (unsigned)grid);
 }
 
 int catccos_b200_mx_fp4_matvec(void* stream, const void* x_bf16, const void* w, const void* w_scale, const int32_t* ids, void* out,

@@ -904,7 +904,7 @@ __global__ void __launch_bounds__(kCombineThreads) moe_dispatch_kernel(const Dis
     }
 }
 
-constexpr uint32_t kCombineGradThreads = 256, kCombineGradRoutes = 4;
+constexpr uint32_t kCombineGradThreads = 256;
 
 struct CombineGradParams {
     const uint8_t* d_out;      // [tokens, n], 16-bit floats
@@ -914,63 +914,72 @@ struct CombineGradParams {
     uint8_t* d_y;              // [rows, n]
     float* d_weights;          // [tokens, top_k]
     uint32_t tokens, rows, top_k;
-    uint32_t vectors;          // 16-byte pieces of a row
-    uint32_t chunks;           // CTAs of a token: its routes in groups of kCombineGradRoutes
+    uint32_t vectors;          // pieces of a row: of 16 bytes, or 32 in the wide form
+    uint32_t chunks;           // CTAs of a token: its routes in groups of kRoutes
 };
 
 // out[t] = sum over r of weights[t, r] * y[row_index[t, r]] backwards:
 //   d_y[row_index[t, r]] = weights[t, r] * d_out[t];   d_weights[t, r] = sum over columns of d_out[t] * y[row_index[t, r]]
-// A CTA has a token and four of its routes.  Bound by memory: d_out once, a row read and a row written for every live route.  The
+// A CTA has a token and kRoutes of its routes.  Bound by memory: d_out once, a row read and a row written for every live route.  The
 // sums are fp32, a thread's columns ascending, then lanes and warps in a fixed order.
-template <typename T>
+template <typename T, uint32_t kRoutes, bool kWide>
 __global__ void __launch_bounds__(kCombineGradThreads) moe_combine_grad_kernel(const CombineGradParams p)
 {
-    __shared__ float partial[kCombineGradThreads / 32][kCombineGradRoutes];
+    constexpr uint32_t kWords = kWide ? 8 : 4;
+    __shared__ float partial[kCombineGradThreads / 32][kRoutes];
     grid_dep_wait();
     grid_dep_launch();
-    const uint32_t token = blockIdx.x / p.chunks, r0 = (blockIdx.x - token * p.chunks) * kCombineGradRoutes;
+    const uint32_t token = blockIdx.x / p.chunks, r0 = (blockIdx.x - token * p.chunks) * kRoutes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    uint32_t index[kCombineGradRoutes];
-    float w[kCombineGradRoutes], sum[kCombineGradRoutes] = {};
+    uint32_t index[kRoutes];
+    float w[kRoutes], sum[kRoutes] = {};
 #pragma unroll
-    for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+    for (uint32_t j = 0; j < kRoutes; ++j) {
         const size_t at = (size_t)token * p.top_k + min(r0 + j, p.top_k - 1u);
         index[j] = r0 + j < p.top_k ? (uint32_t)__ldcg(p.row_index + at) : 0xFFFFFFFFu;  // a dropped route is negative: above any row
         w[j] = __ldcg(p.weights + at);
     }
     for (uint32_t v = threadIdx.x; v < p.vectors; v += blockDim.x) {
-        const uint4 d4 = __ldcg(reinterpret_cast<const uint4*>(p.d_out) + (size_t)token * p.vectors + v);
-        uint4 y4[kCombineGradRoutes];
+        auto load = [&](const uint8_t* base, size_t row, uint32_t (&x)[kWords]) {
+            const uint8_t* src = base + (row * p.vectors + v) * (kWords * 4u);
+            uint4 a, b;
+            if constexpr (kWide) {
+                ld_global_stream_v8(src, a, b);
+                x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+            } else {
+                a = __ldcs(reinterpret_cast<const uint4*>(src));
+            }
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+        };
+        uint32_t d[kWords], y[kRoutes][kWords];
+        load(p.d_out, token, d);
 #pragma unroll
-        for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
-            y4[j] = make_uint4(0, 0, 0, 0);
+        for (uint32_t j = 0; j < kRoutes; ++j) {
             if (index[j] < p.rows) {
-                y4[j] = __ldcs(reinterpret_cast<const uint4*>(p.y) + (size_t)index[j] * p.vectors + v);
+                load(p.y, index[j], y[j]);
             }
         }
-        const uint32_t dw[4] = {d4.x, d4.y, d4.z, d4.w};
-        float2 d[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            d[i] = unpack2<T>(dw[i]);
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+        for (uint32_t j = 0; j < kRoutes; ++j) {
             if (index[j] < p.rows) {
-                const uint32_t yw[4] = {y4[j].x, y4[j].y, y4[j].z, y4[j].w};
-                uint32_t o[4];
+                uint32_t o[kWords];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const float2 f = unpack2<T>(yw[i]);
-                    sum[j] = fmaf(d[i].x, f.x, fmaf(d[i].y, f.y, sum[j]));
-                    o[i] = pack2<T>(w[j] * d[i].x, w[j] * d[i].y);
+                for (uint32_t i = 0; i < kWords; ++i) {
+                    const float2 f = unpack2<T>(y[j][i]), g = unpack2<T>(d[i]);
+                    sum[j] = fmaf(g.x, f.x, fmaf(g.y, f.y, sum[j]));
+                    o[i] = pack2<T>(w[j] * g.x, w[j] * g.y);
                 }
-                __stcs(reinterpret_cast<uint4*>(p.d_y) + (size_t)index[j] * p.vectors + v, make_uint4(o[0], o[1], o[2], o[3]));
+                uint8_t* dst = p.d_y + ((size_t)index[j] * p.vectors + v) * (kWords * 4u);
+                if constexpr (kWide) {
+                    st_global_v8(dst, o);
+                } else {
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+                }
             }
         }
     }
 #pragma unroll
-    for (uint32_t j = 0; j < kCombineGradRoutes; ++j) {
+    for (uint32_t j = 0; j < kRoutes; ++j) {
 #pragma unroll
         for (uint32_t d = 16; d > 0; d >>= 1) {
             sum[j] += __shfl_xor_sync(0xFFFFFFFFu, sum[j], d);
@@ -980,7 +989,7 @@ __global__ void __launch_bounds__(kCombineGradThreads) moe_combine_grad_kernel(c
         }
     }
     __syncthreads();
-    if (threadIdx.x < kCombineGradRoutes && r0 + threadIdx.x < p.top_k) {
+    if (threadIdx.x < kRoutes && r0 + threadIdx.x < p.top_k) {
         float s = 0.0f;
         for (uint32_t i = 0; i < blockDim.x / 32; ++i) {
             s += partial[i][threadIdx.x];
