@@ -148,15 +148,16 @@ __device__ __forceinline__ void fma_2(float& a0, float& a1, float x0, float x1, 
         : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
 
-// sixteen sums += f * the columns of this lane's row; by column: f * scale[column] * them (scale 16-byte aligned)
+// sixteen sums += f * the columns of this lane's row; by column: f * scale[column] * them (scale: address in shared memory, 16-byte
+// aligned)
 template <bool kByColumn>
-__device__ __forceinline__ void add_scaled(float* acc, const float (&v)[16], float f, const float* scale)
+__device__ __forceinline__ void add_scaled(float* acc, const float (&v)[16], float f, uint32_t scale)
 {
 #pragma unroll
     for (uint32_t c = 0; c < 16; c += 4) {
         float4 g = make_float4(f, f, f, f);
         if (kByColumn) {
-            const float4 s = *reinterpret_cast<const float4*>(scale + c);
+            const float4 s = ld_shared_v4(scale + c * 4u);
             g = make_float4(f * s.x, f * s.y, f * s.z, f * s.w);
         }
         fma_2(acc[c], acc[c + 1], v[c], v[c + 1], g.x, g.y);

@@ -7,19 +7,19 @@
 // A block's way from the tensor core through the promotion and back is far longer than its products (256 cycles at best): some 1000
 // cycles until a finished product is seen, 300 to load the tile, 300 until the issuer knows that it is free again.  So four tiles
 // take turns (all that tensor memory holds), a tile goes back as soon as it is in registers, and no warp that promotes looks at a
-// barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: two other warps do, and named
-// barriers join them.  256 x 256 tiles, which read less of A and B, have room for two tiles only: 8192 x 2304 x 7168 took 153 us.
+// barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: another warp does, and named barriers
+// pass it on.  256 x 256 tiles, which read less of A and B, have room for two tiles only: 8192 x 2304 x 7168 took 153 us.
 //
 //   full[s], tmem_empty[b]    live in the leader; both CTAs' TMA bytes, and the other CTA's word that it has read a tile, go there
 //   empty[s], tmem_full[b]    live in each CTA; the leader's tcgen05.commit arrives on both copies
+//   tile_read[b]              lives in each CTA: its promotion warps have read a tile
 //   scale_full[i], scale_empty[i]   live in each CTA: the factors of its rows (and, by column, of the columns) for a group of four
 //                             blocks of K (every unit begins with a group of its own)
-//   named barriers 1 + b, 5 + b   tile b may be read; tile b has been read
+//   named barriers 1 + b      tile b may be read (nothing else waits on one: their waits have no limit)
 //
 // A role takes 300 to 600 cycles for a block whatever its size (a look at a barrier, then instructions of one lane), hence so many of
 // them.  448 threads: warps 0-7 promotion and output (warp w: lane quarter w % 4, columns 64 (w / 4)), 8 and 9 TMA for A and B, 10
-// and 11 MMA, each every second block (in the other CTA they pass on that tiles have been read), 12 tells the promotion of tiles
-// and factors, 13 makes the factors, a row's scale times the columns'.
+// and 11 MMA, each every second block (in the other CTA they pass on that tiles have been read), 12 tells the promotion of tiles and factors, 13 makes the factors, a row's scale times the columns'.
 #pragma once
 
 #include "block_gemm.cuh"
@@ -45,7 +45,7 @@ struct BlockPairSmem {
     static constexpr uint32_t kOffFactor = kOffOut + kBlockPairPromoters * kOutBytes;  // [128 rows][4 blocks] a slot
     static constexpr uint32_t kOffScale = kOffFactor + kScaleSlots * 128 * 16;         // by column: [4 blocks][128 columns] a slot
     static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * kBlockPairN * 16;
-    static constexpr uint32_t kNumBars = 2 * kStages + 2 * kTiles + 2 * kScaleSlots;
+    static constexpr uint32_t kNumBars = 2 * kStages + 3 * kTiles + 2 * kScaleSlots;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // the step (counted from 1) whose wait has given up
     static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
@@ -151,7 +151,8 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     uint64_t* empty = full + kStages;
     uint64_t* tmem_full = empty + kStages;
     uint64_t* tmem_empty = tmem_full + S::kTiles;
-    uint64_t* scale_full = tmem_empty + S::kTiles;
+    uint64_t* tile_read = tmem_empty + S::kTiles;
+    uint64_t* scale_full = tile_read + S::kTiles;
     uint64_t* scale_empty = scale_full + S::kScaleSlots;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + S::kOffDead);
@@ -173,11 +174,12 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         }
         for (uint32_t b = 0; b < S::kTiles; ++b) {
             mbar_init(&tmem_full[b], 1);
-            mbar_init(&tmem_empty[b], 1);  // of the other CTA
+            mbar_init(&tmem_empty[b], 1);  // warps 10 and 11 of the other CTA
+            mbar_init(&tile_read[b], kBlockPairPromoters);
         }
         for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
             mbar_init(&scale_full[i], kByColumn ? 2 : 1);  // the rows' factors (and the columns' bytes)
-            mbar_init(&scale_empty[i], 1);
+            mbar_init(&scale_empty[i], kBlockPairPromoters);
         }
         *dead = 0u;
         mbar_fence_init();
@@ -287,31 +289,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             }
         }
     } else if (warp == 10 || warp == 11) {
-        // ------------------------------- MMA issuers (leader), tiles given back -----------
-        const uint32_t mine = warp - 10u;  // steps of this parity
-        // Hears that all promotion warps of this CTA have read the tile of step `it`, of whose unit it is the i-th, and tells the
-        // makers of factors when that was the first step of a group (the group before is done with); false once the promotion has ended.
-        uint32_t read = mine, read_i = 0, group = 0;
-        auto skip = [&] {  // a step of the other warp's, or of this one
-            group += (read_i & 3u) == 0u ? 1u : 0u;
-            read_i = read_i + 1u == k_blocks ? 0u : read_i + 1u;
-        };
-        if (mine) {
-            skip();
-        }
-        auto hear = [&] {
-            named_sync(5u + (read & 3u));
-            if (*dead == read + 1u) {
-                alive = false;
-                return;
-            }
-            if ((read_i & 3u) == 0u && group != 0u && lane == 0) {
-                mbar_arrive(&scale_empty[(group - 1u) % S::kScaleSlots]);
-            }
-            skip();
-            skip();
-            read += 2u;
-        };
+        // ------------------------------- MMA issuers (leader CTA only) --------------------
         if (cta == 0) {
             const uint32_t idesc0 = make_idesc_f8(kBlockPairM, 0, p.a_fmt, p.b_fmt, p.a_cols != 0u, p.b_rows == 0u);
             const uint64_t desc_k = make_smem_desc(0, 16, 1024, 2);
@@ -320,9 +298,9 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const uint32_t a_lo0 = (uint32_t)desc_a | (smem_u32(smem + S::kOffA) >> 4);
             const uint32_t b_lo0 = (uint32_t)desc_b | (smem_u32(smem + S::kOffB) >> 4);
             const uint32_t step_a = (p.a_cols ? 4096u : 32u) >> 4, step_b = (p.b_rows ? 32u : 2048u) >> 4;
-            uint32_t unit = pair, i = mine;  // of step `it`: its unit, the how manieth there
+            uint32_t unit = pair, i = warp - 10u;  // of step `it`: its unit, the how manieth there
             uint32_t idesc = 0, of_unit = 0xFFFFFFFFu;
-            for (uint32_t it = mine; it < steps; it += 2u, i += 2u) {
+            for (uint32_t it = warp - 10u; it < steps; it += 2u, i += 2u) {
                 while (i >= k_blocks) {
                     i -= k_blocks;
                     unit += num_pairs;
@@ -334,10 +312,9 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     of_unit = unit;
                 }
                 const uint32_t b = it & 3u, s = it % kStages;
-                if (it >= S::kTiles) {
-                    hear();
-                }
-                alive = alive && mbar_wait_both(&full[s], (it / kStages) & 1u, &tmem_empty[b], ((it >> 2) & 1u) ^ 1u, p.status, 501, b, bar_ns);
+                const uint32_t free_ph = ((it >> 2) & 1u) ^ 1u;
+                alive = mbar_wait_both(&tile_read[b], free_ph, &tmem_empty[b], free_ph, p.status, 501, b, bar_ns) &&
+                        mbar_wait_soon(&full[s], (it / kStages) & 1u, p.status, 503, s, bar_ns);
                 if (!alive) {
                     break;  // nothing is issued, and no tile reported, after a wait has given up
                 }
@@ -345,15 +322,15 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 umma_f8_pair_block(tmem_base + b * kBlockPairN, a_lo0 + s * (S::kABytes >> 4), hi_a, step_a, b_lo0 + s * (S::kBBytes >> 4), hi_b, step_b,
                                    idesc, &tmem_full[b], &empty[s]);
             }
-            while (alive && read < steps) {
-                hear();
-            }
         } else {
             const uint32_t free_bar = map_to_cta(smem_u32(&tmem_empty[0]), 0);
-            while (alive && read < steps) {
-                const uint32_t b = read & 3u;
-                hear();
-                if (alive && lane == 0) {
+            for (uint32_t it = warp - 10u; it < steps; it += 2u) {
+                const uint32_t b = it & 3u;
+                alive = mbar_wait_soon(&tile_read[b], (it >> 2) & 1u, p.status, 502, b, bar_ns);
+                if (!alive) {
+                    break;
+                }
+                if (lane == 0) {
                     mbar_arrive_cluster(free_bar + b * 8u);
                 }
                 __syncwarp();
@@ -362,7 +339,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     } else if (warp == 12) {
         // ------------------------------- tells of tiles and factors -----------------------
         // It is never two turns ahead on a named barrier: tile b is filled again after all have read it.  When a wait gives up, the
-        // promotion and warps 10 and 11 are told with that step and end with it.
+        // promotion is told with that step and ends with it.
         uint32_t i = 0, group = 0;
         for (uint32_t it = 0; alive && it < steps; ++it) {
             const uint32_t b = it & 3u, slot = group % S::kScaleSlots;
@@ -385,10 +362,10 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         // ------------------------------- promotion and output (both CTAs, own 128 rows) ---
         const uint32_t q = warp & 3u, col = (warp >> 2) * kCols;
         const uint32_t tmem = tmem_base + ((q * 32u) << 16) + col;
-        const float4* factors = reinterpret_cast<const float4*>(smem + S::kOffFactor) + q * 32u + lane;
+        const uint32_t factors = smem_u32(smem + S::kOffFactor) + (q * 32u + lane) * 16u;
+        const uint32_t scales = smem_u32(smem + S::kOffScale) + col * 4u;
         uint8_t* out = smem + S::kOffOut + warp * S::kOutBytes;
         uint32_t it = 0, group = 0;
-        float4 f4 = {};  // the factors of a group
         for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
             const Unit u = unit_at(unit);
             const uint32_t row0 = u.m0 + cta * 128u + q * 32u, col0 = u.n0 + col;
@@ -397,7 +374,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             // Sixteen columns are added while the next are on their way, a step's last while the next step's first are; a tile goes
             // back when its last are in registers.
             float v[2][16], f = 0.0f;
-            const float* scale = nullptr;
+            uint32_t scale = 0;
             for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
                 const uint32_t b = it & 3u, j = i & 3u;
                 named_sync(1u + b);
@@ -406,24 +383,29 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 if (live) {
                     const uint32_t tile = tmem + b * kBlockPairN;
                     tmem_ld_16(tile, v[0]);
-                    if (j == 0u) {
-                        f4 = factors[group % S::kScaleSlots * 128u];
-                    }
+                    float f_next;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f_next) : "r"(factors + (group % S::kScaleSlots * 128u) * 16u + j * 4u));
                     if (i != 0u) {
-                        add_scaled<kByColumn>(&acc[48], v[1], f, scale + 48);
+                        add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
                     }
-                    f = j == 0u ? f4.x : (j == 1u ? f4.y : (j == 2u ? f4.z : f4.w));
-                    scale = reinterpret_cast<const float*>(smem + S::kOffScale) + (group % S::kScaleSlots * 4u + j) * kBlockPairN + col;
+                    f = f_next;
+                    scale = scales + (group % S::kScaleSlots * 4u + j) * (kBlockPairN * 4u);
                     tmem_ld_fence(v[0]);
 #pragma unroll
                     for (uint32_t c = 0; c < 3; ++c) {
                         tmem_ld_16(tile + 16u * c + 16u, v[(c + 1) & 1]);
-                        add_scaled<kByColumn>(&acc[16 * c], v[c & 1], f, scale + 16 * c);
+                        add_scaled<kByColumn>(&acc[16 * c], v[c & 1], f, scale + 64u * c);
                         tmem_ld_fence(v[(c + 1) & 1]);
                     }
                 }
                 tcgen05_fence_before();
-                named_arrive(5u + b);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tile_read[b]);
+                    if (j == 0u && group != 0u) {
+                        mbar_arrive(&scale_empty[(group - 1u) % S::kScaleSlots]);  // what it had has been added
+                    }
+                }
                 if (dead_step == it + 1u) {
                     alive = false;  // a tile that never filled is not written out
                     break;
@@ -431,7 +413,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 group += j == 3u || i + 1u == k_blocks ? 1u : 0u;
             }
             if (live) {
-                add_scaled<kByColumn>(&acc[48], v[1], f, scale + 48);
+                add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
             }
             if (live && alive) {
                 if (row0 + 32u <= u.end || p.offsets == nullptr) {
