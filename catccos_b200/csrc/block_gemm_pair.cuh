@@ -4,11 +4,17 @@
 // CTA r of a pair loads rows [128 r, +128) of A and columns [64 r, +64) of B with plain TMA; the leader issues the products of both,
 // and each CTA has the results for its own 128 rows and all 128 columns in its own tensor memory.
 //
-// A block's way from the tensor core through the promotion and back is far longer than its products (256 cycles at best): some 1000
-// cycles until a finished product is seen, 300 to load the tile, 300 until the issuer knows that it is free again.  So four tiles
-// take turns (all that tensor memory holds), a tile goes back as soon as it is in registers, and no warp that promotes looks at a
-// barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: another warp does, and named barriers
-// pass it on.  256 x 256 tiles, which read less of A and B, have room for two tiles only: 8192 x 2304 x 7168 took 153 us.
+// A block's way from the tensor core through the promotion and back is far longer than its products (256 cycles at best): some 500
+// cycles until a finished product is seen, 400 to load and add the tile, 300 until the issuer knows that it is free again.  So four
+// tiles take turns (all that tensor memory holds), a tile goes back as soon as its last columns are in registers, and no warp that
+// promotes looks at a barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: another warp does,
+// and named barriers pass it on.  (With each promotion warp looking for itself 8192 x 2304 x 7168 takes 171 us.)
+//
+// What bounds it, at 8192 x 2304 x 7168: 154 us (1.76 PFLOP/s), 0.34 us a block of K.  With the promotion left out it is 127, with its
+// loads alone 135: operands come at 24 KB a block and SM, 85 GB/s, about what a K tile of 192 rows takes in mx_gemm_pair.cuh.  256 x
+// 256 tiles read a third less of A and B, but have room for two tiles only, and came to 153; at 3001 x 7168 x 2304 to 84 against 78.
+// Sixteen promotion warps of 32 columns: 160.  By column (the scales of 128 columns in shared memory, one more product a value): 7168
+// x 2304 x 4096 136 us, bound by the promotion.
 //
 //   full[s], tmem_empty[b]    live in the leader; both CTAs' TMA bytes, and the other CTA's word that it has read a tile, go there
 //   empty[s], tmem_full[b]    live in each CTA; the leader's tcgen05.commit arrives on both copies

@@ -5,7 +5,9 @@
 // keeps both quotients finite and normal; a block of zeros has codes of zero.  An infinity or a NaN makes its block's scale and
 // codes NaN.
 //
-// Bound by memory: 2 bytes read and 1 + 4 / 128 written an element (with row_index: the written part for every route).
+// Bound by memory: 2 bytes read and 1 + 4 / 128 written an element (with row_index: the written part for every route).  Measured:
+// 4096 x 7168 to 8 routes each 51.7 us (5.8 TB/s, 90 % of a plain copy), 8190 x 2304 by column 14.0 (4.1 TB/s: 1152 CTAs that each load,
+// meet once and store).
 #pragma once
 
 #include <cuda_bf16.h>
