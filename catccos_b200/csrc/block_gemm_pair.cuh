@@ -14,7 +14,7 @@
 // loads alone 135: operands come at 24 KB a block and SM, 85 GB/s, about what a K tile of 192 rows takes in mx_gemm_pair.cuh.  256 x
 // 256 tiles read a third less of A and B, but have room for two tiles only, and came to 153; at 3001 x 7168 x 2304 to 84 against 78.
 // Sixteen promotion warps of 32 columns: 160.  By column (the scales of 128 columns in shared memory, one more product a value): 7168
-// x 2304 x 4096 136 us, bound by the promotion.
+// x 2304 x 4096 128 to 134 us, bound by the promotion.
 //
 //   full[s], tmem_empty[b]    live in the leader; both CTAs' TMA bytes, and the other CTA's word that it has read a tile, go there
 //   empty[s], tmem_full[b]    live in each CTA; the leader's tcgen05.commit arrives on both copies
@@ -149,6 +149,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 {
     using S = BlockPairSmem<OutT>;
     constexpr uint32_t kStages = S::kStages, kCols = 64;  // columns of a promotion warp
+    constexpr bool kLater = !kByColumn;
 
     grid_dep_launch();
     extern __shared__ uint8_t smem_raw[];
@@ -377,8 +378,8 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const uint32_t row0 = u.m0 + cta * 128u + q * 32u, col0 = u.n0 + col;
             const bool live = row0 < u.end && col0 < p.N;  // else there is nothing to fetch
             float acc[kCols] = {};
-            // Sixteen columns are added while the next are on their way, a step's last while the next step's first are; a tile goes
-            // back when its last are in registers.
+            // Sixteen columns are added while the next are on their way, a step's last while the next step's first are (by column, which
+            // has no registers left for that, at once: 140 -> 128 us on one GPU); a tile goes back when its last are in registers.
             float v[2][16], f = 0.0f;
             uint32_t scale = 0;
             for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
@@ -391,7 +392,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     tmem_ld_16(tile, v[0]);
                     float f_next;
                     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f_next) : "r"(factors + (group % S::kScaleSlots * 128u) * 16u + j * 4u));
-                    if (i != 0u) {
+                    if (kLater && i != 0u) {
                         add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
                     }
                     f = f_next;
@@ -412,13 +413,16 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                         mbar_arrive(&scale_empty[(group - 1u) % S::kScaleSlots]);  // what it had has been added
                     }
                 }
+                if (!kLater && live) {
+                    add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
+                }
                 if (dead_step == it + 1u) {
                     alive = false;  // a tile that never filled is not written out
                     break;
                 }
                 group += j == 3u || i + 1u == k_blocks ? 1u : 0u;
             }
-            if (live) {
+            if (kLater && live) {
                 add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
             }
             if (live && alive) {
