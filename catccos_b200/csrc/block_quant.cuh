@@ -6,7 +6,7 @@
 // codes NaN.
 //
 // Bound by memory: 2 bytes read and 1 + 4 / 128 written an element (with row_index: the written part for every route).  Measured:
-// 4096 x 7168 to 8 routes each 51.7 us (5.8 TB/s, 90 % of a plain copy), 8190 x 2304 by column 14.0 (4.1 TB/s: 1152 CTAs that each load,
+// 4096 x 7168 to 8 routes each 51.7 us (5.8 TB/s, 90 % of a plain copy), 8190 x 2304 by column 13.7 (4.2 TB/s: 1152 CTAs that each load,
 // meet once and store).
 #pragma once
 
@@ -150,9 +150,10 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_rows_kernel(co
 }
 
 // Blocks of 128 x 1 and of 128 x 128: a CTA has 128 rows of 128 columns in registers, as they are stored (as fp32 the 16-bit types
-// would leave room for half as many CTAs: 8190 x 2304 by column 20.0 us), a thread 8 columns of every 16th row.
+// would leave room for half as many CTAs: 8190 x 2304 by column 20.0 us), a thread 8 columns of every 16th row. Four CTAs an SM of the
+// 16-bit types against three: bf16 8190 x 2304 by column 14.0 -> 13.2 us, 8192 x 7168 37.5 -> 36.1, but 512 x 2304 3.7 -> 3.9.
 template <typename T, bool kE5m2, bool kSquare>
-__global__ void __launch_bounds__(kBlockQuantThreads) block_quant_tiles_kernel(const BlockQuantParams p)
+__global__ void __launch_bounds__(kBlockQuantThreads, sizeof(T) == 2 ? 4 : 2) block_quant_tiles_kernel(const BlockQuantParams p)
 {
     __shared__ __align__(16) uint32_t tops[kBlockQuantThreads / 32][kBlockSize];
     grid_dep_wait();
@@ -181,6 +182,13 @@ __global__ void __launch_bounds__(kBlockQuantThreads) block_quant_tiles_kernel(c
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
             top[j] = max(top[j], abs_bits(v[j]));
+        }
+    }
+    // the values are made from the stored ones again below: kept as fp32 they would not fit (fp16 by column 13.4 -> 18.8 us)
+    if (sizeof(T) == 2) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            asm volatile("" : "+r"(w[i][0].x), "+r"(w[i][0].y), "+r"(w[i][0].z), "+r"(w[i][0].w));
         }
     }
     if (kSquare) {
