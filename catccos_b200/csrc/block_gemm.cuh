@@ -148,6 +148,20 @@ __device__ __forceinline__ void fma_2(float& a0, float& a1, float x0, float x1, 
         : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
 
+// (x0, x1) *= (y0, y1)
+__device__ __forceinline__ void mul_2(float& x0, float& x1, float y0, float y1)
+{
+    asm("{\n\t"
+        ".reg .b64 x, y;\n\t"
+        "mov.b64 x, {%0, %1};\n\t"
+        "mov.b64 y, {%2, %3};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t"
+        "}"
+        : "+f"(x0), "+f"(x1)
+        : "f"(y0), "f"(y1));
+}
+
 // sixteen sums += f * the columns of this lane's row; by column: f * scale[column] * them (scale: address in shared memory, 16-byte
 // aligned)
 template <bool kByColumn>
@@ -163,6 +177,13 @@ __device__ __forceinline__ void add_scaled(float* acc, const float (&v)[16], flo
         fma_2(acc[c], acc[c + 1], v[c], v[c + 1], g.x, g.y);
         fma_2(acc[c + 2], acc[c + 3], v[c + 2], v[c + 3], g.z, g.w);
     }
+}
+
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
 }
 
 // 32 columns of row `lane` to a box of 32 rows in shared memory that TMA stores: 16-byte pieces in its swizzle of 64 (16-bit types) or
@@ -185,7 +206,7 @@ __device__ __forceinline__ void stage_out(uint8_t* box, uint32_t lane, const flo
     }
 }
 
-// A line's scales of blocks kb .. kb + 3 of K (those behind the last: 0); they are `step` floats apart.
+// A line's scales of blocks kb .. kb + 3 of K (those behind the last: 1, an ordinary one); they are `step` floats apart.
 __device__ __forceinline__ void load_scales(const float* line, size_t step, uint32_t kb, uint32_t blocks, float (&v)[4])
 {
     const float* at = line + kb * step;
@@ -195,8 +216,87 @@ __device__ __forceinline__ void load_scales(const float* line, size_t step, uint
     } else {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            v[j] = kb + j < blocks ? __ldcg(at + j * step) : 0.0f;
+            v[j] = kb + j < blocks ? __ldcg(at + j * step) : 1.0f;
         }
+    }
+}
+
+// ---- two scales whose product is not in fp32's range ----
+// A block's sum v (with finite codes 0, or 2^-32 to 2^39 in size) is added as v * f, f = 2^40 * sa * sb: one product of the scales for many
+// sums.  What is held is 2^40 times the result, so that f is a normal number from products of 2^-166 on: a block of zeros has a scale of
+// 2^-109 or 2^-116 from the quantiser, a row of zeros beside small weights is ordinary.  f is below 2^64, so that no sum of blocks overflows.
+//
+// Other scales, finite and not zero, would give NaN for v = 0 or lose bits that v * sa * sb keeps.  The warp that makes the factors looks
+// for them and marks their group of four blocks of K; with it the promotion goes on to a second loop up to the end of the unit, which holds
+// the result itself and adds (v * g) * f with g = 2^64 or 2^-64 and f that much smaller or larger: v * g is exact, and what is then outside of
+// f's range is outside of the result's.  With the choice inside one loop, or with more work in the warp of the factors, calls without such
+// scales took 5 to 25 % longer.  A row's result is the same in both loops.
+constexpr float kHeld = 0x1p40f;
+
+// a factor in range: 2^-126 <= |f| < 2^64
+__device__ __forceinline__ bool is_ordinary(float f) { return __float_as_uint(f) * 2u - 0x01000000u < 0xBE000000u; }
+
+__device__ __forceinline__ bool is_finite_and_not_zero(float f) { return __float_as_uint(f) * 2u - 1u < 0xFEFFFFFFu; }
+
+__device__ __forceinline__ bool is_finite(float f) { return __float_as_uint(f) * 2u < 0xFF000000u; }
+
+// Whether f, as 2^40 times the product of the two scales, may not stand for them (NaN may be 0 times 2^40 * sb)
+__device__ __forceinline__ bool needs_both_scales(float sa, float sb, float f)
+{
+    return !is_ordinary(f) && is_finite(sa) && is_finite(sb) && (f != 0.0f || (sa != 0.0f && sb != 0.0f));
+}
+
+// The factor of a marked group: v * sa * sb is (v * g) * it.
+__device__ __forceinline__ float wide_factor(float sa, float sb, float& g)
+{
+    float f = sa * sb;
+    const float size = fabsf(f);
+    g = 1.0f;
+    if (!(size >= 0x1p-126f && size <= 0x1.fffffep127f) && is_finite_and_not_zero(sa) && is_finite_and_not_zero(sb)) {
+        // of a product of 2^128 or more neither scale is below 1, of one below 2^-126 neither is above 2^23
+        const bool large = size > 1.0f;
+        const float shift = large ? 0x1p-32f : 0x1p32f;
+        f = (sa * shift) * (sb * shift);
+        f = fminf(fmaxf(f, -0x1.fffffep127f), 0x1.fffffep127f);  // above 2^192 in all: any v but 0 is infinite, and 0 is 0
+        g = large ? 0x1p64f : 0x1p-64f;
+    }
+    return f;
+}
+
+// sums *= s
+template <uint32_t kCount>
+__device__ __forceinline__ void scale_sums(float (&sums)[kCount], float s)
+{
+#pragma unroll
+    for (uint32_t i = 0; i < kCount; i += 2) {
+        mul_2(sums[i], sums[i + 1], s, s);
+    }
+}
+
+// s = near * rest, exactly: rest a power of two, near from 2^-86 to 2^65 (an infinity or a NaN stays in near)
+__device__ __forceinline__ void split_scale(float s, float& near, float& rest)
+{
+    const int e = (int)((__float_as_uint(s) >> 23) & 0xFFu) - 127;
+    const int shift = e - min(max(e, -64), 64);
+    near = s * __uint_as_float((uint32_t)(127 - shift) << 23);
+    rest = __uint_as_float((uint32_t)(127 + shift) << 23);
+}
+
+// By column, in the second loop: sixteen sums += f * scale[column] * the columns of this lane's row, as ((v * near) * scale) * rest with f =
+// near * rest: the products on the way are outside of fp32's range only where the result is.
+__device__ __forceinline__ void add_scaled_apart(float* acc, float (&v)[16], float f, uint32_t scale)
+{
+    float near, rest;
+    split_scale(f, near, rest);
+#pragma unroll
+    for (uint32_t c = 0; c < 16; c += 4) {
+        const float4 s = ld_shared_v4(scale + c * 4u);
+        mul_2(v[c], v[c + 1], near, near);
+        mul_2(v[c + 2], v[c + 3], near, near);
+        mul_2(v[c], v[c + 1], s.x, s.y);
+        mul_2(v[c + 2], v[c + 3], s.z, s.w);
+        fma_2(acc[c], acc[c + 1], v[c], v[c + 1], rest, rest);
+        fma_2(acc[c + 2], acc[c + 3], v[c + 2], v[c + 3], rest, rest);
     }
 }
 
@@ -298,7 +398,9 @@ struct BlockFewSmem {
     static constexpr uint32_t kNumBars = 2 * kStages + 2 * kTiles + 2 * kGroups;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
-    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
+    static constexpr uint32_t kOffApart = kOffTmemPtr + 16;            // [groups] words: its products of scales leave fp32's range
+    static constexpr uint32_t kOffPower = kOffApart + kGroups * 4;     // [groups][4 blocks][kRows] bytes: then g's exponents
+    static constexpr uint32_t kOffTiles = kOffPower + kGroups * 4 * kRows;
     static constexpr uint32_t kPitch = kRows + 4;  // floats of a weight column's sums in the exchange
     static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
     static_assert(kBlockFewColumns * kPitch * 4 <= kOffX, "the sums of all parts fit the idle ring");
@@ -322,6 +424,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     uint64_t* scale_empty = scale_full + S::kGroups;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
+    volatile uint32_t* apart_of = reinterpret_cast<volatile uint32_t*>(smem + S::kOffApart);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
@@ -427,6 +530,40 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
                 for (uint32_t i = 0; i < kPerLane; ++i) {
                     load_scales(p.a_scales + min(row + 32u * i, end - 1u) * p.a_scale_row, p.a_scale_block, kb, kb1, x[i]);
                 }
+                float f[kPerLane][4];
+                bool odd = false;
+#pragma unroll
+                for (uint32_t i = 0; i < kPerLane; ++i) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        f[i][j] = x[i][j] * (w[j] * kHeld);
+                        odd = odd || !is_ordinary(f[i][j]);
+                    }
+                }
+                bool apart = __any_sync(0xFFFFFFFFu, odd);
+                uint32_t power[kPerLane] = {};  // of four blocks
+                if (__builtin_expect(apart, 0)) {
+                    odd = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < kPerLane; ++i) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            odd = odd || needs_both_scales(x[i][j], w[j], f[i][j]);
+                        }
+                    }
+                    apart = __any_sync(0xFFFFFFFFu, odd);
+                }
+                if (__builtin_expect(apart, 0)) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kPerLane; ++i) {
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            float g;
+                            f[i][j] = wide_factor(x[i][j], w[j], g);
+                            power[i] |= (__float_as_uint(g) >> 23) << (8u * j);
+                        }
+                    }
+                }
                 const uint32_t slot = group % S::kGroups;
                 alive = mbar_wait_soon(&scale_empty[slot], ((group / S::kGroups) & 1u) ^ 1u, p.status, 405, slot, bar_ns);
                 if (!alive) {
@@ -438,9 +575,15 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
                     for (uint32_t i = 0; i < kPerLane; ++i) {
 #pragma unroll
                         for (uint32_t j = 0; j < 4; ++j) {
-                            factor[j * kRows + 32u * i] = x[i][j] * w[j];
+                            factor[j * kRows + 32u * i] = f[i][j];
+                            if (apart) {
+                                smem[S::kOffPower + (slot * 4u + j) * kRows + lane + 32u * i] = (uint8_t)(power[i] >> (8u * j));
+                            }
                         }
                     }
+                }
+                if (lane == 0) {
+                    apart_of[slot] = apart ? 1u : 0u;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -452,25 +595,58 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         // ------------------------------- promotion and output -----------------------------
         const uint32_t tmem = tmem_base + ((warp * 32u) << 16), column = warp * 32u + lane;
         uint32_t it = 0, group = 0;
+        bool apart = false;  // the group that comes next is marked
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
             const uint32_t first = row_begin[walk.e] + tc.m_tile * kRows, rows = min(row_end[walk.e] - first, kRows);
             const uint32_t n0 = tc.n_tile * kBlockFewColumns;
             float acc[kRows] = {};
-            for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t b = it % kTiles, slot = group % S::kGroups, j = (kb - kb0) & 3u;
-                alive = j == 0u ? mbar_wait_both(&tmem_full[b], (it / kTiles) & 1u, &scale_full[slot], (group / S::kGroups) & 1u, p.status, 406, b, bar_ns)
-                                : mbar_wait_soon(&tmem_full[b], (it / kTiles) & 1u, p.status, 406, b, bar_ns);
+            // A block of K: waits for its tile and, at the end of a group, for the next one's factors.
+            struct Step {
+                uint32_t b, slot, j;
+                bool group_end;
+            };
+            auto begin = [&](uint32_t kb) {
+                Step t = {it % kTiles, group % S::kGroups, (kb - kb0) & 3u, false};
+                t.group_end = t.j == 3u || kb + 1u == kb1;
+                const uint32_t next = (group + 1u) % S::kGroups;
+                if (t.group_end && (kb + 1u < kb1 || unit + stride < num_units)) {
+                    alive = mbar_wait_both(&tmem_full[t.b], (it / kTiles) & 1u, &scale_full[next], ((group + 1u) / S::kGroups) & 1u, p.status, 406, t.b, bar_ns);
+                    apart = __any_sync(0xFFFFFFFFu, apart_of[next] != 0u);
+                } else {
+                    alive = mbar_wait_soon(&tmem_full[t.b], (it / kTiles) & 1u, p.status, 406, t.b, bar_ns);
+                }
+                tcgen05_fence_after();
+                return t;
+            };
+            auto give_back = [&](const Step& t) {
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tmem_empty[t.b]);
+                    if (t.group_end) {
+                        mbar_arrive(&scale_empty[t.slot]);
+                    }
+                }
+                group += t.group_end ? 1u : 0u;
+                ++it;
+            };
+            if (unit == first_unit) {
+                alive = mbar_wait_soon(&scale_full[0], 0u, p.status, 407, 0, bar_ns);
+                apart = __any_sync(0xFFFFFFFFu, apart_of[0] != 0u);
+            }
+            uint32_t kb = kb0;
+            while (alive && kb < kb1 && !apart) {
+                const Step t = begin(kb);
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
-                tcgen05_fence_after();
-                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (slot * 4u + j) * (kRows / 4);
+                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (t.slot * 4u + t.j) * (kRows / 4);
 #pragma unroll
                 for (uint32_t c = 0; c < kRows; c += 16) {
                     if (c < rows) {
                         float v[16];
-                        tmem_ld_16(tmem + b * kRows + c, v);
+                        tmem_ld_16(tmem + t.b * kRows + c, v);
                         tmem_ld_fence(v);
 #pragma unroll
                         for (uint32_t i = 0; i < 16; i += 4) {
@@ -480,17 +656,43 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
                         }
                     }
                 }
-                tcgen05_fence_before();
-                __syncwarp();
-                const bool group_end = j == 3u || kb + 1u == kb1;
-                if (lane == 0) {
-                    mbar_arrive(&tmem_empty[b]);
-                    if (group_end) {
-                        mbar_arrive(&scale_empty[slot]);
+                give_back(t);
+                ++kb;
+            }
+            float back = 1.0f / kHeld;
+            if (kb < kb1) {
+                scale_sums(acc, back);
+                back = 1.0f;
+            }
+            while (alive && kb < kb1) {  // from a marked group to the end of the unit
+                const uint32_t marked = apart_of[group % S::kGroups];
+                const Step t = begin(kb);
+                if (!alive) {
+                    break;
+                }
+                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (t.slot * 4u + t.j) * (kRows / 4);
+                const uint32_t* power = reinterpret_cast<const uint32_t*>(smem + S::kOffPower) + (t.slot * 4u + t.j) * (kRows / 4);
+#pragma unroll
+                for (uint32_t c = 0; c < kRows; c += 16) {
+                    if (c < rows) {
+                        float v[16];
+                        tmem_ld_16(tmem + t.b * kRows + c, v);
+                        tmem_ld_fence(v);
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i += 4) {
+                            const float4 f = factor[(c + i) / 4];
+                            const uint32_t e = marked ? power[(c + i) / 4] : 0x57575757u;  // 2^-40
+                            mul_2(v[i], v[i + 1], __uint_as_float((e & 0xFFu) << 23), __uint_as_float((e >> 8 & 0xFFu) << 23));
+                            mul_2(v[i + 2], v[i + 3], __uint_as_float((e >> 16 & 0xFFu) << 23), __uint_as_float((e >> 24) << 23));
+                            fma_2(acc[c + i], acc[c + i + 1], v[i], v[i + 1], f.x, f.y);
+                            fma_2(acc[c + i + 2], acc[c + i + 3], v[i + 2], v[i + 3], f.z, f.w);
+                        }
                     }
                 }
-                group += group_end ? 1u : 0u;
+                give_back(t);
+                ++kb;
             }
+            scale_sums(acc, back);
             OutT* out = static_cast<OutT*>(p.c) + (size_t)first * p.N + n0;
             if (p.parts == 1u) {
                 if (alive && n0 + column < p.N) {

@@ -21,7 +21,8 @@
 //   tile_read[b]              lives in each CTA: its promotion warps have read a tile
 //   scale_full[i], scale_empty[i]   live in each CTA: the factors of its rows (and, by column, of the columns) for a group of four
 //                             blocks of K (every unit begins with a group of its own)
-//   named barriers 1 + b      tile b may be read (nothing else waits on one: their waits have no limit)
+//   named barriers 1 + b      tile b may be read; 5: the first group's factors are there (the warp that arrives on them always does, and nothing
+//                             else waits on one: their waits have no limit)
 //
 // A role takes 300 to 600 cycles for a block whatever its size (a look at a barrier, then instructions of one lane), hence so many of
 // them.  448 threads: warps 0-7 promotion and output (warp w: lane quarter w % 4, columns 64 (w / 4)), 8 and 9 TMA for A and B, 10
@@ -49,13 +50,16 @@ struct BlockPairSmem {
     static constexpr uint32_t kOffB = kOffA + kStages * kABytes;
     static constexpr uint32_t kOffOut = kOffB + kStages * kBBytes;
     static constexpr uint32_t kOffFactor = kOffOut + kBlockPairPromoters * kOutBytes;  // [128 rows][4 blocks] a slot
-    static constexpr uint32_t kOffScale = kOffFactor + kScaleSlots * 128 * 16;         // by column: [4 blocks][128 columns] a slot
+    static constexpr uint32_t kOffScale = kOffFactor + kScaleSlots * 128 * 16;         // by column: [4 blocks][128 columns] a slot; else g as the factors
     static constexpr uint32_t kOffBar = kOffScale + kScaleSlots * kBlockPairN * 16;
     static constexpr uint32_t kNumBars = 2 * kStages + 3 * kTiles + 2 * kScaleSlots;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // the step (counted from 1) whose wait has given up
-    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
+    static constexpr uint32_t kOffDead = kOffTmemPtr + 4;   // the step (counted from 1) whose wait has given up; ~0: before the first
+    static constexpr uint32_t kOffLeave = kOffTmemPtr + 16;               // [tiles]: the step (from 1) with which the promotion leaves its loop
+    static constexpr uint32_t kOffApart = kOffLeave + kTiles * 4;         // [slots] words: the group's products of scales leave fp32's range
+    static constexpr uint32_t kOffTiles = kOffApart + kScaleSlots * 4;
     static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
+    static_assert(kScaleSlots * 128 * 16 <= kOffBar - kOffScale, "a marked group's g lie where the columns' scales would");
 };
 static_assert(BlockPairSmem<float>::dynamic_bytes(kGroupedMaxExperts) <= 232448 && BlockPairSmem<__half>::dynamic_bytes(kGroupedMaxExperts) <= 232448,
               "one CTA's shared memory");
@@ -129,7 +133,38 @@ __device__ __forceinline__ void tma_expect_and_load_3d_pair(void* smem_dst, cons
         : "memory");
 }
 
+// By column: whether some product of a row's and a column's scale, of the whole warp's, may not be ordinary.  Looks at the largest and the
+// smallest ones (as ordered bits), and only when these say so at the finite ones other than zero alone.
+__device__ __forceinline__ bool scales_apart(const float (&rows)[4][4], const float4 (&columns)[4])
+{
+    auto outside = [&](bool all) {
+        uint32_t most[2] = {0u, 0u}, least[2] = {0x7F800000u, 0x7F800000u};
+        auto see = [&](uint32_t side, float s) {
+            if (all || is_finite_and_not_zero(s)) {
+                const uint32_t size = __float_as_uint(s) & 0x7FFFFFFFu;
+                most[side] = max(most[side], size);
+                least[side] = min(least[side], size);
+            }
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            see(0, rows[i][0]), see(0, rows[i][1]), see(0, rows[i][2]), see(0, rows[i][3]);
+            see(1, columns[i].x), see(1, columns[i].y), see(1, columns[i].z), see(1, columns[i].w);
+        }
+        float top = kHeld, bottom = kHeld;
+#pragma unroll
+        for (uint32_t side = 0; side < 2; ++side) {
+            top *= __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, most[side]));
+            bottom *= __uint_as_float(__reduce_min_sync(0xFFFFFFFFu, least[side]));
+        }
+        // without any finite scale, or none but zeros: 0 and infinity, or NaN
+        return all ? !is_ordinary(top) || !is_ordinary(bottom) : top >= 0x1p64f || bottom < 0x1p-126f;
+    };
+    return __builtin_expect(outside(true), 0) && outside(false);
+}
+
 constexpr uint32_t kBlockPairJoined = 32 * (kBlockPairPromoters + 1);  // threads of a named barrier
+constexpr uint32_t kBlockPairFirst = 5;                                // the named barrier of the first factors
 
 __device__ __forceinline__ void named_sync(uint32_t id)
 {
@@ -163,6 +198,8 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     uint64_t* scale_empty = scale_full + S::kScaleSlots;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     volatile uint32_t* dead = reinterpret_cast<volatile uint32_t*>(smem + S::kOffDead);
+    volatile uint32_t* leave = reinterpret_cast<volatile uint32_t*>(smem + S::kOffLeave);
+    volatile uint32_t* apart_of = reinterpret_cast<volatile uint32_t*>(smem + S::kOffApart);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
@@ -183,6 +220,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             mbar_init(&tmem_full[b], 1);
             mbar_init(&tmem_empty[b], 1);  // warps 10 and 11 of the other CTA
             mbar_init(&tile_read[b], kBlockPairPromoters);
+            leave[b] = 0u;
         }
         for (uint32_t i = 0; i < S::kScaleSlots; ++i) {
             mbar_init(&scale_full[i], kByColumn ? 2 : 1);  // the rows' factors (and the columns' bytes)
@@ -267,8 +305,15 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 for (uint32_t i = 0; i < 4; ++i) {
                     load_scales(p.a_scales + min(row + 32u * i, u.end - 1u) * p.a_scale_row, p.a_scale_block, kb, k_blocks, a[i]);
                 }
+                float4 columns[4];  // by column: of four of them
                 if (!kByColumn) {
                     load_scales(b_scales, p.b_scale_block, kb, k_blocks, b);
+                } else {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const float* at = p.b_scales + (kb + j) * p.b_scale_block + u.n0 + 4u * lane;
+                        columns[j] = kb + j < k_blocks && u.n0 + 4u * lane < p.N ? __ldcg(reinterpret_cast<const float4*>(at)) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                    }
                 }
                 const uint32_t slot = group % S::kScaleSlots;
                 alive = mbar_wait_soon(&scale_empty[slot], ((group / S::kScaleSlots) & 1u) ^ 1u, p.status, 505, slot, bar_ns);
@@ -284,10 +329,53 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     }
                 }
                 __syncwarp();
+                // whether some product may not stand for its two scales; by column: of the group's largest or smallest ones
+                float f[4][4];
+                bool apart;
+                if (kByColumn) {
+                    apart = scales_apart(a, columns);
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        f[i / 4][i % 4] = a[i / 4][i % 4] * kHeld;
+                    }
+                } else {
+                    bool odd = false;
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        f[i / 4][i % 4] = a[i / 4][i % 4] * (b[i % 4] * kHeld);
+                        odd = odd || !is_ordinary(f[i / 4][i % 4]);
+                    }
+                    apart = __any_sync(0xFFFFFFFFu, odd);
+                    if (__builtin_expect(apart, 0)) {
+                        odd = false;
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            odd = odd || needs_both_scales(a[i / 4][i % 4], b[i % 4], f[i / 4][i % 4]);
+                        }
+                        apart = __any_sync(0xFFFFFFFFu, odd);
+                    }
+                }
+                if (__builtin_expect(apart, 0)) {
+                    float4* power = reinterpret_cast<float4*>(smem + S::kOffScale) + slot * 128u + lane;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        float g[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; ++j) {
+                            f[i][j] = kByColumn ? a[i][j] : wide_factor(a[i][j], b[j], g[j]);
+                        }
+                        if (!kByColumn) {
+                            power[32u * i] = make_float4(g[0], g[1], g[2], g[3]);
+                        }
+                    }
+                }
                 float4* factor = reinterpret_cast<float4*>(smem + S::kOffFactor) + slot * 128u + lane;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
-                    factor[32u * i] = make_float4(a[i][0] * b[0], a[i][1] * b[1], a[i][2] * b[2], a[i][3] * b[3]);
+                    factor[32u * i] = make_float4(f[i][0], f[i][1], f[i][2], f[i][3]);
+                }
+                if (lane == 0) {
+                    apart_of[slot] = apart ? 1u : 0u;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -345,20 +433,35 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         }
     } else if (warp == 12) {
         // ------------------------------- tells of tiles and factors -----------------------
-        // It is never two turns ahead on a named barrier: tile b is filled again after all have read it.  When a wait gives up, the
-        // promotion is told with that step and ends with it.
+        // It is never two turns ahead on a named barrier: tile b is filled again after all have read it.  With the last block of a group it
+        // waits for the next one's factors as well: when that is marked, or when a wait gives up, the promotion leaves its loop with
+        // this step.
         uint32_t i = 0, group = 0;
+        if (steps != 0u) {
+            alive = mbar_wait_soon(&scale_full[0], 0u, p.status, 507, 0, bar_ns);
+            if (!alive && lane == 0) {
+                *dead = 0xFFFFFFFFu;
+            }
+            __syncwarp();
+            named_arrive(kBlockPairFirst);
+        }
         for (uint32_t it = 0; alive && it < steps; ++it) {
-            const uint32_t b = it & 3u, slot = group % S::kScaleSlots;
-            if ((i & 3u) == 0u) {
-                alive = mbar_wait_both(&tmem_full[b], (it >> 2) & 1u, &scale_full[slot], (group / S::kScaleSlots) & 1u, p.status, 506, b, bar_ns);
-                ++group;
+            const uint32_t b = it & 3u, next = (group + 1u) % S::kScaleSlots;
+            const bool group_end = (i & 3u) == 3u || i + 1u == k_blocks;
+            uint32_t apart = 0;
+            if (group_end && it + 1u < steps) {
+                alive = mbar_wait_both(&tmem_full[b], (it >> 2) & 1u, &scale_full[next], ((group + 1u) / S::kScaleSlots) & 1u, p.status, 506, b, bar_ns);
+                apart = apart_of[next];
             } else {
                 alive = mbar_wait_soon(&tmem_full[b], (it >> 2) & 1u, p.status, 506, b, bar_ns);
             }
+            group += group_end ? 1u : 0u;
             i = i + 1u == k_blocks ? 0u : i + 1u;
-            if (!alive && lane == 0) {
-                *dead = it + 1u;
+            if ((!alive || apart != 0u) && lane == 0) {
+                if (!alive) {
+                    *dead = it + 1u;
+                }
+                leave[b] = it + 1u;
             }
             __syncwarp();
             tcgen05_fence_after();
@@ -373,6 +476,12 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
         const uint32_t scales = smem_u32(smem + S::kOffScale) + col * 4u;
         uint8_t* out = smem + S::kOffOut + warp * S::kOutBytes;
         uint32_t it = 0, group = 0;
+        bool apart = false;  // the group that comes next is marked
+        if (steps != 0u) {
+            named_sync(kBlockPairFirst);
+            alive = *dead != 0xFFFFFFFFu;
+            apart = apart_of[0] != 0u;
+        }
         for (uint32_t unit = pair; alive && unit < num_units; unit += num_pairs) {
             const Unit u = unit_at(unit);
             const uint32_t row0 = u.m0 + cta * 128u + q * 32u, col0 = u.n0 + col;
@@ -382,11 +491,13 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             // has no registers left for that, at once: 140 -> 128 us on one GPU); a tile goes back when its last are in registers.
             float v[2][16], f = 0.0f;
             uint32_t scale = 0;
-            for (uint32_t i = 0; i < k_blocks; ++i, ++it) {
+            uint32_t i = 0;
+            bool left = false;
+            for (; !apart && i < k_blocks; ++i, ++it) {
                 const uint32_t b = it & 3u, j = i & 3u;
                 named_sync(1u + b);
                 tcgen05_fence_after();
-                const uint32_t dead_step = *dead;
+                const uint32_t leave_step = leave[b];
                 if (live) {
                     const uint32_t tile = tmem + b * kBlockPairN;
                     tmem_ld_16(tile, v[0]);
@@ -416,16 +527,79 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                 if (!kLater && live) {
                     add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
                 }
-                if (dead_step == it + 1u) {
-                    alive = false;  // a tile that never filled is not written out
+                if (leave_step == it + 1u) {
+                    left = true;
                     break;
                 }
                 group += j == 3u || i + 1u == k_blocks ? 1u : 0u;
             }
-            if (kLater && live) {
+            if (kLater && live && !apart) {
                 add_scaled<kByColumn>(&acc[48], v[1], f, scale + 192u);
             }
+            if (left) {
+                alive = *dead != it + 1u;  // a tile that never filled is not written out
+                apart = true;
+                ++group, ++i, ++it;
+            }
+            float back = 1.0f / kHeld;
+            if (apart) {
+                scale_sums(acc, back);
+                back = 1.0f;
+            }
+            for (uint32_t marked = 0; alive && i < k_blocks; ++i, ++it) {  // from a marked group to the end of the unit
+                const uint32_t b = it & 3u, j = i & 3u, slot = group % S::kScaleSlots;
+                named_sync(1u + b);
+                tcgen05_fence_after();
+                const uint32_t leave_step = leave[b];
+                marked = j == 0u ? apart_of[slot] : marked;
+                const uint32_t tile = tmem + b * kBlockPairN, of_row = (slot * 128u) * 16u + j * 4u;
+                scale = scales + (slot * 4u + j) * (kBlockPairN * 4u);
+                float g = 1.0f / kHeld;
+                auto add = [&](uint32_t c) {
+                    float(&x)[16] = v[c & 1];
+                    if (kByColumn) {
+                        add_scaled_apart(&acc[16 * c], x, f, scale + 64u * c);
+                    } else {
+                        scale_sums(x, g);
+                        add_scaled<false>(&acc[16 * c], x, f, 0u);
+                    }
+                };
+                if (live) {
+                    tmem_ld_16(tile, v[0]);
+                    f = ld_shared_f32(factors + of_row);
+                    if (kByColumn) {
+                        f = marked ? f : f * g;
+                    } else if (marked) {
+                        g = ld_shared_f32(factors + S::kOffScale - S::kOffFactor + of_row);
+                    }
+                    tmem_ld_fence(v[0]);
+#pragma unroll
+                    for (uint32_t c = 0; c < 3; ++c) {
+                        tmem_ld_16(tile + 16u * c + 16u, v[(c + 1) & 1]);
+                        add(c);
+                        tmem_ld_fence(v[(c + 1) & 1]);
+                    }
+                }
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&tile_read[b]);
+                    if (j == 0u && group != 0u) {
+                        mbar_arrive(&scale_empty[(group - 1u) % S::kScaleSlots]);
+                    }
+                }
+                if (live) {
+                    add(3);
+                }
+                group += j == 3u || i + 1u == k_blocks ? 1u : 0u;
+                apart = leave_step == it + 1u;
+                if (apart && *dead == it + 1u) {
+                    alive = false;
+                    break;
+                }
+            }
             if (live && alive) {
+                scale_sums(acc, back);
                 if (row0 + 32u <= u.end || p.offsets == nullptr) {
                     // twice 32 rows of 32 columns, in the order that TMA reads with its swizzle; what lies outside the matrix is not written
                     if (lane == 0) {

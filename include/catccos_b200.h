@@ -281,7 +281,8 @@ typedef struct catccos_b200_block_operand {
  *   x W       x in blocks 1 x 128, W [k, n] in blocks 128 x 128 (or the checkpoint's [n, k], transposed)
  *   dy W^T    the same W, transposed the other way
  *   x^T dy    both in blocks 128 x 1, x transposed, dy per_column
- * The products of a block are summed by the tensor core, the blocks in fp32, in a fixed order.  n % 16 == 0, k % 16 == 0, a
+ * The products of a block are summed by the tensor core, the blocks in fp32, in a fixed order.  Scales are any fp32 values: a block's
+ * sum times its two scales counts, also where the product of the scales by itself is outside of fp32's range.  n % 16 == 0, k % 16 == 0, a
  * transposed: m % 16 == 0; c 32-byte aligned, overlapping nothing. */
 int catccos_b200_block_gemm(void* stream, const catccos_b200_block_operand_t* a, const catccos_b200_block_operand_t* b, void* c, uint32_t m,
                             uint32_t n, uint32_t k, int c_type);
