@@ -577,6 +577,21 @@ at::ScalarType code_dtype(PyObject* dtype)
     return type;
 }
 
+// Rows of a dispatch: those of the output that is given, the number that is, or one for each route.  An int32 names no more than whole().
+int64_t dispatch_rows(PyObject* out, PyObject* rows, int64_t tokens, int64_t top_k)
+{
+    if (out != Py_None) {
+        return tensor(out).size(0);
+    }
+    if (rows != Py_None) {
+        return whole(rows, "rows");
+    }
+    if (tokens * top_k > 0x7FFFFFFFll) {  // both factors are below 2^31
+        refuse("rows", "tokens * top_k below 2^31");
+    }
+    return tokens * top_k;
+}
+
 // x, dtype, block, row_index, rows, codes, scales
 CALL(block_quant, 7)
     const at::Tensor& x = plain(a[0], "x", "a bf16, fp16 or fp32 CUDA matrix, its columns next to one another", {kBf16, kF16, kF32}, 2, nullptr, false);
@@ -592,7 +607,7 @@ CALL(block_quant, 7)
             refuse("row_index", "a row for each row of x");
         }
         top_k = index.size(1);
-        rows = a[5] != Py_None ? tensor(a[5]).size(0) : (a[4] != Py_None ? whole(a[4], "rows") : m * top_k);
+        rows = dispatch_rows(a[5], a[4], m, top_k);
     } else if (a[4] != Py_None) {
         refuse("rows", "None without row_index");
     }
@@ -724,7 +739,7 @@ CALL(moe_dispatch, 4)
     if (index.size(0) != tokens) {
         refuse("row_index", "a row for each row of x");
     }
-    const int64_t rows = a[3] != Py_None ? tensor(a[3]).size(0) : (a[2] != Py_None ? whole(a[2], "rows") : tokens * top_k);
+    const int64_t rows = dispatch_rows(a[3], a[2], tokens, top_k);
     const OnDevice on(x);
     const at::Tensor out = result(a[3], "a contiguous matrix [rows, n] of x's type and device", {x.scalar_type()}, x, rows, n, x.scalar_type());
     void *in = x.data_ptr(), *i = index.data_ptr(), *o = out.data_ptr();
