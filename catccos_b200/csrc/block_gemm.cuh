@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "block_plan.hpp"
 #include "common.cuh"
 #include "mx_gemm_small.cuh"
 #include "mx_grouped_gemm.cuh"
@@ -24,8 +25,6 @@
 namespace catccos {
 
 constexpr uint32_t kBlockFewThreads = 256;
-constexpr uint32_t kBlockFewColumns = 128;  // of the weight, to a tile
-constexpr uint32_t kBlockFewMaxParts = 8;
 
 struct BlockGemmParams {
     const float* a_scales;

@@ -36,7 +36,6 @@ namespace catccos {
 
 constexpr uint32_t kBlockPairThreads = 448;
 constexpr uint32_t kBlockPairPromoters = 8;  // warps
-constexpr uint32_t kBlockPairM = 256, kBlockPairN = 128;
 
 template <typename OutT>
 struct BlockPairSmem {

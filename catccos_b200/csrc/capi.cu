@@ -1803,12 +1803,7 @@ int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmPa
                     : encode_map_3d(&maps[2], o.b->codes, p.N, p.K, p.experts, columns, 128, ldb, plane);
 }
 
-// Units of a launch of single CTAs (with offsets: as many as there may be, one row tile that is not full for every expert with rows).
-uint64_t block_units(const BlockGemmParams& p, uint32_t tile_rows, uint32_t tile_columns)
-{
-    const uint64_t tiles = p.offsets ? p.rows / tile_rows + std::min(p.rows, p.experts) : (p.rows + tile_rows - 1) / tile_rows;
-    return tiles * ((p.N + tile_columns - 1) / tile_columns);
-}
+BlockCall block_call(const BlockGemmParams& p, bool by_column) { return {p.rows, p.experts, p.N, p.K, p.offsets != nullptr, p.a_cols != 0 || by_column}; }
 
 template <uint32_t kRows, typename OutT>
 int launch_block_few(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const BlockGemmParams& p)
@@ -1820,7 +1815,7 @@ int launch_block_few(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const
     CUtensorMap maps[3];
     int rcode = block_maps(maps, o, p, kRows, kBlockFewColumns);
     if (rcode != 0) return rcode;
-    const uint64_t units = block_units(p, kRows, kBlockFewColumns);
+    const uint64_t units = block_units(block_call(p, false), kRows, kBlockFewColumns);
     const uint32_t smem = S::dynamic_bytes(p.experts);
     if (p.parts > 1) {
         CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockFewThreads, smem, st, maps[1], maps[2], p));
@@ -1843,64 +1838,17 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     int rcode = block_maps(maps, o, p, 32, 64);
     if (rcode == 0) rcode = encode_map_2d(&out, p.c, p.N, p.rows, 32, 32, false, sizeof(OutT));
     if (rcode != 0) return rcode;
-    const uint64_t units = block_units(p, kBlockPairM, kBlockPairN);
+    const uint64_t units = block_units(block_call(p, kByColumn), kBlockPairM, kBlockPairN);
     CUDA_TRY(launch_after(kern, dim3(2u * (unsigned)std::min<uint64_t>(units, (uint64_t)pairs)), kBlockPairThreads, S::dynamic_bytes(p.experts), st,
                           maps[0], maps[1], maps[2], out, p));
     return 0;
 }
 
-// Which form a launch takes: CTA pairs (rows 0), or tiles of so many rows with K in so many parts.  The one that takes least by a fit
-// to 600 measured calls (dense with 1 to 1024 rows, experts with 1 to 512 rows each; 14 to 22 % off): a launch, then for each round of
-// units a block of K, which takes longer the more SMs are busy, and the output; the meeting of the parts.  So chosen, a call takes
-// 2.4 % more than in the best form; by the rows alone (16, 32, 64, pairs above 128 rows an expert) it would be 13 %.  An expert's rows are
-// reckoned with as in plan_grouped.
-struct BlockPlan {
-    uint32_t rows, parts;
-};
-
-BlockPlan plan_block_gemm(const RankCtx& rc, const BlockGemmParams& p, bool by_column)
-{
-    struct Cost {
-        uint32_t rows;
-        double launch, block, busy_block, round, meeting;
-    };
-    constexpr Cost costs[] = {{0, 4.28, 0.299, 0.053, 0.50, 0}, {16, 3.71, 0.219, 0.205, 0.28, 1.29}, {32, 3.82, 0.241, 0.235, 0.56, 1.96}, {64, 5.06, 0.286, 0.360, 0.72, 2.37}};
-    if (p.a_cols || by_column || g.cta_pair == 1) {
-        return {0, 1};  // the form for few rows has neither
-    }
-    const uint32_t k_blocks = (p.K + 127u) / 128u;
-    const double active = std::min(p.rows, p.experts) < 2 ? 1.0 : 0.9 * std::min(p.rows, p.experts);
-    BlockPlan best = {0, 0};
-    double least = 0;
-    for (const Cost& c : costs) {
-        if ((g.block_rows != 0 && (uint32_t)g.block_rows != c.rows) || (g.block_rows == 0 && g.cta_pair == 2 && c.rows == 0)) {
-            continue;  // a test names the form
-        }
-        const uint32_t tile_rows = c.rows ? c.rows : kBlockPairM;
-        uint32_t parts = 1;
-        const uint64_t most = block_units(p, tile_rows, kBlockFewColumns);
-        while (c.rows != 0 && parts < kBlockFewMaxParts && most * parts * 2 <= 2 * (uint64_t)rc.num_sms && parts * 2 <= k_blocks &&
-               (g.split_k == 0 || parts * 2 <= (uint32_t)g.split_k)) {
-            parts *= 2;
-        }
-        const double tiles = p.offsets ? std::max(active, p.rows / (double)tile_rows + 0.7 * active) : std::ceil(p.rows / (double)tile_rows);
-        const double units = tiles * ((p.N + kBlockFewColumns - 1) / kBlockFewColumns) * parts, slots = c.rows ? 2 * rc.num_sms : rc.num_sms / 2;
-        const double time = c.launch + (parts > 1 ? c.meeting : 0) +
-                            std::ceil(units / slots) * ((k_blocks + parts - 1) / parts * (c.block + c.busy_block * std::min(1.0, units / slots)) + c.round);
-        if (best.parts == 0 || time < least) {
-            best = {c.rows, parts};
-            least = time;
-        }
-    }
-    return best;
-}
-static_assert(kBlockPairN == kBlockFewColumns, "the plan counts columns of tiles alike");
-
 template <typename OutT>
 int launch_block_gemm(RankCtx& rc, cudaStream_t st, const BlockOperands& o, BlockGemmParams p)
 {
     const bool by_column = o.b->per_column != 0;
-    const BlockPlan plan = plan_block_gemm(rc, p, by_column);
+    const BlockPlan plan = plan_block_gemm(block_call(p, by_column), {g.block_rows, g.split_k, g.cta_pair}, (uint32_t)rc.num_sms);
     p.parts = plan.parts;
     switch (plan.rows) {
         case 0: return by_column ? launch_block_pair<OutT, true>(rc, st, o, p) : launch_block_pair<OutT, false>(rc, st, o, p);
