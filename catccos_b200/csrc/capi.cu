@@ -1789,18 +1789,19 @@ struct BlockOperands {
     const catccos_b200_block_operand_t *a, *b;
 };
 
-// Maps of the rows of a (boxes of `most` and, in maps[1], of `few` rows; stored by column: boxes of 128 x 128) and of b (`columns`
-// wide).
-int block_maps(CUtensorMap (&maps)[3], const BlockOperands& o, const BlockGemmParams& p, uint32_t few, uint32_t columns)
+// Map of the rows of a in boxes of so many (stored by column: boxes of 128 x 128)
+int block_row_map(CUtensorMap* map, const BlockOperands& o, const BlockGemmParams& p, uint32_t box_rows)
 {
-    const void* a = o.a->codes;
-    const uint64_t lda = o.a->line_bytes, ldb = o.b->line_bytes;
-    int rcode = p.a_cols ? encode_map_2d(&maps[0], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[0], a, p.K, p.rows, 128, 128, false, 1, lda);
-    if (rcode == 0) rcode = p.a_cols ? encode_map_2d(&maps[1], a, p.rows, p.K, 128, 128, false, 1, lda) : encode_map_2d(&maps[1], a, p.K, p.rows, 128, few, false, 1, lda);
-    if (rcode != 0) return rcode;
-    const uint64_t plane = p.experts > 1 ? o.b->matrix_bytes : ldb * (p.b_rows ? p.N : p.K);
-    return p.b_rows ? encode_map_3d(&maps[2], o.b->codes, p.K, p.N, p.experts, 128, columns, ldb, plane)
-                    : encode_map_3d(&maps[2], o.b->codes, p.N, p.K, p.experts, columns, 128, ldb, plane);
+    return p.a_cols ? encode_map_2d(map, o.a->codes, p.rows, p.K, 128, 128, false, 1, o.a->line_bytes)
+                    : encode_map_2d(map, o.a->codes, p.K, p.rows, 128, box_rows, false, 1, o.a->line_bytes);
+}
+
+// Map of b in boxes of so many columns
+int block_weight_map(CUtensorMap* map, const BlockOperands& o, const BlockGemmParams& p, uint32_t columns)
+{
+    const uint64_t ldb = o.b->line_bytes, plane = p.experts > 1 ? o.b->matrix_bytes : ldb * (p.b_rows ? p.N : p.K);
+    return p.b_rows ? encode_map_3d(map, o.b->codes, p.K, p.N, p.experts, 128, columns, ldb, plane)
+                    : encode_map_3d(map, o.b->codes, p.N, p.K, p.experts, columns, 128, ldb, plane);
 }
 
 BlockCall block_call(const BlockGemmParams& p, bool by_column) { return {p.rows, p.experts, p.N, p.K, p.offsets != nullptr, p.a_cols != 0 || by_column}; }
@@ -1812,16 +1813,17 @@ int launch_block_few(RankCtx& rc, cudaStream_t st, const BlockOperands& o, const
     auto kern = block_gemm_few_kernel<kRows, OutT>;
     static PerDevice<bool, kMaxRanks * 2> done;
     CUDA_TRY(allow_smem(kern, S::dynamic_bytes(kGroupedMaxExperts), done));
-    CUtensorMap maps[3];
-    int rcode = block_maps(maps, o, p, kRows, kBlockFewColumns);
+    CUtensorMap rows, weight;
+    int rcode = block_row_map(&rows, o, p, kRows);
+    if (rcode == 0) rcode = block_weight_map(&weight, o, p, kBlockFewColumns);
     if (rcode != 0) return rcode;
     const uint64_t units = block_units(block_call(p, false), kRows, kBlockFewColumns);
     const uint32_t smem = S::dynamic_bytes(p.experts);
     if (p.parts > 1) {
-        CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockFewThreads, smem, st, maps[1], maps[2], p));
+        CUDA_TRY(launch_clusters_after(kern, dim3((unsigned)(units * p.parts)), p.parts, kBlockFewThreads, smem, st, rows, weight, p));
     } else {
         const uint32_t grid = (uint32_t)std::min<uint64_t>(units, 2 * (uint64_t)rc.num_sms);
-        CUDA_TRY(launch_after(kern, dim3(grid), kBlockFewThreads, smem, st, maps[1], maps[2], p));
+        CUDA_TRY(launch_after(kern, dim3(grid), kBlockFewThreads, smem, st, rows, weight, p));
     }
     return 0;
 }
@@ -1835,7 +1837,9 @@ int launch_block_pair(RankCtx& rc, cudaStream_t st, const BlockOperands& o, cons
     int pairs = 0;
     CUDA_TRY(resident_clusters_of_two(rc, kern, kBlockPairThreads, S::dynamic_bytes(kGroupedMaxExperts), resident, &pairs));
     CUtensorMap maps[3], out;
-    int rcode = block_maps(maps, o, p, 32, 64);
+    int rcode = block_row_map(&maps[0], o, p, 128);
+    if (rcode == 0) rcode = block_row_map(&maps[1], o, p, 32);
+    if (rcode == 0) rcode = block_weight_map(&maps[2], o, p, 64);
     if (rcode == 0) rcode = encode_map_2d(&out, p.c, p.N, p.rows, 32, 32, false, sizeof(OutT));
     if (rcode != 0) return rcode;
     const uint64_t units = block_units(block_call(p, kByColumn), kBlockPairM, kBlockPairN);
