@@ -1728,9 +1728,22 @@ int moe_sum(const char* name, void* stream, const void* expert_out, uint32_t row
     return 0;
 }
 
-uint32_t combine_grad_routes(uint32_t tokens, uint32_t top_k)
+// Routes of a CTA.  Long rows read by whole sectors (wide): one, whose rows are spread best over the SMs (what other routes read of the
+// token's gradient comes from L2).  Short rows are bound by the number of CTAs: two, or four where they are many.  Rows read in pieces of 16
+// bytes have too few bytes on their way with one route: more of them as soon as the SMs have enough CTAs.  One / two / four routes in us:
+//   wide       4096 tokens x 6 routes x 7168 119 / 122 / 127   4096 x 8 x 2304 60.6 / 62.8 / 63.0   8192 x 8 x 1536 71.7 / 74.2 / 70.3
+//              1024 x 8 x 1024 9.7 / 8.2 / 8.6   4096 x 2 x 1024 9.7 / 8.9 / 10.6   256 x 4 x 512 2.1 / 1.9 / 2.3
+//              512 x 8 x 512 5.3 / 3.9 / 4.3     4096 x 4 x 512 18.0 / 9.7 / 8.9    1024 x 8 x 64 9.3 / 5.1 / 3.6
+//   of 16      64 x 8 x 7176 6.2 / 6.6 / 7.3     512 x 8 x 7176 27.1 / 25.9 / 26.1  4096 x 8 x 7176 198 / 184 / 178
+//              64 x 8 x 1032 2.3 / 2.5 / 2.6     256 x 4 x 1032 3.0 / 2.7 / 2.9     1024 x 4 x 1032 7.4 / 6.5 / 6.1
+//              256 x 8 x 264 3.0 / 2.5 / 2.7     1024 x 4 x 264 5.2 / 3.4 / 3.0     4096 x 2 x 264 9.5 / 5.3 / 5.8
+uint32_t combine_grad_routes(uint32_t tokens, uint32_t n, uint32_t top_k, bool wide)
 {
-    return top_k <= 1 || (uint64_t)tokens * top_k <= 512 ? 1 : (top_k <= 2 || (uint64_t)tokens * top_k <= 2048 ? 2 : 4);
+    const uint64_t routes = (uint64_t)tokens * top_k;
+    if (top_k == 1 || (wide ? n > 1024 : n > 512 && routes <= 512)) {
+        return 1;
+    }
+    return top_k > 2 && (wide ? n <= 512 && routes >= 8192 : routes >= 4096) ? 4 : 2;
 }
 
 template <typename T, bool kWide>
@@ -3027,8 +3040,7 @@ int catccos_b200_moe_combine_grad(void* stream, const void* d_out, const void* e
     p.top_k = top_k;
     const bool wide = n % 16 == 0 && !misaligned(d_out, 32) && !misaligned(expert_out, 32) && !misaligned(d_expert_out, 32);
     p.vectors = wide ? n / 16 : n / 8;
-    // four routes a CTA read a token's gradient less often; with few tokens one or two spread the rows over the SMs
-    const uint32_t routes = combine_grad_routes(tokens, top_k);
+    const uint32_t routes = combine_grad_routes(tokens, n, top_k, wide);
     p.chunks = (top_k + routes - 1) / routes;
     const uint64_t grid = (uint64_t)tokens * p.chunks;
     if (grid > 0x7FFFFFFFull) {

@@ -923,7 +923,7 @@ struct CombineGradParams {
 //   d_y[row_index[t, r]] = weights[t, r] * d_out[t];   d_weights[t, r] = sum over columns of d_out[t] * y[row_index[t, r]]
 // A CTA has a token and kRoutes of its routes.  Bound by memory: d_out once, a row read and a row written for every live route.  The
 // sums are fp32, a thread's columns ascending, then lanes and warps in a fixed order.  4095 tokens x 6 rows of 5120 columns: 92 us with
-// four routes and whole sectors (6.0 TB/s), 104 with 16-byte pieces; 64 tokens x 8 x 7168 4.4 us with one route, 5.7 with four.
+// four routes and whole sectors, 85 with one (6.4 TB/s, a plain copy's rate), 104 with four and 16-byte pieces; how many: combine_grad_routes().
 template <typename T, uint32_t kRoutes, bool kWide>
 __global__ void __launch_bounds__(kCombineGradThreads) moe_combine_grad_kernel(const CombineGradParams p)
 {
