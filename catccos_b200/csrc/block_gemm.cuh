@@ -375,8 +375,8 @@ __device__ __forceinline__ bool mbar_wait_both(uint64_t* bar1, uint32_t parity1,
 // Up to 64 rows (of an expert) are bound by streaming the weights and by latencies, so the operands change sides: 128 columns of the
 // weight are the rows of a tile, kRows rows of A its columns.  A lane then has one weight column and kRows sums, and every warp of
 // the promotion has work however few the rows are.  (With the rows of A on the lanes the one warp that has 16 rows took 600 cycles a
-// block and 16 x 4096 x 7168 12.9 us.)  Measured: 16 x 4096 x 7168 9.0 us (3.3 TB/s; launch and set-up 3, the meeting 1.3, the weights
-// alone 4.6), 128 rows over 32 experts of 4096 x 7168 126 us: the used experts' weights at HBM's rate.
+// block and 16 x 4096 x 7168 12.9 us.)  Measured: 16 x 4096 x 7168 9.3 us in a caller's loop (3.2 TB/s; launch and set-up 3, the meeting 1.3,
+// the weights alone 4.6), 10.8 back to back; 128 rows over 32 experts of 4096 x 7168 128 us: the used experts' weights at HBM's rate.
 //
 // K may be cut over the CTAs of a cluster (p.parts: 1, 2, 4 or 8), so that calls of few tiles stream their weights with every SM.
 // Their sums meet in distributed shared memory: part d owns 128 / parts of the weight columns, the others push theirs into its idle

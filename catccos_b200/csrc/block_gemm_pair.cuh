@@ -10,11 +10,11 @@
 // promotes looks at a barrier in shared memory, which takes some 150 cycles even if there is nothing to wait for: another warp does,
 // and named barriers pass it on.  (With each promotion warp looking for itself 8192 x 2304 x 7168 takes 171 us.)
 //
-// What bounds it, at 8192 x 2304 x 7168: 154 us (1.76 PFLOP/s), 0.34 us a block of K.  With the promotion left out it is 127, with its
-// loads alone 135: operands come at 24 KB a block and SM, 85 GB/s, about what a K tile of 192 rows takes in mx_gemm_pair.cuh.  256 x
+// What bounds it, at 8192 x 2304 x 7168: 153 us back to back on two sets of operands (1.77 PFLOP/s; 177 in a caller's loop with new operands,
+// 1.53), 0.34 us a block of K.  With the promotion left out it is 127, with its loads alone 135: operands come at 24 KB a block and SM, 85 GB/s, about what a K tile of 192 rows takes in mx_gemm_pair.cuh.  256 x
 // 256 tiles read a third less of A and B, but have room for two tiles only, and came to 153; at 3001 x 7168 x 2304 to 84 against 78.
 // Sixteen promotion warps of 32 columns: 160.  By column (the scales of 128 columns in shared memory, one more product a value): 7168
-// x 2304 x 4096 128 to 134 us, bound by the promotion.
+// x 2304 x 4096 127 to 134 us, bound by the promotion.  (All figures back to back.)
 //
 //   full[s], tmem_empty[b]    live in the leader; both CTAs' TMA bytes, and the other CTA's word that it has read a tile, go there
 //   empty[s], tmem_full[b]    live in each CTA; the leader's tcgen05.commit arrives on both copies
@@ -487,7 +487,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
             const bool live = row0 < u.end && col0 < p.N;  // else there is nothing to fetch
             float acc[kCols] = {};
             // Sixteen columns are added while the next are on their way, a step's last while the next step's first are (by column, which
-            // has no registers left for that, at once: 140 -> 128 us on one GPU); a tile goes back when its last are in registers.
+            // has no registers left for that, at once: 143 -> 132 us); a tile goes back when its last are in registers.
             float v[2][16], f = 0.0f;
             uint32_t scale = 0;
             uint32_t i = 0;
