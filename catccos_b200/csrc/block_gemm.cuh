@@ -27,6 +27,8 @@ namespace catccos {
 constexpr uint32_t kBlockFewThreads = 256;
 
 struct BlockGemmParams {
+    const uint8_t *a, *b;                                  // the codes, for block_few_again
+    size_t a_line, b_line, b_matrix;                       // bytes from one line, one expert's matrix to the next
     const float* a_scales;
     size_t a_scale_row, a_scale_block;                     // floats from one row's (block's) scale to the next
     const float* b_scales;
@@ -221,28 +223,31 @@ __device__ __forceinline__ void load_scales(const float* line, size_t step, uint
 }
 
 // ---- two scales whose product is not in fp32's range ----
-// A block's sum v (with finite codes 0, or 2^-32 to 2^39 in size) is added as v * f, f = 2^40 * sa * sb: one product of the scales for many
-// sums.  What is held is 2^40 times the result, so that f is a normal number from products of 2^-166 on: a block of zeros has a scale of
-// 2^-109 or 2^-116 from the quantiser, a row of zeros beside small weights is ordinary.  f is below 2^64, so that no sum of blocks overflows.
+// A block's sum v (with finite codes 0, or 2^-32 to 2^39 in size) is added as v * f, one product of the scales for many sums.  f is kHeld * sa *
+// sb, and what is held is kHeld times the result: where f is below fp32's normal numbers, v * f is then off by 2^39 * 2^-150 / 2^40 of the
+// result at most, less than half of fp32's smallest step.  (Without kHeld the product for a block of zeros, whose scale is 2^-109 or 2^-116,
+// and small weights would be there already.)
 //
-// Other scales, finite and not zero, would give NaN for v = 0 or lose bits that v * sa * sb keeps.  The warp that makes the factors looks
-// for them and marks their group of four blocks of K; with it the promotion goes on to a second loop up to the end of the unit, which holds
-// the result itself and adds (v * g) * f with g = 2^64 or 2^-64 and f that much smaller or larger: v * g is exact, and what is then outside of
-// f's range is outside of the result's.  With the choice inside one loop, or with more work in the warp of the factors, calls without such
-// scales took 5 to 25 % longer.  A row's result is the same in both loops.
+// Upwards, f has to stay below 2^64, so that no sum of blocks overflows where the result does not, and that v = 0 stays 0 beside finite
+// scales.  The warps that make the factors look for larger ones.
+//   CTA pairs: the group of four blocks of K is marked; with it the promotion goes on to a second loop up to the end of the unit, which holds
+//   the result itself and adds (v * g) * f with g = 2^64 or 2^-64 and f that much smaller or larger: v * g is exact, and what is then outside
+//   of f's range is outside of the result's.  By column: ((v * near) * sb) * rest with sa = near * rest.
+//   Few rows: before a CTA ends, rows with such a block are computed again from the codes in global memory.
+// A row without such blocks gets the same result whatever the others have (by column: but for its last bit).  With such scales in 5 % of the
+// rows 8192 x 2304 x 7168 takes 220 us (150), 16 x 4096 x 7168 with one such row 91 (10.9).  Other calls pay 0 to 2 %, short ones (5 to 20 us) 1 to
+// 4, on pairs 4 to 8.  A choice inside one loop cost them 5 to 25 %, for few rows a second loop 2 to 7, on pairs the rows at the end 3 on large products.
 constexpr float kHeld = 0x1p40f;
-
-// a factor in range: 2^-126 <= |f| < 2^64
-__device__ __forceinline__ bool is_ordinary(float f) { return __float_as_uint(f) * 2u - 0x01000000u < 0xBE000000u; }
-
-__device__ __forceinline__ bool is_finite_and_not_zero(float f) { return __float_as_uint(f) * 2u - 1u < 0xFEFFFFFFu; }
+constexpr uint32_t kFactorLimit = 0x5F800000u;  // 2^64 as bits; a negative factor, an infinity and a NaN are above it, too, and looked at again
 
 __device__ __forceinline__ bool is_finite(float f) { return __float_as_uint(f) * 2u < 0xFF000000u; }
 
-// Whether f, as 2^40 times the product of the two scales, may not stand for them (NaN may be 0 times 2^40 * sb)
+__device__ __forceinline__ bool is_finite_and_not_zero(float f) { return __float_as_uint(f) * 2u - 1u < 0xFEFFFFFFu; }
+
+// Whether f, as kHeld times the product of the two scales, does not stand for them (NaN may be 0 times kHeld * sb)
 __device__ __forceinline__ bool needs_both_scales(float sa, float sb, float f)
 {
-    return !is_ordinary(f) && is_finite(sa) && is_finite(sb) && (f != 0.0f || (sa != 0.0f && sb != 0.0f));
+    return !(fabsf(f) < 0x1p64f) && is_finite(sa) && is_finite(sb);
 }
 
 // The factor of a marked group: v * sa * sb is (v * g) * it.
@@ -397,13 +402,113 @@ struct BlockFewSmem {
     static constexpr uint32_t kNumBars = 2 * kStages + 2 * kTiles + 2 * kGroups;
     static constexpr uint32_t kOffTmemPtr = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffDead = kOffTmemPtr + 4;  // a part of this cluster has given up
-    static constexpr uint32_t kOffApart = kOffTmemPtr + 16;            // [groups] words: its products of scales leave fp32's range
-    static constexpr uint32_t kOffPower = kOffApart + kGroups * 4;     // [groups][4 blocks][kRows] bytes: then g's exponents
-    static constexpr uint32_t kOffTiles = kOffPower + kGroups * 4 * kRows;
+    static constexpr uint32_t kOffLarge = kOffTmemPtr + 8;  // some factor was too large, in this CTA or another part
+    static constexpr uint32_t kOffTiles = kOffTmemPtr + 16;
     static constexpr uint32_t kPitch = kRows + 4;  // floats of a weight column's sums in the exchange
     static constexpr uint32_t dynamic_bytes(uint32_t experts) { return kOffTiles + (3u * experts + 1u) * 4u + 1024u; }
-    static_assert(kBlockFewColumns * kPitch * 4 <= kOffX, "the sums of all parts fit the idle ring");
+    static_assert(kBlockFewColumns * kPitch * 4 <= kOffX && kBlockFewThreads / 32 * kBlockFewColumns * 4 <= kOffX, "the sums of all parts fit the idle ring");
 };
+
+// The values of two codes
+__device__ __forceinline__ float2 code_values(uint32_t two, uint32_t e5m2)
+{
+    uint32_t halves;
+    if (e5m2) {
+        asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e5m2x2 %0, c;\n\t}" : "=r"(halves) : "r"(two));
+    } else {
+        asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(halves) : "r"(two));
+    }
+    return __half22float2(*reinterpret_cast<const __half2*>(&halves));
+}
+
+// The units of a CTA once more (with parts, the columns that it owns), after a factor was too large: rows of which a block needs both
+// scales are computed again.  All warps have a row together, a warp every eighth block of K, a lane four columns and sixteen steps of K at
+// a time; sums: the idle ring.
+template <uint32_t kRows, typename OutT>
+__device__ __forceinline__ void block_few_again(const BlockGemmParams& p, const uint32_t* tiles, float* sums)
+{
+    constexpr uint32_t kWarps = kBlockFewThreads / 32;
+    const uint32_t n_tiles = (p.N + kBlockFewColumns - 1) / kBlockFewColumns, k_blocks = (p.K + 127u) / 128u;
+    const uint32_t own = kBlockFewColumns / p.parts, clusters = gridDim.x / p.parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t* row_begin = tiles + p.experts + 1u;
+    const uint32_t num_units = p.parts > 1u ? min(tiles[p.experts] * n_tiles, clusters) : tiles[p.experts] * n_tiles;
+    GroupedWalk walk;
+    for (uint32_t unit = blockIdx.x / p.parts; unit < num_units; unit += clusters) {
+        const TileCoord tc = walk.seek(tiles, n_tiles, unit);
+        const uint32_t first = row_begin[walk.e] + tc.m_tile * kRows, rows = min(row_begin[p.experts + walk.e] - first, kRows);
+        const uint32_t n0 = tc.n_tile * kBlockFewColumns + (blockIdx.x & (p.parts - 1u)) * own, n = n0 + 4u * lane;
+        const uint32_t columns = n0 < p.N ? min(p.N - n0, own) : 0u;  // a multiple of 16
+        const uint8_t* b_codes = p.b + walk.e * p.b_matrix;
+        const float* sb_of = p.b_scales + walk.e * p.b_scale_matrix + tc.n_tile * p.b_scale_col;
+        for (uint32_t r = 0; r < rows; ++r) {
+            const size_t row = first + r;
+            const float* sa_of = p.a_scales + row * p.a_scale_row;
+            bool both = false;
+            for (uint32_t kb = threadIdx.x; kb < k_blocks; kb += kBlockFewThreads) {
+                const float sa = __ldcg(sa_of + kb * p.a_scale_block), sb = __ldcg(sb_of + kb * p.b_scale_block);
+                both = both || needs_both_scales(sa, sb, sa * (sb * kHeld));
+            }
+            if (!__syncthreads_or(both)) {
+                continue;
+            }
+            float acc[4] = {};
+            for (uint32_t kb = warp; kb < k_blocks && 4u * lane < columns; kb += kWarps) {
+                float v[4] = {}, near, rest;
+                const uint32_t end = min(p.K, kb * 128u + 128u);  // a multiple of 16
+#pragma unroll 2
+                for (uint32_t k = kb * 128u; k < end; k += 16u) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p.a + row * p.a_line + k);
+                    const uint32_t a[4] = {x.x, x.y, x.z, x.w};
+                    uint32_t b[16];  // four steps of each of four columns, four times
+                    if (p.b_rows) {
+#pragma unroll
+                        for (uint32_t c = 0; c < 4; ++c) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(b_codes + (n + c) * p.b_line + k);
+                            b[c] = w.x, b[4 + c] = w.y, b[8 + c] = w.z, b[12 + c] = w.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i += 4) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (uint32_t j = 0; j < 4; ++j) {
+                                w[j] = *reinterpret_cast<const uint32_t*>(b_codes + (k + i + j) * p.b_line + n);
+                            }
+#pragma unroll
+                            for (uint32_t c = 0; c < 4; ++c) {
+                                b[i + c] = __byte_perm(__byte_perm(w[0], w[1], c | ((4u + c) << 4)), __byte_perm(w[2], w[3], c | ((4u + c) << 4)), 0x5410u);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; i += 2) {
+                        const float2 xs = code_values(a[i / 4] >> (8u * (i & 3u)) & 0xFFFFu, p.a_fmt);
+#pragma unroll
+                        for (uint32_t c = 0; c < 4; ++c) {
+                            const float2 ws = code_values(b[i / 4 * 4 + c] >> (8u * (i & 3u)) & 0xFFFFu, p.b_fmt);
+                            v[c] = fmaf(xs.y, ws.y, fmaf(xs.x, ws.x, v[c]));
+                        }
+                    }
+                }
+                split_scale(__ldcg(sa_of + kb * p.a_scale_block), near, rest);
+                const float sb = __ldcg(sb_of + kb * p.b_scale_block);
+#pragma unroll
+                for (uint32_t c = 0; c < 4; ++c) {
+                    acc[c] = fmaf(v[c] * near * sb, rest, acc[c]);
+                }
+            }
+            *reinterpret_cast<float4*>(sums + warp * kBlockFewColumns + 4u * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            __syncthreads();
+            if (threadIdx.x < columns) {
+                float sum = sums[threadIdx.x];
+                for (uint32_t w = 1; w < kWarps; ++w) {
+                    sum += sums[w * kBlockFewColumns + threadIdx.x];
+                }
+                static_cast<OutT*>(p.c)[row * p.N + n0 + threadIdx.x] = static_cast<OutT>(sum);
+            }
+        }
+    }
+}
 
 template <uint32_t kRows, typename OutT>
 __global__ void __launch_bounds__(kBlockFewThreads, 2)
@@ -423,7 +528,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     uint64_t* scale_empty = scale_full + S::kGroups;
     uint32_t* tmem_ptr_smem = reinterpret_cast<uint32_t*>(smem + S::kOffTmemPtr);
     uint32_t* dead = reinterpret_cast<uint32_t*>(smem + S::kOffDead);
-    volatile uint32_t* apart_of = reinterpret_cast<volatile uint32_t*>(smem + S::kOffApart);
+    volatile uint32_t* large = reinterpret_cast<volatile uint32_t*>(smem + S::kOffLarge);
     uint32_t* tiles = reinterpret_cast<uint32_t*>(smem + S::kOffTiles);
     uint32_t* row_begin = tiles + p.experts + 1u;
     uint32_t* row_end = row_begin + p.experts;
@@ -449,6 +554,7 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
             mbar_init(&scale_empty[i], 4);
         }
         *dead = 0u;
+        *large = 0u;
         mbar_fence_init();
         tma_prefetch_desc(&tmap_x);
         tma_prefetch_desc(&tmap_w);
@@ -529,60 +635,32 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
                 for (uint32_t i = 0; i < kPerLane; ++i) {
                     load_scales(p.a_scales + min(row + 32u * i, end - 1u) * p.a_scale_row, p.a_scale_block, kb, kb1, x[i]);
                 }
-                float f[kPerLane][4];
-                bool odd = false;
-#pragma unroll
-                for (uint32_t i = 0; i < kPerLane; ++i) {
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; ++j) {
-                        f[i][j] = x[i][j] * (w[j] * kHeld);
-                        odd = odd || !is_ordinary(f[i][j]);
-                    }
-                }
-                bool apart = __any_sync(0xFFFFFFFFu, odd);
-                uint32_t power[kPerLane] = {};  // of four blocks
-                if (__builtin_expect(apart, 0)) {
-                    odd = false;
-#pragma unroll
-                    for (uint32_t i = 0; i < kPerLane; ++i) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) {
-                            odd = odd || needs_both_scales(x[i][j], w[j], f[i][j]);
-                        }
-                    }
-                    apart = __any_sync(0xFFFFFFFFu, odd);
-                }
-                if (__builtin_expect(apart, 0)) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kPerLane; ++i) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) {
-                            float g;
-                            f[i][j] = wide_factor(x[i][j], w[j], g);
-                            power[i] |= (__float_as_uint(g) >> 23) << (8u * j);
-                        }
-                    }
-                }
                 const uint32_t slot = group % S::kGroups;
                 alive = mbar_wait_soon(&scale_empty[slot], ((group / S::kGroups) & 1u) ^ 1u, p.status, 405, slot, bar_ns);
                 if (!alive) {
                     break;
                 }
                 float* factor = reinterpret_cast<float*>(smem + S::kOffFactor) + slot * (4u * kRows) + lane;
-                if (lane < kRows) {
+                uint32_t most = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const float w_held = w[j] * kHeld;
 #pragma unroll
                     for (uint32_t i = 0; i < kPerLane; ++i) {
-#pragma unroll
-                        for (uint32_t j = 0; j < 4; ++j) {
-                            factor[j * kRows + 32u * i] = f[i][j];
-                            if (apart) {
-                                smem[S::kOffPower + (slot * 4u + j) * kRows + lane + 32u * i] = (uint8_t)(power[i] >> (8u * j));
-                            }
+                        const float f = x[i][j] * w_held;
+                        most = max(most, __float_as_uint(f));
+                        if (lane < kRows) {
+                            factor[j * kRows + 32u * i] = f;
                         }
                     }
                 }
-                if (lane == 0) {
-                    apart_of[slot] = apart ? 1u : 0u;
+                if (__builtin_expect(most >= kFactorLimit, 0)) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kPerLane * 4; ++i) {
+                        if (needs_both_scales(x[i / 4][i % 4], w[i % 4], x[i / 4][i % 4] * (w[i % 4] * kHeld))) {
+                            *large = 1u;
+                        }
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -594,58 +672,25 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         // ------------------------------- promotion and output -----------------------------
         const uint32_t tmem = tmem_base + ((warp * 32u) << 16), column = warp * 32u + lane;
         uint32_t it = 0, group = 0;
-        bool apart = false;  // the group that comes next is marked
         for (uint32_t unit = first_unit; alive && unit < num_units; unit += stride) {
             const TileCoord tc = walk.seek(tiles, n_tiles, unit);
             const uint32_t first = row_begin[walk.e] + tc.m_tile * kRows, rows = min(row_end[walk.e] - first, kRows);
             const uint32_t n0 = tc.n_tile * kBlockFewColumns;
             float acc[kRows] = {};
-            // A block of K: waits for its tile and, at the end of a group, for the next one's factors.
-            struct Step {
-                uint32_t b, slot, j;
-                bool group_end;
-            };
-            auto begin = [&](uint32_t kb) {
-                Step t = {it % kTiles, group % S::kGroups, (kb - kb0) & 3u, false};
-                t.group_end = t.j == 3u || kb + 1u == kb1;
-                const uint32_t next = (group + 1u) % S::kGroups;
-                if (t.group_end && (kb + 1u < kb1 || unit + stride < num_units)) {
-                    alive = mbar_wait_both(&tmem_full[t.b], (it / kTiles) & 1u, &scale_full[next], ((group + 1u) / S::kGroups) & 1u, p.status, 406, t.b, bar_ns);
-                    apart = __any_sync(0xFFFFFFFFu, apart_of[next] != 0u);
-                } else {
-                    alive = mbar_wait_soon(&tmem_full[t.b], (it / kTiles) & 1u, p.status, 406, t.b, bar_ns);
-                }
-                tcgen05_fence_after();
-                return t;
-            };
-            auto give_back = [&](const Step& t) {
-                tcgen05_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&tmem_empty[t.b]);
-                    if (t.group_end) {
-                        mbar_arrive(&scale_empty[t.slot]);
-                    }
-                }
-                group += t.group_end ? 1u : 0u;
-                ++it;
-            };
-            if (unit == first_unit) {
-                alive = mbar_wait_soon(&scale_full[0], 0u, p.status, 407, 0, bar_ns);
-                apart = __any_sync(0xFFFFFFFFu, apart_of[0] != 0u);
-            }
-            uint32_t kb = kb0;
-            while (alive && kb < kb1 && !apart) {
-                const Step t = begin(kb);
+            for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t b = it % kTiles, slot = group % S::kGroups, j = (kb - kb0) & 3u;
+                alive = j == 0u ? mbar_wait_both(&tmem_full[b], (it / kTiles) & 1u, &scale_full[slot], (group / S::kGroups) & 1u, p.status, 406, b, bar_ns)
+                                : mbar_wait_soon(&tmem_full[b], (it / kTiles) & 1u, p.status, 406, b, bar_ns);
                 if (!alive) {
                     break;  // a tile that never filled is not written out
                 }
-                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (t.slot * 4u + t.j) * (kRows / 4);
+                tcgen05_fence_after();
+                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (slot * 4u + j) * (kRows / 4);
 #pragma unroll
                 for (uint32_t c = 0; c < kRows; c += 16) {
                     if (c < rows) {
                         float v[16];
-                        tmem_ld_16(tmem + t.b * kRows + c, v);
+                        tmem_ld_16(tmem + b * kRows + c, v);
                         tmem_ld_fence(v);
 #pragma unroll
                         for (uint32_t i = 0; i < 16; i += 4) {
@@ -655,43 +700,18 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
                         }
                     }
                 }
-                give_back(t);
-                ++kb;
-            }
-            float back = 1.0f / kHeld;
-            if (kb < kb1) {
-                scale_sums(acc, back);
-                back = 1.0f;
-            }
-            while (alive && kb < kb1) {  // from a marked group to the end of the unit
-                const uint32_t marked = apart_of[group % S::kGroups];
-                const Step t = begin(kb);
-                if (!alive) {
-                    break;
-                }
-                const float4* factor = reinterpret_cast<const float4*>(smem + S::kOffFactor) + (t.slot * 4u + t.j) * (kRows / 4);
-                const uint32_t* power = reinterpret_cast<const uint32_t*>(smem + S::kOffPower) + (t.slot * 4u + t.j) * (kRows / 4);
-#pragma unroll
-                for (uint32_t c = 0; c < kRows; c += 16) {
-                    if (c < rows) {
-                        float v[16];
-                        tmem_ld_16(tmem + t.b * kRows + c, v);
-                        tmem_ld_fence(v);
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; i += 4) {
-                            const float4 f = factor[(c + i) / 4];
-                            const uint32_t e = marked ? power[(c + i) / 4] : 0x57575757u;  // 2^-40
-                            mul_2(v[i], v[i + 1], __uint_as_float((e & 0xFFu) << 23), __uint_as_float((e >> 8 & 0xFFu) << 23));
-                            mul_2(v[i + 2], v[i + 3], __uint_as_float((e >> 16 & 0xFFu) << 23), __uint_as_float((e >> 24) << 23));
-                            fma_2(acc[c + i], acc[c + i + 1], v[i], v[i + 1], f.x, f.y);
-                            fma_2(acc[c + i + 2], acc[c + i + 3], v[i + 2], v[i + 3], f.z, f.w);
-                        }
+                tcgen05_fence_before();
+                __syncwarp();
+                const bool group_end = j == 3u || kb + 1u == kb1;
+                if (lane == 0) {
+                    mbar_arrive(&tmem_empty[b]);
+                    if (group_end) {
+                        mbar_arrive(&scale_empty[slot]);
                     }
                 }
-                give_back(t);
-                ++kb;
+                group += group_end ? 1u : 0u;
             }
-            scale_sums(acc, back);
+            scale_sums(acc, 1.0f / kHeld);
             OutT* out = static_cast<OutT*>(p.c) + (size_t)first * p.N + n0;
             if (p.parts == 1u) {
                 if (alive && n0 + column < p.N) {
@@ -707,9 +727,9 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
             // The sums of all parts.  Every CTA of the cluster has multiplied its last block: the rings are idle.
             const uint32_t shift = __ffs(kBlockFewColumns / p.parts) - 1;  // of a part's columns
             cluster_sync_all();
-            if (!alive && lane == 0) {
+            if (lane == 0 && (!alive || *large != 0u)) {
                 for (uint32_t d = 0; d < p.parts; ++d) {
-                    st_shared_cluster_u32(map_to_cta(smem_u32(dead), d), 1u);
+                    st_shared_cluster_u32(map_to_cta(smem_u32(smem) + (alive ? S::kOffLarge : S::kOffDead), d), 1u);
                 }
             }
             __syncwarp();
@@ -751,6 +771,8 @@ block_gemm_few_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     tcgen05_fence_before();
     if (__syncthreads_or(alive ? 0 : 1)) {
         drain_after_abort(p.status);
+    } else if (__builtin_expect(*large != 0u, 0)) {
+        block_few_again<kRows, OutT>(p, tiles, reinterpret_cast<float*>(smem));
     }
     if (warp == 6) {
         tcgen05_fence_after();

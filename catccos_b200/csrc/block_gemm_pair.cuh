@@ -132,32 +132,22 @@ __device__ __forceinline__ void tma_expect_and_load_3d_pair(void* smem_dst, cons
         : "memory");
 }
 
-// By column: whether some product of a row's and a column's scale, of the whole warp's, may not be ordinary.  Looks at the largest and the
-// smallest ones (as ordered bits), and only when these say so at the finite ones other than zero alone.
+// By column: whether some product of a row's and a column's scale, of the whole warp's, may not stand for them.  Looks at the largest ones by
+// their bits, and only when these say so at the finite ones alone.
 __device__ __forceinline__ bool scales_apart(const float (&rows)[4][4], const float4 (&columns)[4])
 {
     auto outside = [&](bool all) {
-        uint32_t most[2] = {0u, 0u}, least[2] = {0x7F800000u, 0x7F800000u};
+        uint32_t most[2] = {0u, 0u};  // of the rows' scales, of the columns'
         auto see = [&](uint32_t side, float s) {
-            if (all || is_finite_and_not_zero(s)) {
-                const uint32_t size = __float_as_uint(s) & 0x7FFFFFFFu;
-                most[side] = max(most[side], size);
-                least[side] = min(least[side], size);
-            }
+            most[side] = max(most[side], all ? __float_as_uint(s) : (is_finite(s) ? __float_as_uint(s) & 0x7FFFFFFFu : 0u));
         };
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
             see(0, rows[i][0]), see(0, rows[i][1]), see(0, rows[i][2]), see(0, rows[i][3]);
             see(1, columns[i].x), see(1, columns[i].y), see(1, columns[i].z), see(1, columns[i].w);
         }
-        float top = kHeld, bottom = kHeld;
-#pragma unroll
-        for (uint32_t side = 0; side < 2; ++side) {
-            top *= __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, most[side]));
-            bottom *= __uint_as_float(__reduce_min_sync(0xFFFFFFFFu, least[side]));
-        }
-        // without any finite scale, or none but zeros: 0 and infinity, or NaN
-        return all ? !is_ordinary(top) || !is_ordinary(bottom) : top >= 0x1p64f || bottom < 0x1p-126f;
+        const float top = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, most[0])) * kHeld * __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, most[1]));
+        return __float_as_uint(top) >= kFactorLimit;
     };
     return __builtin_expect(outside(true), 0) && outside(false);
 }
@@ -311,7 +301,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j) {
                         const float* at = p.b_scales + (kb + j) * p.b_scale_block + u.n0 + 4u * lane;
-                        columns[j] = kb + j < k_blocks && u.n0 + 4u * lane < p.N ? __ldcg(reinterpret_cast<const float4*>(at)) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+                        columns[j] = kb + j < k_blocks && u.n0 + 4u * lane < p.N ? __ldcg(reinterpret_cast<const float4*>(at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
                 }
                 const uint32_t slot = group % S::kScaleSlots;
@@ -338,15 +328,19 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                         f[i / 4][i % 4] = a[i / 4][i % 4] * kHeld;
                     }
                 } else {
-                    bool odd = false;
+                    uint32_t most = 0;
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        f[i / 4][i % 4] = a[i / 4][i % 4] * (b[i % 4] * kHeld);
-                        odd = odd || !is_ordinary(f[i / 4][i % 4]);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const float held = b[j] * kHeld;
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            f[i][j] = a[i][j] * held;
+                            most = max(most, __float_as_uint(f[i][j]));
+                        }
                     }
-                    apart = __any_sync(0xFFFFFFFFu, odd);
+                    apart = __any_sync(0xFFFFFFFFu, most >= kFactorLimit);
                     if (__builtin_expect(apart, 0)) {
-                        odd = false;
+                        bool odd = false;
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) {
                             odd = odd || needs_both_scales(a[i / 4][i % 4], b[i % 4], f[i / 4][i % 4]);

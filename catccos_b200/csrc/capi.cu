@@ -1943,6 +1943,11 @@ int block_product(const char* name, void* stream, const catccos_b200_block_opera
         return CATCCOS_B200_ESTATE;  // the record of its waits is on the rank's device
     }
     BlockGemmParams p = {};
+    p.a = static_cast<const uint8_t*>(a->codes);
+    p.b = static_cast<const uint8_t*>(b->codes);
+    p.a_line = a->line_bytes;
+    p.b_line = b->line_bytes;
+    p.b_matrix = experts > 1 ? b->matrix_bytes : 0;
     p.a_scales = a->scales;
     p.a_scale_row = a->scale_row;
     p.a_scale_block = a->scale_col;

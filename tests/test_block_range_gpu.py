@@ -73,7 +73,8 @@ def test_blocks_of_zeros_between_others(capi, cuda, a_e, b_e, form, by_column):
         c = capi.block_gemm(a, a_scales, b, b_scales, out_dtype=torch.float32)
     assert bool(torch.isfinite(c).all()) and bool(_check(torch, c, a, a_scales, b, b_scales).all())
     if not by_column:  # a row's result does not depend on the others
-        assert torch.equal(c, clean)
+        others = torch.arange(m, device="cuda") != 3
+        assert torch.equal(c[others], clean[others])
 
 
 @pytest.mark.parametrize("form,by_column", [(f, False) for f in FORMS] + [(f, True) for f in PAIR], ids=IDS + ["by_column"])
