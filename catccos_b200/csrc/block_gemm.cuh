@@ -236,7 +236,8 @@ __device__ __forceinline__ void load_scales(const float* line, size_t step, uint
 //   Few rows: before a CTA ends, rows with such a block are computed again from the codes in global memory.
 // A row without such blocks gets the same result whatever the others have (by column: but for its last bit).  With such scales in 5 % of the
 // rows 8192 x 2304 x 7168 takes 220 us (150), 16 x 4096 x 7168 with one such row 91 (10.9).  Other calls pay 0 to 2 %, short ones (5 to 20 us) 1 to
-// 4, on pairs 4 to 8.  A choice inside one loop cost them 5 to 25 %, for few rows a second loop 2 to 7, on pairs the rows at the end 3 on large products.
+// 4, on pairs 4 to 10.  A choice inside one loop cost them 5 to 25 %, for few rows a second loop 2 to 7, on pairs the rows at the end 3 on large
+// products.
 constexpr float kHeld = 0x1p40f;
 constexpr uint32_t kFactorLimit = 0x5F800000u;  // 2^64 as bits; a negative factor, an infinity and a NaN are above it, too, and looked at again
 
