@@ -318,7 +318,7 @@ block_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                     }
                 }
                 __syncwarp();
-                // whether some product may not stand for its two scales; by column: of the group's largest or smallest ones
+                // whether some product may not stand for its two scales; by column: of the group's largest ones
                 float f[4][4];
                 bool apart;
                 if (kByColumn) {
